@@ -132,7 +132,7 @@ def prepare(case, seed):
     randn = lambda tokens, heads, scale: (torch.randn(tokens, heads, hd, generator=g, device="cuda") * scale).to(dtype)  # noqa: E731
     s = {"case": c, "longest": max(lengths)}
     q_heads, rows = c["kv_heads"] * c["share"], c["batch"] if kind == "decode" else sum(lengths)
-    s["q"] = randn(rows, q_heads, 1.25)
+    s["q"] = randn(rows, q_heads, 1.0)
     if kind != "decode":
         s["k"], s["v"] = randn(rows, c["kv_heads"], 1.0), randn(rows, c["kv_heads"], 1.0)
         s["ends"] = _ints(_ends(lengths))

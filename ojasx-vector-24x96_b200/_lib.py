@@ -7,7 +7,7 @@ import os
 PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(PKG_DIR, "libojasx_lut_b200.so")
 
-_vp, _i, _sz, _f = C.c_void_p, C.c_int, C.c_size_t, C.c_float
+_vp, _i, _sz, _f, _ll = C.c_void_p, C.c_int, C.c_size_t, C.c_float, C.c_longlong
 
 
 
@@ -121,6 +121,12 @@ SIGNATURES = {
     "ojasx_b200_rmsnorm": (_i, [_vp, _vp, _vp, _vp, _i, _i, _f, _i, _vp]),
     "ojasx_b200_rope_qk": (_i, [_vp, _vp, _vp, _i, _i, _i, _i, _f, _i, _vp]),
     "ojasx_b200_add_int": (_i, [_vp, _i, _i, _vp]),
+    "ojasx_b200_q4kv_page_bytes": (_sz, [_i, _i, _i]),
+    "ojasx_b200_q4kv_append": (_i, [_vp, _ll, _vp, _ll, _vp, _ll, _vp, _vp, _vp, _vp, _vp, _vp, _vp] + [_i] * 9 + [_vp]),
+    "ojasx_b200_q4kv_read": (_i, [_vp] * 7 + [_i] * 8 + [_vp]),
+    "ojasx_b200_q4kv_decode_workspace": (_sz, [_i] * 6),
+    "ojasx_b200_q4kv_decode": (_i, [_vp] * 6 + [_i] * 7 + [_f, _i, _vp, _sz, _vp]),
+    "ojasx_b200_prompt_attention": (_i, [_vp, _ll, _ll] * 3 + [_vp] * 3 + [_i] * 6 + [_f, _i, _vp]),
 }
 
 _lib = None

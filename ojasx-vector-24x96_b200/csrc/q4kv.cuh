@@ -1,0 +1,60 @@
+// Layout of the 4-bit paged KV cache.
+//
+// 32 consecutive dimensions of a token's key or value form a group with a bf16 minimum and a bf16 scale: minimum = floor(min x) and
+// scale = ceil((max x - minimum) / 15), to the neighbouring bf16 number, code = round((x - minimum) / scale) in 0..15.  Rounding the
+// two outwards keeps every x of the group inside the 16 steps, so that it is read back within half a step.  A group with a value
+// that is not finite has a NaN for its scale and its minimum and is read back as NaN.
+//
+// A page of one KV head is page_size / 16 tiles of 16 tokens, each contiguous (2560 bytes at head_dim 128), pools are
+// [pages][kv_heads][tiles].  A tile is laid out as the operands of mma.sync m16n8k16 that the decode kernel makes of it, so that
+// every lane reads whole 8- or 16-byte pieces, G = head_dim / 32 groups:
+//   keys     [token][t = 0..3][g]: words; word (t, g) holds dimensions 32 g + 8 t + j in nibble j
+//   their    [token][g]: words, minimum << 16 | scale
+//   values   [half][c = 0..7][pair = 0..3][g]: words; tokens 8 half + 2 pair (low 16 bits) and + 1 (high 16 bits), dimensions
+//            32 g + 4 c + i in nibble i of either
+//   their    [token][g]: words, minimum << 16 | scale
+#pragma once
+#include "common.cuh"
+
+namespace ojx {
+
+constexpr int kQ4Group = 32;
+constexpr int kQ4Tile = 16;    // tokens of a tile
+
+template <int HD>
+struct Q4Layout {
+    static constexpr int G = HD / kQ4Group;
+    static constexpr int key_meta = kQ4Tile * HD / 2;
+    static constexpr int values = key_meta + kQ4Tile * G * 4;
+    static constexpr int value_meta = values + kQ4Tile * HD / 2;
+    static constexpr int bytes = value_meta + kQ4Tile * G * 4;
+    // dimensions 32 g + 4 c .. + 3 of a token, as 16 bits
+    __host__ __device__ static constexpr int key_at(int token, int g, int c) { return ((token * 4 + (c >> 1)) * G + g) * 4 + (c & 1) * 2; }
+    __host__ __device__ static constexpr int value_at(int token, int g, int c) {
+        return values + ((((token >> 3) * 8 + c) * 4 + ((token >> 1) & 3)) * G + g) * 4 + (token & 1) * 2;
+    }
+    __host__ __device__ static constexpr int meta_at(int token, int g) { return (token * G + g) * 4; }   // from key_meta or value_meta
+};
+
+struct Q4Cache {
+    uint8_t* pool;              // [num_pages][kv_heads][page_size / 16][tile]
+    const int* block_table;     // [batch][max_pages] page ids; ids outside [0, num_pages) hold nothing
+    int* status;                // set to 1 where a token has no page
+    int max_pages, num_pages, page_size, kv_heads;
+};
+
+// Tile of `token` of sequence b for one KV head, or null where the table has no page for it.
+template <int HD>
+__device__ __forceinline__ uint8_t* q4_tile(const Q4Cache& C, int b, int head, int token) {
+    const int p = token / C.page_size;
+    if (token < 0 || p >= C.max_pages) return nullptr;
+    const int id = C.block_table[(size_t)b * C.max_pages + p];
+    if ((unsigned)id >= (unsigned)C.num_pages) return nullptr;
+    const int tiles = C.page_size / kQ4Tile;
+    return C.pool + (((size_t)id * C.kv_heads + head) * tiles + (token - p * C.page_size) / kQ4Tile) * Q4Layout<HD>::bytes;
+}
+
+__device__ __forceinline__ float q4_scale(unsigned meta) { return __uint_as_float(meta << 16); }
+__device__ __forceinline__ float q4_min(unsigned meta) { return __uint_as_float(meta & 0xffff0000u); }
+
+}  // namespace ojx

@@ -435,3 +435,238 @@ class VQKVCache:
             self.close()
         except Exception:
             pass
+
+
+def _index32(t: torch.Tensor, name: str, shape, device) -> torch.Tensor:
+    """An int32 tensor of a call: on the call's device, contiguous, of the given shape."""
+    _require_cuda(t, name)
+    if t.dtype is not torch.int32 or tuple(t.shape) != tuple(shape) or t.device != device or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous int32 tensor of shape {tuple(shape)} on {device}")
+    return t
+
+
+def _heads(t: torch.Tensor, name: str, rows: int, heads: int, head_dim: int, like: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Activations [rows, heads, head_dim] of a call, float32 or bfloat16 like the others."""
+    _require_cuda(t, name)
+    _dtype_code(t)
+    if tuple(t.shape) != (rows, heads, head_dim):
+        raise ValueError(f"{name} must have the shape {(rows, heads, head_dim)}, got {tuple(t.shape)}")
+    if like is not None and (t.dtype != like.dtype or t.device != like.device):
+        raise ValueError(f"{name} must have the dtype and the device of the other activations")
+    return t
+
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """``t`` itself where its heads lie behind one another in rows on 16-byte boundaries (a view into a fused projection does), a copy
+    else."""
+    unit = 16 // t.element_size()
+    fits = t.stride(2) == 1 and t.stride(1) == t.shape[2] and t.stride(0) % unit == 0 and t.stride(0) >= 0 and t.data_ptr() % 16 == 0
+    if t.numel() == 0 or fits:
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+def _out(out: Optional[torch.Tensor], like: torch.Tensor) -> torch.Tensor:
+    if out is None:
+        return torch.empty(like.shape, device=like.device, dtype=like.dtype)
+    if out.shape != like.shape or out.dtype != like.dtype or out.device != like.device or not out.is_contiguous() or out.data_ptr() % 16:
+        raise ValueError("out must be contiguous, 16-byte aligned and of the shape, dtype and device of q")
+    return out
+
+
+class Q4PagedKVCache:
+    """Paged KV cache of one layer in 4 bits: 32 dimensions of a key or value share a bf16 scale and a bf16 minimum, 160 bytes per
+    token and KV head at head_dim 128.
+
+    The cache holds the pages; which page belongs to which sequence, and how many tokens a sequence has, is the caller's and goes
+    into every call: ``block_table`` int32 [batch, pages per sequence] (entries outside the pool, such as -1, are no page) and
+    ``positions`` or ``lengths`` int32 [batch], all on the device, so that layers share them and a captured graph follows them.
+    ``rope_theta``: keys and the queries given with them are turned by ``position * theta^(-2j / head_dim)`` on the way in
+    (``None``: they come as they are to be kept).  A call that finds no page for a token drops it and raises a flag that
+    ``check`` reports."""
+
+    def __init__(self, num_pages: int, page_size: int, kv_heads: int, q_heads: int, head_dim: int, rope_theta: Optional[float] = None,
+                 device: Optional[torch.device] = None):
+        if min(num_pages, page_size, kv_heads, q_heads) <= 0 or q_heads % kv_heads:
+            raise ValueError("num_pages, page_size and the head counts must be positive, q_heads a multiple of kv_heads")
+        if head_dim not in (64, 128) or page_size % 16:
+            raise ValueError("head_dim must be 64 or 128 and page_size a multiple of 16")
+        if rope_theta is not None and not rope_theta > 0:
+            raise ValueError("rope_theta must be positive")
+        self.num_pages, self.page_size, self.kv_heads, self.q_heads = int(num_pages), int(page_size), int(kv_heads), int(q_heads)
+        self.head_dim, self.rope_theta = int(head_dim), rope_theta
+        device = torch.device("cuda") if device is None else torch.device(device)
+        self.device = torch.device("cuda", torch.cuda.current_device()) if device.index is None else device
+        self.page_bytes = int(lib().ojasx_b200_q4kv_page_bytes(self.kv_heads, self.page_size, self.head_dim))
+        self.pool = torch.zeros((self.num_pages, self.page_bytes), dtype=torch.uint8, device=self.device)
+        self._status = torch.zeros(1, dtype=torch.int32, device=self.device)
+        self._turns = None
+        if rope_theta is not None:
+            j = np.arange(self.head_dim // 2, dtype=np.float64)
+            self._turns = torch.from_numpy(float(rope_theta) ** (-2.0 * j / self.head_dim) / (2.0 * np.pi)).to(self.device)
+
+    @property
+    def memory_bytes(self) -> int:
+        return self.pool.numel()
+
+    def check(self) -> None:
+        """Raises if a call since the last check met a token without a page (synchronises)."""
+        if int(self._status.item()):
+            self._status.zero_()
+            raise OjasxB200Error("a call on this cache met a token whose block table entry is no page of the pool")
+
+    # ------------------------------------------------------------------ codes in and out
+    def _tiles(self):
+        """The pool as (key codes, key metas, value codes, value metas) by the layout of csrc/q4kv.cuh, views of int32 words."""
+        G, T = self.head_dim // 32, self.page_size // 16
+        words = self.pool.view(torch.int32).view(self.num_pages, self.kv_heads, T, -1)
+        cuts = [16 * 4 * G, 16 * G, 16 * 4 * G, 16 * G]
+        k, km, v, vm = words.split(cuts, dim=-1)
+        lead = (self.num_pages, self.kv_heads, T)
+        return k.view(*lead, 16, 4, G), km.view(*lead, 16, G), v.view(*lead, 2, 8, 4, G), vm.view(*lead, 16, G)
+
+    def load(self, k_codes, k_scales, k_mins, v_codes, v_scales, v_mins) -> None:
+        """Fills the pool: codes uint8 0..15 [num_pages, kv_heads, page_size, head_dim], scales and minima bf16
+        [num_pages, kv_heads, page_size, head_dim / 32]."""
+        G, T = self.head_dim // 32, self.page_size // 16
+        lead = (self.num_pages, self.kv_heads, T)
+        for name, t, last, dtype in (("k_codes", k_codes, self.head_dim, torch.uint8), ("v_codes", v_codes, self.head_dim, torch.uint8),
+                                     ("k_scales", k_scales, G, torch.bfloat16), ("k_mins", k_mins, G, torch.bfloat16),
+                                     ("v_scales", v_scales, G, torch.bfloat16), ("v_mins", v_mins, G, torch.bfloat16)):
+            if tuple(t.shape) != (self.num_pages, self.kv_heads, self.page_size, last) or t.dtype != dtype:
+                raise ValueError(f"{name} must be {dtype} of shape {(self.num_pages, self.kv_heads, self.page_size, last)}")
+        k, km, v, vm = self._tiles()
+        nibbles = lambda c, n: sum((c[..., i].to(torch.int32) & 15) << (4 * i) for i in range(n))  # noqa: E731
+        word16 = lambda t: t.contiguous().view(torch.int16).to(torch.int32)  # noqa: E731
+        meta = lambda mins, scales: ((word16(mins) << 16) | (word16(scales) & 0xffff)).view(*lead, 16, G)  # noqa: E731
+        k.copy_(nibbles(k_codes.to(self.device).view(*lead, 16, G, 4, 8), 8).transpose(-1, -2))
+        halves = nibbles(v_codes.to(self.device).view(*lead, 2, 4, 2, G, 8, 4), 4)     # [half, pair, odd, g, c]
+        v.copy_(((halves[..., 1, :, :] << 16) | halves[..., 0, :, :]).permute(0, 1, 2, 3, 6, 4, 5))
+        km.copy_(meta(k_mins.to(self.device), k_scales.to(self.device)))
+        vm.copy_(meta(v_mins.to(self.device), v_scales.to(self.device)))
+
+    def unload(self) -> dict:
+        """The pool as ``load`` takes it."""
+        k, km, v, vm = self._tiles()
+        shape = (self.num_pages, self.kv_heads, self.page_size)
+        bf16 = lambda w: w.to(torch.int16).view(torch.bfloat16).reshape(*shape, -1)  # noqa: E731
+        split = lambda w, n: torch.stack([(w >> (4 * i)) & 15 for i in range(n)], -1).to(torch.uint8)  # noqa: E731
+        halves = torch.stack([v & 0xffff, (v >> 16) & 0xffff], -1).permute(0, 1, 2, 3, 5, 7, 6, 4)   # [half, pair, odd, g, c]
+        return {"k_codes": split(k.transpose(-1, -2), 8).reshape(*shape, -1), "k_scales": bf16((km << 16) >> 16), "k_mins": bf16(km >> 16),
+                "v_codes": split(halves, 4).reshape(*shape, -1), "v_scales": bf16((vm << 16) >> 16), "v_mins": bf16(vm >> 16)}
+
+    # ------------------------------------------------------------------ the calls of a model
+    def _table(self, block_table: torch.Tensor, rows: Optional[int] = None) -> torch.Tensor:
+        if block_table.dim() != 2 or block_table.shape[1] == 0 or (rows is not None and block_table.shape[0] != rows):
+            raise ValueError("block_table must be [batch, pages per sequence], a row for every sequence")
+        return _index32(block_table, "block_table", block_table.shape, self.device)
+
+    def append(self, k: torch.Tensor, v: torch.Tensor, block_table: torch.Tensor, positions: torch.Tensor,
+               q: Optional[torch.Tensor] = None, cu_seqlens: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
+        """``k``, ``v`` [tokens, kv_heads, head_dim] behind the ``positions[b]`` tokens that sequence b has: one token per sequence, or
+        with ``cu_seqlens`` int32 [batch + 1] the packed tokens ``cu_seqlens[b] .. cu_seqlens[b + 1]``.  ``q``
+        [tokens, q_heads, head_dim] is turned as the keys are and returned (its rows behind the last sequence are not written)."""
+        B, n = block_table.shape[0], k.shape[0]
+        table = self._table(block_table)
+        _heads(k, "k", n, self.kv_heads, self.head_dim)
+        _heads(v, "v", n, self.kv_heads, self.head_dim, k)
+        if k.device != self.device:
+            raise ValueError(f"the cache is on {self.device}")
+        if cu_seqlens is None and n != B:
+            raise ValueError("one token per sequence, or cu_seqlens")
+        positions = _index32(positions, "positions", (B,), self.device)
+        ends = None if cu_seqlens is None else _index32(cu_seqlens, "cu_seqlens", (B + 1,), self.device).data_ptr()
+        k, v, out = _rows(k), _rows(v), None
+        if q is not None:
+            q = _rows(_heads(q, "q", n, self.q_heads, self.head_dim, k))
+            out = torch.empty(q.shape, device=q.device, dtype=q.dtype)
+        if n and B:
+            with torch.cuda.device(self.device):
+                check(lib().ojasx_b200_q4kv_append(k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0), None if q is None else q.data_ptr(),
+                                                   0 if q is None else q.stride(0), None if q is None else out.data_ptr(), self.pool.data_ptr(),
+                                                   table.data_ptr(), positions.data_ptr(), ends, None if self._turns is None else self._turns.data_ptr(),
+                                                   self._status.data_ptr(), n, B, table.shape[1], self.num_pages, self.page_size, self.kv_heads,
+                                                   self.q_heads, self.head_dim, _dtype_code(k), _stream_ptr(self.device)), "ojasx_b200_q4kv_append")
+        return out
+
+    def read(self, block_table: torch.Tensor, cu_seqlens: torch.Tensor, tokens: int, positions: Optional[torch.Tensor] = None,
+             dtype: torch.dtype = torch.bfloat16):
+        """(k, v) [tokens, kv_heads, head_dim]: the values of ``cu_seqlens[b + 1] - cu_seqlens[b]`` tokens of every sequence, from
+        ``positions[b]`` (default 0) on.  Rows behind the last sequence are not written."""
+        table, B = self._table(block_table), block_table.shape[0]
+        ends = _index32(cu_seqlens, "cu_seqlens", (B + 1,), self.device)
+        positions = None if positions is None else _index32(positions, "positions", (B,), self.device).data_ptr()
+        k = torch.empty((int(tokens), self.kv_heads, self.head_dim), device=self.device, dtype=dtype)
+        v = torch.empty_like(k)
+        if tokens and B:
+            with torch.cuda.device(self.device):
+                check(lib().ojasx_b200_q4kv_read(self.pool.data_ptr(), table.data_ptr(), ends.data_ptr(), positions, k.data_ptr(), v.data_ptr(),
+                                                 self._status.data_ptr(), int(tokens), B, table.shape[1], self.num_pages, self.page_size,
+                                                 self.kv_heads, self.head_dim, _dtype_code(k), _stream_ptr(self.device)), "ojasx_b200_q4kv_read")
+        return k, v
+
+    def decode(self, q: torch.Tensor, block_table: torch.Tensor, lengths: torch.Tensor, scale: float = -1.0,
+               out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """One query per sequence, ``q`` [batch, q_heads, head_dim], over the first ``lengths[b]`` tokens of its sequence (zeros for an
+        empty one); ``scale <= 0`` is 1/sqrt(head_dim)."""
+        B = q.shape[0]
+        table = self._table(block_table, B)
+        q = _heads(q, "q", B, self.q_heads, self.head_dim)
+        if q.device != self.device:
+            raise ValueError(f"the cache is on {self.device}")
+        q = q if q.is_contiguous() and q.data_ptr() % 16 == 0 else q.clone(memory_format=torch.contiguous_format)
+        lengths = _index32(lengths, "lengths", (B,), self.device)
+        o = _out(out, q)
+        if B:
+            size = lib().ojasx_b200_q4kv_decode_workspace(B, table.shape[1], self.page_size, self.kv_heads, self.q_heads, self.head_dim)
+            ws = torch.empty(size, device=self.device, dtype=torch.uint8)     # of this call, so that calls on several streams do not share it
+            with torch.cuda.device(self.device):
+                check(lib().ojasx_b200_q4kv_decode(q.data_ptr(), o.data_ptr(), self.pool.data_ptr(), table.data_ptr(), lengths.data_ptr(),
+                                                   self._status.data_ptr(), B, table.shape[1], self.num_pages, self.page_size, self.kv_heads,
+                                                   self.q_heads, self.head_dim, float(scale), _dtype_code(q), ws.data_ptr() if size else None, size,
+                                                   _stream_ptr(self.device)), "ojasx_b200_q4kv_decode")
+        return o
+
+    def prefill(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, block_table: torch.Tensor, positions: torch.Tensor,
+                cu_seqlens: torch.Tensor, cu_context: torch.Tensor, context_tokens: int, scale: float = -1.0,
+                out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """A chunk of every sequence's prompt, packed by ``cu_seqlens``: its keys and values are appended and every query attends to the
+        cached tokens up to its own, as the cache holds them.  ``cu_context`` int32 [batch + 1]: the tokens of the sequences with the
+        chunk, ends of ``positions[b] + chunk`` each; ``context_tokens``: their sum."""
+        turned = self.append(k, v, block_table, positions, q=q, cu_seqlens=cu_seqlens)
+        keys, values = self.read(block_table, cu_context, context_tokens, dtype=q.dtype)
+        return prompt_attention(turned, keys, values, cu_seqlens, cu_context, scale=scale, out=out)
+
+
+def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor, cu_keys: Optional[torch.Tensor] = None,
+                     scale: float = -1.0, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Causal attention over packed prompts: ``q`` [tokens, q_heads, head_dim], ``k``, ``v`` [keys, kv_heads, head_dim], all float32 or all
+    bfloat16, head_dim 64 or 128.  Sequence b has the rows ``cu_seqlens[b] .. cu_seqlens[b + 1]`` and the keys ``cu_keys[b] ..``
+    (default: the same); its last query sees its last key, the one before it the keys up to the one before, and so on.  A query that
+    sees nothing gives zeros; rows behind the last sequence are not written; ``scale <= 0`` is 1/sqrt(head_dim)."""
+    if q.dim() != 3 or k.dim() != 3 or k.shape[1] == 0 or q.shape[1] % k.shape[1]:
+        raise ValueError("q must be [tokens, q_heads, head_dim] and k [keys, kv_heads, head_dim], q_heads a multiple of kv_heads")
+    T, Hq, hd = q.shape
+    if hd not in (64, 128):
+        raise ValueError("head_dim must be 64 or 128")
+    if Hq // k.shape[1] > 64:
+        raise ValueError("at most 64 query heads share a KV head")
+    _heads(q, "q", T, Hq, hd)
+    _heads(k, "k", k.shape[0], k.shape[1], hd, q)
+    _heads(v, "v", k.shape[0], k.shape[1], hd, q)
+    if cu_seqlens.dim() != 1 or cu_seqlens.shape[0] < 1:
+        raise ValueError("cu_seqlens must be [batch + 1]")
+    B = cu_seqlens.shape[0] - 1
+    ends = _index32(cu_seqlens, "cu_seqlens", (B + 1,), q.device)
+    if cu_keys is None and k.shape[0] != T:
+        raise ValueError("as many keys as queries, or cu_keys")
+    key_ends = ends if cu_keys is None else _index32(cu_keys, "cu_keys", (B + 1,), q.device)
+    o = _out(out, q)
+    q, k, v = _rows(q), _rows(k), _rows(v)
+    if T and B:
+        with torch.cuda.device(q.device):
+            check(lib().ojasx_b200_prompt_attention(q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(),
+                                                    v.stride(0), v.stride(1), o.data_ptr(), ends.data_ptr(), key_ends.data_ptr(), B, T, k.shape[0],
+                                                    Hq, k.shape[1], hd, float(scale), _dtype_code(q), _stream_ptr(q.device)),
+                  "ojasx_b200_prompt_attention")
+    return o

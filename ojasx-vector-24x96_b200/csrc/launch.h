@@ -116,6 +116,8 @@ bool moe_fused_wanted(const MoeProblem& P);   // shape fits and enough routed pa
 int launch_moe_fused(MoeProblem P, cudaStream_t stream, const PeerLink* link = nullptr);   // work list, token tables (unless lut_ready), experts
 int launch_moe_prebuild_blocks(const void* x, int io_dtype, int n_tokens, int H, int D, const float* codebook, int Kcb,
                                float* out, cudaStream_t stream);
+// --- prompt.cu
+int take_prompt_error(int* out);   // a bounded wait of attention over prompts ran out
 // --- moe_gather.cu: experts that several tokens are routed to, on mma.sync operands gathered from the codebooks
 bool moe_gather_wanted(const MoeProblem& P);
 int launch_moe_gather(const MoeProblem& P, cudaStream_t s, const PeerLink& link);   // all but the combine

@@ -121,7 +121,7 @@ OJASX_API int ojasx_b200_linear_forward_tensor(OjasxLinearHandle handle, const v
  * and did nothing.  Bit 2: a bounded wait for a bulk copy of a lookup table ran out, or a whole-expert
  * MoE kernel of the chain walk found the same placement and did nothing.  Bit 3: a kernel that walks four
  * vectors at a time gave up on a wait (its results are NaN) or found that placement.  Bit 4: a launch of
- * attention over prompts gave up on a wait.  Negative = CUDA error. */
+ * attention over prompts gave up on a wait; bit 5: one over the 4-bit cache.  Negative = CUDA error. */
 OJASX_API int ojasx_b200_take_device_error(void);
 
 /* Same computation on borrowed device arrays, no handle: the device twin of
@@ -421,7 +421,8 @@ OJASX_API int ojasx_b200_q4kv_append(const void* d_k, long long k_stride, const 
 OJASX_API int ojasx_b200_q4kv_read(const void* d_pool, const int* d_block_table, const int* d_ends, const int* d_positions, void* d_k,
                                    void* d_v, int* d_status, int n_tokens, int batch, int max_pages, int num_pages, int page_size,
                                    int kv_heads, int head_dim, int io_dtype, void* stream);
-OJASX_API size_t ojasx_b200_q4kv_decode_workspace(int batch, int max_pages, int page_size, int kv_heads, int q_heads, int head_dim);
+OJASX_API size_t ojasx_b200_q4kv_decode_workspace(int batch, int max_pages, int page_size, int kv_heads, int q_heads, int head_dim,
+                                                  int io_dtype);
 OJASX_API int ojasx_b200_q4kv_decode(const void* d_q, void* d_out, const void* d_pool, const int* d_block_table, const int* d_lengths,
                                      int* d_status, int batch, int max_pages, int num_pages, int page_size, int kv_heads, int q_heads,
                                      int head_dim, float scale, int io_dtype, void* workspace, size_t workspace_bytes, void* stream);

@@ -124,7 +124,7 @@ SIGNATURES = {
     "ojasx_b200_q4kv_page_bytes": (_sz, [_i, _i, _i]),
     "ojasx_b200_q4kv_append": (_i, [_vp, _ll, _vp, _ll, _vp, _ll, _vp, _vp, _vp, _vp, _vp, _vp, _vp] + [_i] * 9 + [_vp]),
     "ojasx_b200_q4kv_read": (_i, [_vp] * 7 + [_i] * 8 + [_vp]),
-    "ojasx_b200_q4kv_decode_workspace": (_sz, [_i] * 6),
+    "ojasx_b200_q4kv_decode_workspace": (_sz, [_i] * 7),
     "ojasx_b200_q4kv_decode": (_i, [_vp] * 6 + [_i] * 7 + [_f, _i, _vp, _sz, _vp]),
     "ojasx_b200_prompt_attention": (_i, [_vp, _ll, _ll] * 3 + [_vp] * 3 + [_i] * 6 + [_f, _i, _vp]),
 }

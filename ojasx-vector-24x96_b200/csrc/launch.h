@@ -118,6 +118,8 @@ int launch_moe_prebuild_blocks(const void* x, int io_dtype, int n_tokens, int H,
                                float* out, cudaStream_t stream);
 // --- prompt.cu
 int take_prompt_error(int* out);   // a bounded wait of attention over prompts ran out
+// --- q4kv_decode.cu
+int take_q4_error(int* out);       // the same over the 4-bit cache
 // --- moe_gather.cu: experts that several tokens are routed to, on mma.sync operands gathered from the codebooks
 bool moe_gather_wanted(const MoeProblem& P);
 int launch_moe_gather(const MoeProblem& P, cudaStream_t s, const PeerLink& link);   // all but the combine

@@ -1,5 +1,5 @@
-// 4-bit paged KV cache: appending with the position rotation on the way, reading back, attention of single tokens.  Layout and
-// format: q4kv.cuh.
+// 4-bit paged KV cache: appending with the position rotation on the way, and reading back.  Layout and format: q4kv.cuh; attention of
+// single tokens: q4kv_decode.cu.
 #include <cmath>
 
 #include "handles.h"
@@ -159,86 +159,6 @@ __global__ void __launch_bounds__(128) q4_read_kernel(const __grid_constant__ Q4
     }
 }
 
-constexpr float kLowest = -3.0e38f;
-
-struct Q4DecodeProblem {
-    Q4Cache cache;
-    const void* q;              // [batch][q_heads][head_dim]
-    void* out;
-    const int* lengths;         // [batch]
-    int batch, q_heads;
-    float scale;
-};
-
-// A CTA per query head; a warp takes every eighth token, a lane head_dim / 32 dimensions of it; online softmax per warp.
-template <int HD, bool kBf16>
-__global__ void __launch_bounds__(256) q4_decode_kernel(const __grid_constant__ Q4DecodeProblem P) {
-    constexpr int E = HD / 32;
-    using T = Q4Layout<HD>;
-    __shared__ float sm_m[8], sm_l[8], sm_o[8][HD];
-    chain_begin();
-    const int hq = blockIdx.x, b = blockIdx.y, head = hq / (P.q_heads / P.cache.kv_heads);
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const size_t row = ((size_t)b * P.q_heads + hq) * HD;
-    float q[E], o[E], m = kLowest, l = 0.0f;   // (finite: scores of -inf weigh nothing, a NaN makes its head's result one)
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-        const size_t i = row + lane * E + e;
-        q[e] = (kBf16 ? __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(P.q)[i]) : reinterpret_cast<const float*>(P.q)[i]) * P.scale;
-        o[e] = 0.0f;
-    }
-    const int n = min(P.lengths[b], P.cache.max_pages * P.cache.page_size);
-    for (int t = warp; t < n; t += 8) {
-        const uint8_t* tile = q4_tile<HD>(P.cache, b, head, t);
-        if (!tile) {
-            if (lane == 0) atomicExch(P.cache.status, 1);
-            continue;
-        }
-        const int in = t & (kQ4Tile - 1), d = lane * E, g = d / 32, c = d % 32 / 4, sh = d % 4 * 4;
-        const unsigned kw = *reinterpret_cast<const unsigned short*>(tile + T::key_at(in, g, c)) >> sh;
-        const unsigned vw = *reinterpret_cast<const unsigned short*>(tile + T::value_at(in, g, c)) >> sh;
-        const unsigned km = *reinterpret_cast<const unsigned*>(tile + T::key_meta + T::meta_at(in, g));
-        const unsigned vm = *reinterpret_cast<const unsigned*>(tile + T::value_meta + T::meta_at(in, g));
-        float dot = 0.0f;
-#pragma unroll
-        for (int e = 0; e < E; ++e) dot = fmaf(q[e], fmaf((float)(kw >> (4 * e) & 15), q4_scale(km), q4_min(km)), dot);
-#pragma unroll
-        for (int off = 16; off >= 1; off >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, off);
-        const float top = fmaxf(m, dot), p = __expf(dot - top), keep = __expf(m - top);
-        l = fmaf(l, keep, p);
-#pragma unroll
-        for (int e = 0; e < E; ++e) o[e] = fmaf(o[e], keep, p * fmaf((float)(vw >> (4 * e) & 15), q4_scale(vm), q4_min(vm)));
-        m = top;
-    }
-    if (lane == 0) { sm_m[warp] = m; sm_l[warp] = l; }
-#pragma unroll
-    for (int e = 0; e < E; ++e) sm_o[warp][lane * E + e] = o[e];
-    __syncthreads();
-    float M = kLowest, L = 0.0f, acc = 0.0f;
-    for (int w = 0; w < 8; ++w) M = fmaxf(M, sm_m[w]);
-    if (threadIdx.x < HD) {
-        for (int w = 0; w < 8; ++w) {
-            const float keep = __expf(sm_m[w] - M);
-            L = fmaf(sm_l[w], keep, L);
-            acc = fmaf(sm_o[w][threadIdx.x], keep, acc);
-        }
-        acc = L == 0.0f ? 0.0f : acc / L;
-        if (kBf16) reinterpret_cast<__nv_bfloat16*>(P.out)[row + threadIdx.x] = __float2bfloat16_rn(acc);
-        else reinterpret_cast<float*>(P.out)[row + threadIdx.x] = acc;
-    }
-}
-
-// What every entry point asks of a cache.
-static int q4_check(const void* pool, const int* table, int max_pages, int num_pages, int page_size, int kv_heads, int head_dim, int batch,
-                    int dtype, int* status) {
-    if (!pool || !table || !status || max_pages <= 0 || num_pages <= 0 || kv_heads <= 0 || batch <= 0) return OJX_ERR_ARG;
-    if (dtype != OJX_F32 && dtype != OJX_BF16) return OJX_ERR_ARG;
-    if (page_size <= 0 || page_size % kQ4Tile || (head_dim != 64 && head_dim != 128)) return OJX_ERR_UNSUPPORTED;
-    if ((long long)max_pages * page_size > 0x7fffffffLL) return OJX_ERR_TOO_LARGE;
-    return (reinterpret_cast<uintptr_t>(pool) & 15) ? OJX_ERR_ARG : OJX_OK;
-}
-static bool q4_aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
-
 }  // namespace ojx
 
 using namespace ojx;
@@ -285,31 +205,6 @@ int ojasx_b200_q4kv_read(const void* d_pool, const int* d_block_table, const int
     auto kernel = head_dim == 64 ? (bf ? q4_read_kernel<64, true> : q4_read_kernel<64, false>)
                                  : (bf ? q4_read_kernel<128, true> : q4_read_kernel<128, false>);
     OJX_CUDA_TRY(launch_chained(kernel, n_tokens, 128, 0, static_cast<cudaStream_t>(stream), P));
-    count_launch(1);
-    return OJX_OK;
-}
-
-size_t ojasx_b200_q4kv_decode_workspace(int batch, int max_pages, int page_size, int kv_heads, int q_heads, int head_dim) {
-    (void)batch; (void)max_pages; (void)page_size; (void)kv_heads; (void)q_heads; (void)head_dim;
-    return 0;
-}
-
-int ojasx_b200_q4kv_decode(const void* d_q, void* d_out, const void* d_pool, const int* d_block_table, const int* d_lengths, int* d_status,
-                           int batch, int max_pages, int num_pages, int page_size, int kv_heads, int q_heads, int head_dim, float scale,
-                           int io_dtype, void* workspace, size_t workspace_bytes, void* stream) {
-    (void)workspace; (void)workspace_bytes;
-    const int rc = q4_check(d_pool, d_block_table, max_pages, num_pages, page_size, kv_heads, head_dim, batch, io_dtype, d_status);
-    if (rc != OJX_OK) return rc;
-    if (!d_q || !d_out || !d_lengths || q_heads <= 0 || q_heads % kv_heads || !q4_aligned(d_q) || !q4_aligned(d_out)) return OJX_ERR_ARG;
-    if (batch > 65535) return OJX_ERR_TOO_LARGE;
-    Q4DecodeProblem P{};
-    P.cache = {static_cast<uint8_t*>(const_cast<void*>(d_pool)), d_block_table, d_status, max_pages, num_pages, page_size, kv_heads};
-    P.q = d_q; P.out = d_out; P.lengths = d_lengths; P.batch = batch; P.q_heads = q_heads;
-    P.scale = scale > 0.0f ? scale : 1.0f / sqrtf((float)head_dim);
-    const bool bf = io_dtype == OJX_BF16;
-    auto kernel = head_dim == 64 ? (bf ? q4_decode_kernel<64, true> : q4_decode_kernel<64, false>)
-                                 : (bf ? q4_decode_kernel<128, true> : q4_decode_kernel<128, false>);
-    OJX_CUDA_TRY(launch_chained(kernel, dim3(q_heads, batch), 256, 0, static_cast<cudaStream_t>(stream), P));
     count_launch(1);
     return OJX_OK;
 }

@@ -57,4 +57,15 @@ __device__ __forceinline__ uint8_t* q4_tile(const Q4Cache& C, int b, int head, i
 __device__ __forceinline__ float q4_scale(unsigned meta) { return __uint_as_float(meta << 16); }
 __device__ __forceinline__ float q4_min(unsigned meta) { return __uint_as_float(meta & 0xffff0000u); }
 
+// What every entry point asks of a cache.
+inline int q4_check(const void* pool, const int* table, int max_pages, int num_pages, int page_size, int kv_heads, int head_dim, int batch,
+                    int dtype, int* status) {
+    if (!pool || !table || !status || max_pages <= 0 || num_pages <= 0 || kv_heads <= 0 || batch <= 0) return OJX_ERR_ARG;
+    if (dtype != OJX_F32 && dtype != OJX_BF16) return OJX_ERR_ARG;
+    if (page_size <= 0 || page_size % kQ4Tile || (head_dim != 64 && head_dim != 128)) return OJX_ERR_UNSUPPORTED;
+    if ((long long)max_pages * page_size > 0x7fffffffLL) return OJX_ERR_TOO_LARGE;
+    return (reinterpret_cast<uintptr_t>(pool) & 15) ? OJX_ERR_ARG : OJX_OK;
+}
+inline bool q4_aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
 }  // namespace ojx

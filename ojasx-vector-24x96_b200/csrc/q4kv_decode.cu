@@ -1,0 +1,478 @@
+// Attention of single tokens over the 4-bit paged cache: softmax(q K^T * scale) V of up to eight query heads per KV head at a time.
+//
+// With the codes c, scales s and minima m of a token's groups of 32 dimensions, a score is sum_g (s_g (q_g . c_g) + m_g sum(q_g)) and
+// the result sum_t p_t (s_tg c_t + m_tg) per dimension of group g: both products take the codes as they are, exact in bf16, on
+// mma.sync m16n8k16, and the scales join in fp32 (those of the values before their product, as p * s).  A warp takes tiles of 16 tokens:
+//   S[token][head]  = codes of K (16 x 16 a step) x q (16 x 8)           a group's steps have sums of their own
+//   O[dim][head]   += codes of V, transposed (16 x 16) x p * s_g (16 x 8)    p * s_g turned by movmatrix
+// fp32 queries and weights are three bf16 numbers each (24 bits), a product three products; a bf16 query is one, weights are rounded to
+// bf16 (2^-9 of a weight at random, below the rounding of the result).
+//
+// Work: units of 64 tokens of a (sequence, KV head, eight query heads), all of them in a row, in equal shares for the CTAs whatever the
+// lengths are; the four warps of a CTA take a tile of a unit each, from rings of their own that bulk copies fill.  A share that begins
+// or ends inside a sequence leaves its sums to q4_combine_kernel.
+#include <cmath>
+
+#include "handles.h"
+#include "launch.h"
+#include "q4kv.cuh"
+#include "../../include/ojasx_lut_b200.h"
+
+namespace ojx {
+
+constexpr int kQdThreads = 128, kQdWarps = 4, kQdStages = 3, kQdHeads = 8;
+constexpr int kQdUnit = kQdWarps * kQ4Tile;   // tokens
+constexpr float kQdLowest = -3.0e38f;         // finite: scores of -inf weigh nothing, a NaN makes its head's result one
+constexpr float kQdSlack = 8.0f;              // sums are relative to the maximum when a score was last 2^8 above it
+
+static __device__ int g_q4_error;   // raised when a bounded wait inside a kernel ran out
+
+struct Q4DecodeProblem {
+    Q4Cache cache;
+    const void* q;              // [batch][q_heads][head_dim]
+    void* out;
+    const int* lengths;         // [batch]
+    int2* pieces;               // [CTAs] item that begins and does not end in the CTA's share (-1: none), last CTA with a part of it
+    float* partials;            // [CTAs][2][8][head_dim + 2]: of an item that began before the share, of one that does not end in it
+    int batch, q_heads, share, blocks;   // blocks: of eight query heads per KV head
+    float scale;                // times log2(e)
+};
+
+template <int N> struct Q4Words;
+template <> struct Q4Words<2> { using type = uint2; };
+template <> struct Q4Words<4> { using type = uint4; };
+
+__device__ __forceinline__ void q4_mma(float (&c)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ unsigned q4_turn(unsigned v) {   // an 8 x 8 matrix of 16-bit numbers, a pair per lane
+    unsigned r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
+}
+// Nibbles i and i + 4 of a word as bf16 numbers: 128 + code has the code in its lowest bits.
+__device__ __forceinline__ unsigned q4_pair(unsigned w, int i) {
+    const unsigned v = ((w >> (4 * i)) & 0x000f000fu) | 0x43004300u;
+    const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&v), __floats2bfloat162_rn(128.0f, 128.0f));
+    return *reinterpret_cast<const unsigned*>(&r);
+}
+__device__ __forceinline__ float q4_exp2(float x) {
+    asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(x));
+    return x;
+}
+// The next bf16 part of two numbers, which keep the rest.
+__device__ __forceinline__ unsigned q4_part(float& a, float& b) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    a -= __low2float(h);
+    b -= __high2float(h);
+    return *reinterpret_cast<const unsigned*>(&h);
+}
+
+// A place in the row of units: unit `u` of the `units` of sequence b for (KV head, block of query heads) `hh`.
+struct Q4Place {
+    int b, hh, u, units;
+    __device__ __forceinline__ void skip(const Q4DecodeProblem& P, int heads) {   // to the next unit, on through sequences without any
+        if (++u < units) return;
+        u = 0;
+        if (++hh < heads) return;
+        hh = 0;
+        do ++b;
+        while (b < P.batch && (units = length_units(P, b)) == 0);
+    }
+    static __device__ __forceinline__ int length(const Q4DecodeProblem& P, int b) {
+        return min(max(P.lengths[b], 0), P.cache.max_pages * P.cache.page_size);
+    }
+    static __device__ __forceinline__ int length_units(const Q4DecodeProblem& P, int b) { return (length(P, b) + kQdUnit - 1) / kQdUnit; }
+};
+
+template <int HD>
+struct QdSmem {
+    static constexpr int ring = kQdStages * Q4Layout<HD>::bytes;    // of a warp
+    static constexpr int row = HD + 8;                              // of a head's sums
+    static constexpr int sums = kQdWarps * kQdHeads * row * 4;
+    static constexpr int bytes = kQdWarps * ring + sums;
+};
+
+template <int HD, bool kBf16>
+__global__ void __launch_bounds__(kQdThreads, kBf16 ? 4 : 2) q4_decode_kernel(const __grid_constant__ Q4DecodeProblem P) {
+    constexpr int G = HD / 32, NP = kBf16 ? 1 : 3;
+    using T = Q4Layout<HD>;
+    using M = QdSmem<HD>;
+    using Words = typename Q4Words<G>::type;
+    extern __shared__ __align__(128) unsigned char qd_smem[];
+    __shared__ float s_m[kQdWarps][kQdHeads], s_l[kQdWarps][kQdHeads];
+    __shared__ __align__(8) unsigned long long s_bar[kQdWarps][kQdStages];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, gq = lane >> 2, t = lane & 3;
+    unsigned char* ring = qd_smem + warp * M::ring;
+    float* sums = reinterpret_cast<float*>(qd_smem + kQdWarps * M::ring);
+    const unsigned ring_at = static_cast<unsigned>(__cvta_generic_to_shared(ring)), bar_at = static_cast<unsigned>(__cvta_generic_to_shared(&s_bar[warp][0]));
+    if (lane == 0) {
+        for (int i = 0; i < kQdStages; ++i) asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(bar_at + 8 * i) : "memory");
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    chain_begin();
+    const int heads = P.cache.kv_heads * P.blocks;
+
+    // this CTA's share of all units, and the place where it begins
+    long long total = 0;
+    for (int b0 = 0; b0 < P.batch; b0 += 32) {
+        int n = b0 + lane < P.batch ? Q4Place::length_units(P, b0 + lane) : 0;
+        total += __reduce_add_sync(0xffffffffu, (unsigned)n);
+    }
+    const long long all = total * heads, n_ctas = min((long long)gridDim.x, all), cta = min((long long)blockIdx.x, n_ctas);
+    const long long first = cta < n_ctas ? all * cta / n_ctas : all, last = cta < n_ctas ? all * (cta + 1) / n_ctas : all;
+    // an empty sequence has no units: its zeros come from here
+    for (int b = blockIdx.x; b < P.batch; b += gridDim.x) {
+        if (Q4Place::length(P, b) > 0) continue;
+        for (int i = tid; i < P.q_heads * HD; i += kQdThreads) {
+            if (kBf16) reinterpret_cast<__nv_bfloat16*>(P.out)[(size_t)b * P.q_heads * HD + i] = __float2bfloat16_rn(0.0f);
+            else reinterpret_cast<float*>(P.out)[(size_t)b * P.q_heads * HD + i] = 0.0f;
+        }
+    }
+    if (tid == 0) P.pieces[blockIdx.x] = make_int2(-1, 0);
+    if (first >= last) return;
+    Q4Place at{0, 0, 0, 0};
+    {
+        long long before = 0;
+        for (int b0 = 0; b0 < P.batch; b0 += 32) {
+            const int n = b0 + lane < P.batch ? Q4Place::length_units(P, b0 + lane) : 0;
+            int sum = n;
+#pragma unroll
+            for (int off = 1; off < 32; off <<= 1) {
+                const int o = __shfl_up_sync(0xffffffffu, sum, off);
+                if (lane >= off) sum += o;
+            }
+            const unsigned in = __ballot_sync(0xffffffffu, first < (before + sum) * heads);
+            if (in) {
+                const int src = __ffs(in) - 1;
+                at.b = b0 + src;
+                at.units = __shfl_sync(0xffffffffu, n, src);
+                const long long rest = first - (before + __shfl_sync(0xffffffffu, sum - n, src)) * heads;
+                at.hh = (int)(rest / at.units);
+                at.u = (int)(rest - (long long)at.hh * at.units);
+                break;
+            }
+            before += __shfl_sync(0xffffffffu, sum, 31);
+        }
+    }
+    __syncwarp();
+
+    // Copies run ahead of the tiles by the stages of the ring; a tile that is not there (behind the last token, or without a page) is
+    // passed over by both.
+    Q4Place ahead = at;
+    long long issue = first;
+    int filled = 0, taken = 0;
+    auto tile_of = [&](const Q4Place& p) -> const unsigned char* {
+        const int token = (p.u * kQdWarps + warp) * kQ4Tile;
+        if (token >= Q4Place::length(P, p.b)) return nullptr;
+        const unsigned char* tile = q4_tile<HD>(P.cache, p.b, p.hh / P.blocks, token);
+        if (!tile && lane == 0) atomicExch(P.cache.status, 1);
+        return tile;
+    };
+    auto fill = [&]() {   // the next tile that is there
+        while (issue < last) {
+            const unsigned char* tile = tile_of(ahead);
+            ++issue;
+            if (issue < last) ahead.skip(P, heads);
+            if (!tile) continue;
+            if (lane == 0) {
+                const int slot = filled % kQdStages;
+                asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar_at + 8 * slot), "n"(T::bytes) : "memory");
+                asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(ring_at + slot * T::bytes),
+                             "l"(tile), "n"(T::bytes), "r"(bar_at + 8 * slot)
+                             : "memory");
+            }
+            ++filled;
+            break;
+        }
+    };
+    for (int i = 0; i < kQdStages; ++i) fill();
+
+    bool ok = true;
+    for (long long unit = first; unit < last;) {
+        const int head = at.hh / P.blocks, h0 = (at.hh % P.blocks) * kQdHeads, n_heads = min(kQdHeads, P.share - h0), length = Q4Place::length(P, at.b);
+        const size_t row0 = ((size_t)at.b * P.q_heads + head * P.share + h0) * HD;
+        const bool begins = at.u == 0;
+        // the queries as the second operand: lane (head gq, t) has the dimensions 32 g + 8 t + 0..7, pairs i and i + 4
+        unsigned qf[NP][G][4];
+        float qsum[G][2];
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+            float x[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = 0.0f;
+            if (gq < n_heads) {
+                const size_t i = row0 + gq * HD + 32 * g + 8 * t;
+                if (kBf16) {
+                    const uint4 w = *reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(P.q) + i);
+                    const unsigned ws[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) { x[2 * e] = __uint_as_float(ws[e] << 16); x[2 * e + 1] = __uint_as_float(ws[e] & 0xffff0000u); }
+                } else {
+                    const float4 a = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(P.q) + i);
+                    const float4 c = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(P.q) + i + 4);
+                    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = c.x; x[5] = c.y; x[6] = c.z; x[7] = c.w;
+                }
+            }
+            float sum = ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
+            sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+            sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+            qsum[g][0] = __shfl_sync(0xffffffffu, sum, 8 * t);        // heads 2 t and 2 t + 1
+            qsum[g][1] = __shfl_sync(0xffffffffu, sum, 8 * t + 4);
+#pragma unroll
+            for (int p = 0; p < NP; ++p)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) qf[p][g][i] = q4_part(x[i], x[i + 4]);
+        }
+        float top[2] = {kQdLowest, kQdLowest}, l[2] = {0.0f, 0.0f}, o[2 * G][4], mins[G][2];
+#pragma unroll
+        for (int m = 0; m < 2 * G; ++m)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[m][e] = 0.0f;
+#pragma unroll
+        for (int g = 0; g < G; ++g) mins[g][0] = mins[g][1] = 0.0f;
+
+        const int u0 = at.u, u1 = (int)min((long long)at.units, at.u + (last - unit));
+        for (int u = u0; u < u1 && ok; ++u) {
+            const int token = (u * kQdWarps + warp) * kQ4Tile;
+            if (token >= length) break;
+            {   // (as the copies passed over it)
+                const int p = token / P.cache.page_size;
+                if ((unsigned)P.cache.block_table[(size_t)at.b * P.cache.max_pages + p] >= (unsigned)P.cache.num_pages) continue;
+            }
+            const int slot = taken % kQdStages;
+            if (!(ok = __all_sync(0xffffffffu, bar_wait(bar_at + 8 * slot, (taken / kQdStages) & 1)))) break;
+            const unsigned char* tile = ring + slot * T::bytes;
+            const bool live[2] = {token + gq < length, token + gq + 8 < length};
+            float x[4];
+            {
+                const Words ka = *reinterpret_cast<const Words*>(tile + (gq * 4 + t) * (4 * G)), kb = *reinterpret_cast<const Words*>(tile + ((gq + 8) * 4 + t) * (4 * G));
+                const Words ma = *reinterpret_cast<const Words*>(tile + T::key_meta + gq * (4 * G)), mb = *reinterpret_cast<const Words*>(tile + T::key_meta + (gq + 8) * (4 * G));
+                const unsigned *wa = reinterpret_cast<const unsigned*>(&ka), *wb = reinterpret_cast<const unsigned*>(&kb);
+                const unsigned *na = reinterpret_cast<const unsigned*>(&ma), *nb = reinterpret_cast<const unsigned*>(&mb);
+                x[0] = x[1] = x[2] = x[3] = 0.0f;
+#pragma unroll
+                for (int g = 0; g < G; ++g) {
+                    unsigned a[4], b[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) { a[i] = q4_pair(wa[g], i); b[i] = q4_pair(wb[g], i); }
+                    float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (int p = NP - 1; p >= 0; --p) {
+                        q4_mma(c, a[0], b[0], a[1], b[1], qf[p][g][0], qf[p][g][1]);
+                        q4_mma(c, a[2], b[2], a[3], b[3], qf[p][g][2], qf[p][g][3]);
+                    }
+                    x[0] = fmaf(q4_scale(na[g]), c[0], fmaf(q4_min(na[g]), qsum[g][0], x[0]));
+                    x[1] = fmaf(q4_scale(na[g]), c[1], fmaf(q4_min(na[g]), qsum[g][1], x[1]));
+                    x[2] = fmaf(q4_scale(nb[g]), c[2], fmaf(q4_min(nb[g]), qsum[g][0], x[2]));
+                    x[3] = fmaf(q4_scale(nb[g]), c[3], fmaf(q4_min(nb[g]), qsum[g][1], x[3]));
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] = live[e >> 1] ? x[e] * P.scale : -INFINITY;
+            float now[2] = {fmaxf(x[0], x[2]), fmaxf(x[1], x[3])};
+#pragma unroll
+            for (int off = 4; off < 32; off <<= 1) {
+                now[0] = fmaxf(now[0], __shfl_xor_sync(0xffffffffu, now[0], off));
+                now[1] = fmaxf(now[1], __shfl_xor_sync(0xffffffffu, now[1], off));
+            }
+            const bool up[2] = {now[0] > top[0] + kQdSlack, now[1] > top[1] + kQdSlack};
+            if (__any_sync(0xffffffffu, up[0] || up[1])) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const float keep = up[h] ? q4_exp2(top[h] - now[h]) : 1.0f;
+                    top[h] = up[h] ? now[h] : top[h];
+                    l[h] *= keep;
+#pragma unroll
+                    for (int g = 0; g < G; ++g) mins[g][h] *= keep;
+#pragma unroll
+                    for (int m = 0; m < 2 * G; ++m) { o[m][h] *= keep; o[m][h + 2] *= keep; }
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] = q4_exp2(x[e] - top[e & 1]);
+            l[0] += x[0] + x[2];
+            l[1] += x[1] + x[3];
+            {
+                const Words va = *reinterpret_cast<const Words*>(tile + T::values + (gq * 4 + t) * (4 * G)),
+                            vb = *reinterpret_cast<const Words*>(tile + T::values + (32 + gq * 4 + t) * (4 * G));
+                const Words ma = *reinterpret_cast<const Words*>(tile + T::value_meta + gq * (4 * G)), mb = *reinterpret_cast<const Words*>(tile + T::value_meta + (gq + 8) * (4 * G));
+                const unsigned *wa = reinterpret_cast<const unsigned*>(&va), *wb = reinterpret_cast<const unsigned*>(&vb);
+                const unsigned *na = reinterpret_cast<const unsigned*>(&ma), *nb = reinterpret_cast<const unsigned*>(&mb);
+#pragma unroll
+                for (int g = 0; g < G; ++g) {
+                    const unsigned mna = live[0] ? na[g] : 0u, mnb = live[1] ? nb[g] : 0u;   // (what is behind the last token may be anything)
+                    mins[g][0] = fmaf(x[0], q4_min(mna), fmaf(x[2], q4_min(mnb), mins[g][0]));
+                    mins[g][1] = fmaf(x[1], q4_min(mna), fmaf(x[3], q4_min(mnb), mins[g][1]));
+                    float y[4] = {x[0] * q4_scale(mna), x[1] * q4_scale(mna), x[2] * q4_scale(mnb), x[3] * q4_scale(mnb)};
+                    unsigned b0[NP], b1[NP];
+#pragma unroll
+                    for (int p = 0; p < NP; ++p) { b0[p] = q4_turn(q4_part(y[0], y[1])); b1[p] = q4_turn(q4_part(y[2], y[3])); }
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const unsigned a0 = q4_pair(wa[g], 2 * h), a1 = q4_pair(wa[g], 2 * h + 1), a2 = q4_pair(wb[g], 2 * h), a3 = q4_pair(wb[g], 2 * h + 1);
+                        if (NP == 1) {
+                            q4_mma(o[2 * g + h], a0, a1, a2, a3, b0[0], b1[0]);
+                        } else {   // (the tensor cores cut what they add to a sum: a tile's products are summed on their own)
+                            float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                            for (int p = NP - 1; p >= 0; --p) q4_mma(c, a0, a1, a2, a3, b0[p], b1[p]);
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) o[2 * g + h][e] += c[e];
+                        }
+                    }
+                }
+            }
+            ++taken;
+            __syncwarp();   // the stage has been read
+            fill();
+        }
+
+        // the warps' sums joined, and out
+#pragma unroll
+        for (int off = 4; off < 32; off <<= 1)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                l[h] += __shfl_xor_sync(0xffffffffu, l[h], off);
+#pragma unroll
+                for (int g = 0; g < G; ++g) mins[g][h] += __shfl_xor_sync(0xffffffffu, mins[g][h], off);
+            }
+        if (gq == 0) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) { s_m[warp][2 * t + h] = top[h]; s_l[warp][2 * t + h] = l[h]; }
+        }
+#pragma unroll
+        for (int m = 0; m < 2 * G; ++m)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                float* to = sums + (warp * kQdHeads + 2 * t + h) * M::row + 32 * (m >> 1) + 4 * gq + 2 * (m & 1);
+                *reinterpret_cast<float2*>(to) = make_float2(o[m][h] + mins[m >> 1][h], o[m][h + 2] + mins[m >> 1][h]);
+            }
+        __syncthreads();
+        unit += u1 - u0;
+        const bool ends = u1 == at.units;
+        float* part = P.partials + ((size_t)blockIdx.x * 2 + (begins ? 1 : 0)) * kQdHeads * (HD + 2);
+        for (int i = tid; i < n_heads * HD; i += kQdThreads) {
+            const int h = i / HD, d = i % HD;
+            float most = kQdLowest, acc = 0.0f, weight = 0.0f;
+#pragma unroll
+            for (int w = 0; w < kQdWarps; ++w) most = fmaxf(most, s_m[w][h]);
+#pragma unroll
+            for (int w = 0; w < kQdWarps; ++w) {
+                const float keep = q4_exp2(s_m[w][h] - most);
+                acc = fmaf(sums[(w * kQdHeads + h) * M::row + d], keep, acc);
+                weight = fmaf(s_l[w][h], keep, weight);
+            }
+            if (begins && ends) {
+                acc = weight == 0.0f ? 0.0f : acc / weight;
+                if (kBf16) reinterpret_cast<__nv_bfloat16*>(P.out)[row0 + i] = __float2bfloat16_rn(acc);
+                else reinterpret_cast<float*>(P.out)[row0 + i] = acc;
+            } else {
+                part[h * (HD + 2) + 2 + d] = acc;
+                if (d == 0) { part[h * (HD + 2)] = most; part[h * (HD + 2) + 1] = weight; }
+            }
+        }
+        if (begins && !ends && tid == 0) {
+            // the CTA of the item's last unit: unit v is in share i of n where i all / n <= v < (i + 1) all / n, rounded down
+            const long long end = unit + (at.units - u1) - 1;
+            P.pieces[blockIdx.x] = make_int2(at.b * heads + at.hh, (int)(((end + 1) * n_ctas - 1) / all));
+        }
+        __syncthreads();   // the sums have been read
+        at.u = u1 - 1;
+        if (unit < last) at.skip(P, heads);
+    }
+    if (!ok) {
+        for (int i = taken; i < filled; ++i) bar_wait(bar_at + 8 * (i % kQdStages), (i / kQdStages) & 1);   // nothing may land after the CTA has left
+        atomicExch(&g_q4_error, 1);
+    }
+}
+
+// Items that several CTAs have parts of; a CTA per CTA of the decode.
+template <int HD, bool kBf16>
+__global__ void __launch_bounds__(kQdThreads) q4_combine_kernel(const __grid_constant__ Q4DecodeProblem P) {
+    chain_begin();
+    const int2 piece = P.pieces[blockIdx.x];
+    if (piece.x < 0) return;
+    const int heads = P.cache.kv_heads * P.blocks, b = piece.x / heads, hh = piece.x % heads, h0 = (hh % P.blocks) * kQdHeads;
+    const int n_heads = min(kQdHeads, P.share - h0);
+    const size_t row0 = ((size_t)b * P.q_heads + hh / P.blocks * P.share + h0) * HD;
+    auto part = [&](int c) { return P.partials + ((size_t)c * 2 + (c == (int)blockIdx.x ? 1 : 0)) * kQdHeads * (HD + 2); };
+    for (int i = threadIdx.x; i < n_heads * HD; i += kQdThreads) {
+        const int h = i / HD, d = i % HD;
+        float most = kQdLowest, acc = 0.0f, weight = 0.0f;
+        for (int c = blockIdx.x; c <= piece.y; ++c) most = fmaxf(most, part(c)[h * (HD + 2)]);
+        for (int c = blockIdx.x; c <= piece.y; ++c) {
+            const float* p = part(c) + h * (HD + 2);
+            const float keep = q4_exp2(p[0] - most);
+            acc = fmaf(p[2 + d], keep, acc);
+            weight = fmaf(p[1], keep, weight);
+        }
+        acc = weight == 0.0f ? 0.0f : acc / weight;
+        if (kBf16) reinterpret_cast<__nv_bfloat16*>(P.out)[row0 + i] = __float2bfloat16_rn(acc);
+        else reinterpret_cast<float*>(P.out)[row0 + i] = acc;
+    }
+}
+
+// CTAs of a decode: what the GPU holds at a time, or a unit each where the tables have room for fewer.
+static int q4_decode_ctas(int batch, int max_pages, int page_size, int kv_heads, int share, int dtype) {
+    const long long units = (long long)batch * kv_heads * ((share + kQdHeads - 1) / kQdHeads) * (((long long)max_pages * page_size + kQdUnit - 1) / kQdUnit);
+    const int most = num_sms() * (dtype == OJX_BF16 ? 4 : 2);
+    return units < most ? (int)units : most;
+}
+static size_t q4_decode_bytes(int ctas, int head_dim) {
+    return ((size_t)ctas * sizeof(int2) + 15) / 16 * 16 + (size_t)ctas * 2 * kQdHeads * (head_dim + 2) * sizeof(float);
+}
+
+template <int HD, bool kBf16>
+static int launch_q4_decode(const Q4DecodeProblem& P, int ctas, cudaStream_t s) {
+    static std::atomic<bool> opted[64];
+    OJX_CUDA_TRY(opt_in_smem(reinterpret_cast<const void*>(q4_decode_kernel<HD, kBf16>), QdSmem<HD>::bytes, opted));
+    OJX_CUDA_TRY(launch_chained(q4_decode_kernel<HD, kBf16>, ctas, kQdThreads, QdSmem<HD>::bytes, s, P));
+    OJX_CUDA_TRY(launch_chained(q4_combine_kernel<HD, kBf16>, ctas, kQdThreads, 0, s, P));
+    count_launch(2);
+    return OJX_OK;
+}
+
+int take_q4_error(int* out) {
+    int v = 0, zero = 0;
+    OJX_CUDA_TRY(cudaMemcpyFromSymbol(&v, g_q4_error, sizeof(int)));
+    if (v) OJX_CUDA_TRY(cudaMemcpyToSymbol(g_q4_error, &zero, sizeof(int)));
+    *out = v;
+    return OJX_OK;
+}
+
+}  // namespace ojx
+
+using namespace ojx;
+
+extern "C" {
+
+size_t ojasx_b200_q4kv_decode_workspace(int batch, int max_pages, int page_size, int kv_heads, int q_heads, int head_dim, int io_dtype) {
+    if (batch <= 0 || max_pages <= 0 || page_size <= 0 || kv_heads <= 0 || q_heads <= 0) return 0;
+    return q4_decode_bytes(q4_decode_ctas(batch, max_pages, page_size, kv_heads, q_heads / kv_heads, io_dtype), head_dim);
+}
+
+int ojasx_b200_q4kv_decode(const void* d_q, void* d_out, const void* d_pool, const int* d_block_table, const int* d_lengths, int* d_status,
+                           int batch, int max_pages, int num_pages, int page_size, int kv_heads, int q_heads, int head_dim, float scale,
+                           int io_dtype, void* workspace, size_t workspace_bytes, void* stream) {
+    const int rc = q4_check(d_pool, d_block_table, max_pages, num_pages, page_size, kv_heads, head_dim, batch, io_dtype, d_status);
+    if (rc != OJX_OK) return rc;
+    if (!d_q || !d_out || !d_lengths || q_heads <= 0 || q_heads % kv_heads || !q4_aligned(d_q) || !q4_aligned(d_out)) return OJX_ERR_ARG;
+    const int share = q_heads / kv_heads, ctas = q4_decode_ctas(batch, max_pages, page_size, kv_heads, share, io_dtype);
+    if (!workspace || !q4_aligned(workspace) || workspace_bytes < q4_decode_bytes(ctas, head_dim)) return OJX_ERR_ARG;
+    if ((long long)batch * q_heads > 0x7fffffffLL) return OJX_ERR_TOO_LARGE;
+    Q4DecodeProblem P{};
+    P.cache = {static_cast<uint8_t*>(const_cast<void*>(d_pool)), d_block_table, d_status, max_pages, num_pages, page_size, kv_heads};
+    P.q = d_q; P.out = d_out; P.lengths = d_lengths; P.batch = batch; P.q_heads = q_heads; P.share = share;
+    P.blocks = (share + kQdHeads - 1) / kQdHeads;
+    P.pieces = static_cast<int2*>(workspace);
+    P.partials = reinterpret_cast<float*>(static_cast<char*>(workspace) + ((size_t)ctas * sizeof(int2) + 15) / 16 * 16);
+    P.scale = (scale > 0.0f ? scale : 1.0f / sqrtf((float)head_dim)) * 1.4426950408889634f;
+    const cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (io_dtype == OJX_BF16) return head_dim == 64 ? launch_q4_decode<64, true>(P, ctas, s) : launch_q4_decode<128, true>(P, ctas, s);
+    return head_dim == 64 ? launch_q4_decode<64, false>(P, ctas, s) : launch_q4_decode<128, false>(P, ctas, s);
+}
+
+}  // extern "C"

@@ -618,12 +618,13 @@ class Q4PagedKVCache:
         lengths = _index32(lengths, "lengths", (B,), self.device)
         o = _out(out, q)
         if B:
-            size = lib().ojasx_b200_q4kv_decode_workspace(B, table.shape[1], self.page_size, self.kv_heads, self.q_heads, self.head_dim)
+            size = lib().ojasx_b200_q4kv_decode_workspace(B, table.shape[1], self.page_size, self.kv_heads, self.q_heads, self.head_dim,
+                                                          _dtype_code(q))
             ws = torch.empty(size, device=self.device, dtype=torch.uint8)     # of this call, so that calls on several streams do not share it
             with torch.cuda.device(self.device):
                 check(lib().ojasx_b200_q4kv_decode(q.data_ptr(), o.data_ptr(), self.pool.data_ptr(), table.data_ptr(), lengths.data_ptr(),
                                                    self._status.data_ptr(), B, table.shape[1], self.num_pages, self.page_size, self.kv_heads,
-                                                   self.q_heads, self.head_dim, float(scale), _dtype_code(q), ws.data_ptr() if size else None, size,
+                                                   self.q_heads, self.head_dim, float(scale), _dtype_code(q), ws.data_ptr(), size,
                                                    _stream_ptr(self.device)), "ojasx_b200_q4kv_decode")
         return o
 

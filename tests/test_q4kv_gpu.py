@@ -44,8 +44,8 @@ def test_c_entries_refuse_missing_and_unfit_arguments():
     assert append(mp=1 << 20, ps=4096) == -5
     assert append(n=0, ends=one) == 0
     decode = lambda **kw: L.ojasx_b200_q4kv_decode(*{**dict(q=one, o=one, pool=one, table=one, n=one, status=one, b=1, mp=1, np_=1, ps=16, kv=2, qh=4,
-             hd=64, sc=-1.0, io=1, ws=None, size=0, st=None), **kw}.values())  # noqa: E731
-    for bad in (dict(q=None), dict(o=None), dict(n=None), dict(qh=3), dict(qh=0), dict(q=one + 2), dict(o=one + 8)):
+             hd=64, sc=-1.0, io=1, ws=one, size=1 << 30, st=None), **kw}.values())  # noqa: E731
+    for bad in (dict(q=None), dict(o=None), dict(n=None), dict(qh=3), dict(qh=0), dict(q=one + 2), dict(o=one + 8), dict(ws=None), dict(size=1000), dict(ws=one + 4)):
         assert decode(**bad) == -1, bad
     read = lambda **kw: L.ojasx_b200_q4kv_read(*{**dict(pool=one, table=one, ends=one, pos=None, k=one, v=one, status=one, n=1, b=1, mp=1, np_=1, ps=16,
              kv=1, hd=64, io=0, st=None), **kw}.values())  # noqa: E731

@@ -42,7 +42,7 @@ __device__ __forceinline__ unsigned q4_encode(float4 x, unsigned& meta) {
     const __nv_bfloat16 sb = __float2bfloat16_ru(wide ? hi / 15.0f - m / 15.0f : __fdiv_rn(range, 15.0f));
     const float s = __bfloat162float(sb);
     if (!(odd == 0.0f) || isinf(m) || isinf(s)) {
-        meta = 0x7fff7fffu;
+        meta = 0x7fff0000u;
         return 0u;
     }
     meta = (unsigned)__bfloat16_as_ushort(mb) << 16 | __bfloat16_as_ushort(sb);

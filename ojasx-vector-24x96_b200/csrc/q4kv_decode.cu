@@ -1,18 +1,25 @@
 // Attention of single tokens over the 4-bit paged cache: softmax(q K^T * scale) V of up to eight query heads per KV head at a time.
 //
 // With the codes c, scales s and minima m of a token's groups of 32 dimensions, a score is sum_g (s_g (q_g . c_g) + m_g sum(q_g)) and
-// the result sum_t p_t (s_tg c_t + m_tg) per dimension of group g: both products take the codes as they are, exact in bf16, on
-// mma.sync m16n8k16, and the scales join in fp32 (those of the values before their product, as p * s).  A warp takes tiles of 16 tokens:
+// the result sum_t p_t (s_tg c_t + m_tg) per dimension of group g: both products take the codes as they are on mma.sync m16n8k16, and
+// the scales join in fp32 (those of the values before their product, as p * s).  A nibble in the lowest bits of an fp16 number is the
+// subnormal c * 2^-24, in the next ones 16 times that, exact in the tensor cores: a word of eight codes becomes operands with five
+// integer instructions, and the powers of two are taken out of the queries and the results (12 for bf16 numbers, which need an
+// exponent and its subtraction: 295 against XXX us at 16 sequences of 32768 tokens, 8 KV heads of 4 query heads of 128).
+// A warp takes tiles of 16 tokens:
 //   S[token][head]  = codes of K (16 x 16 a step) x q (16 x 8)           a group's steps have sums of their own
 //   O[dim][head]   += codes of V, transposed (16 x 16) x p * s_g (16 x 8)    p * s_g turned by movmatrix
-// fp32 queries and weights are three bf16 numbers each (24 bits), a product three products; a bf16 query is one, weights are rounded to
-// bf16 (2^-9 of a weight at random, below the rounding of the result).
+// A bf16 query is one fp16 number where a power of two brings the head's largest to 2^15 (what is 2^29 below it loses bits), an fp32
+// one two of them (22 bits); so is p * s, one with bf16 activations (11 bits, below the rounding of the result), two with fp32.  The
+// reference of the weights is the largest score plus the exponent of its token's largest scale, so that p * s is in the range of fp16
+// whatever the scales are.
 //
 // Work: units of 64 tokens of a (sequence, KV head, eight query heads), all of them in a row, in equal shares for the CTAs whatever the
 // lengths are; the four warps of a CTA take a tile of a unit each, from rings of their own that bulk copies fill.  A share that begins
 // or ends inside a sequence leaves its sums to q4_combine_kernel.
 #include <cmath>
 
+#include "gather_mma.cuh"
 #include "handles.h"
 #include "launch.h"
 #include "q4kv.cuh"
@@ -23,7 +30,9 @@ namespace ojx {
 constexpr int kQdThreads = 128, kQdWarps = 4, kQdStages = 3, kQdHeads = 8;
 constexpr int kQdUnit = kQdWarps * kQ4Tile;   // tokens
 constexpr float kQdLowest = -3.0e38f;         // finite: scores of -inf weigh nothing, a NaN makes its head's result one
-constexpr float kQdSlack = 8.0f;              // sums are relative to the maximum when a score was last 2^8 above it
+constexpr float kQdSlack = 8.0f;              // sums are relative to a reference, until a score is 2^8 above it ...
+constexpr float kQdRoom = 5.0f;               // ... and the largest p * s is 2^5 then: 2^14 at most
+constexpr float kQdCode = 16777216.0f;        // 2^24: a code is a subnormal of fp16
 
 static __device__ int g_q4_error;   // raised when a bounded wait inside a kernel ran out
 
@@ -42,32 +51,34 @@ template <int N> struct Q4Words;
 template <> struct Q4Words<2> { using type = uint2; };
 template <> struct Q4Words<4> { using type = uint4; };
 
-__device__ __forceinline__ void q4_mma(float (&c)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
 __device__ __forceinline__ unsigned q4_turn(unsigned v) {   // an 8 x 8 matrix of 16-bit numbers, a pair per lane
     unsigned r;
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
     return r;
 }
-// Nibbles i and i + 4 of a word as bf16 numbers: 128 + code has the code in its lowest bits.
-__device__ __forceinline__ unsigned q4_pair(unsigned w, int i) {
-    const unsigned v = ((w >> (4 * i)) & 0x000f000fu) | 0x43004300u;
-    const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&v), __floats2bfloat162_rn(128.0f, 128.0f));
-    return *reinterpret_cast<const unsigned*>(&r);
+// Nibbles i and i + 4 of a word as fp16 numbers, c * 2^-24 for even i and 16 c * 2^-24 for odd i.
+__device__ __forceinline__ void q4_codes(unsigned w, unsigned (&c)[4]) {
+    const unsigned v = w >> 8;
+    c[0] = w & 0x000f000fu;
+    c[1] = w & 0x00f000f0u;
+    c[2] = v & 0x000f000fu;
+    c[3] = v & 0x00f000f0u;
 }
 __device__ __forceinline__ float q4_exp2(float x) {
     asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(x));
     return x;
 }
-// The next bf16 part of two numbers, which keep the rest.
+// The next fp16 part of two numbers, which keep the rest.
 __device__ __forceinline__ unsigned q4_part(float& a, float& b) {
-    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    const __half2 h = __floats2half2_rn(a, b);
     a -= __low2float(h);
     b -= __high2float(h);
     return *reinterpret_cast<const unsigned*>(&h);
+}
+// Exponent of a positive fp32 number, kept in -20..100.
+__device__ __forceinline__ float q4_exponent(float s) {
+    const unsigned e = min(max(__float_as_uint(s) >> 23, 107u), 227u);
+    return __uint_as_float(0x4b000000u | e) - (8388608.0f + 127.0f);
 }
 
 // A place in the row of units: unit `u` of the `units` of sequence b for (KV head, block of query heads) `hh`.
@@ -95,9 +106,11 @@ struct QdSmem {
     static constexpr int bytes = kQdWarps * ring + sums;
 };
 
+constexpr int kQdCtas(bool bf16) { return bf16 ? 4 : 3; }   // per SM
+
 template <int HD, bool kBf16>
-__global__ void __launch_bounds__(kQdThreads, kBf16 ? 4 : 2) q4_decode_kernel(const __grid_constant__ Q4DecodeProblem P) {
-    constexpr int G = HD / 32, NP = kBf16 ? 1 : 3;
+__global__ void __launch_bounds__(kQdThreads, kQdCtas(kBf16)) q4_decode_kernel(const __grid_constant__ Q4DecodeProblem P) {
+    constexpr int G = HD / 32, NP = kBf16 ? 1 : 2;
     using T = Q4Layout<HD>;
     using M = QdSmem<HD>;
     using Words = typename Q4Words<G>::type;
@@ -159,35 +172,62 @@ __global__ void __launch_bounds__(kQdThreads, kBf16 ? 4 : 2) q4_decode_kernel(co
     }
     __syncwarp();
 
-    // Copies run ahead of the tiles by the stages of the ring; a tile that is not there (behind the last token, or without a page) is
-    // passed over by both.
-    Q4Place ahead = at;
-    long long issue = first;
-    int filled = 0, taken = 0;
-    auto tile_of = [&](const Q4Place& p) -> const unsigned char* {
-        const int token = (p.u * kQdWarps + warp) * kQ4Tile;
-        if (token >= Q4Place::length(P, p.b)) return nullptr;
-        const unsigned char* tile = q4_tile<HD>(P.cache, p.b, p.hh / P.blocks, token);
-        if (!tile && lane == 0) atomicExch(P.cache.status, 1);
-        return tile;
+    // Copies run ahead of the tiles by the stages of the ring.  Every tile that begins before its sequence's end has a stage; one without a
+    // page stays as it is and is marked.  The page of the next copy is looked up a tile ahead.
+    struct {
+        Q4Place at;
+        long long rest;       // units of the share from here on
+        const int* table;
+        int tile, in, page, id, tiles;   // tile of the sequence, its place in its page, the page's place in the table and its id
+        size_t head;          // bytes of the heads before this one in a page
+    } ahead{at, last - first, nullptr, 0, 0, 0, 0, 0, 0};
+    const int page_tiles = P.cache.page_size / kQ4Tile;
+    const size_t head_bytes = (size_t)page_tiles * T::bytes, page_bytes = head_bytes * P.cache.kv_heads;
+    unsigned missing = 0;
+    auto enter = [&]() {   // an item, at its unit `ahead.at.u`
+        ahead.tiles = (Q4Place::length(P, ahead.at.b) + kQ4Tile - 1) / kQ4Tile;
+        ahead.table = P.cache.block_table + (size_t)ahead.at.b * P.cache.max_pages;
+        ahead.head = ahead.at.hh / P.blocks * head_bytes;
+        ahead.tile = ahead.at.u * kQdWarps + warp;
+        ahead.page = ahead.tile / page_tiles;
+        ahead.in = ahead.tile - ahead.page * page_tiles;
+        ahead.id = ahead.tile < ahead.tiles ? ahead.table[ahead.page] : 0;
     };
-    auto fill = [&]() {   // the next tile that is there
-        while (issue < last) {
-            const unsigned char* tile = tile_of(ahead);
-            ++issue;
-            if (issue < last) ahead.skip(P, heads);
-            if (!tile) continue;
-            if (lane == 0) {
-                const int slot = filled % kQdStages;
-                asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar_at + 8 * slot), "n"(T::bytes) : "memory");
-                asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(ring_at + slot * T::bytes),
-                             "l"(tile), "n"(T::bytes), "r"(bar_at + 8 * slot)
-                             : "memory");
-            }
-            ++filled;
-            break;
+    auto next = [&]() {
+        --ahead.rest;
+        if (ahead.at.u + 1 < ahead.at.units) {
+            ++ahead.at.u;
+            ahead.tile += kQdWarps;
+            ahead.in += kQdWarps;
+            while (ahead.in >= page_tiles) { ahead.in -= page_tiles; ++ahead.page; }
+            ahead.id = ahead.tile < ahead.tiles ? ahead.table[ahead.page] : 0;
+        } else if (ahead.rest > 0) {
+            ahead.at.skip(P, heads);
+            enter();
         }
     };
+    int filled = 0, taken = 0, into = 0, from = 0, phase = 0;   // stages used so far, the next ones and the phase of the next to be read
+    auto fill = [&]() {
+        while (ahead.rest > 0 && ahead.tile >= ahead.tiles) next();
+        if (ahead.rest <= 0) return;
+        const bool there = (unsigned)ahead.id < (unsigned)P.cache.num_pages;
+        missing = there ? missing & ~(1u << into) : missing | 1u << into;
+        if (lane == 0) {
+            if (there) {
+                asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar_at + 8 * into), "n"(T::bytes) : "memory");
+                asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(ring_at + into * T::bytes),
+                             "l"(P.cache.pool + (size_t)ahead.id * page_bytes + ahead.head + ahead.in * T::bytes), "n"(T::bytes), "r"(bar_at + 8 * into)
+                             : "memory");
+            } else {
+                asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar_at + 8 * into) : "memory");
+                atomicExch(P.cache.status, 1);
+            }
+        }
+        ++filled;
+        into = into + 1 == kQdStages ? 0 : into + 1;
+        next();
+    };
+    enter();
     for (int i = 0; i < kQdStages; ++i) fill();
 
     bool ok = true;
@@ -197,34 +237,55 @@ __global__ void __launch_bounds__(kQdThreads, kBf16 ? 4 : 2) q4_decode_kernel(co
         const bool begins = at.u == 0;
         // the queries as the second operand: lane (head gq, t) has the dimensions 32 g + 8 t + 0..7, pairs i and i + 4
         unsigned qf[NP][G][4];
-        float qsum[G][2];
+        float qsum[G][2], unscale[2];
+        {
+            float x[G][8];
+            unsigned most = 0;
 #pragma unroll
-        for (int g = 0; g < G; ++g) {
-            float x[8];
+            for (int g = 0; g < G; ++g) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = 0.0f;
-            if (gq < n_heads) {
-                const size_t i = row0 + gq * HD + 32 * g + 8 * t;
-                if (kBf16) {
-                    const uint4 w = *reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(P.q) + i);
-                    const unsigned ws[4] = {w.x, w.y, w.z, w.w};
+                for (int e = 0; e < 8; ++e) x[g][e] = 0.0f;
+                if (gq < n_heads) {
+                    const size_t i = row0 + gq * HD + 32 * g + 8 * t;
+                    if (kBf16) {
+                        const uint4 w = *reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(P.q) + i);
+                        const unsigned ws[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) { x[2 * e] = __uint_as_float(ws[e] << 16); x[2 * e + 1] = __uint_as_float(ws[e] & 0xffff0000u); }
-                } else {
-                    const float4 a = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(P.q) + i);
-                    const float4 c = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(P.q) + i + 4);
-                    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = c.x; x[5] = c.y; x[6] = c.z; x[7] = c.w;
+                        for (int e = 0; e < 4; ++e) { x[g][2 * e] = __uint_as_float(ws[e] << 16); x[g][2 * e + 1] = __uint_as_float(ws[e] & 0xffff0000u); }
+                    } else {
+                        const float4 a = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(P.q) + i);
+                        const float4 c = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(P.q) + i + 4);
+                        x[g][0] = a.x; x[g][1] = a.y; x[g][2] = a.z; x[g][3] = a.w; x[g][4] = c.x; x[g][5] = c.y; x[g][6] = c.z; x[g][7] = c.w;
+                    }
                 }
+#pragma unroll
+                for (int e = 0; e < 8; ++e) most = max(most, __float_as_uint(x[g][e]) & 0x7fffffffu);
             }
-            float sum = ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
-            sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-            sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-            qsum[g][0] = __shfl_sync(0xffffffffu, sum, 8 * t);        // heads 2 t and 2 t + 1
-            qsum[g][1] = __shfl_sync(0xffffffffu, sum, 8 * t + 4);
+            most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
+            most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
+            float up, down;
+            gm_scale(most, up, down);
+            // a score comes out of the products with 2^24 too little and this factor too much
+            const float back = fminf(down * (P.scale * kQdCode), 3.0e38f);
+            unscale[0] = __shfl_sync(0xffffffffu, back, 8 * t);        // heads 2 t and 2 t + 1
+            unscale[1] = __shfl_sync(0xffffffffu, back, 8 * t + 4);
 #pragma unroll
-            for (int p = 0; p < NP; ++p)
+            for (int g = 0; g < G; ++g) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) qf[p][g][i] = q4_part(x[i], x[i + 4]);
+                for (int e = 0; e < 8; ++e) x[g][e] *= up;
+                float sum = ((x[g][0] + x[g][1]) + (x[g][2] + x[g][3])) + ((x[g][4] + x[g][5]) + (x[g][6] + x[g][7]));
+                sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+                sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+                sum *= 1.0f / kQdCode;
+                qsum[g][0] = __shfl_sync(0xffffffffu, sum, 8 * t);
+                qsum[g][1] = __shfl_sync(0xffffffffu, sum, 8 * t + 4);
+#pragma unroll
+                for (int i = 1; i < 8; i += 2) x[g][i] *= 0.0625f;     // (the codes of odd nibbles are 16 times as large)
+#pragma unroll
+                for (int p = 0; p < NP; ++p)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) qf[p][g][i] = q4_part(x[g][i], x[g][i + 4]);
+            }
         }
         float top[2] = {kQdLowest, kQdLowest}, l[2] = {0.0f, 0.0f}, o[2 * G][4], mins[G][2];
 #pragma unroll
@@ -238,14 +299,10 @@ __global__ void __launch_bounds__(kQdThreads, kBf16 ? 4 : 2) q4_decode_kernel(co
         for (int u = u0; u < u1 && ok; ++u) {
             const int token = (u * kQdWarps + warp) * kQ4Tile;
             if (token >= length) break;
-            {   // (as the copies passed over it)
-                const int p = token / P.cache.page_size;
-                if ((unsigned)P.cache.block_table[(size_t)at.b * P.cache.max_pages + p] >= (unsigned)P.cache.num_pages) continue;
-            }
-            const int slot = taken % kQdStages;
-            if (!(ok = __all_sync(0xffffffffu, bar_wait(bar_at + 8 * slot, (taken / kQdStages) & 1)))) break;
-            const unsigned char* tile = ring + slot * T::bytes;
-            const bool live[2] = {token + gq < length, token + gq + 8 < length};
+            if (!(ok = __all_sync(0xffffffffu, bar_wait(bar_at + 8 * from, phase)))) break;
+            const unsigned char* tile = ring + from * T::bytes;
+            const int seen = missing >> from & 1 ? 0 : length - token;
+            const bool live[2] = {gq < seen, gq + 8 < seen};
             float x[4];
             {
                 const Words ka = *reinterpret_cast<const Words*>(tile + (gq * 4 + t) * (4 * G)), kb = *reinterpret_cast<const Words*>(tile + ((gq + 8) * 4 + t) * (4 * G));
@@ -256,13 +313,13 @@ __global__ void __launch_bounds__(kQdThreads, kBf16 ? 4 : 2) q4_decode_kernel(co
 #pragma unroll
                 for (int g = 0; g < G; ++g) {
                     unsigned a[4], b[4];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) { a[i] = q4_pair(wa[g], i); b[i] = q4_pair(wb[g], i); }
+                    q4_codes(wa[g], a);
+                    q4_codes(wb[g], b);
                     float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                     for (int p = NP - 1; p >= 0; --p) {
-                        q4_mma(c, a[0], b[0], a[1], b[1], qf[p][g][0], qf[p][g][1]);
-                        q4_mma(c, a[2], b[2], a[3], b[3], qf[p][g][2], qf[p][g][3]);
+                        gm_mma(c, {a[0], b[0], a[1], b[1]}, qf[p][g][0], qf[p][g][1]);
+                        gm_mma(c, {a[2], b[2], a[3], b[3]}, qf[p][g][2], qf[p][g][3]);
                     }
                     x[0] = fmaf(q4_scale(na[g]), c[0], fmaf(q4_min(na[g]), qsum[g][0], x[0]));
                     x[1] = fmaf(q4_scale(na[g]), c[1], fmaf(q4_min(na[g]), qsum[g][1], x[1]));
@@ -271,8 +328,22 @@ __global__ void __launch_bounds__(kQdThreads, kBf16 ? 4 : 2) q4_decode_kernel(co
                 }
             }
 #pragma unroll
-            for (int e = 0; e < 4; ++e) x[e] = live[e >> 1] ? x[e] * P.scale : -INFINITY;
-            float now[2] = {fmaxf(x[0], x[2]), fmaxf(x[1], x[3])};
+            for (int e = 0; e < 4; ++e) x[e] = live[e >> 1] ? x[e] * unscale[e & 1] : -INFINITY;
+            const Words va = *reinterpret_cast<const Words*>(tile + T::values + (gq * 4 + t) * (4 * G)),
+                        vb = *reinterpret_cast<const Words*>(tile + T::values + (32 + gq * 4 + t) * (4 * G));
+            const Words ma = *reinterpret_cast<const Words*>(tile + T::value_meta + gq * (4 * G)), mb = *reinterpret_cast<const Words*>(tile + T::value_meta + (gq + 8) * (4 * G));
+            const unsigned *na = reinterpret_cast<const unsigned*>(&ma), *nb = reinterpret_cast<const unsigned*>(&mb);
+            float sa[G], sb[G], ba = 0.0f, bb = 0.0f;   // (what is behind the last token may be anything)
+#pragma unroll
+            for (int g = 0; g < G; ++g) {
+                sa[g] = live[0] ? q4_scale(na[g]) : 0.0f;
+                sb[g] = live[1] ? q4_scale(nb[g]) : 0.0f;
+                ba = fmaxf(ba, sa[g]);
+                bb = fmaxf(bb, sb[g]);
+            }
+            ba = q4_exponent(ba) - kQdRoom;
+            bb = q4_exponent(bb) - kQdRoom;
+            float now[2] = {fmaxf(x[0] + ba, x[2] + bb), fmaxf(x[1] + ba, x[3] + bb)};
 #pragma unroll
             for (int off = 4; off < 32; off <<= 1) {
                 now[0] = fmaxf(now[0], __shfl_xor_sync(0xffffffffu, now[0], off));
@@ -296,29 +367,26 @@ __global__ void __launch_bounds__(kQdThreads, kBf16 ? 4 : 2) q4_decode_kernel(co
             l[0] += x[0] + x[2];
             l[1] += x[1] + x[3];
             {
-                const Words va = *reinterpret_cast<const Words*>(tile + T::values + (gq * 4 + t) * (4 * G)),
-                            vb = *reinterpret_cast<const Words*>(tile + T::values + (32 + gq * 4 + t) * (4 * G));
-                const Words ma = *reinterpret_cast<const Words*>(tile + T::value_meta + gq * (4 * G)), mb = *reinterpret_cast<const Words*>(tile + T::value_meta + (gq + 8) * (4 * G));
                 const unsigned *wa = reinterpret_cast<const unsigned*>(&va), *wb = reinterpret_cast<const unsigned*>(&vb);
-                const unsigned *na = reinterpret_cast<const unsigned*>(&ma), *nb = reinterpret_cast<const unsigned*>(&mb);
 #pragma unroll
                 for (int g = 0; g < G; ++g) {
-                    const unsigned mna = live[0] ? na[g] : 0u, mnb = live[1] ? nb[g] : 0u;   // (what is behind the last token may be anything)
-                    mins[g][0] = fmaf(x[0], q4_min(mna), fmaf(x[2], q4_min(mnb), mins[g][0]));
-                    mins[g][1] = fmaf(x[1], q4_min(mna), fmaf(x[3], q4_min(mnb), mins[g][1]));
-                    float y[4] = {x[0] * q4_scale(mna), x[1] * q4_scale(mna), x[2] * q4_scale(mnb), x[3] * q4_scale(mnb)};
-                    unsigned b0[NP], b1[NP];
+                    const float low = live[0] ? q4_min(na[g]) : 0.0f, high = live[1] ? q4_min(nb[g]) : 0.0f;
+                    mins[g][0] = fmaf(x[0], low, fmaf(x[2], high, mins[g][0]));
+                    mins[g][1] = fmaf(x[1], low, fmaf(x[3], high, mins[g][1]));
+                    float y[4] = {x[0] * sa[g], x[1] * sa[g], x[2] * sb[g], x[3] * sb[g]};
+                    unsigned b0[NP], b1[NP], a[4], b[4];
 #pragma unroll
                     for (int p = 0; p < NP; ++p) { b0[p] = q4_turn(q4_part(y[0], y[1])); b1[p] = q4_turn(q4_part(y[2], y[3])); }
+                    q4_codes(wa[g], a);
+                    q4_codes(wb[g], b);
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
-                        const unsigned a0 = q4_pair(wa[g], 2 * h), a1 = q4_pair(wa[g], 2 * h + 1), a2 = q4_pair(wb[g], 2 * h), a3 = q4_pair(wb[g], 2 * h + 1);
                         if (NP == 1) {
-                            q4_mma(o[2 * g + h], a0, a1, a2, a3, b0[0], b1[0]);
+                            gm_mma(o[2 * g + h], {a[2 * h], a[2 * h + 1], b[2 * h], b[2 * h + 1]}, b0[0], b1[0]);
                         } else {   // (the tensor cores cut what they add to a sum: a tile's products are summed on their own)
                             float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                            for (int p = NP - 1; p >= 0; --p) q4_mma(c, a0, a1, a2, a3, b0[p], b1[p]);
+                            for (int p = NP - 1; p >= 0; --p) gm_mma(c, {a[2 * h], a[2 * h + 1], b[2 * h], b[2 * h + 1]}, b0[p], b1[p]);
 #pragma unroll
                             for (int e = 0; e < 4; ++e) o[2 * g + h][e] += c[e];
                         }
@@ -326,6 +394,8 @@ __global__ void __launch_bounds__(kQdThreads, kBf16 ? 4 : 2) q4_decode_kernel(co
                 }
             }
             ++taken;
+            from = from + 1 == kQdStages ? 0 : from + 1;
+            phase ^= from == 0;
             __syncwarp();   // the stage has been read
             fill();
         }
@@ -348,7 +418,7 @@ __global__ void __launch_bounds__(kQdThreads, kBf16 ? 4 : 2) q4_decode_kernel(co
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 float* to = sums + (warp * kQdHeads + 2 * t + h) * M::row + 32 * (m >> 1) + 4 * gq + 2 * (m & 1);
-                *reinterpret_cast<float2*>(to) = make_float2(o[m][h] + mins[m >> 1][h], o[m][h + 2] + mins[m >> 1][h]);
+                *reinterpret_cast<float2*>(to) = make_float2(fmaf(o[m][h], kQdCode, mins[m >> 1][h]), fmaf(o[m][h + 2], kQdCode / 16.0f, mins[m >> 1][h]));
             }
         __syncthreads();
         unit += u1 - u0;
@@ -418,7 +488,7 @@ __global__ void __launch_bounds__(kQdThreads) q4_combine_kernel(const __grid_con
 // CTAs of a decode: what the GPU holds at a time, or a unit each where the tables have room for fewer.
 static int q4_decode_ctas(int batch, int max_pages, int page_size, int kv_heads, int share, int dtype) {
     const long long units = (long long)batch * kv_heads * ((share + kQdHeads - 1) / kQdHeads) * (((long long)max_pages * page_size + kQdUnit - 1) / kQdUnit);
-    const int most = num_sms() * (dtype == OJX_BF16 ? 4 : 2);
+    const int most = num_sms() * kQdCtas(dtype == OJX_BF16);
     return units < most ? (int)units : most;
 }
 static size_t q4_decode_bytes(int ctas, int head_dim) {

@@ -14,9 +14,10 @@
 // reference of the weights is the largest score plus the exponent of its token's largest scale, so that p * s is in the range of fp16
 // whatever the scales are.
 //
-// Work: units of 64 tokens of a (sequence, KV head, eight query heads), all of them in a row, in equal shares for the CTAs whatever the
-// lengths are; the four warps of a CTA take a tile of a unit each, from rings of their own that bulk copies fill.  A share that begins
+// Work: units of 128 tokens of a (sequence, KV head, eight query heads), all of them in a row, in equal shares for the CTAs whatever the
+// lengths are; the four warps of a CTA take two tiles of a unit each, from rings of their own that bulk copies fill.  A share that begins
 // or ends inside a sequence leaves its sums to q4_combine_kernel.
+#include <algorithm>
 #include <cmath>
 
 #include "gather_mma.cuh"
@@ -27,8 +28,8 @@
 
 namespace ojx {
 
-constexpr int kQdThreads = 128, kQdWarps = 4, kQdStages = 3, kQdHeads = 8;
-constexpr int kQdUnit = kQdWarps * kQ4Tile;   // tokens
+constexpr int kQdThreads = 128, kQdWarps = 4, kQdStages = 2, kQdHeads = 8, kQdPair = 2;
+constexpr int kQdUnit = kQdWarps * kQdPair * kQ4Tile;   // tokens
 constexpr float kQdLowest = -3.0e38f;         // finite: scores of -inf weigh nothing, a NaN makes its head's result one
 constexpr float kQdSlack = 8.0f;              // sums are relative to a reference, until a score is 2^8 above it ...
 constexpr float kQdRoom = 5.0f;               // ... and the largest p * s is 2^5 then: 2^14 at most
@@ -51,6 +52,11 @@ template <int N> struct Q4Words;
 template <> struct Q4Words<2> { using type = uint2; };
 template <> struct Q4Words<4> { using type = uint4; };
 
+__device__ __forceinline__ void q4_mma(float (&c)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
 __device__ __forceinline__ unsigned q4_turn(unsigned v) {   // an 8 x 8 matrix of 16-bit numbers, a pair per lane
     unsigned r;
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
@@ -100,10 +106,9 @@ struct Q4Place {
 
 template <int HD>
 struct QdSmem {
-    static constexpr int ring = kQdStages * Q4Layout<HD>::bytes;    // of a warp
+    static constexpr int stage = kQdPair * Q4Layout<HD>::bytes, ring = kQdStages * stage;    // of a warp
     static constexpr int row = HD + 8;                              // of a head's sums
-    static constexpr int sums = kQdWarps * kQdHeads * row * 4;
-    static constexpr int bytes = kQdWarps * ring + sums;
+    static constexpr int bytes(int heads) { return kQdWarps * (ring + heads * row * 4); }
 };
 
 constexpr int kQdCtas(bool bf16) { return bf16 ? 4 : 3; }   // per SM
@@ -117,7 +122,7 @@ __global__ void __launch_bounds__(kQdThreads, kQdCtas(kBf16)) q4_decode_kernel(c
     extern __shared__ __align__(128) unsigned char qd_smem[];
     __shared__ float s_m[kQdWarps][kQdHeads], s_l[kQdWarps][kQdHeads];
     __shared__ __align__(8) unsigned long long s_bar[kQdWarps][kQdStages];
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, gq = lane >> 2, t = lane & 3;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, gq = lane >> 2, t = lane & 3, sum_heads = min(P.share, kQdHeads);
     unsigned char* ring = qd_smem + warp * M::ring;
     float* sums = reinterpret_cast<float*>(qd_smem + kQdWarps * M::ring);
     const unsigned ring_at = static_cast<unsigned>(__cvta_generic_to_shared(ring)), bar_at = static_cast<unsigned>(__cvta_generic_to_shared(&s_bar[warp][0]));
@@ -172,8 +177,9 @@ __global__ void __launch_bounds__(kQdThreads, kQdCtas(kBf16)) q4_decode_kernel(c
     }
     __syncwarp();
 
-    // Copies run ahead of the tiles by the stages of the ring.  Every tile that begins before its sequence's end has a stage; one without a
-    // page stays as it is and is marked.  The page of the next copy is looked up a tile ahead.
+    // Copies run ahead by the stages of the ring, two tiles each: lanes 0 and 1 have a tile to themselves (the others do as they do).  A
+    // pair that begins before its sequence's end has a stage; a tile behind the end or without a page stays as it is, the latter is
+    // marked.  The pages of the next copies are looked up a pair ahead.
     struct {
         Q4Place at;
         long long rest;       // units of the share from here on
@@ -183,12 +189,12 @@ __global__ void __launch_bounds__(kQdThreads, kQdCtas(kBf16)) q4_decode_kernel(c
     } ahead{at, last - first, nullptr, 0, 0, 0, 0, 0, 0};
     const int page_tiles = P.cache.page_size / kQ4Tile;
     const size_t head_bytes = (size_t)page_tiles * T::bytes, page_bytes = head_bytes * P.cache.kv_heads;
-    unsigned missing = 0;
+    unsigned missing = 0;     // two bits for each stage
     auto enter = [&]() {   // an item, at its unit `ahead.at.u`
         ahead.tiles = (Q4Place::length(P, ahead.at.b) + kQ4Tile - 1) / kQ4Tile;
         ahead.table = P.cache.block_table + (size_t)ahead.at.b * P.cache.max_pages;
         ahead.head = ahead.at.hh / P.blocks * head_bytes;
-        ahead.tile = ahead.at.u * kQdWarps + warp;
+        ahead.tile = (ahead.at.u * kQdWarps + warp) * kQdPair + (lane & 1);
         ahead.page = ahead.tile / page_tiles;
         ahead.in = ahead.tile - ahead.page * page_tiles;
         ahead.id = ahead.tile < ahead.tiles ? ahead.table[ahead.page] : 0;
@@ -197,9 +203,10 @@ __global__ void __launch_bounds__(kQdThreads, kQdCtas(kBf16)) q4_decode_kernel(c
         --ahead.rest;
         if (ahead.at.u + 1 < ahead.at.units) {
             ++ahead.at.u;
-            ahead.tile += kQdWarps;
-            ahead.in += kQdWarps;
+            ahead.tile += kQdWarps * kQdPair;
+            ahead.in += kQdWarps * kQdPair;
             while (ahead.in >= page_tiles) { ahead.in -= page_tiles; ++ahead.page; }
+            __syncwarp();
             ahead.id = ahead.tile < ahead.tiles ? ahead.table[ahead.page] : 0;
         } else if (ahead.rest > 0) {
             ahead.at.skip(P, heads);
@@ -208,21 +215,22 @@ __global__ void __launch_bounds__(kQdThreads, kQdCtas(kBf16)) q4_decode_kernel(c
     };
     int filled = 0, taken = 0, into = 0, from = 0, phase = 0;   // stages used so far, the next ones and the phase of the next to be read
     auto fill = [&]() {
-        while (ahead.rest > 0 && ahead.tile >= ahead.tiles) next();
+        while (ahead.rest > 0 && ahead.tile - (lane & 1) >= ahead.tiles) next();
         if (ahead.rest <= 0) return;
-        const bool there = (unsigned)ahead.id < (unsigned)P.cache.num_pages;
-        missing = there ? missing & ~(1u << into) : missing | 1u << into;
+        const bool want = ahead.tile < ahead.tiles, there = want && (unsigned)ahead.id < (unsigned)P.cache.num_pages;
+        const unsigned none = __ballot_sync(0xffffffffu, want && !there) & 3u, copies = __ballot_sync(0xffffffffu, there) & 3u;
+        missing = (missing & ~(3u << (2 * into))) | none << (2 * into);
+        const unsigned bar = bar_at + 8 * into;
         if (lane == 0) {
-            if (there) {
-                asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar_at + 8 * into), "n"(T::bytes) : "memory");
-                asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(ring_at + into * T::bytes),
-                             "l"(P.cache.pool + (size_t)ahead.id * page_bytes + ahead.head + ahead.in * T::bytes), "n"(T::bytes), "r"(bar_at + 8 * into)
-                             : "memory");
-            } else {
-                asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar_at + 8 * into) : "memory");
-                atomicExch(P.cache.status, 1);
-            }
+            if (copies) asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(__popc(copies) * T::bytes) : "memory");
+            else asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+            if (none) atomicExch(P.cache.status, 1);
         }
+        __syncwarp();
+        if (lane < kQdPair && there)
+            asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(ring_at + into * M::stage + lane * T::bytes),
+                         "l"(P.cache.pool + (size_t)ahead.id * page_bytes + ahead.head + ahead.in * T::bytes), "n"(T::bytes), "r"(bar)
+                         : "memory");
         ++filled;
         into = into + 1 == kQdStages ? 0 : into + 1;
         next();
@@ -237,7 +245,8 @@ __global__ void __launch_bounds__(kQdThreads, kQdCtas(kBf16)) q4_decode_kernel(c
         const bool begins = at.u == 0;
         // the queries as the second operand: lane (head gq, t) has the dimensions 32 g + 8 t + 0..7, pairs i and i + 4
         unsigned qf[NP][G][4];
-        float qsum[G][2], unscale[2];
+        unsigned qs[2];       // sums over the groups in three bf16 parts, as an operand: k = 4 part + group
+        float unscale[2];
         {
             float x[G][8];
             unsigned most = 0;
@@ -269,6 +278,7 @@ __global__ void __launch_bounds__(kQdThreads, kQdCtas(kBf16)) q4_decode_kernel(c
             const float back = fminf(down * (P.scale * kQdCode), 3.0e38f);
             unscale[0] = __shfl_sync(0xffffffffu, back, 8 * t);        // heads 2 t and 2 t + 1
             unscale[1] = __shfl_sync(0xffffffffu, back, 8 * t + 4);
+            float total[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int g = 0; g < G; ++g) {
 #pragma unroll
@@ -277,14 +287,24 @@ __global__ void __launch_bounds__(kQdThreads, kQdCtas(kBf16)) q4_decode_kernel(c
                 sum += __shfl_xor_sync(0xffffffffu, sum, 1);
                 sum += __shfl_xor_sync(0xffffffffu, sum, 2);
                 sum *= 1.0f / kQdCode;
-                qsum[g][0] = __shfl_sync(0xffffffffu, sum, 8 * t);
-                qsum[g][1] = __shfl_sync(0xffffffffu, sum, 8 * t + 4);
+                total[g] = sum;
 #pragma unroll
                 for (int i = 1; i < 8; i += 2) x[g][i] *= 0.0625f;     // (the codes of odd nibbles are 16 times as large)
 #pragma unroll
                 for (int p = 0; p < NP; ++p)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) qf[p][g][i] = q4_part(x[g][i], x[g][i + 4]);
+            }
+            // lane t has k = 2 t and 2 t + 1 (parts 0 and 1), and 8 on (part 2)
+            float s0 = t & 1 ? total[2] : total[0], s1 = t & 1 ? total[3] : total[1];
+#pragma unroll
+            for (int p = 0; p < 3; ++p) {
+                const __nv_bfloat162 h = __floats2bfloat162_rn(s0, s1);
+                s0 -= __low2float(h);
+                s1 -= __high2float(h);
+                const unsigned w = *reinterpret_cast<const unsigned*>(&h);
+                if (p == 2) qs[1] = t < 2 ? w : 0u;
+                else if (p == t >> 1) qs[0] = w;
             }
         }
         float top[2] = {kQdLowest, kQdLowest}, l[2] = {0.0f, 0.0f}, o[2 * G][4], mins[G][2];
@@ -297,19 +317,32 @@ __global__ void __launch_bounds__(kQdThreads, kQdCtas(kBf16)) q4_decode_kernel(c
 
         const int u0 = at.u, u1 = (int)min((long long)at.units, at.u + (last - unit));
         for (int u = u0; u < u1 && ok; ++u) {
-            const int token = (u * kQdWarps + warp) * kQ4Tile;
+            const int token = (u * kQdWarps + warp) * kQdPair * kQ4Tile;
             if (token >= length) break;
             if (!(ok = __all_sync(0xffffffffu, bar_wait(bar_at + 8 * from, phase)))) break;
-            const unsigned char* tile = ring + from * T::bytes;
-            const int seen = missing >> from & 1 ? 0 : length - token;
-            const bool live[2] = {gq < seen, gq + 8 < seen};
-            float x[4];
-            {
+            const unsigned char* stage = ring + from * M::stage;
+            const unsigned none = missing >> (2 * from) & 3u;
+            // tokens of the two tiles that are there
+            const int seen[2] = {none & 1 ? 0 : length - token, none & 2 ? 0 : length - token - kQ4Tile};
+            const bool part = min(seen[0], seen[1]) < kQ4Tile;
+            float x[kQdPair][4];
+            float now[2] = {kQdLowest, kQdLowest};
+#pragma unroll
+            for (int i = 0; i < kQdPair; ++i) {
+                const unsigned char* tile = stage + i * T::bytes;
                 const Words ka = *reinterpret_cast<const Words*>(tile + (gq * 4 + t) * (4 * G)), kb = *reinterpret_cast<const Words*>(tile + ((gq + 8) * 4 + t) * (4 * G));
                 const Words ma = *reinterpret_cast<const Words*>(tile + T::key_meta + gq * (4 * G)), mb = *reinterpret_cast<const Words*>(tile + T::key_meta + (gq + 8) * (4 * G));
+                const Words va = *reinterpret_cast<const Words*>(tile + T::value_meta + gq * (4 * G)), vb = *reinterpret_cast<const Words*>(tile + T::value_meta + (gq + 8) * (4 * G));
                 const unsigned *wa = reinterpret_cast<const unsigned*>(&ka), *wb = reinterpret_cast<const unsigned*>(&kb);
-                const unsigned *na = reinterpret_cast<const unsigned*>(&ma), *nb = reinterpret_cast<const unsigned*>(&mb);
-                x[0] = x[1] = x[2] = x[3] = 0.0f;
+                const unsigned *ca = reinterpret_cast<const unsigned*>(&ma), *cb = reinterpret_cast<const unsigned*>(&mb);
+                const unsigned *ua = reinterpret_cast<const unsigned*>(&va), *ub = reinterpret_cast<const unsigned*>(&vb);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[i][e] = 0.0f;
+                {   // sum_g m_g sum(q_g): the minima, bf16 as they are, times the sums in three parts
+                    const bool odd = G == 4 && (t & 1);
+                    const unsigned a = __byte_perm(odd ? ca[G - 2] : ca[0], odd ? ca[G - 1] : ca[1], 0x7632), b = __byte_perm(odd ? cb[G - 2] : cb[0], odd ? cb[G - 1] : cb[1], 0x7632);
+                    q4_mma(x[i], a, b, a, b, qs[0], qs[1]);
+                }
 #pragma unroll
                 for (int g = 0; g < G; ++g) {
                     unsigned a[4], b[4];
@@ -321,40 +354,40 @@ __global__ void __launch_bounds__(kQdThreads, kQdCtas(kBf16)) q4_decode_kernel(c
                         gm_mma(c, {a[0], b[0], a[1], b[1]}, qf[p][g][0], qf[p][g][1]);
                         gm_mma(c, {a[2], b[2], a[3], b[3]}, qf[p][g][2], qf[p][g][3]);
                     }
-                    x[0] = fmaf(q4_scale(na[g]), c[0], fmaf(q4_min(na[g]), qsum[g][0], x[0]));
-                    x[1] = fmaf(q4_scale(na[g]), c[1], fmaf(q4_min(na[g]), qsum[g][1], x[1]));
-                    x[2] = fmaf(q4_scale(nb[g]), c[2], fmaf(q4_min(nb[g]), qsum[g][0], x[2]));
-                    x[3] = fmaf(q4_scale(nb[g]), c[3], fmaf(q4_min(nb[g]), qsum[g][1], x[3]));
+                    x[i][0] = fmaf(q4_scale(ca[g]), c[0], x[i][0]);
+                    x[i][1] = fmaf(q4_scale(ca[g]), c[1], x[i][1]);
+                    x[i][2] = fmaf(q4_scale(cb[g]), c[2], x[i][2]);
+                    x[i][3] = fmaf(q4_scale(cb[g]), c[3], x[i][3]);
                 }
-            }
 #pragma unroll
-            for (int e = 0; e < 4; ++e) x[e] = live[e >> 1] ? x[e] * unscale[e & 1] : -INFINITY;
-            const Words va = *reinterpret_cast<const Words*>(tile + T::values + (gq * 4 + t) * (4 * G)),
-                        vb = *reinterpret_cast<const Words*>(tile + T::values + (32 + gq * 4 + t) * (4 * G));
-            const Words ma = *reinterpret_cast<const Words*>(tile + T::value_meta + gq * (4 * G)), mb = *reinterpret_cast<const Words*>(tile + T::value_meta + (gq + 8) * (4 * G));
-            const unsigned *na = reinterpret_cast<const unsigned*>(&ma), *nb = reinterpret_cast<const unsigned*>(&mb);
-            float sa[G], sb[G], ba = 0.0f, bb = 0.0f;   // (what is behind the last token may be anything)
+                for (int e = 0; e < 4; ++e) x[i][e] *= unscale[e & 1];
+                if (part) {   // what is behind the last token may be anything
+                    if (gq >= seen[i]) x[i][0] = x[i][1] = -INFINITY;
+                    if (gq + 8 >= seen[i]) x[i][2] = x[i][3] = -INFINITY;
+                }
+                float ba = 0.0f, bb = 0.0f;
 #pragma unroll
-            for (int g = 0; g < G; ++g) {
-                sa[g] = live[0] ? q4_scale(na[g]) : 0.0f;
-                sb[g] = live[1] ? q4_scale(nb[g]) : 0.0f;
-                ba = fmaxf(ba, sa[g]);
-                bb = fmaxf(bb, sb[g]);
+                for (int g = 0; g < G; ++g) {
+                    ba = fmaxf(ba, q4_scale(ua[g]));
+                    bb = fmaxf(bb, q4_scale(ub[g]));
+                }
+                ba = q4_exponent(ba);
+                bb = q4_exponent(bb);
+                now[0] = fmaxf(now[0], fmaxf(x[i][0] + ba, x[i][2] + bb));
+                now[1] = fmaxf(now[1], fmaxf(x[i][1] + ba, x[i][3] + bb));
             }
-            ba = q4_exponent(ba) - kQdRoom;
-            bb = q4_exponent(bb) - kQdRoom;
-            float now[2] = {fmaxf(x[0] + ba, x[2] + bb), fmaxf(x[1] + ba, x[3] + bb)};
+            // (the reference has to move for a row only where one of its lanes sees a score too far above it)
+            if (__any_sync(0xffffffffu, now[0] > top[0] + (kQdSlack + kQdRoom) || now[1] > top[1] + (kQdSlack + kQdRoom))) {
 #pragma unroll
-            for (int off = 4; off < 32; off <<= 1) {
-                now[0] = fmaxf(now[0], __shfl_xor_sync(0xffffffffu, now[0], off));
-                now[1] = fmaxf(now[1], __shfl_xor_sync(0xffffffffu, now[1], off));
-            }
-            const bool up[2] = {now[0] > top[0] + kQdSlack, now[1] > top[1] + kQdSlack};
-            if (__any_sync(0xffffffffu, up[0] || up[1])) {
+                for (int off = 4; off < 32; off <<= 1) {
+                    now[0] = fmaxf(now[0], __shfl_xor_sync(0xffffffffu, now[0], off));
+                    now[1] = fmaxf(now[1], __shfl_xor_sync(0xffffffffu, now[1], off));
+                }
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    const float keep = up[h] ? q4_exp2(top[h] - now[h]) : 1.0f;
-                    top[h] = up[h] ? now[h] : top[h];
+                    const bool up = now[h] > top[h] + (kQdSlack + kQdRoom);
+                    const float to = up ? now[h] - kQdRoom : top[h], keep = up ? q4_exp2(top[h] - to) : 1.0f;
+                    top[h] = to;
                     l[h] *= keep;
 #pragma unroll
                     for (int g = 0; g < G; ++g) mins[g][h] *= keep;
@@ -363,17 +396,27 @@ __global__ void __launch_bounds__(kQdThreads, kQdCtas(kBf16)) q4_decode_kernel(c
                 }
             }
 #pragma unroll
-            for (int e = 0; e < 4; ++e) x[e] = q4_exp2(x[e] - top[e & 1]);
-            l[0] += x[0] + x[2];
-            l[1] += x[1] + x[3];
-            {
+            for (int i = 0; i < kQdPair; ++i) {
+                const unsigned char* tile = stage + i * T::bytes;
+                const Words va = *reinterpret_cast<const Words*>(tile + T::values + (gq * 4 + t) * (4 * G)),
+                            vb = *reinterpret_cast<const Words*>(tile + T::values + (32 + gq * 4 + t) * (4 * G));
+                Words ma = *reinterpret_cast<const Words*>(tile + T::value_meta + gq * (4 * G)), mb = *reinterpret_cast<const Words*>(tile + T::value_meta + (gq + 8) * (4 * G));
+                if (part) {
+                    if (gq >= seen[i]) ma = Words{};
+                    if (gq + 8 >= seen[i]) mb = Words{};
+                }
+                const unsigned *na = reinterpret_cast<const unsigned*>(&ma), *nb = reinterpret_cast<const unsigned*>(&mb);
                 const unsigned *wa = reinterpret_cast<const unsigned*>(&va), *wb = reinterpret_cast<const unsigned*>(&vb);
 #pragma unroll
+                for (int e = 0; e < 4; ++e) x[i][e] = q4_exp2(x[i][e] - top[e & 1]);
+                l[0] += x[i][0] + x[i][2];
+                l[1] += x[i][1] + x[i][3];
+#pragma unroll
                 for (int g = 0; g < G; ++g) {
-                    const float low = live[0] ? q4_min(na[g]) : 0.0f, high = live[1] ? q4_min(nb[g]) : 0.0f;
-                    mins[g][0] = fmaf(x[0], low, fmaf(x[2], high, mins[g][0]));
-                    mins[g][1] = fmaf(x[1], low, fmaf(x[3], high, mins[g][1]));
-                    float y[4] = {x[0] * sa[g], x[1] * sa[g], x[2] * sb[g], x[3] * sb[g]};
+                    const float low = q4_min(na[g]), high = q4_min(nb[g]), sa = q4_scale(na[g]), sb = q4_scale(nb[g]);
+                    mins[g][0] = fmaf(x[i][0], low, fmaf(x[i][2], high, mins[g][0]));
+                    mins[g][1] = fmaf(x[i][1], low, fmaf(x[i][3], high, mins[g][1]));
+                    float y[4] = {x[i][0] * sa, x[i][1] * sa, x[i][2] * sb, x[i][3] * sb};
                     unsigned b0[NP], b1[NP], a[4], b[4];
 #pragma unroll
                     for (int p = 0; p < NP; ++p) { b0[p] = q4_turn(q4_part(y[0], y[1])); b1[p] = q4_turn(q4_part(y[2], y[3])); }
@@ -417,7 +460,8 @@ __global__ void __launch_bounds__(kQdThreads, kQdCtas(kBf16)) q4_decode_kernel(c
         for (int m = 0; m < 2 * G; ++m)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                float* to = sums + (warp * kQdHeads + 2 * t + h) * M::row + 32 * (m >> 1) + 4 * gq + 2 * (m & 1);
+                if (2 * t + h >= sum_heads) continue;
+                float* to = sums + (warp * sum_heads + 2 * t + h) * M::row + 32 * (m >> 1) + 4 * gq + 2 * (m & 1);
                 *reinterpret_cast<float2*>(to) = make_float2(fmaf(o[m][h], kQdCode, mins[m >> 1][h]), fmaf(o[m][h + 2], kQdCode / 16.0f, mins[m >> 1][h]));
             }
         __syncthreads();
@@ -432,7 +476,7 @@ __global__ void __launch_bounds__(kQdThreads, kQdCtas(kBf16)) q4_decode_kernel(c
 #pragma unroll
             for (int w = 0; w < kQdWarps; ++w) {
                 const float keep = q4_exp2(s_m[w][h] - most);
-                acc = fmaf(sums[(w * kQdHeads + h) * M::row + d], keep, acc);
+                acc = fmaf(sums[(w * sum_heads + h) * M::row + d], keep, acc);
                 weight = fmaf(s_l[w][h], keep, weight);
             }
             if (begins && ends) {
@@ -498,8 +542,8 @@ static size_t q4_decode_bytes(int ctas, int head_dim) {
 template <int HD, bool kBf16>
 static int launch_q4_decode(const Q4DecodeProblem& P, int ctas, cudaStream_t s) {
     static std::atomic<bool> opted[64];
-    OJX_CUDA_TRY(opt_in_smem(reinterpret_cast<const void*>(q4_decode_kernel<HD, kBf16>), QdSmem<HD>::bytes, opted));
-    OJX_CUDA_TRY(launch_chained(q4_decode_kernel<HD, kBf16>, ctas, kQdThreads, QdSmem<HD>::bytes, s, P));
+    OJX_CUDA_TRY(opt_in_smem(reinterpret_cast<const void*>(q4_decode_kernel<HD, kBf16>), QdSmem<HD>::bytes(kQdHeads), opted));
+    OJX_CUDA_TRY(launch_chained(q4_decode_kernel<HD, kBf16>, ctas, kQdThreads, QdSmem<HD>::bytes(std::min(P.share, kQdHeads)), s, P));
     OJX_CUDA_TRY(launch_chained(q4_combine_kernel<HD, kBf16>, ctas, kQdThreads, 0, s, P));
     count_launch(2);
     return OJX_OK;

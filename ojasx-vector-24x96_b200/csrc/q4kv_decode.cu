@@ -180,47 +180,44 @@ __global__ void __launch_bounds__(kQdThreads, kQdCtas(kBf16)) q4_decode_kernel(c
     // Copies run ahead by the stages of the ring, two tiles each: lanes 0 and 1 have a tile to themselves (the others do as they do).  A
     // pair that begins before its sequence's end has a stage; a tile behind the end or without a page stays as it is, the latter is
     // marked.  The pages of the next copies are looked up a pair ahead.
-    struct {
-        Q4Place at;
-        long long rest;       // units of the share from here on
-        const int* table;
-        int tile, in, page, id, tiles;   // tile of the sequence, its place in its page, the page's place in the table and its id
-        size_t head;          // bytes of the heads before this one in a page
-    } ahead{at, last - first, nullptr, 0, 0, 0, 0, 0, 0};
-    const int page_tiles = P.cache.page_size / kQ4Tile;
+    Q4Place ahead = at;
+    int rest = (int)(last - first);    // units from `ahead` on
+    int left, in, id;                  // tiles of the sequence from this lane's next one on, that one's place in its page, the page's id
+    const int* page;                   // its entry in the table
+    const uint8_t* head;               // the head's part of page 0
+    const int page_tiles = P.cache.page_size / kQ4Tile, step_pages = kQdWarps * kQdPair / page_tiles, step_in = kQdWarps * kQdPair % page_tiles;
     const size_t head_bytes = (size_t)page_tiles * T::bytes, page_bytes = head_bytes * P.cache.kv_heads;
     unsigned missing = 0;     // two bits for each stage
-    auto enter = [&]() {   // an item, at its unit `ahead.at.u`
-        ahead.tiles = (Q4Place::length(P, ahead.at.b) + kQ4Tile - 1) / kQ4Tile;
-        ahead.table = P.cache.block_table + (size_t)ahead.at.b * P.cache.max_pages;
-        ahead.head = ahead.at.hh / P.blocks * head_bytes;
-        ahead.tile = (ahead.at.u * kQdWarps + warp) * kQdPair + (lane & 1);
-        ahead.page = ahead.tile / page_tiles;
-        ahead.in = ahead.tile - ahead.page * page_tiles;
-        ahead.id = ahead.tile < ahead.tiles ? ahead.table[ahead.page] : 0;
+    auto enter = [&]() {   // an item, at its unit `ahead.u`
+        const int tile = (ahead.u * kQdWarps + warp) * kQdPair + (lane & 1);
+        left = (Q4Place::length(P, ahead.b) + kQ4Tile - 1) / kQ4Tile - tile;
+        page = P.cache.block_table + (size_t)ahead.b * P.cache.max_pages + tile / page_tiles;
+        head = P.cache.pool + ahead.hh / P.blocks * head_bytes;
+        in = tile % page_tiles;
+        id = left > 0 ? *page : 0;
     };
     auto next = [&]() {
-        --ahead.rest;
-        if (ahead.at.u + 1 < ahead.at.units) {
-            ++ahead.at.u;
-            ahead.tile += kQdWarps * kQdPair;
-            ahead.in += kQdWarps * kQdPair;
-            while (ahead.in >= page_tiles) { ahead.in -= page_tiles; ++ahead.page; }
+        --rest;
+        if (ahead.u + 1 < ahead.units) {
+            ++ahead.u;
+            left -= kQdWarps * kQdPair;
+            in += step_in;
+            page += step_pages;
+            if (in >= page_tiles) { in -= page_tiles; ++page; }
             __syncwarp();
-            ahead.id = ahead.tile < ahead.tiles ? ahead.table[ahead.page] : 0;
-        } else if (ahead.rest > 0) {
-            ahead.at.skip(P, heads);
+            if (left > 0) id = *page;
+        } else if (rest > 0) {
+            ahead.skip(P, heads);
             enter();
         }
     };
-    int filled = 0, taken = 0, into = 0, from = 0, phase = 0;   // stages used so far, the next ones and the phase of the next to be read
-    auto fill = [&]() {
-        while (ahead.rest > 0 && ahead.tile - (lane & 1) >= ahead.tiles) next();
-        if (ahead.rest <= 0) return;
-        const bool want = ahead.tile < ahead.tiles, there = want && (unsigned)ahead.id < (unsigned)P.cache.num_pages;
-        const unsigned none = __ballot_sync(0xffffffffu, want && !there) & 3u, copies = __ballot_sync(0xffffffffu, there) & 3u;
-        missing = (missing & ~(3u << (2 * into))) | none << (2 * into);
-        const unsigned bar = bar_at + 8 * into;
+    auto fill = [&](int stage) {   // true: there was a pair
+        while (rest > 0 && left + (lane & 1) <= 0) next();
+        if (rest <= 0) return false;
+        const bool there = left > 0 && (unsigned)id < (unsigned)P.cache.num_pages;
+        const unsigned none = __ballot_sync(0xffffffffu, left > 0 && !there) & 3u, copies = __ballot_sync(0xffffffffu, there) & 3u;
+        missing = (missing & ~(3u << (2 * stage))) | none << (2 * stage);
+        const unsigned bar = bar_at + 8 * stage;
         if (lane == 0) {
             if (copies) asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(__popc(copies) * T::bytes) : "memory");
             else asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
@@ -228,15 +225,15 @@ __global__ void __launch_bounds__(kQdThreads, kQdCtas(kBf16)) q4_decode_kernel(c
         }
         __syncwarp();
         if (lane < kQdPair && there)
-            asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(ring_at + into * M::stage + lane * T::bytes),
-                         "l"(P.cache.pool + (size_t)ahead.id * page_bytes + ahead.head + ahead.in * T::bytes), "n"(T::bytes), "r"(bar)
+            asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(ring_at + stage * M::stage + lane * T::bytes),
+                         "l"(head + (size_t)id * page_bytes + in * T::bytes), "n"(T::bytes), "r"(bar)
                          : "memory");
-        ++filled;
-        into = into + 1 == kQdStages ? 0 : into + 1;
         next();
+        return true;
     };
+    int filled = 0, taken = 0;
     enter();
-    for (int i = 0; i < kQdStages; ++i) fill();
+    for (int i = 0; i < kQdStages; ++i) filled += fill(i);
 
     bool ok = true;
     for (long long unit = first; unit < last;) {
@@ -319,7 +316,8 @@ __global__ void __launch_bounds__(kQdThreads, kQdCtas(kBf16)) q4_decode_kernel(c
         for (int u = u0; u < u1 && ok; ++u) {
             const int token = (u * kQdWarps + warp) * kQdPair * kQ4Tile;
             if (token >= length) break;
-            if (!(ok = __all_sync(0xffffffffu, bar_wait(bar_at + 8 * from, phase)))) break;
+            const int from = taken % kQdStages;
+            if (!(ok = __all_sync(0xffffffffu, bar_wait(bar_at + 8 * from, taken / kQdStages & 1)))) break;
             const unsigned char* stage = ring + from * M::stage;
             const unsigned none = missing >> (2 * from) & 3u;
             // tokens of the two tiles that are there
@@ -359,8 +357,6 @@ __global__ void __launch_bounds__(kQdThreads, kQdCtas(kBf16)) q4_decode_kernel(c
                     x[i][2] = fmaf(q4_scale(cb[g]), c[2], x[i][2]);
                     x[i][3] = fmaf(q4_scale(cb[g]), c[3], x[i][3]);
                 }
-#pragma unroll
-                for (int e = 0; e < 4; ++e) x[i][e] *= unscale[e & 1];
                 if (part) {   // what is behind the last token may be anything
                     if (gq >= seen[i]) x[i][0] = x[i][1] = -INFINITY;
                     if (gq + 8 >= seen[i]) x[i][2] = x[i][3] = -INFINITY;
@@ -373,8 +369,8 @@ __global__ void __launch_bounds__(kQdThreads, kQdCtas(kBf16)) q4_decode_kernel(c
                 }
                 ba = q4_exponent(ba);
                 bb = q4_exponent(bb);
-                now[0] = fmaxf(now[0], fmaxf(x[i][0] + ba, x[i][2] + bb));
-                now[1] = fmaxf(now[1], fmaxf(x[i][1] + ba, x[i][3] + bb));
+                now[0] = fmaxf(now[0], fmaxf(fmaf(x[i][0], unscale[0], ba), fmaf(x[i][2], unscale[0], bb)));
+                now[1] = fmaxf(now[1], fmaxf(fmaf(x[i][1], unscale[1], ba), fmaf(x[i][3], unscale[1], bb)));
             }
             // (the reference has to move for a row only where one of its lanes sees a score too far above it)
             if (__any_sync(0xffffffffu, now[0] > top[0] + (kQdSlack + kQdRoom) || now[1] > top[1] + (kQdSlack + kQdRoom))) {
@@ -408,7 +404,7 @@ __global__ void __launch_bounds__(kQdThreads, kQdCtas(kBf16)) q4_decode_kernel(c
                 const unsigned *na = reinterpret_cast<const unsigned*>(&ma), *nb = reinterpret_cast<const unsigned*>(&mb);
                 const unsigned *wa = reinterpret_cast<const unsigned*>(&va), *wb = reinterpret_cast<const unsigned*>(&vb);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) x[i][e] = q4_exp2(x[i][e] - top[e & 1]);
+                for (int e = 0; e < 4; ++e) x[i][e] = q4_exp2(fmaf(x[i][e], unscale[e & 1], -top[e & 1]));
                 l[0] += x[i][0] + x[i][2];
                 l[1] += x[i][1] + x[i][3];
 #pragma unroll
@@ -437,10 +433,8 @@ __global__ void __launch_bounds__(kQdThreads, kQdCtas(kBf16)) q4_decode_kernel(c
                 }
             }
             ++taken;
-            from = from + 1 == kQdStages ? 0 : from + 1;
-            phase ^= from == 0;
             __syncwarp();   // the stage has been read
-            fill();
+            filled += fill(from);
         }
 
         // the warps' sums joined, and out

@@ -430,11 +430,14 @@ OJASX_API int ojasx_b200_q4kv_decode(const void* d_q, void* d_out, const void* d
  * of a head in elements, the dimensions of a head together) into d_out [n_rows, q_heads, head_dim].  Rows d_ends[b] .. and keys
  * d_key_ends[b] .. belong to sequence b, whose last query sees its last key, the one before it the keys up to the one before, and so
  * on; a query that sees nothing gives zeros; rows behind the last sequence are left as they were.  Keys that a query does not see
- * have no part in its result, whatever they hold. */
+ * have no part in its result, whatever they hold.  workspace: ojasx_b200_prompt_workspace bytes (0 for bf16) for this call alone,
+ * 256-byte aligned; the others 16-byte aligned, strides whole multiples of 16 bytes. */
+OJASX_API size_t ojasx_b200_prompt_workspace(int n_keys, int kv_heads, int head_dim, int io_dtype);
 OJASX_API int ojasx_b200_prompt_attention(const void* d_q, long long q_row, long long q_head, const void* d_k, long long k_row,
                                           long long k_head, const void* d_v, long long v_row, long long v_head, void* d_out,
                                           const int* d_ends, const int* d_key_ends, int batch, int n_rows, int n_keys, int q_heads,
-                                          int kv_heads, int head_dim, float scale, int io_dtype, void* stream);
+                                          int kv_heads, int head_dim, float scale, int io_dtype, void* workspace,
+                                          size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

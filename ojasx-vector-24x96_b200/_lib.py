@@ -126,7 +126,8 @@ SIGNATURES = {
     "ojasx_b200_q4kv_read": (_i, [_vp] * 7 + [_i] * 8 + [_vp]),
     "ojasx_b200_q4kv_decode_workspace": (_sz, [_i] * 7),
     "ojasx_b200_q4kv_decode": (_i, [_vp] * 6 + [_i] * 7 + [_f, _i, _vp, _sz, _vp]),
-    "ojasx_b200_prompt_attention": (_i, [_vp, _ll, _ll] * 3 + [_vp] * 3 + [_i] * 6 + [_f, _i, _vp]),
+    "ojasx_b200_prompt_workspace": (_sz, [_i] * 4),
+    "ojasx_b200_prompt_attention": (_i, [_vp, _ll, _ll] * 3 + [_vp] * 3 + [_i] * 6 + [_f, _i, _vp, _sz, _vp]),
 }
 
 _lib = None

@@ -5,6 +5,7 @@
 #include <algorithm>
 #include <cmath>
 
+#include "gather_mma.cuh"
 #include "handles.h"
 #include "launch.h"
 #include "packed.cuh"
@@ -22,131 +23,6 @@ struct PromptProblem {
     float scale;
 };
 
-// fp32 tiles of 64 rows x 64 keys, sixteen threads to four rows, four keys of a thread.
-template <int HD>
-__global__ void __launch_bounds__(256) prompt_tile_kernel(const __grid_constant__ PromptProblem P) {
-    constexpr int R = 64, C = 64, W = HD + 4;
-    extern __shared__ __align__(16) float sm[];
-    float *qs = sm, *ks = qs + R * W, *vs = ks + C * W, *ps = vs + C * W;   // ps [R][C + 4]
-    __shared__ int s_seq, s_part;
-    chain_begin();
-    const int per = R / P.share, tid = threadIdx.x, tx = tid & 15, ty = tid >> 4, head = blockIdx.y;
-    if (tid < 32) {
-        int seq = -1, part = 0;
-        const bool in = packed_part(P.batch, blockIdx.x, [&](int b) { return (packed_range(P.ends, b, P.n_rows).count + per - 1) / per; }, seq, part);
-        if (tid == 0) { s_seq = in ? seq : -1; s_part = part; }
-    }
-    __syncthreads();
-    if (s_seq < 0) return;
-    const PackedRange rows = packed_range(P.ends, s_seq, P.n_rows), keys = packed_range(P.key_ends, s_seq, P.n_keys);
-    const int p0 = s_part * per, live = min(per, rows.count - p0) * P.share, ahead = keys.count - rows.count;
-    auto load = [](const void* p, size_t i) { return reinterpret_cast<const float*>(p)[i]; };
-    for (int i = tid; i < R * HD; i += 256) {
-        const int r = i / HD, d = i % HD;
-        qs[r * W + d] = r < live ? load(P.q, (size_t)(rows.first + p0 + r / P.share) * P.q_row + (size_t)(head * P.share + r % P.share) * P.q_head + d) * P.scale : 0.0f;
-    }
-    float m[4], l[4], o[4][HD / 16];
-    int last[4];   // last key that the row sees
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int r = ty * 4 + i;
-        m[i] = -INFINITY; l[i] = 0.0f;
-        last[i] = r < live ? p0 + r / P.share + ahead : -1;
-#pragma unroll
-        for (int j = 0; j < HD / 16; ++j) o[i][j] = 0.0f;
-    }
-    const int n = min(keys.count, p0 + (live - 1) / P.share + ahead + 1);
-    for (int k0 = 0; k0 < n; k0 += C) {
-        __syncthreads();
-        for (int i = tid; i < C * HD; i += 256) {
-            const int c = i / HD, d = i % HD;
-            const bool in = k0 + c < n;
-            ks[c * W + d] = in ? load(P.k, (size_t)(keys.first + k0 + c) * P.k_row + (size_t)head * P.k_head + d) : 0.0f;
-            vs[c * W + d] = in ? load(P.v, (size_t)(keys.first + k0 + c) * P.v_row + (size_t)head * P.v_head + d) : 0.0f;
-        }
-        __syncthreads();
-        float s[4][4] = {};
-        for (int d = 0; d < HD; d += 4) {
-            float4 a[4], b[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                a[i] = *reinterpret_cast<const float4*>(qs + (ty * 4 + i) * W + d);
-                b[i] = *reinterpret_cast<const float4*>(ks + (tx + 16 * i) * W + d);
-            }
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) s[i][j] = fmaf(a[i].x, b[j].x, fmaf(a[i].y, b[j].y, fmaf(a[i].z, b[j].z, fmaf(a[i].w, b[j].w, s[i][j]))));
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            float top = m[i];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                if (k0 + tx + 16 * j > last[i]) s[i][j] = -INFINITY;
-                top = fmaxf(top, s[i][j]);
-            }
-#pragma unroll
-            for (int off = 8; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-            const float base = top == -INFINITY ? 0.0f : top, keep = __expf(m[i] - base);
-            float sum = 0.0f;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const float p = __expf(s[i][j] - base);
-                sum += p;
-                ps[(ty * 4 + i) * (C + 4) + tx + 16 * j] = p;
-            }
-#pragma unroll
-            for (int off = 8; off >= 1; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
-            l[i] = fmaf(l[i], keep, sum);
-            m[i] = top;
-#pragma unroll
-            for (int j = 0; j < HD / 16; ++j) o[i][j] *= keep;
-        }
-        __syncwarp();   // (a row's sixteen threads are in one warp)
-        for (int c = 0; c < C; ++c) {
-            float v[HD / 16];
-#pragma unroll
-            for (int j = 0; j < HD / 16; ++j) v[j] = vs[c * W + tx + 16 * j];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float p = ps[(ty * 4 + i) * (C + 4) + c];
-                if (k0 + c > last[i]) continue;   // (what a row does not see may be infinite)
-#pragma unroll
-                for (int j = 0; j < HD / 16; ++j) o[i][j] = fmaf(p, v[j], o[i][j]);
-            }
-        }
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int r = ty * 4 + i;
-        if (r >= live) continue;
-        const float inv = l[i] == 0.0f ? 0.0f : 1.0f / l[i];
-        const size_t to = ((size_t)(rows.first + p0 + r / P.share) * P.q_heads + head * P.share + r % P.share) * HD;
-#pragma unroll
-        for (int j = 0; j < HD / 16; ++j) {
-            reinterpret_cast<float*>(P.out)[to + tx + 16 * j] = o[i][j] * inv;
-        }
-    }
-}
-
-template <int HD>
-constexpr size_t prompt_tile_smem() { return sizeof(float) * (3 * 64 * (HD + 4) + 64 * 68); }
-
-template <int HD>
-static int launch_prompt_tile(const PromptProblem& P, cudaStream_t s) {
-    static std::atomic<bool> opted[64];
-    constexpr size_t smem = prompt_tile_smem<HD>();
-    OJX_CUDA_TRY(opt_in_smem(reinterpret_cast<const void*>(prompt_tile_kernel<HD>), smem, opted));
-    const int per = 64 / P.share;
-    // as many tiles as the sequences can have: each has at most one that is not full
-    const long long tiles = P.n_rows / per + std::min(P.batch, P.n_rows);
-    if (tiles > 0x7fffffffLL) return OJX_ERR_TOO_LARGE;
-    OJX_CUDA_TRY(launch_chained(prompt_tile_kernel<HD>, dim3((unsigned)tiles, P.kv_heads), 256, smem, s, P));
-    count_launch(1);
-    return OJX_OK;
-}
-
 // ------------------------------------------------------------------------------------ bf16 on the 5th-generation tensor cores
 //
 // A CTA has two tiles of 128 rows of one sequence and KV head (rows are (position, head of the KV head)) and walks the keys 128 at a
@@ -154,7 +30,7 @@ static int launch_prompt_tile(const PromptProblem& P, cudaStream_t s) {
 // the weights back over S as bf16, O += P V with P read from tensor memory.  The two tiles take turns: while the tensor cores are at
 // one, 128 threads are at the other's exponentials.
 //   warps 0..3, 4..7: the rows of the two tiles; warp 8: issues the products; warp 9: the copies of Q, K and V (K and V in a ring);
-//   warps 10, 11: none (registers are moved between groups of four warps: 384 * 168 = 64512 are 2 * 128 * 216 + 128 * 64 and some)
+//   warps 10, 11: none, but for the keys' factors of fp32 (registers are moved between groups of four warps: 384 * 168 = 64512 are 2 * 128 * 216 + 128 * 64 and some)
 // Maxima are left behind: a row's sums are relative to the maximum it had when a score was last more than 2^8 above it, so that
 // O is rescaled a few times per row and not once per step (weights up to 2^8 cost nothing in bf16 or in fp32 sums).
 constexpr int kPaRows = 128, kPaKeys = 128, kPaThreads = 384;
@@ -483,6 +359,461 @@ static int launch_prompt_tc(const PromptProblem& P, cudaStream_t s) {
     return OJX_OK;
 }
 
+// ------------------------------------------------------------------------------------ fp32 on the 5th-generation tensor cores
+//
+// The bf16 kernel's two tiles and turns, on operands that are two fp16 numbers each, x = (hi + lo) / scale: 22 bits, and three products
+// for one (lo hi, hi lo, hi hi).  Every row of Q, K and V has a power of two of its own that brings its largest element to 2^14..2^15:
+//   those of Q and K are taken out of the scores (a factor per row, a factor per key);
+//   those of V go into the weights, y = 2^(x + e - reference) with e the exponent of the key's largest value, so that a weight times its
+//   value is what it is, and the sum of weights takes y * 2^-e.  e stays in -20..100: the values of a smaller row keep fewer bits.
+// Steps are of 48 keys (two tiles' Q take 128 KB, two steps' K and V 96).  The tensor cores cut what they add to a sum, so a step's
+// products with V are summed on their own and join the row's fp32 sums, which are in its thread's registers.
+constexpr int kPpKeys = 48;
+constexpr float kPpRoom = 5.0f;   // y is 2^5 at most when the reference is set, 2^13 later on
+
+template <int HD>
+struct PpSmem {
+    static constexpr int plane = 128 * HD * 2, tile = 2 * plane;              // of Q
+    static constexpr int part = kPpKeys * HD * 2, slot = 2 * part;            // of K or V: two planes
+    static constexpr int slots = HD == 128 ? 4 : 8;
+    static constexpr int ring = 2 * tile, factors = ring + slots * slot;      // [2][3][48]: of K, e, 2^-e
+    static constexpr int bars = factors + 2 * 3 * kPpKeys * 4;
+    static constexpr int bytes = bars + 256 + 1024;
+};
+
+struct PromptSplit {
+    __half* planes[4];      // K hi, K lo, V hi, V lo: [n_keys][kv_heads][head_dim]
+    float2* factors;        // [kv_heads][n_keys]: 1 / scale of the key's row of K, e of its row of V
+};
+
+// A row of K or V per HD / 4 lanes.
+template <int HD>
+__global__ void __launch_bounds__(256) prompt_split_kernel(const __grid_constant__ PromptProblem P, const __grid_constant__ PromptSplit S) {
+    constexpr int L = HD / 4;
+    chain_begin();
+    const long long row = ((long long)blockIdx.x * 256 + threadIdx.x) / L, rows = (long long)P.n_keys * P.kv_heads;
+    const int l = threadIdx.x % L;
+    if (row >= 2 * rows) return;   // (a whole warp's rows or half of them: the shuffles stay within L lanes)
+    const bool values = row >= rows;
+    const long long r = values ? row - rows : row;
+    const long long key = r / P.kv_heads;
+    const int head = (int)(r - key * P.kv_heads);
+    const float4 x = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(values ? P.v : P.k) + key * (values ? P.v_row : P.k_row) +
+                                                      head * (values ? P.v_head : P.k_head) + 4 * l);
+    const float xs[4] = {x.x, x.y, x.z, x.w};
+    unsigned most = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const unsigned b = __float_as_uint(xs[e]) & 0x7fffffffu;
+        if (b < 0x7f800000u) most = max(most, b);
+    }
+    const unsigned lanes = __activemask();
+#pragma unroll
+    for (int off = L / 2; off >= 1; off >>= 1) most = max(most, __shfl_xor_sync(lanes, most, off));
+    float up, down, e = 0.0f;
+    if (values) {
+        const int p = min(max((int)(most >> 23) - 127, -20), 100);
+        up = __uint_as_float((unsigned)(127 + 14 - p) << 23);
+        e = (float)p;
+    } else {
+        gm_scale(most, up, down);
+    }
+    unsigned hi[2], lo[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const float a = xs[2 * i] * up, b = xs[2 * i + 1] * up;
+        const __half2 h = __floats2half2_rn(a, b);
+        hi[i] = *reinterpret_cast<const unsigned*>(&h);
+        lo[i] = gm_pack(a - __low2float(h), b - __high2float(h));
+    }
+    const size_t to = (size_t)r * HD + 4 * l;
+    *reinterpret_cast<uint2*>(S.planes[values ? 2 : 0] + to) = make_uint2(hi[0], hi[1]);
+    *reinterpret_cast<uint2*>(S.planes[values ? 3 : 1] + to) = make_uint2(lo[0], lo[1]);
+    // (a value is 2^(14 - e) times as large, its weight 2^e: 2^14 is left for the end)
+    if (l == 0) {
+        float* f = reinterpret_cast<float*>(S.factors + (size_t)head * P.n_keys + key);
+        f[values] = values ? e : down;
+    }
+}
+
+template <int HD>
+__global__ void __launch_bounds__(kPaThreads, 1) prompt_pair_kernel(const __grid_constant__ PromptProblem P, const __grid_constant__ PromptSplit S,
+                                                                    const __grid_constant__ CUtensorMap k_hi, const __grid_constant__ CUtensorMap k_lo,
+                                                                    const __grid_constant__ CUtensorMap v_hi, const __grid_constant__ CUtensorMap v_lo) {
+    using M = PpSmem<HD>;
+    constexpr int NS = M::slots, C = HD / 64, N = kPpKeys;
+    extern __shared__ unsigned char pa_raw[];
+    unsigned char* smem = pa_raw + ((1024u - (tc_smem(pa_raw) & 1023u)) & 1023u);
+    __shared__ int s_seq, s_part, s_gone, s_odd[2];
+    __shared__ unsigned s_tmem;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const unsigned base = tc_smem(smem), bars = base + M::bars;
+    const unsigned full = bars, empty = bars + 8 * NS, q_full = empty + 8 * NS, s_full = q_full + 16, p_full = s_full + 16, o_full = p_full + 16,
+                   checked = o_full + 16, f_full = checked + 16, f_empty = f_full + 16, ended = f_empty + 16, gone = tc_smem(&s_gone);
+    const int head = blockIdx.x % P.kv_heads, per = kPaRows / P.share;
+    if (tid == 0) {
+        for (int i = 0; i < NS; ++i) { tc_bar_init(full + 8 * i, 1); tc_bar_init(empty + 8 * i, 1); }
+        for (int i = 0; i < 2; ++i) {
+            tc_bar_init(q_full + 8 * i, 4);
+            tc_bar_init(s_full + 8 * i, 1);
+            tc_bar_init(p_full + 8 * i, 4);
+            tc_bar_init(o_full + 8 * i, 1);
+            tc_bar_init(checked + 8 * i, 4);
+            tc_bar_init(f_full + 8 * i, 32);
+            tc_bar_init(f_empty + 8 * i, 8);
+            s_odd[i] = 0;
+        }
+        tc_bar_init(ended, 1);
+        s_gone = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    chain_begin();
+    if (warp == 0) {
+        int seq = -1, part = 0;   // (the last parts first)
+        const bool in = packed_part(P.batch, (int)(gridDim.x / P.kv_heads) - 1 - (int)blockIdx.x / P.kv_heads,
+                                    [&](int b) { return (packed_range(P.ends, b, P.n_rows).count + 2 * per - 1) / (2 * per); }, seq, part);
+        if (lane == 0) { s_seq = in ? seq : -1; s_part = part; }
+    }
+    __syncthreads();
+    if (s_seq < 0) return;
+    if (warp == 8) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(tc_smem(&s_tmem)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_before();
+    __syncthreads();
+    tc_after();
+    const unsigned tmem = s_tmem;   // S and then the weights of tile i at 64 i (hi 24 columns, lo 24), a step's O at 256 + 128 i
+    const PackedRange rows = packed_range(P.ends, s_seq, P.n_rows), keys = packed_range(P.key_ends, s_seq, P.n_keys);
+    const int ahead = keys.count - rows.count;
+    int pos[2], live[2], steps[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        pos[i] = (s_part * 2 + i) * per;
+        live[i] = max(0, min(per, rows.count - pos[i]));
+        steps[i] = live[i] > 0 ? max(0, pos[i] + live[i] + ahead + N - 1) / N : 0;
+    }
+    const int n = max(steps[0], steps[1]);
+    bool ok = true;
+
+    if (warp >= 8) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+        if (warp == 9 && lane == 0) {
+            int s = 0;
+            for (; s < 2 * n; ++s) {   // K of step 0, V of step 0, K of step 1, ...
+                const int slot = s % NS;
+                if (s >= NS && !(ok = bar_wait(empty + 8 * slot, (s / NS - 1) & 1, gone))) break;
+                tc_bar_expect(full + 8 * slot, M::slot);
+                for (int c = 0; c < C; ++c)
+                    for (int p = 0; p < 2; ++p)
+                        tc_load3(base + M::ring + slot * M::slot + p * M::part + c * (M::part / C), s & 1 ? (p ? &v_lo : &v_hi) : (p ? &k_lo : &k_hi), 64 * c,
+                                 head, keys.first + (s >> 1) * N, full + 8 * slot);
+            }
+            if (!ok)   // nothing may land after the CTA has left
+                for (int u = max(0, s - NS); u < s; ++u) bar_wait(full + 8 * (u % NS), (u / NS) & 1);
+        }
+        if (warp == 10) {
+            for (int j = 0; j < n; ++j) {
+                if (j >= 2 && !(ok = bar_wait(f_empty + 8 * (j & 1), (j / 2 - 1) & 1, gone))) break;
+                float* f = reinterpret_cast<float*>(smem + M::factors) + (j & 1) * 3 * N;
+                for (int c = lane; c < N; c += 32) {
+                    const int key = j * N + c;
+                    const float2 x = key < keys.count ? S.factors[(size_t)head * P.n_keys + keys.first + key] : make_float2(0.0f, 0.0f);
+                    f[c] = x.x;
+                    f[N + c] = x.y;
+                    f[2 * N + c] = __uint_as_float((unsigned)(127 - (int)x.y) << 23);
+                }
+                tc_bar_arrive(f_full + 8 * (j & 1));
+            }
+        }
+        if (warp == 8 && lane == 0) {
+            constexpr unsigned iq = tc_idesc<false, false>(N), iv = tc_idesc<false, true>(HD);
+            auto slot_at = [&](int s) { return base + M::ring + (s % NS) * M::slot; };
+            auto wait_slot = [&](int s) { return bar_wait(full + 8 * (s % NS), (s / NS) & 1, gone); };
+            auto scores = [&](int i, int j) {
+#pragma unroll
+                for (int p = 0; p < 3; ++p) {   // lo hi, hi lo, hi hi
+                    const unsigned a = base + i * M::tile + (p == 0) * M::plane, b = slot_at(2 * j) + (p == 1) * M::part;
+#pragma unroll
+                    for (int k = 0; k < HD / 16; ++k)
+                        tc_mma(tmem + i * 64, tc_desc(a + (k / 4) * (M::plane / C) + (k % 4) * 32), tc_desc(b + (k / 4) * (M::part / C) + (k % 4) * 32), iq, p > 0 || k > 0);
+                }
+                tc_commit(s_full + 8 * i);
+            };
+            if (n > 0) ok = wait_slot(0);
+            for (int i = 0; i < 2 && ok; ++i)
+                if (steps[i]) {
+                    ok = bar_wait(q_full + 8 * i, 0, gone);
+                    tc_after();
+                    if (ok) scores(i, 0);
+                }
+            if (n > 0 && ok) tc_commit(empty);
+            for (int j = 0; j < n && ok; ++j) {
+                ok = wait_slot(2 * j + 1);
+                for (int i = 0; i < 2 && ok; ++i) {
+                    if (j >= steps[i]) continue;
+                    if (!(ok = bar_wait(p_full + 8 * i, j & 1, gone))) break;
+                    tc_after();
+                    if (*reinterpret_cast<volatile int*>(&s_odd[i]) != j + 1) {
+#pragma unroll
+                        for (int p = 0; p < 3; ++p) {
+                            const unsigned a = tmem + i * 64 + (p == 0) * (N / 2), b = slot_at(2 * j + 1) + (p == 1) * M::part;
+#pragma unroll
+                            for (int k = 0; k < N / 16; ++k) tc_mma_ts(tmem + 256 + i * 128, a + k * 8, tc_desc(b + k * 2048, M::part / C), iv, p > 0 || k > 0);
+                        }
+                    }
+                    if (j + 1 < steps[i]) {
+                        if (!(ok = wait_slot(2 * j + 2))) break;
+                        scores(i, j + 1);   // (in order: its commit says that O is there, too)
+                    } else {
+                        tc_commit(o_full + 8 * i);
+                    }
+                }
+                if (!ok) break;
+                tc_commit(empty + 8 * ((2 * j + 1) % NS));
+                if (j + 1 < n) tc_commit(empty + 8 * ((2 * j + 2) % NS));
+            }
+            if (!ok) {
+                tc_commit(ended);
+                bar_wait(ended, 0);
+            }
+        }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+        const int i = warp >> 2, row = tid & 127;
+        const int at = min(row, max(live[i] * P.share - 1, 0)), last = pos[i] + at / P.share + ahead;
+        const bool out = row < live[i] * P.share;
+        const unsigned lanes = (unsigned)((warp & 3) * 32) << 16, st = tmem + i * 64 + lanes, ot = tmem + 256 + i * 128 + lanes;
+        const size_t where = out ? (size_t)(rows.first + pos[i] + row / P.share) : 0;
+        const int q_head = head * P.share + (out ? row % P.share : 0);
+        int checks = 0;
+        auto wait = [&](unsigned bar, unsigned parity) { return (bool)__all_sync(0xffffffffu, bar_wait(bar, parity, gone)); };
+        float unscale = 0.0f;
+        if (steps[i]) {   // the row of Q
+            const float* q = reinterpret_cast<const float*>(P.q) + where * P.q_row + (size_t)q_head * P.q_head;
+            unsigned most = 0;
+            for (int d = 0; d < HD; d += 4) {
+                const float4 x = out ? *reinterpret_cast<const float4*>(q + d) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                most = max(max(most, __float_as_uint(x.x) & 0x7fffffffu), max(__float_as_uint(x.y) & 0x7fffffffu, max(__float_as_uint(x.z) & 0x7fffffffu, __float_as_uint(x.w) & 0x7fffffffu)));
+            }
+            float up, down;
+            gm_scale(most, up, down);
+            unscale = down * (P.scale * 1.4426950408889634f);
+            unsigned char* to = smem + i * M::tile + row * 128;
+            for (int d = 0; d < HD; d += 8) {
+                const float4 x = out ? *reinterpret_cast<const float4*>(q + d) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                const float4 y = out ? *reinterpret_cast<const float4*>(q + d + 4) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                const float xs[8] = {x.x * up, x.y * up, x.z * up, x.w * up, y.x * up, y.y * up, y.z * up, y.w * up};
+                unsigned hi[4], lo[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const __half2 h = __floats2half2_rn(xs[2 * e], xs[2 * e + 1]);
+                    hi[e] = *reinterpret_cast<const unsigned*>(&h);
+                    lo[e] = gm_pack(xs[2 * e] - __low2float(h), xs[2 * e + 1] - __high2float(h));
+                }
+                const int off = (d / 64) * (M::plane / C) + (((d % 64) / 8 ^ (row & 7)) << 4);
+                *reinterpret_cast<uint4*>(to + off) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                *reinterpret_cast<uint4*>(to + M::plane + off) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) tc_bar_arrive(q_full + 8 * i);
+        }
+        float top = -INFINITY, sum[2] = {0.0f, 0.0f}, o[HD];
+#pragma unroll
+        for (int d = 0; d < HD; ++d) o[d] = 0.0f;
+        bool parted = false;   // a step's O is in tensor memory
+        auto join = [&]() {
+#pragma unroll
+            for (int c = 0; c < HD; c += 32) {
+                unsigned x[32];
+                tc_ld32(ot + c, x);
+                tc_wait_ld();
+                tc_pin32(x);
+#pragma unroll
+                for (int e = 0; e < 32; ++e) o[c + e] += __uint_as_float(x[e]);
+            }
+        };
+        for (int j = 0; j < n; ++j) {
+            if (j >= steps[i]) {   // (the other tile has more steps: the keys' factors have to go on)
+                if (!(ok = wait(f_full + 8 * (j & 1), (j / 2) & 1))) break;
+                __syncwarp();
+                if (lane == 0) tc_bar_arrive(f_empty + 8 * (j & 1));
+                continue;
+            }
+            if (!(ok = wait(s_full + 8 * i, j & 1))) break;
+            tc_after();
+            if (parted) join();
+            unsigned s[N];
+            tc_ld32(st, s);
+            tc_ld16(st + 32, s + 32);
+            if (!(ok = wait(f_full + 8 * (j & 1), (j / 2) & 1))) break;
+            tc_wait_ld();
+            tc_pin32(s);
+            tc_pin16(s + 32);
+            const float* f = reinterpret_cast<const float*>(smem + M::factors) + (j & 1) * 3 * N;
+            const bool masked = (j + 1) * N - 1 > pos[i] + ahead;
+            const int see = last - j * N;
+            float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+            for (int e = 0; e < N; e += 4) {
+                const float4 kf = *reinterpret_cast<const float4*>(f + e), ex = *reinterpret_cast<const float4*>(f + N + e);
+                const float kfs[4] = {kf.x, kf.y, kf.z, kf.w}, exs[4] = {ex.x, ex.y, ex.z, ex.w};
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    float x = fmaf(__uint_as_float(s[e + u]) * kfs[u], unscale, exs[u]);
+                    if (masked) x = e + u > see ? -INFINITY : x;
+                    s[e + u] = __float_as_uint(x);
+                    m[u] = fmaxf(m[u], x);
+                }
+            }
+            const float now = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])) - kPpRoom;
+            const bool up = now > top + kPaSlack;
+            if (j == 0) {
+                top = now;
+            } else if (__any_sync(0xffffffffu, up)) {
+                const float by = up ? exp2f(top - now) : 1.0f;
+                top = up ? now : top;
+                sum[0] *= by;
+                sum[1] *= by;
+#pragma unroll
+                for (int d = 0; d < HD; ++d) o[d] *= by;
+            }
+            const float off = top == -INFINITY ? 0.0f : top;
+            unsigned w[N / 2];   // low parts; the high ones take the scores' place
+#pragma unroll
+            for (int e = 0; e < N; e += 4) {
+                const float4 vf = *reinterpret_cast<const float4*>(f + 2 * N + e);
+                const float vfs[4] = {vf.x, vf.y, vf.z, vf.w};
+                float y[4];
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    y[u] = __uint_as_float(s[e + u]) - off;
+                    asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(y[u]));
+                    sum[u & 1] = fmaf(y[u], vfs[u], sum[u & 1]);
+                }
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const __half2 h = __floats2half2_rn(y[2 * u], y[2 * u + 1]);
+                    s[e / 2 + u] = *reinterpret_cast<const unsigned*>(&h);
+                    w[e / 2 + u] = gm_pack(y[2 * u] - __low2float(h), y[2 * u + 1] - __high2float(h));
+                }
+            }
+            tc_st16(st, s);
+            tc_st8(st + 16, s + 16);
+            tc_st16(st + N / 2, w);
+            tc_st8(st + N / 2 + 16, w + 16);
+            parted = true;
+            if (masked) {   // (as in the bf16 kernel: values that are not finite among those that are not seen)
+                if (!(ok = wait(full + 8 * ((2 * j + 1) % NS), ((2 * j + 1) / NS) & 1))) break;
+                const unsigned char* v = smem + M::ring + ((2 * j + 1) % NS) * M::slot;
+                unsigned odd = 0;
+                for (int e = row; e < M::part / 16; e += 128) {
+                    const uint4 x = reinterpret_cast<const uint4*>(v)[e];
+                    odd |= (((x.x & 0x7c007c00u) + 0x04000400u) | ((x.y & 0x7c007c00u) + 0x04000400u) | ((x.z & 0x7c007c00u) + 0x04000400u) |
+                            ((x.w & 0x7c007c00u) + 0x04000400u)) & 0x80008000u;
+                }
+                odd = __reduce_or_sync(0xffffffffu, odd);
+                if (lane == 0) {
+                    if (odd) *reinterpret_cast<volatile int*>(&s_odd[i]) = j + 1;
+                    tc_bar_arrive(checked + 8 * i);
+                }
+                if (!(ok = wait(checked + 8 * i, checks++ & 1))) break;
+                if (*reinterpret_cast<volatile int*>(&s_odd[i]) == j + 1) {
+                    tc_wait_st();
+                    parted = false;
+                    const int end = min(see, N - 1);
+#pragma unroll
+                    for (int c = 0; c < HD; c += 32)
+                        for (int k = 0; k < N; ++k) {
+                            unsigned hi = tc_ld1(st + (k >> 1)), lo = tc_ld1(st + N / 2 + (k >> 1));
+                            tc_wait_ld();
+                            asm volatile("" : "+r"(hi), "+r"(lo));
+                            if (k <= end) {
+                                const __half2 a = *reinterpret_cast<const __half2*>(&hi), b = *reinterpret_cast<const __half2*>(&lo);
+                                const float y = k & 1 ? __high2float(a) + __high2float(b) : __low2float(a) + __low2float(b);
+                                const unsigned char* line = v + (c / 64) * (M::part / C) + k * 128;
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) {
+                                    const int piece = (((c % 64) / 8 + e) ^ (k & 7)) * 16;
+                                    const uint4 xh = *reinterpret_cast<const uint4*>(line + piece), xl = *reinterpret_cast<const uint4*>(line + M::part + piece);
+                                    const unsigned hs[4] = {xh.x, xh.y, xh.z, xh.w}, ls[4] = {xl.x, xl.y, xl.z, xl.w};
+#pragma unroll
+                                    for (int h = 0; h < 4; ++h) {
+                                        const __half2 vh = *reinterpret_cast<const __half2*>(&hs[h]), vl = *reinterpret_cast<const __half2*>(&ls[h]);
+                                        o[c + 8 * e + 2 * h] = fmaf(y, __low2float(vh) + __low2float(vl), o[c + 8 * e + 2 * h]);
+                                        o[c + 8 * e + 2 * h + 1] = fmaf(y, __high2float(vh) + __high2float(vl), o[c + 8 * e + 2 * h + 1]);
+                                    }
+                                }
+                            }
+                            __syncwarp();
+                        }
+                }
+            }
+            tc_wait_st();
+            tc_before();
+            __syncwarp();
+            if (lane == 0) {
+                tc_bar_arrive(f_empty + 8 * (j & 1));
+                tc_bar_arrive(p_full + 8 * i);
+            }
+        }
+        if (ok && live[i] > 0) {
+            if (steps[i]) {
+                ok = wait(o_full + 8 * i, 0);
+                tc_after();
+                if (ok && parted) join();
+            }
+            const float total = sum[0] + sum[1], inv = total == 0.0f ? 0.0f : 1.0f / (total * 16384.0f);   // (values are 2^14 times as large as their exponents say)
+            if (ok && out) {
+                float4* to = reinterpret_cast<float4*>(reinterpret_cast<float*>(P.out) + (where * P.q_heads + q_head) * HD);
+#pragma unroll
+                for (int d = 0; d < HD; d += 4) to[d / 4] = make_float4(o[d] * inv, o[d + 1] * inv, o[d + 2] * inv, o[d + 3] * inv);
+            }
+        }
+    }
+    if (!ok) atomicExch(&g_prompt_error, 1);
+    tc_before();
+    __syncthreads();
+    if (warp == 8) {
+        tc_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+    }
+}
+
+// Bytes of the planes and factors of K and V.
+static size_t prompt_split_plane(int n_keys, int kv_heads, int head_dim) { return ((size_t)std::max(n_keys, 1) * kv_heads * head_dim * 2 + 255) / 256 * 256; }
+
+template <int HD>
+static int launch_prompt_pair(const PromptProblem& P, void* workspace, cudaStream_t s) {
+    static std::atomic<bool> opted[64];
+    constexpr int smem = PpSmem<HD>::bytes;
+    OJX_CUDA_TRY(opt_in_smem(reinterpret_cast<const void*>(prompt_pair_kernel<HD>), smem, opted));
+    const int per = kPaRows / P.share;
+    const long long parts = P.n_rows / (2 * per) + std::min(P.batch, P.n_rows);
+    const long long split = ((long long)P.n_keys * P.kv_heads * 2 * (HD / 4) + 255) / 256;
+    if (parts * P.kv_heads > 0x7fffffffLL || split > 0x7fffffffLL) return OJX_ERR_TOO_LARGE;
+    PromptSplit S{};
+    const size_t plane = prompt_split_plane(P.n_keys, P.kv_heads, HD);
+    char* at = static_cast<char*>(workspace);
+    CUtensorMap maps[4];
+    for (int i = 0; i < 4; ++i, at += plane) {
+        S.planes[i] = reinterpret_cast<__half*>(at);
+        if (!tc_map3(&maps[i], false, at, HD, P.kv_heads, std::max(P.n_keys, 1), HD, (unsigned long long)P.kv_heads * HD, 64, 1, kPpKeys)) {
+            set_last_error_msg("prompt attention: no tensor map");
+            return OJX_ERR_CUDA;
+        }
+    }
+    S.factors = reinterpret_cast<float2*>(at);
+    if (split) {
+        OJX_CUDA_TRY(launch_chained(prompt_split_kernel<HD>, dim3((unsigned)split), 256, 0, s, P, S));
+        count_launch(1);
+    }
+    OJX_CUDA_TRY(launch_chained(prompt_pair_kernel<HD>, dim3((unsigned)(parts * P.kv_heads)), kPaThreads, smem, s, P, S, maps[0], maps[1], maps[2], maps[3]));
+    count_launch(1);
+    return OJX_OK;
+}
+
 int take_prompt_error(int* out) {
     int v = 0, zero = 0;
     OJX_CUDA_TRY(cudaMemcpyFromSymbol(&v, g_prompt_error, sizeof(int)));
@@ -495,16 +826,29 @@ int take_prompt_error(int* out) {
 
 using namespace ojx;
 
-extern "C" int ojasx_b200_prompt_attention(const void* d_q, long long q_row, long long q_head, const void* d_k, long long k_row,
-                                           long long k_head, const void* d_v, long long v_row, long long v_head, void* d_out,
-                                           const int* d_ends, const int* d_key_ends, int batch, int n_rows, int n_keys, int q_heads,
-                                           int kv_heads, int head_dim, float scale, int io_dtype, void* stream) {
-    if (!d_q || (n_keys > 0 && (!d_k || !d_v)) || !d_out || !d_ends || !d_key_ends || batch <= 0 || n_rows < 0 || n_keys < 0 || kv_heads <= 0 || q_heads <= 0 ||
-        q_heads % kv_heads)
+extern "C" {
+
+size_t ojasx_b200_prompt_workspace(int n_keys, int kv_heads, int head_dim, int io_dtype) {
+    if (io_dtype != OJX_F32 || n_keys < 0 || kv_heads <= 0 || head_dim <= 0) return 0;
+    return 4 * prompt_split_plane(n_keys, kv_heads, head_dim) + (size_t)n_keys * kv_heads * sizeof(float2);
+}
+
+int ojasx_b200_prompt_attention(const void* d_q, long long q_row, long long q_head, const void* d_k, long long k_row, long long k_head,
+                                const void* d_v, long long v_row, long long v_head, void* d_out, const int* d_ends, const int* d_key_ends,
+                                int batch, int n_rows, int n_keys, int q_heads, int kv_heads, int head_dim, float scale, int io_dtype,
+                                void* workspace, size_t workspace_bytes, void* stream) {
+    if (!d_q || (n_keys > 0 && (!d_k || !d_v)) || !d_out || !d_ends || !d_key_ends || batch <= 0 || n_rows < 0 || n_keys < 0 || kv_heads <= 0 ||
+        q_heads <= 0 || q_heads % kv_heads)
         return OJX_ERR_ARG;
     if (io_dtype != OJX_F32 && io_dtype != OJX_BF16) return OJX_ERR_ARG;
+    const int unit = io_dtype == OJX_F32 ? 4 : 8;   // elements of 16 bytes
+    for (const long long stride : {q_row, q_head, k_row, k_head, v_row, v_head})
+        if (stride < 0 || stride % unit) return OJX_ERR_ARG;
+    for (const void* p : {d_q, d_k, d_v, static_cast<const void*>(d_out)})
+        if (reinterpret_cast<uintptr_t>(p) & 15) return OJX_ERR_ARG;
     if ((head_dim != 64 && head_dim != 128) || q_heads / kv_heads > 64) return OJX_ERR_UNSUPPORTED;
-    if (kv_heads > 65535) return OJX_ERR_TOO_LARGE;
+    const size_t need = ojasx_b200_prompt_workspace(n_keys, kv_heads, head_dim, io_dtype);
+    if (need && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255) || workspace_bytes < need)) return OJX_ERR_ARG;
     if (n_rows == 0) return OJX_OK;
     PromptProblem P{};
     P.q = d_q; P.k = d_k; P.v = d_v; P.out = d_out;
@@ -514,5 +858,7 @@ extern "C" int ojasx_b200_prompt_attention(const void* d_q, long long q_row, lon
     P.scale = scale > 0.0f ? scale : 1.0f / sqrtf((float)head_dim);
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (io_dtype == OJX_BF16) return head_dim == 64 ? launch_prompt_tc<64>(P, s) : launch_prompt_tc<128>(P, s);
-    return head_dim == 64 ? launch_prompt_tile<64>(P, s) : launch_prompt_tile<128>(P, s);
+    return head_dim == 64 ? launch_prompt_pair<64>(P, workspace, s) : launch_prompt_pair<128>(P, workspace, s);
 }
+
+}  // extern "C"

@@ -460,7 +460,7 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
     """``t`` itself where its heads lie behind one another in rows on 16-byte boundaries (a view into a fused projection does), a copy
     else."""
     unit = 16 // t.element_size()
-    fits = t.stride(2) == 1 and t.stride(1) == t.shape[2] and t.stride(0) % unit == 0 and t.stride(0) >= 0 and t.data_ptr() % 16 == 0
+    fits = t.stride(2) == 1 and t.stride(1) == t.shape[2] and t.stride(0) % unit == 0 and t.stride(0) >= t.shape[1] * t.shape[2] and t.data_ptr() % 16 == 0
     if t.numel() == 0 or fits:
         return t
     return t.clone(memory_format=torch.contiguous_format)
@@ -665,9 +665,11 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     o = _out(out, q)
     q, k, v = _rows(q), _rows(k), _rows(v)
     if T and B:
+        size = lib().ojasx_b200_prompt_workspace(k.shape[0], k.shape[1], hd, _dtype_code(q))
+        ws = torch.empty(size, device=q.device, dtype=torch.uint8) if size else None
         with torch.cuda.device(q.device):
             check(lib().ojasx_b200_prompt_attention(q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(),
                                                     v.stride(0), v.stride(1), o.data_ptr(), ends.data_ptr(), key_ends.data_ptr(), B, T, k.shape[0],
-                                                    Hq, k.shape[1], hd, float(scale), _dtype_code(q), _stream_ptr(q.device)),
-                  "ojasx_b200_prompt_attention")
+                                                    Hq, k.shape[1], hd, float(scale), _dtype_code(q), None if ws is None else ws.data_ptr(), size,
+                                                    _stream_ptr(q.device)), "ojasx_b200_prompt_attention")
     return o

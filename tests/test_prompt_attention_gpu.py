@@ -40,9 +40,10 @@ def _check(q, k, v, lengths, key_lengths, got, scale=None):
 def test_c_entry_refuses_missing_and_unfit_arguments():
     one = 4096
     call = lambda **kw: lib().ojasx_b200_prompt_attention(*{**dict(q=one, qr=128, qh=64, k=one, kr=64, kh=64, v=one, vr=64, vh=64, o=one, e=one, ke=one,
-           b=1, n=1, m=1, hq=2, hkv=1, hd=64, sc=-1.0, io=0, st=None), **kw}.values())  # noqa: E731
+           b=1, n=1, m=1, hq=2, hkv=1, hd=64, sc=-1.0, io=0, ws=one, size=1 << 20, st=None), **kw}.values())  # noqa: E731
     for bad in (dict(q=None), dict(k=None), dict(v=None), dict(o=None), dict(e=None), dict(ke=None), dict(b=0), dict(n=-1), dict(m=-1), dict(hq=0),
-                dict(hkv=0), dict(hq=3, hkv=2), dict(io=2)):
+                dict(hkv=0), dict(hq=3, hkv=2), dict(io=2), dict(ws=None), dict(size=100), dict(ws=one + 16), dict(q=one + 8), dict(o=one + 4), dict(kr=66),
+                dict(vh=-64), dict(io=1, qh=68)):
         assert call(**bad) == -1, bad
     for bad in (dict(hd=32), dict(hd=256), dict(hq=65)):
         assert call(**bad) == -4, bad

@@ -55,7 +55,7 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_tc_kernel(const __grid_c
     unsigned char* smem = pa_raw + ((1024u - (tc_smem(pa_raw) & 1023u)) & 1023u);
     __shared__ int s_seq, s_part, s_gone, s_odd[2];
     __shared__ unsigned s_tmem;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;   // (the same for a warp, as the compiler sees)
     const unsigned base = tc_smem(smem), bars = base + M::bars;
     const unsigned full = bars, empty = bars + 8 * NS, q_full = empty + 8 * NS, s_full = q_full + 16, p_full = s_full + 16, o_full = p_full + 16,
                    checked = o_full + 16, ended = checked + 16, gone = tc_smem(&s_gone);
@@ -91,7 +91,7 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_tc_kernel(const __grid_c
     tc_before();
     __syncthreads();
     tc_after();
-    const unsigned tmem = s_tmem;
+    const unsigned tmem = __shfl_sync(0xffffffffu, s_tmem, 0);
     const PackedRange rows = packed_range(P.ends, s_seq, P.n_rows), keys = packed_range(P.key_ends, s_seq, P.n_keys);
     const int ahead = keys.count - rows.count;
     int pos[2], live[2], steps[2];   // first position, positions and steps of the tiles
@@ -103,6 +103,7 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_tc_kernel(const __grid_c
     }
     const int n = max(steps[0], steps[1]);
     bool ok = true;
+    auto wait = [&](unsigned bar, unsigned parity) { return (bool)__all_sync(0xffffffffu, bar_wait(bar, parity, gone)); };   // of a warp
 
     if (warp >= 8) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
@@ -125,46 +126,49 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_tc_kernel(const __grid_c
                 for (int i = 0; i < 2; ++i) if (steps[i]) bar_wait(q_full + 8 * i, 0);
             }
         }
-        if (warp == 8 && lane == 0) {
+        if (warp == 8) {
+            const unsigned lead = tc_lead();
             constexpr unsigned iq = tc_idesc<true, false>(kPaKeys), iv = tc_idesc<true, true>(HD);
             auto slot_at = [&](int s) { return base + M::ring + (s % NS) * M::tile; };
-            auto wait_slot = [&](int s) { return bar_wait(full + 8 * (s % NS), (s / NS) & 1, gone); };
+            auto wait_slot = [&](int s) { return wait(full + 8 * (s % NS), (s / NS) & 1); };
             auto scores = [&](int i, int j) {
-                const unsigned a = base + i * M::tile, b = slot_at(2 * j);
+                const unsigned long long a = tc_desc(base + i * M::tile), b = tc_desc(slot_at(2 * j));
 #pragma unroll
-                for (int k = 0; k < HD / 16; ++k)
-                    tc_mma(tmem + i * 128, tc_desc(a + (k / 4) * (M::tile / C) + (k % 4) * 32), tc_desc(b + (k / 4) * (M::tile / C) + (k % 4) * 32), iq, k > 0);
-                tc_commit(s_full + 8 * i);
+                for (int k = 0; k < HD / 16; ++k) {
+                    const int off = (k / 4) * (M::tile / C) + (k % 4) * 32;
+                    tc_mma(lead, tmem + i * 128, tc_at(a, off), tc_at(b, off), iq, k > 0);
+                }
+                tc_commit(lead, s_full + 8 * i);
             };
             if (n > 0) ok = wait_slot(0);
             for (int i = 0; i < 2 && ok; ++i)
                 if (steps[i]) {
-                    ok = bar_wait(q_full + 8 * i, 0, gone);
+                    ok = wait(q_full + 8 * i, 0);
                     if (ok) scores(i, 0);
                 }
-            if (n > 0 && ok) tc_commit(empty);
+            if (n > 0 && ok) tc_commit(lead, empty);
             for (int j = 0; j < n && ok; ++j) {
                 if (j + 1 < n) ok = wait_slot(2 * j + 2);
                 if (ok) ok = wait_slot(2 * j + 1);
                 for (int i = 0; i < 2 && ok; ++i) {
                     if (j >= steps[i]) continue;
-                    if (!(ok = bar_wait(p_full + 8 * i, j & 1, gone))) break;
+                    if (!(ok = wait(p_full + 8 * i, j & 1))) break;
                     tc_after();
                     if (*reinterpret_cast<volatile int*>(&s_odd[i]) != j + 1) {   // (else the rows have added their products themselves)
-                        const unsigned b = slot_at(2 * j + 1);
+                        const unsigned long long b = tc_desc(slot_at(2 * j + 1), M::tile / C);
 #pragma unroll
                         for (int k = 0; k < kPaKeys / 16; ++k)
-                            tc_mma_ts(tmem + 256 + i * 128, tmem + i * 128 + k * 8, tc_desc(b + k * 2048, M::tile / C), iv, j > 0 || k > 0);
+                            tc_mma_ts(lead, tmem + 256 + i * 128, tmem + i * 128 + k * 8, tc_at(b, k * 2048), iv, j > 0 || k > 0);
                     }
                     if (j + 1 < steps[i]) scores(i, j + 1);   // (in order: its commit says that O is up to date, too)
-                    else tc_commit(o_full + 8 * i);
+                    else tc_commit(lead, o_full + 8 * i);
                 }
                 if (!ok) break;
-                tc_commit(empty + 8 * ((2 * j + 1) % NS));
-                if (j + 1 < n) tc_commit(empty + 8 * ((2 * j + 2) % NS));
+                tc_commit(lead, empty + 8 * ((2 * j + 1) % NS));
+                if (j + 1 < n) tc_commit(lead, empty + 8 * ((2 * j + 2) % NS));
             }
             if (!ok) {
-                tc_commit(ended);
+                tc_commit(lead, ended);
                 bar_wait(ended, 0);
             }
         }
@@ -176,7 +180,6 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_tc_kernel(const __grid_c
         const float scale = P.scale * 1.4426950408889634f;
         float top = 0.0f, sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
         int checks = 0;
-        auto wait = [&](unsigned bar, unsigned parity) { return (bool)__all_sync(0xffffffffu, bar_wait(bar, parity, gone)); };
         auto rescale = [&](float by) {   // the warp's rows of O
             for (int c = 0; c < HD; c += 32) {
                 unsigned o[32];
@@ -446,7 +449,7 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_pair_kernel(const __grid
     unsigned char* smem = pa_raw + ((1024u - (tc_smem(pa_raw) & 1023u)) & 1023u);
     __shared__ int s_seq, s_part, s_gone, s_odd[2];
     __shared__ unsigned s_tmem;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;   // (the same for a warp, as the compiler sees)
     const unsigned base = tc_smem(smem), bars = base + M::bars;
     const unsigned full = bars, empty = bars + 8 * NS, q_full = empty + 8 * NS, s_full = q_full + 16, p_full = s_full + 16, o_full = p_full + 16,
                    checked = o_full + 16, f_full = checked + 16, f_empty = f_full + 16, ended = f_empty + 16, gone = tc_smem(&s_gone);
@@ -483,7 +486,7 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_pair_kernel(const __grid
     tc_before();
     __syncthreads();
     tc_after();
-    const unsigned tmem = s_tmem;   // S and then the weights of tile i at 64 i (hi 24 columns, lo 24), a step's O at 256 + 128 i
+    const unsigned tmem = __shfl_sync(0xffffffffu, s_tmem, 0);   // S and then the weights of tile i at 64 i (hi 24 columns, lo 24), a step's O at 256 + 128 i
     const PackedRange rows = packed_range(P.ends, s_seq, P.n_rows), keys = packed_range(P.key_ends, s_seq, P.n_keys);
     const int ahead = keys.count - rows.count;
     int pos[2], live[2], steps[2];
@@ -495,6 +498,7 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_pair_kernel(const __grid
     }
     const int n = max(steps[0], steps[1]);
     bool ok = true;
+    auto wait = [&](unsigned bar, unsigned parity) { return (bool)__all_sync(0xffffffffu, bar_wait(bar, parity, gone)); };   // of a warp
 
     if (warp >= 8) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
@@ -526,55 +530,57 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_pair_kernel(const __grid
                 tc_bar_arrive(f_full + 8 * (j & 1));
             }
         }
-        if (warp == 8 && lane == 0) {
+        if (warp == 8) {
+            const unsigned lead = tc_lead();
             constexpr unsigned iq = tc_idesc<false, false>(N), iv = tc_idesc<false, true>(HD);
             auto slot_at = [&](int s) { return base + M::ring + (s % NS) * M::slot; };
-            auto wait_slot = [&](int s) { return bar_wait(full + 8 * (s % NS), (s / NS) & 1, gone); };
+            auto wait_slot = [&](int s) { return wait(full + 8 * (s % NS), (s / NS) & 1); };
             auto scores = [&](int i, int j) {
+                const unsigned long long a = tc_desc(base + i * M::tile), b = tc_desc(slot_at(2 * j));
 #pragma unroll
                 for (int p = 0; p < 3; ++p) {   // lo hi, hi lo, hi hi
-                    const unsigned a = base + i * M::tile + (p == 0) * M::plane, b = slot_at(2 * j) + (p == 1) * M::part;
 #pragma unroll
                     for (int k = 0; k < HD / 16; ++k)
-                        tc_mma(tmem + i * 64, tc_desc(a + (k / 4) * (M::plane / C) + (k % 4) * 32), tc_desc(b + (k / 4) * (M::part / C) + (k % 4) * 32), iq, p > 0 || k > 0);
+                        tc_mma(lead, tmem + i * 64, tc_at(a, (p == 0) * M::plane + (k / 4) * (M::plane / C) + (k % 4) * 32),
+                               tc_at(b, (p == 1) * M::part + (k / 4) * (M::part / C) + (k % 4) * 32), iq, p > 0 || k > 0);
                 }
-                tc_commit(s_full + 8 * i);
+                tc_commit(lead, s_full + 8 * i);
             };
             if (n > 0) ok = wait_slot(0);
             for (int i = 0; i < 2 && ok; ++i)
                 if (steps[i]) {
-                    ok = bar_wait(q_full + 8 * i, 0, gone);
+                    ok = wait(q_full + 8 * i, 0);
                     tc_after();
                     if (ok) scores(i, 0);
                 }
-            if (n > 0 && ok) tc_commit(empty);
+            if (n > 0 && ok) tc_commit(lead, empty);
             for (int j = 0; j < n && ok; ++j) {
                 ok = wait_slot(2 * j + 1);
                 for (int i = 0; i < 2 && ok; ++i) {
                     if (j >= steps[i]) continue;
-                    if (!(ok = bar_wait(p_full + 8 * i, j & 1, gone))) break;
+                    if (!(ok = wait(p_full + 8 * i, j & 1))) break;
                     tc_after();
                     if (*reinterpret_cast<volatile int*>(&s_odd[i]) != j + 1) {
+                        const unsigned long long b = tc_desc(slot_at(2 * j + 1), M::part / C);
 #pragma unroll
-                        for (int p = 0; p < 3; ++p) {
-                            const unsigned a = tmem + i * 64 + (p == 0) * (N / 2), b = slot_at(2 * j + 1) + (p == 1) * M::part;
+                        for (int p = 0; p < 3; ++p)
 #pragma unroll
-                            for (int k = 0; k < N / 16; ++k) tc_mma_ts(tmem + 256 + i * 128, a + k * 8, tc_desc(b + k * 2048, M::part / C), iv, p > 0 || k > 0);
-                        }
+                            for (int k = 0; k < N / 16; ++k)
+                                tc_mma_ts(lead, tmem + 256 + i * 128, tmem + i * 64 + (p == 0) * (N / 2) + k * 8, tc_at(b, (p == 1) * M::part + k * 2048), iv, p > 0 || k > 0);
                     }
                     if (j + 1 < steps[i]) {
                         if (!(ok = wait_slot(2 * j + 2))) break;
                         scores(i, j + 1);   // (in order: its commit says that O is there, too)
                     } else {
-                        tc_commit(o_full + 8 * i);
+                        tc_commit(lead, o_full + 8 * i);
                     }
                 }
                 if (!ok) break;
-                tc_commit(empty + 8 * ((2 * j + 1) % NS));
-                if (j + 1 < n) tc_commit(empty + 8 * ((2 * j + 2) % NS));
+                tc_commit(lead, empty + 8 * ((2 * j + 1) % NS));
+                if (j + 1 < n) tc_commit(lead, empty + 8 * ((2 * j + 2) % NS));
             }
             if (!ok) {
-                tc_commit(ended);
+                tc_commit(lead, ended);
                 bar_wait(ended, 0);
             }
         }
@@ -587,34 +593,32 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_pair_kernel(const __grid
         const size_t where = out ? (size_t)(rows.first + pos[i] + row / P.share) : 0;
         const int q_head = head * P.share + (out ? row % P.share : 0);
         int checks = 0;
-        auto wait = [&](unsigned bar, unsigned parity) { return (bool)__all_sync(0xffffffffu, bar_wait(bar, parity, gone)); };
         float unscale = 0.0f;
-        if (steps[i]) {   // the row of Q
-            const float* q = reinterpret_cast<const float*>(P.q) + where * P.q_row + (size_t)q_head * P.q_head;
-            unsigned most = 0;
-            for (int d = 0; d < HD; d += 4) {
-                const float4 x = out ? *reinterpret_cast<const float4*>(q + d) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                most = max(max(most, __float_as_uint(x.x) & 0x7fffffffu), max(__float_as_uint(x.y) & 0x7fffffffu, max(__float_as_uint(x.z) & 0x7fffffffu, __float_as_uint(x.w) & 0x7fffffffu)));
-            }
-            float up, down;
-            gm_scale(most, up, down);
-            unscale = down * (P.scale * 1.4426950408889634f);
-            unsigned char* to = smem + i * M::tile + row * 128;
-            for (int d = 0; d < HD; d += 8) {
-                const float4 x = out ? *reinterpret_cast<const float4*>(q + d) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                const float4 y = out ? *reinterpret_cast<const float4*>(q + d + 4) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                const float xs[8] = {x.x * up, x.y * up, x.z * up, x.w * up, y.x * up, y.y * up, y.z * up, y.w * up};
-                unsigned hi[4], lo[4];
+        if (steps[i]) {   // the warp's rows of Q, HD / 4 lanes to a row
+            constexpr int L = HD / 4, R = 32 / L;
+            const int r0 = (warp & 3) * 32 + lane / L, l = lane % L;
+#pragma unroll 4
+            for (int r = 0; r < 32; r += R) {
+                const int mine = r0 + r;
+                float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                if (mine < live[i] * P.share)
+                    x = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(P.q) + (size_t)(rows.first + pos[i] + mine / P.share) * P.q_row +
+                                                         (size_t)(head * P.share + mine % P.share) * P.q_head + 4 * l);
+                unsigned most = max(max(__float_as_uint(x.x) & 0x7fffffffu, __float_as_uint(x.y) & 0x7fffffffu),
+                                    max(__float_as_uint(x.z) & 0x7fffffffu, __float_as_uint(x.w) & 0x7fffffffu));
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const __half2 h = __floats2half2_rn(xs[2 * e], xs[2 * e + 1]);
-                    hi[e] = *reinterpret_cast<const unsigned*>(&h);
-                    lo[e] = gm_pack(xs[2 * e] - __low2float(h), xs[2 * e + 1] - __high2float(h));
-                }
-                const int off = (d / 64) * (M::plane / C) + (((d % 64) / 8 ^ (row & 7)) << 4);
-                *reinterpret_cast<uint4*>(to + off) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-                *reinterpret_cast<uint4*>(to + M::plane + off) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                for (int off = L / 2; off >= 1; off >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, off));
+                float up, down;
+                gm_scale(most, up, down);
+                const float a = x.x * up, b = x.y * up, c = x.z * up, d = x.w * up;
+                const __half2 h0 = __floats2half2_rn(a, b), h1 = __floats2half2_rn(c, d);
+                unsigned char* to = smem + i * M::tile + (4 * l / 64) * (M::plane / C) + mine * 128 + (((l % 16) / 2 ^ (mine & 7)) << 4) + (l & 1) * 8;
+                *reinterpret_cast<uint2*>(to) = make_uint2(*reinterpret_cast<const unsigned*>(&h0), *reinterpret_cast<const unsigned*>(&h1));
+                *reinterpret_cast<uint2*>(to + M::plane) = make_uint2(gm_pack(a - __low2float(h0), b - __high2float(h0)), gm_pack(c - __low2float(h1), d - __high2float(h1)));
+                const float back = __shfl_sync(0xffffffffu, down, (lane - r) * L & 31);   // lane r + k takes that of the k-th row of these
+                if (lane >= r && lane < r + R) unscale = back;
             }
+            unscale *= P.scale * 1.4426950408889634f;
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
             if (lane == 0) tc_bar_arrive(q_full + 8 * i);

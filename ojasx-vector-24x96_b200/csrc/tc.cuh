@@ -31,26 +31,42 @@ __device__ __forceinline__ unsigned long long tc_desc(unsigned addr, unsigned ne
            (unsigned long long)1 << 46 | (unsigned long long)2 << 61;
 }
 
+// The same `bytes` further on (whole multiples of 16; shared memory ends before the address field does).
+__device__ __forceinline__ unsigned long long tc_at(unsigned long long desc, int bytes) { return desc + (unsigned)(bytes >> 4); }
+
 // Instruction descriptor: fp32 sums, operands of 16 bits (bf16, or fp16), M = 128; kMnB: the B operand is MN-major.
 template <bool kBf16, bool kMnB>
 __device__ __forceinline__ constexpr unsigned tc_idesc(int n) {
     return 1u << 4 | (kBf16 ? 1u << 7 | 1u << 10 : 0u) | (kMnB ? 1u << 16 : 0u) | (unsigned)(n >> 3) << 17 | (unsigned)(128 >> 4) << 24;
 }
 
-__device__ __forceinline__ void tc_mma(unsigned d, unsigned long long a, unsigned long long b, unsigned idesc, bool add) {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b),
-                 "r"(idesc), "r"((unsigned)add)
-                 : "memory");
+// Products and commits are issued by whole warps, of which one lane (`lead`) acts: descriptors and addresses that are the same in all
+// lanes stay in uniform registers, where the instruction takes them from.  Issued from a branch of one lane they were moved there
+// for every product, 126 to 180 clocks each.
+__device__ __forceinline__ unsigned tc_lead() {
+    unsigned lead;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(lead));
+    return lead;
+}
+__device__ __forceinline__ void tc_mma(unsigned lead, unsigned d, unsigned long long a, unsigned long long b, unsigned idesc, bool add) {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"((unsigned)add), "r"(lead)
+        : "memory");
 }
 // The A operand in tensor memory: a row per lane, two 16-bit elements per column.
-__device__ __forceinline__ void tc_mma_ts(unsigned d, unsigned a, unsigned long long b, unsigned idesc, bool add) {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b),
-                 "r"(idesc), "r"((unsigned)add)
-                 : "memory");
+__device__ __forceinline__ void tc_mma_ts(unsigned lead, unsigned d, unsigned a, unsigned long long b, unsigned idesc, bool add) {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"((unsigned)add), "r"(lead)
+        : "memory");
 }
 // Arrives at `bar` when the products issued so far are done.
-__device__ __forceinline__ void tc_commit(unsigned bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+__device__ __forceinline__ void tc_commit(unsigned lead, unsigned bar) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar),
+        "r"(lead)
+        : "memory");
 }
 
 #define OJX_R8(v, i) "=r"((v)[i]), "=r"((v)[i + 1]), "=r"((v)[i + 2]), "=r"((v)[i + 3]), "=r"((v)[i + 4]), "=r"((v)[i + 5]), "=r"((v)[i + 6]), "=r"((v)[i + 7])

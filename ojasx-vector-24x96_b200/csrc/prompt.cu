@@ -44,6 +44,34 @@ struct PaSmem {
     static constexpr int bytes = bars + 256 + 1024;               // (swizzled tiles begin on 1024 bytes)
 };
 
+// Two fp32 numbers in one register pair: half the instructions for what is done to all scores.
+__device__ __forceinline__ unsigned long long pa_pair(float a, float b) { return (unsigned long long)__float_as_uint(b) << 32 | __float_as_uint(a); }
+__device__ __forceinline__ unsigned long long pa_fma2(unsigned long long a, unsigned long long b, unsigned long long c) {
+    unsigned long long d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ unsigned long long pa_add2(unsigned long long a, unsigned long long b) {
+    unsigned long long d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ unsigned long long pa_mul2(unsigned long long a, unsigned long long b) {
+    unsigned long long d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ float pa_max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+__device__ __forceinline__ unsigned long long pa_exp2(unsigned long long x) {
+    float a = __uint_as_float((unsigned)x), b = __uint_as_float((unsigned)(x >> 32));
+    asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(a));
+    asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(b));
+    return pa_pair(a, b);
+}
 static __device__ int g_prompt_error;   // raised when a bounded wait inside a kernel ran out
 
 template <int HD>
@@ -58,13 +86,14 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_tc_kernel(const __grid_c
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;   // (the same for a warp, as the compiler sees)
     const unsigned base = tc_smem(smem), bars = base + M::bars;
     const unsigned full = bars, empty = bars + 8 * NS, q_full = empty + 8 * NS, s_full = q_full + 16, p_full = s_full + 16, o_full = p_full + 16,
-                   checked = o_full + 16, ended = checked + 16, gone = tc_smem(&s_gone);
+                   checked = o_full + 16, p_half = checked + 16, ended = p_half + 16, gone = tc_smem(&s_gone);
     const int head = blockIdx.x % P.kv_heads, per = kPaRows / P.share;
     if (tid == 0) {
         for (int i = 0; i < NS; ++i) { tc_bar_init(full + 8 * i, 1); tc_bar_init(empty + 8 * i, 1); }
         for (int i = 0; i < 2; ++i) {
             tc_bar_init(q_full + 8 * i, 1);
             tc_bar_init(s_full + 8 * i, 1);
+            tc_bar_init(p_half + 8 * i, 4);
             tc_bar_init(p_full + 8 * i, 4);
             tc_bar_init(o_full + 8 * i, 1);
             tc_bar_init(checked + 8 * i, 4);
@@ -103,7 +132,7 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_tc_kernel(const __grid_c
     }
     const int n = max(steps[0], steps[1]);
     bool ok = true;
-    auto wait = [&](unsigned bar, unsigned parity) { return (bool)__all_sync(0xffffffffu, bar_wait(bar, parity, gone)); };   // of a warp
+    auto wait = [&](unsigned bar, unsigned parity) { return tc_wait(bar, parity, gone); };
 
     if (warp >= 8) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
@@ -129,10 +158,9 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_tc_kernel(const __grid_c
         if (warp == 8) {
             const unsigned lead = tc_lead();
             constexpr unsigned iq = tc_idesc<true, false>(kPaKeys), iv = tc_idesc<true, true>(HD);
-            auto slot_at = [&](int s) { return base + M::ring + (s % NS) * M::tile; };
-            auto wait_slot = [&](int s) { return wait(full + 8 * (s % NS), (s / NS) & 1); };
-            auto scores = [&](int i, int j) {
-                const unsigned long long a = tc_desc(base + i * M::tile), b = tc_desc(slot_at(2 * j));
+            const unsigned long long ring_k = tc_desc(base + M::ring), ring_v = tc_desc(base + M::ring, M::tile / C), q_desc = tc_desc(base);
+            auto scores = [&](int i, int slot) {
+                const unsigned long long a = tc_at(q_desc, i * M::tile), b = tc_at(ring_k, slot * M::tile);
 #pragma unroll
                 for (int k = 0; k < HD / 16; ++k) {
                     const int off = (k / 4) * (M::tile / C) + (k % 4) * 32;
@@ -140,32 +168,47 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_tc_kernel(const __grid_c
                 }
                 tc_commit(lead, s_full + 8 * i);
             };
-            if (n > 0) ok = wait_slot(0);
-            for (int i = 0; i < 2 && ok; ++i)
-                if (steps[i]) {
+            TcRing<NS> kr{0, 0}, vr{1, 0};
+            if (n > 0) ok = wait(full, 0);
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+                if (ok && steps[i]) {
                     ok = wait(q_full + 8 * i, 0);
                     if (ok) scores(i, 0);
                 }
             if (n > 0 && ok) tc_commit(lead, empty);
             for (int j = 0; j < n && ok; ++j) {
-                if (j + 1 < n) ok = wait_slot(2 * j + 2);
-                if (ok) ok = wait_slot(2 * j + 1);
-                for (int i = 0; i < 2 && ok; ++i) {
-                    if (j >= steps[i]) continue;
-                    if (!(ok = wait(p_full + 8 * i, j & 1))) break;
-                    tc_after();
-                    if (*reinterpret_cast<volatile int*>(&s_odd[i]) != j + 1) {   // (else the rows have added their products themselves)
-                        const unsigned long long b = tc_desc(slot_at(2 * j + 1), M::tile / C);
+                kr.next(2);
+                bool loaded = false;   // K of the next step
+                ok = wait(full + 8 * vr.slot, vr.parity);
 #pragma unroll
-                        for (int k = 0; k < kPaKeys / 16; ++k)
+                for (int i = 0; i < 2; ++i) {
+                    if (j >= steps[i] || !ok) continue;
+                    // the first 64 keys' weights come earlier, so that their product runs beside the other half's exponentials
+                    const unsigned long long b = tc_at(ring_v, vr.slot * M::tile);
+                    const bool maybe = (j + 1) * kPaKeys - 1 > pos[i] + ahead;
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) {
+                        if (!(ok = wait((half ? p_full : p_half) + 8 * i, j & 1))) break;
+                        tc_after();
+                        if (maybe && *reinterpret_cast<volatile int*>(&s_odd[i]) == j + 1) continue;   // (the rows have added their products themselves)
+#pragma unroll
+                        for (int k = half * kPaKeys / 32; k < (half + 1) * kPaKeys / 32; ++k)
                             tc_mma_ts(lead, tmem + 256 + i * 128, tmem + i * 128 + k * 8, tc_at(b, k * 2048), iv, j > 0 || k > 0);
                     }
-                    if (j + 1 < steps[i]) scores(i, j + 1);   // (in order: its commit says that O is up to date, too)
-                    else tc_commit(lead, o_full + 8 * i);
+                    if (!ok) continue;
+                    if (j + 1 < steps[i]) {
+                        if (!loaded && !(ok = wait(full + 8 * kr.slot, kr.parity))) continue;
+                        loaded = true;
+                        scores(i, kr.slot);   // (in order: its commit says that O is up to date, too)
+                    } else {
+                        tc_commit(lead, o_full + 8 * i);
+                    }
                 }
                 if (!ok) break;
-                tc_commit(lead, empty + 8 * ((2 * j + 1) % NS));
-                if (j + 1 < n) tc_commit(lead, empty + 8 * ((2 * j + 2) % NS));
+                tc_commit(lead, empty + 8 * vr.slot);
+                if (j + 1 < n) tc_commit(lead, empty + 8 * kr.slot);
+                vr.next(2);
             }
             if (!ok) {
                 tc_commit(lead, ended);
@@ -178,7 +221,8 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_tc_kernel(const __grid_c
         const int at = min(row, max(live[i] * P.share - 1, 0)), last = pos[i] + at / P.share + ahead;   // last key that the row sees
         const unsigned lanes = (unsigned)((warp & 3) * 32) << 16, st = tmem + i * 128 + lanes, ot = tmem + 256 + i * 128 + lanes;
         const float scale = P.scale * 1.4426950408889634f;
-        float top = 0.0f, sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        float top = 0.0f;
+        unsigned long long sum2[2] = {0, 0};
         int checks = 0;
         auto rescale = [&](float by) {   // the warp's rows of O
             for (int c = 0; c < HD; c += 32) {
@@ -208,9 +252,9 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_tc_kernel(const __grid_c
             }
             float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-            for (int e = 0; e < 128; e += 4)
+            for (int e = 0; e < 128; e += 8)
 #pragma unroll
-                for (int u = 0; u < 4; ++u) m[u] = fmaxf(m[u], __uint_as_float(s[e + u]));
+                for (int u = 0; u < 4; ++u) m[u] = pa_max3(m[u], __uint_as_float(s[e + 2 * u]), __uint_as_float(s[e + 2 * u + 1]));
             const float now = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
             const bool up = (now - top) * scale > kPaSlack;   // (by the row's own scores: its result does not depend on its neighbours)
             if (j == 0) {
@@ -218,25 +262,30 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_tc_kernel(const __grid_c
             } else if (__any_sync(0xffffffffu, up)) {
                 const float to = up ? now : top, by = up ? exp2f((top - now) * scale) : 1.0f;
                 rescale(by);
-#pragma unroll
-                for (int u = 0; u < 4; ++u) sum[u] *= by;
+                sum2[0] = pa_mul2(sum2[0], pa_pair(by, by));
+                sum2[1] = pa_mul2(sum2[1], pa_pair(by, by));
                 top = to;
             }
             const float off = top == -INFINITY ? 0.0f : top * scale;   // (a row that has seen nothing: its weights are exp(-inf))
+            const unsigned long long scale2 = pa_pair(scale, scale), off2 = pa_pair(-off, -off);
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
                 unsigned w[32];
 #pragma unroll
                 for (int e = 0; e < 32; ++e) {
-                    float a = fmaf(__uint_as_float(s[64 * c + 2 * e]), scale, -off), b = fmaf(__uint_as_float(s[64 * c + 2 * e + 1]), scale, -off);
-                    asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(a));
-                    asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(b));
-                    sum[e & 1] += a;
-                    sum[2 + (e & 1)] += b;
-                    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+                    unsigned long long x = pa_fma2((unsigned long long)s[64 * c + 2 * e + 1] << 32 | s[64 * c + 2 * e], scale2, off2);
+                    x = pa_exp2(x);
+                    sum2[e & 1] = pa_add2(sum2[e & 1], x);
+                    const __nv_bfloat162 h = __floats2bfloat162_rn(__uint_as_float((unsigned)x), __uint_as_float((unsigned)(x >> 32)));
                     w[e] = *reinterpret_cast<const unsigned*>(&h);
                 }
                 tc_st32(st + 32 * c, w);
+                if (c == 0 && !masked) {
+                    tc_wait_st();
+                    tc_before();
+                    __syncwarp();
+                    if (lane == 0) tc_bar_arrive(p_half + 8 * i);
+                }
             }
             if (masked) {
                 // A weight of zero times an infinity is a NaN, and the products take all keys of the step.  Where a value among them is
@@ -297,12 +346,16 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_tc_kernel(const __grid_c
             tc_wait_st();
             tc_before();
             __syncwarp();
-            if (lane == 0) tc_bar_arrive(p_full + 8 * i);
+            if (lane == 0) {
+                if (masked) tc_bar_arrive(p_half + 8 * i);
+                tc_bar_arrive(p_full + 8 * i);
+            }
         }
         if (ok && live[i] > 0) {
             const int position = row / P.share;
             const bool out = position < live[i] && row < per * P.share;
-            const float total = (sum[0] + sum[1]) + (sum[2] + sum[3]), inv = total == 0.0f ? 0.0f : 1.0f / total;
+            sum2[0] = pa_add2(sum2[0], sum2[1]);
+            const float total = __uint_as_float((unsigned)sum2[0]) + __uint_as_float((unsigned)(sum2[0] >> 32)), inv = total == 0.0f ? 0.0f : 1.0f / total;
             uint4* to = reinterpret_cast<uint4*>(reinterpret_cast<__nv_bfloat16*>(P.out) +
                                                  ((size_t)(rows.first + pos[i] + (out ? position : 0)) * P.q_heads + head * P.share + (out ? row % P.share : 0)) * HD);
             if (steps[i]) {
@@ -498,7 +551,7 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_pair_kernel(const __grid
     }
     const int n = max(steps[0], steps[1]);
     bool ok = true;
-    auto wait = [&](unsigned bar, unsigned parity) { return (bool)__all_sync(0xffffffffu, bar_wait(bar, parity, gone)); };   // of a warp
+    auto wait = [&](unsigned bar, unsigned parity) { return tc_wait(bar, parity, gone); };
 
     if (warp >= 8) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
@@ -533,10 +586,9 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_pair_kernel(const __grid
         if (warp == 8) {
             const unsigned lead = tc_lead();
             constexpr unsigned iq = tc_idesc<false, false>(N), iv = tc_idesc<false, true>(HD);
-            auto slot_at = [&](int s) { return base + M::ring + (s % NS) * M::slot; };
-            auto wait_slot = [&](int s) { return wait(full + 8 * (s % NS), (s / NS) & 1); };
-            auto scores = [&](int i, int j) {
-                const unsigned long long a = tc_desc(base + i * M::tile), b = tc_desc(slot_at(2 * j));
+            const unsigned long long ring_k = tc_desc(base + M::ring), ring_v = tc_desc(base + M::ring, M::part / C), q_desc = tc_desc(base);
+            auto scores = [&](int i, int slot) {
+                const unsigned long long a = tc_at(q_desc, i * M::tile), b = tc_at(ring_k, slot * M::slot);
 #pragma unroll
                 for (int p = 0; p < 3; ++p) {   // lo hi, hi lo, hi hi
 #pragma unroll
@@ -546,22 +598,27 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_pair_kernel(const __grid
                 }
                 tc_commit(lead, s_full + 8 * i);
             };
-            if (n > 0) ok = wait_slot(0);
-            for (int i = 0; i < 2 && ok; ++i)
-                if (steps[i]) {
+            TcRing<NS> kr{0, 0}, vr{1, 0};
+            if (n > 0) ok = wait(full, 0);
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+                if (ok && steps[i]) {
                     ok = wait(q_full + 8 * i, 0);
                     tc_after();
                     if (ok) scores(i, 0);
                 }
             if (n > 0 && ok) tc_commit(lead, empty);
             for (int j = 0; j < n && ok; ++j) {
-                ok = wait_slot(2 * j + 1);
-                for (int i = 0; i < 2 && ok; ++i) {
-                    if (j >= steps[i]) continue;
-                    if (!(ok = wait(p_full + 8 * i, j & 1))) break;
+                kr.next(2);
+                bool loaded = false;
+                ok = wait(full + 8 * vr.slot, vr.parity);
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    if (j >= steps[i] || !ok) continue;
+                    if (!(ok = wait(p_full + 8 * i, j & 1))) continue;
                     tc_after();
-                    if (*reinterpret_cast<volatile int*>(&s_odd[i]) != j + 1) {
-                        const unsigned long long b = tc_desc(slot_at(2 * j + 1), M::part / C);
+                    if (!((j + 1) * N - 1 > pos[i] + ahead && *reinterpret_cast<volatile int*>(&s_odd[i]) == j + 1)) {
+                        const unsigned long long b = tc_at(ring_v, vr.slot * M::slot);
 #pragma unroll
                         for (int p = 0; p < 3; ++p)
 #pragma unroll
@@ -569,15 +626,17 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_pair_kernel(const __grid
                                 tc_mma_ts(lead, tmem + 256 + i * 128, tmem + i * 64 + (p == 0) * (N / 2) + k * 8, tc_at(b, (p == 1) * M::part + k * 2048), iv, p > 0 || k > 0);
                     }
                     if (j + 1 < steps[i]) {
-                        if (!(ok = wait_slot(2 * j + 2))) break;
-                        scores(i, j + 1);   // (in order: its commit says that O is there, too)
+                        if (!loaded && !(ok = wait(full + 8 * kr.slot, kr.parity))) continue;
+                        loaded = true;
+                        scores(i, kr.slot);   // (in order: its commit says that O is there, too)
                     } else {
                         tc_commit(lead, o_full + 8 * i);
                     }
                 }
                 if (!ok) break;
-                tc_commit(lead, empty + 8 * ((2 * j + 1) % NS));
-                if (j + 1 < n) tc_commit(lead, empty + 8 * ((2 * j + 2) % NS));
+                tc_commit(lead, empty + 8 * vr.slot);
+                if (j + 1 < n) tc_commit(lead, empty + 8 * kr.slot);
+                vr.next(2);
             }
             if (!ok) {
                 tc_commit(lead, ended);

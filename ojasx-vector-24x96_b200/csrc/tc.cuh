@@ -17,6 +17,23 @@ __device__ __forceinline__ void tc_bar_expect(unsigned bar, unsigned bytes) {
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
 
+// Waits of a warp for a phase: one look where it is there already, else as bar_wait waits.  False: it ran out.
+__device__ __forceinline__ bool tc_wait(unsigned bar, unsigned parity, unsigned gone) {
+    unsigned done;
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(done) : "r"(bar), "r"(parity) : "memory");
+    return __all_sync(0xffffffffu, done) || __all_sync(0xffffffffu, bar_wait(bar, parity, gone));
+}
+// A place in a ring of N stages and the parity of its next phase.
+template <int N>
+struct TcRing {
+    int slot;
+    unsigned parity;
+    __device__ __forceinline__ void next(int by) {
+        slot += by;
+        if (slot >= N) { slot -= N; parity ^= 1u; }
+    }
+};
+
 // Box of a 3-dimensional tensor map to shared memory; x in elements, a multiple of 16 bytes.
 __device__ __forceinline__ void tc_load3(unsigned to, const CUtensorMap* map, int x, int y, int z, unsigned bar) {
     asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(to),

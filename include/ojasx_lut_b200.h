@@ -394,38 +394,39 @@ OJASX_API int ojasx_b200_paged_kv_decode(const void* d_q, void* d_out, const int
                                          float* d_scratch, int* d_counters, void* stream);
 
 /* ---- 4-bit paged KV cache and attention over whole prompts (no counterpart in the reference, whose paged cache holds int8 and
- * whose attention is over padded batches, ojasx_24x96/long_context.py:92-279).  Device pointers throughout, 16-byte aligned; row
+ * whose attention is over padded batches, ojasx_24x96/long_context.py:92-279).  Tensors are device pointers, 16-byte aligned; row
  * strides in elements, multiples of 4.
  *
  * Format: 32 consecutive dimensions of a token's key or value share a bf16 minimum (the largest not above their own) and a bf16
  * scale (the smallest not below (max - minimum) / 15); a value is a code 0..15 and reads as code * scale + minimum, within half a
  * scale of what it was.  A group that holds an infinity or a NaN reads as NaN.
- * The pool is num_pages pages of ojasx_b200_q4kv_page_bytes (0: not supported) for one layer; d_block_table [batch, max_pages]
- * int32 names the pages of every sequence.  Entries outside [0, num_pages) are no page: tokens there are dropped by an append, read
- * as zeros and weigh nothing in a decode, and *d_status becomes 1.  head_dim 64 or 128, page_size a multiple of 16.
+ * d_block_table [batch, max_pages] int32 names the pages of every sequence.  Entries outside [0, num_pages) are no page: tokens
+ * there are dropped by an append, read as zeros and weigh nothing in a decode, and *status becomes 1.
  *
  * append: token i of d_k, d_v [n_tokens, kv_heads, head_dim] goes to its place behind the d_positions[b] tokens of its sequence.
  * d_ends [batch + 1]: the tokens of sequence b are d_ends[b] .. d_ends[b + 1] - 1 (tokens behind the last one are left alone); NULL:
- * one token per sequence.  d_turns [head_dim / 2] (float64) or NULL: keys, and the queries d_q [n_tokens, q_heads, head_dim] if
- * there are any, are turned on the way, dimensions j and j + head_dim / 2 by position * d_turns[j] full turns; the queries go to
- * d_q_out.
+ * one token per sequence.  Keys, and the queries d_q [n_tokens, q_heads, head_dim] if there are any, are turned on the way where the
+ * cache has `turns`; the queries go to d_q_out.
  * read: tokens d_positions[b] (NULL: 0) and on of every sequence into d_k, d_v, packed as d_ends says.
  * decode: one query per sequence, d_q, d_out [batch, q_heads, head_dim], over its first d_lengths[b] tokens; a length of zero gives
- * zeros; scale <= 0 means 1/sqrt(head_dim).  workspace: ojasx_b200_q4kv_decode_workspace bytes for this call alone.
+ * zeros; scale <= 0 means 1/sqrt(head_dim).  Values up to 2^100.  workspace: ojasx_b200_q4kv_decode_workspace bytes for this call.
  * None of them waits for the GPU; lengths, positions and tables are read on the device, so the calls can be captured in a graph. */
-OJASX_API size_t ojasx_b200_q4kv_page_bytes(int kv_heads, int page_size, int head_dim);
-OJASX_API int ojasx_b200_q4kv_append(const void* d_k, long long k_stride, const void* d_v, long long v_stride, const void* d_q,
-                                     long long q_stride, void* d_q_out, void* d_pool, const int* d_block_table, const int* d_positions,
-                                     const int* d_ends, const double* d_turns, int* d_status, int n_tokens, int batch, int max_pages,
-                                     int num_pages, int page_size, int kv_heads, int q_heads, int head_dim, int io_dtype, void* stream);
-OJASX_API int ojasx_b200_q4kv_read(const void* d_pool, const int* d_block_table, const int* d_ends, const int* d_positions, void* d_k,
-                                   void* d_v, int* d_status, int n_tokens, int batch, int max_pages, int num_pages, int page_size,
-                                   int kv_heads, int head_dim, int io_dtype, void* stream);
-OJASX_API size_t ojasx_b200_q4kv_decode_workspace(int batch, int max_pages, int page_size, int kv_heads, int q_heads, int head_dim,
-                                                  int io_dtype);
-OJASX_API int ojasx_b200_q4kv_decode(const void* d_q, void* d_out, const void* d_pool, const int* d_block_table, const int* d_lengths,
-                                     int* d_status, int batch, int max_pages, int num_pages, int page_size, int kv_heads, int q_heads,
-                                     int head_dim, float scale, int io_dtype, void* workspace, size_t workspace_bytes, void* stream);
+typedef struct {
+    void* pool;             /* num_pages pages of ojasx_b200_q4kv_page_bytes each */
+    int* status;            /* device */
+    const double* turns;    /* device [head_dim / 2] or NULL: dimensions j and j + head_dim / 2 turn by position * turns[j] full turns */
+    int num_pages, page_size, kv_heads, q_heads, head_dim;   /* page_size a multiple of 16, head_dim 64 or 128 */
+} OjasxQ4Cache;
+OJASX_API size_t ojasx_b200_q4kv_page_bytes(int kv_heads, int page_size, int head_dim);   /* 0: not supported */
+OJASX_API int ojasx_b200_q4kv_append(const OjasxQ4Cache* cache, const void* d_k, long long k_stride, const void* d_v, long long v_stride,
+                                     const void* d_q, long long q_stride, void* d_q_out, const int* d_block_table, int max_pages,
+                                     const int* d_positions, const int* d_ends, int n_tokens, int batch, int io_dtype, void* stream);
+OJASX_API int ojasx_b200_q4kv_read(const OjasxQ4Cache* cache, const int* d_block_table, int max_pages, const int* d_ends,
+                                   const int* d_positions, void* d_k, void* d_v, int n_tokens, int batch, int io_dtype, void* stream);
+OJASX_API size_t ojasx_b200_q4kv_decode_workspace(const OjasxQ4Cache* cache, int batch, int max_pages, int io_dtype);
+OJASX_API int ojasx_b200_q4kv_decode(const OjasxQ4Cache* cache, const void* d_q, void* d_out, const int* d_block_table, int max_pages,
+                                     const int* d_lengths, int batch, float scale, int io_dtype, void* workspace, size_t workspace_bytes,
+                                     void* stream);
 /* Causal attention of packed prompts: d_q [n_rows, q_heads, head_dim], d_k, d_v [n_keys, kv_heads, head_dim] (strides of a row and
  * of a head in elements, the dimensions of a head together) into d_out [n_rows, q_heads, head_dim].  Rows d_ends[b] .. and keys
  * d_key_ends[b] .. belong to sequence b, whose last query sees its last key, the one before it the keys up to the one before, and so

@@ -31,6 +31,12 @@ class GgmlTensor(C.Structure):
         return t
 
 
+class Q4Cache(C.Structure):
+    """``OjasxQ4Cache`` of include/ojasx_lut_b200.h."""
+    _fields_ = [("pool", C.c_void_p), ("status", C.c_void_p), ("turns", C.c_void_p), ("num_pages", C.c_int), ("page_size", C.c_int),
+                ("kv_heads", C.c_int), ("q_heads", C.c_int), ("head_dim", C.c_int)]
+
+
 # name -> (restype, argtypes); mirrors include/ojasx_lut_b200.h and include/ojasx_ggml_b200.h
 SIGNATURES = {
     "ojasx_get_version": (C.c_char_p, []),
@@ -122,10 +128,10 @@ SIGNATURES = {
     "ojasx_b200_rope_qk": (_i, [_vp, _vp, _vp, _i, _i, _i, _i, _f, _i, _vp]),
     "ojasx_b200_add_int": (_i, [_vp, _i, _i, _vp]),
     "ojasx_b200_q4kv_page_bytes": (_sz, [_i, _i, _i]),
-    "ojasx_b200_q4kv_append": (_i, [_vp, _ll, _vp, _ll, _vp, _ll, _vp, _vp, _vp, _vp, _vp, _vp, _vp] + [_i] * 9 + [_vp]),
-    "ojasx_b200_q4kv_read": (_i, [_vp] * 7 + [_i] * 8 + [_vp]),
-    "ojasx_b200_q4kv_decode_workspace": (_sz, [_i] * 7),
-    "ojasx_b200_q4kv_decode": (_i, [_vp] * 6 + [_i] * 7 + [_f, _i, _vp, _sz, _vp]),
+    "ojasx_b200_q4kv_append": (_i, [_vp, _vp, _ll, _vp, _ll, _vp, _ll, _vp, _vp, _i, _vp, _vp, _i, _i, _i, _vp]),
+    "ojasx_b200_q4kv_read": (_i, [_vp, _vp, _i, _vp, _vp, _vp, _vp, _i, _i, _i, _vp]),
+    "ojasx_b200_q4kv_decode_workspace": (_sz, [_vp, _i, _i, _i]),
+    "ojasx_b200_q4kv_decode": (_i, [_vp, _vp, _vp, _vp, _i, _vp, _i, _f, _i, _vp, _sz, _vp]),
     "ojasx_b200_prompt_workspace": (_sz, [_i] * 4),
     "ojasx_b200_prompt_attention": (_i, [_vp, _ll, _ll] * 3 + [_vp] * 3 + [_i] * 6 + [_f, _i, _vp, _sz, _vp]),
 }

@@ -1,5 +1,6 @@
 // 4-bit paged KV cache: appending with the position rotation on the way, and reading back.  Layout and format: q4kv.cuh; attention of
 // single tokens: q4kv_decode.cu.
+#include <algorithm>
 #include <cmath>
 
 #include "handles.h"
@@ -25,30 +26,52 @@ __device__ __forceinline__ void q4_store4(void* p, size_t i, bool bf16, float4 v
         make_uint2(*reinterpret_cast<const unsigned*>(&a), *reinterpret_cast<const unsigned*>(&b));
 }
 
+// Minimum and maximum that a NaN makes NaN.
+__device__ __forceinline__ float q4_less(float a, float b) {
+    asm("min.NaN.f32 %0, %0, %1;" : "+f"(a) : "f"(b));
+    return a;
+}
+__device__ __forceinline__ float q4_more(float a, float b) {
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(a) : "f"(b));
+    return a;
+}
+
 // Four values of a group whose other 28 are with the neighbouring seven lanes, as nibbles; `meta`: the group's minimum and scale.
+// Quotients are those of IEEE division: with the rounded reciprocal r of s, q = v r, and q + (v - q s) r is v / s rounded (Markstein's
+// theorem) where nothing leaves the range of fp32, which the branch sees to.  v - minimum is not negative and at most 15 scales.
 __device__ __forceinline__ unsigned q4_encode(float4 x, unsigned& meta) {
-    float lo = fminf(fminf(x.x, x.y), fminf(x.z, x.w)), hi = fmaxf(fmaxf(x.x, x.y), fmaxf(x.z, x.w));
-    float odd = (x.x - x.x) + (x.y - x.y) + (x.z - x.z) + (x.w - x.w);   // NaN for an infinity or a NaN (which the maxima pass over)
+    float lo = q4_less(q4_less(x.x, x.y), q4_less(x.z, x.w)), hi = q4_more(q4_more(x.x, x.y), q4_more(x.z, x.w));
 #pragma unroll
     for (int off = 1; off < 8; off <<= 1) {
-        lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, off));
-        hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, off));
-        odd += __shfl_xor_sync(0xffffffffu, odd, off);
+        lo = q4_less(lo, __shfl_xor_sync(0xffffffffu, lo, off));
+        hi = q4_more(hi, __shfl_xor_sync(0xffffffffu, hi, off));
     }
-    const __nv_bfloat16 mb = __float2bfloat16_rd(lo);
-    const float m = __bfloat162float(mb);
-    const float range = hi - m;
-    const bool wide = isinf(range);   // beyond fp32: quotients first, then their difference
-    const __nv_bfloat16 sb = __float2bfloat16_ru(wide ? hi / 15.0f - m / 15.0f : __fdiv_rn(range, 15.0f));
-    const float s = __bfloat162float(sb);
-    if (!(odd == 0.0f) || isinf(m) || isinf(s)) {
-        meta = 0x7fff0000u;
-        return 0u;
+    const unsigned lb = __float_as_uint(lo), mb = (lb + ((unsigned)((int)lb >> 31) & 0xffffu)) & 0xffff0000u;   // down to bf16
+    const float m = __uint_as_float(mb), range = hi - m;
+    unsigned sb = (__float_as_uint(__fdiv_rn(range, 15.0f)) + 0xffffu) & 0xffff0000u;                          // up
+    float s = __uint_as_float(sb);
+    unsigned code;
+    if (s > 0x1p-90f && s < 0x1p90f) {
+        const float r = __frcp_rn(s);
+        auto step = [&](float v) {   // rounded by an addition: the code is in the lowest bits
+            const float d = v - m, q = d * r;
+            return __float_as_uint(fmaf(fmaf(-q, s, d), r, q) + 12582912.0f) & 15u;
+        };
+        code = step(x.x) | step(x.y) << 4 | step(x.z) << 8 | step(x.w) << 12;
+    } else {
+        const bool wide = isinf(range);   // beyond fp32: quotients first, then their difference
+        if (wide) sb = (__float_as_uint(hi / 15.0f - m / 15.0f) + 0xffffu) & 0xffff0000u;
+        s = __uint_as_float(sb);
+        const float d = s > 0.0f ? s : 1.0f;   // a group of one value that bf16 holds has no steps
+        auto step = [&](float v) { return (unsigned)fminf(fmaxf(rintf(wide ? v / d - m / d : __fdiv_rn(v - m, d)), 0.0f), 15.0f); };
+        code = step(x.x) | step(x.y) << 4 | step(x.z) << 8 | step(x.w) << 12;
+        if (!isfinite(lo) || !isfinite(hi) || isinf(m) || isinf(s)) {
+            meta = 0x7fff0000u;
+            return 0u;
+        }
     }
-    meta = (unsigned)__bfloat16_as_ushort(mb) << 16 | __bfloat16_as_ushort(sb);
-    const float d = s > 0.0f ? s : 1.0f;   // a group of one value that bf16 holds has no steps
-    auto code = [&](float v) { return (unsigned)fminf(fmaxf(rintf(wide ? v / d - m / d : __fdiv_rn(v - m, d)), 0.0f), 15.0f); };
-    return code(x.x) | code(x.y) << 4 | code(x.z) << 8 | code(x.w) << 12;
+    meta = mb | sb >> 16;
+    return code;
 }
 
 struct Q4AppendProblem {
@@ -71,59 +94,179 @@ __device__ __forceinline__ void q4_angles(const double* turns, int j, int pos, f
     }
 }
 
-// One token per CTA; HD / 8 lanes share a vector, each with four dimensions of either half (a rotated pair is in one lane, a group
-// is eight lanes).  Keys and queries are turned by position * turns[j], keys and values go to the cache as 4 bits.
+__device__ __forceinline__ void q4_rotate(float4& a, float4& d, const float (&c)[4], const float (&s)[4]) {
+    const float4 x = a, y = d;
+    a = make_float4(x.x * c[0] - y.x * s[0], x.y * c[1] - y.y * s[1], x.z * c[2] - y.z * s[2], x.w * c[3] - y.w * s[3]);
+    d = make_float4(y.x * c[0] + x.x * s[0], y.y * c[1] + x.y * s[1], y.z * c[2] + x.z * s[2], y.w * c[3] + x.w * s[3]);
+}
+
+// Few tokens: 1024 / HD vectors (keys, values and queries of one token) per CTA, HD / 8 lanes to a vector, each with four dimensions of
+// either half (a rotated pair is in one lane, a group is eight lanes).  Bound by latency: everything that does not wait for the
+// position is asked for before it, the page while the angles are made.
 template <int HD, bool kBf16>
 __global__ void __launch_bounds__(128) q4_append_kernel(const __grid_constant__ Q4AppendProblem P) {
-    constexpr int L = HD / 8, G = HD / 32;
+    constexpr int L = HD / 8, G = HD / 32, V = 128 / L;
     using T = Q4Layout<HD>;
     chain_begin();
-    const int token = blockIdx.x, l = threadIdx.x % L, task0 = threadIdx.x / L, step = 128 / L;
+    const int kv = P.cache.kv_heads, tasks = 2 * kv + (P.q ? P.q_heads : 0), parts = (tasks + V - 1) / V;
+    const int token = blockIdx.x / parts, l = threadIdx.x % L, first = blockIdx.x % parts * V + threadIdx.x / L;
+    const int task = min(first, tasks - 1);      // (the lanes of a warp stay together for the shuffles)
+    const int kind = task < kv ? 0 : task < 2 * kv ? 1 : 2, head = kind == 2 ? task - 2 * kv : task - kind * kv;
+    const void* src = kind == 0 ? P.k : kind == 1 ? P.v : P.q;
+    const size_t at = (size_t)token * (kind == 0 ? P.k_stride : kind == 1 ? P.v_stride : P.q_stride) + (size_t)head * HD + 4 * l;
+    float4 a = q4_load4(src, at, kBf16), d = q4_load4(src, at + HD / 2, kBf16);
     int b = token, pos;
     if (P.ends) {
         b = packed_owner(P.ends, P.batch, token);
-        if (b < 0) return;
+        if (b < 0) return;   // (of the whole CTA)
         pos = P.positions[b] + token - P.ends[b];
     } else {
         pos = P.positions[b];
     }
-    float c[4] = {1.0f, 1.0f, 1.0f, 1.0f}, s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (P.turns) q4_angles(P.turns, 4 * l, pos, c, s);
-    const int kv = P.cache.kv_heads, tasks = 2 * kv + (P.q ? P.q_heads : 0);
-    const int rounds = (tasks + step - 1) / step;
-    for (int r = 0; r < rounds; ++r) {
-        const int task = min(r * step + task0, tasks - 1);      // (the lanes of a warp stay together for the shuffles)
-        const bool live = r * step + task0 < tasks;
-        const int kind = task < kv ? 0 : task < 2 * kv ? 1 : 2, head = kind == 2 ? task - 2 * kv : task - kind * kv;
-        const void* src = kind == 0 ? P.k : kind == 1 ? P.v : P.q;
-        const long long stride = kind == 0 ? P.k_stride : kind == 1 ? P.v_stride : P.q_stride;
-        const size_t at = (size_t)token * stride + (size_t)head * HD + 4 * l;
-        float4 a = q4_load4(src, at, kBf16), d = q4_load4(src, at + HD / 2, kBf16);
-        if (kind != 1 && P.turns) {
-            const float4 x = a, y = d;
-            a = make_float4(x.x * c[0] - y.x * s[0], x.y * c[1] - y.y * s[1], x.z * c[2] - y.z * s[2], x.w * c[3] - y.w * s[3]);
-            d = make_float4(y.x * c[0] + x.x * s[0], y.y * c[1] + x.y * s[1], y.z * c[2] + x.z * s[2], y.w * c[3] + x.w * s[3]);
-        }
-        unsigned meta[2];
-        const unsigned code[2] = {q4_encode(a, meta[0]), q4_encode(d, meta[1])};
-        if (!live) continue;
-        if (kind == 2) {
-            const size_t to = ((size_t)token * P.q_heads + head) * HD + 4 * l;
-            q4_store4(P.q_out, to, kBf16, a);
-            q4_store4(P.q_out, to + HD / 2, kBf16, d);
-            continue;
-        }
-        uint8_t* tile = q4_tile<HD>(P.cache, b, head, pos);
-        if (!tile) {
-            if (l == 0) atomicExch(P.cache.status, 1);
-            continue;
-        }
-        const int in = pos % kQ4Tile;
+    uint8_t* tile = kind == 2 ? nullptr : q4_tile<HD>(P.cache, b, head, pos);
+    if (kind != 1 && P.turns) {
+        float c[4], s[4];
+        q4_angles(P.turns, 4 * l, pos, c, s);
+        q4_rotate(a, d, c, s);
+    }
+    unsigned meta[2];
+    const unsigned code[2] = {q4_encode(a, meta[0]), q4_encode(d, meta[1])};
+    if (first >= tasks) return;
+    if (kind == 2) {
+        const size_t to = ((size_t)token * P.q_heads + head) * HD + 4 * l;
+        q4_store4(P.q_out, to, kBf16, a);
+        q4_store4(P.q_out, to + HD / 2, kBf16, d);
+        return;
+    }
+    if (!tile) {
+        if (l == 0) atomicExch(P.cache.status, 1);
+        return;
+    }
+    const int in = pos % kQ4Tile;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int g = h * (G / 2) + l / 8;
-            *reinterpret_cast<unsigned short*>(tile + (kind ? T::value_at(in, g, l % 8) : T::key_at(in, g, l % 8))) = (unsigned short)code[h];
-            if (l % 8 == 0) *reinterpret_cast<unsigned*>(tile + (kind ? T::value_meta : T::key_meta) + T::meta_at(in, g)) = meta[h];
+    for (int h = 0; h < 2; ++h) {
+        const int g = h * (G / 2) + l / 8;
+        *reinterpret_cast<unsigned short*>(tile + (kind ? T::value_at(in, g, l % 8) : T::key_at(in, g, l % 8))) = (unsigned short)code[h];
+        if (l % 8 == 0) *reinterpret_cast<unsigned*>(tile + (kind ? T::value_meta : T::key_meta) + T::meta_at(in, g)) = meta[h];
+    }
+}
+
+// A tile of the cache that tokens `from` to `to` (in it) of a CTA's rows lie in: its sequence, the first one's row and position.
+struct Q4Span { int b, row, pos, from, to; };
+
+// Span `index` of the tiles that the packed tokens of all sequences touch; all lanes of a warp call it together.
+__device__ __forceinline__ bool q4_span(const int* ends, const int* positions, int batch, int rows, int index, Q4Span& S) {
+    int part = 0;
+    auto tiles = [&](int b) {
+        const PackedRange r = packed_range(ends, b, rows);
+        if (r.count == 0 || (positions && positions[b] < 0)) return 0;
+        const int in = (positions ? positions[b] : 0) % kQ4Tile;
+        return (in + r.count + kQ4Tile - 1) / kQ4Tile;
+    };
+    if (!packed_part(batch, index, tiles, S.b, part)) return false;
+    const PackedRange r = packed_range(ends, S.b, rows);
+    const int begin = positions ? positions[S.b] : 0, in = begin % kQ4Tile;
+    S.from = part == 0 ? in : 0;
+    S.to = min(kQ4Tile, in + r.count - part * kQ4Tile);
+    S.pos = begin - in + part * kQ4Tile;     // of the tile's first token
+    S.row = r.first - in + part * kQ4Tile;   // (whose row may be another sequence's)
+    return true;
+}
+// Tiles that packed tokens can touch.
+static long long q4_spans(int rows, int batch) { return rows / kQ4Tile + 2LL * std::min(rows, batch); }
+
+// Prompts: a tile of 16 tokens per CTA and some of the heads, a token to HD / 8 lanes (or two of them at head_dim 64), which make its
+// angles once.  A head's tile is put together in shared memory and written in 16-byte pieces: its words hold two tokens each.
+template <int HD, bool kBf16>
+__global__ void __launch_bounds__(256) q4_append_tile_kernel(const __grid_constant__ Q4AppendProblem P, int slices) {
+    constexpr int L = HD / 8, G = HD / 32, W = 256 / (kQ4Tile * L);   // W: vectors of a token at a time
+    using T = Q4Layout<HD>;
+    __shared__ __align__(16) unsigned char s_tile[2][W * T::bytes];
+    __shared__ Q4Span s_span;
+    chain_begin();
+    if (threadIdx.x < 32) {
+        Q4Span S{-1, 0, 0, 0, 0};
+        if (!q4_span(P.ends, P.positions, P.batch, P.n_tokens, blockIdx.x / slices, S)) S.b = -1;
+        if (threadIdx.x == 0) s_span = S;
+    }
+    __syncthreads();
+    const Q4Span S = s_span;
+    if (S.b < 0) return;
+    const int kv = P.cache.kv_heads, slice = blockIdx.x % slices, l = threadIdx.x % L, w = threadIdx.x / L % W, in = threadIdx.x / (L * W);
+    const bool live = in >= S.from && in < S.to;
+    const size_t row = (size_t)(S.row + (live ? in : S.from));   // (the lanes of a warp stay together for the shuffles)
+    float c[4] = {}, s[4] = {};
+    if (P.turns) q4_angles(P.turns, 4 * l, S.pos + in, c, s);
+    uint8_t* const tile = q4_tile<HD>(P.cache, S.b, 0, S.pos);
+    if (!tile && threadIdx.x == 0) atomicExch(P.cache.status, 1);
+    const size_t head_bytes = (size_t)(P.cache.page_size / kQ4Tile) * T::bytes;
+
+    if (P.q) {
+        const int h1 = (int)((long long)P.q_heads * (slice + 1) / slices);
+        for (int h = (int)((long long)P.q_heads * slice / slices) + w; h < h1; h += 4 * W) {
+            float4 a[4], d[4];   // loads ahead of what is done with them
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const size_t at = row * P.q_stride + (size_t)min(h + u * W, h1 - 1) * HD + 4 * l;
+                a[u] = q4_load4(P.q, at, kBf16);
+                d[u] = q4_load4(P.q, at + HD / 2, kBf16);
+            }
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                if (!live || h + u * W >= h1) continue;
+                if (P.turns) q4_rotate(a[u], d[u], c, s);
+                const size_t to = (row * P.q_heads + h + u * W) * HD + 4 * l;
+                q4_store4(P.q_out, to, kBf16, a[u]);
+                q4_store4(P.q_out, to + HD / 2, kBf16, d[u]);
+            }
+        }
+    }
+    const int h0 = (int)((long long)kv * slice / slices), h1 = (int)((long long)kv * (slice + 1) / slices);
+    if (!tile || h0 >= h1) return;
+    float4 x[2][2];   // [keys, values][halves]
+    auto load = [&](int h) {
+#pragma unroll
+        for (int which = 0; which < 2; ++which) {
+            const size_t at = row * (which ? P.v_stride : P.k_stride) + (size_t)min(h, h1 - 1) * HD + 4 * l;
+            x[which][0] = q4_load4(which ? P.v : P.k, at, kBf16);
+            x[which][1] = q4_load4(which ? P.v : P.k, at + HD / 2, kBf16);
+        }
+    };
+    load(h0 + w);
+    int turn = 0;
+    for (int h = h0; h < h1; h += W, turn ^= 1) {
+        unsigned char* to = s_tile[turn] + w * T::bytes;
+        float4 y[2][2];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) y[i >> 1][i & 1] = x[i >> 1][i & 1];
+        if (h + W < h1) load(h + W + w);
+        if (P.turns) q4_rotate(y[0][0], y[0][1], c, s);
+#pragma unroll
+        for (int which = 0; which < 2; ++which)
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const int g = half * (G / 2) + l / 8;
+                unsigned meta;
+                const unsigned code = q4_encode(y[which][half], meta);
+                *reinterpret_cast<unsigned short*>(to + (which ? T::value_at(in, g, l % 8) : T::key_at(in, g, l % 8))) = (unsigned short)code;
+                if (l % 8 == 0) *reinterpret_cast<unsigned*>(to + (which ? T::value_meta : T::key_meta) + T::meta_at(in, g)) = meta;
+            }
+        __syncthreads();   // (the other buffer's pieces were read before the barrier of the turn before)
+        const int heads = min(W, h1 - h);
+        if (S.from == 0 && S.to == kQ4Tile) {
+            for (int i = threadIdx.x; i < heads * (T::bytes / 16); i += 256) {
+                const int head = i / (T::bytes / 16), piece = i % (T::bytes / 16);
+                *reinterpret_cast<uint4*>(tile + (h + head) * head_bytes + piece * 16) = *reinterpret_cast<const uint4*>(s_tile[turn] + i * 16);
+            }
+        } else {   // only these tokens' parts
+            constexpr int pieces = 2 * (8 * G + 2 * G);   // of 16 bits, of a token
+            for (int i = threadIdx.x; i < heads * kQ4Tile * pieces; i += 256) {
+                const int head = i / (kQ4Tile * pieces), token = i / pieces % kQ4Tile, piece = i % pieces, which = piece / (10 * G), p = piece % (10 * G);
+                if (token < S.from || token >= S.to) continue;
+                const int at = p < 8 * G ? (which ? T::value_at(token, p / 8, p % 8) : T::key_at(token, p / 8, p % 8))
+                                         : (which ? T::value_meta : T::key_meta) + T::meta_at(token, 0) + (p - 8 * G) * 2;
+                *reinterpret_cast<unsigned short*>(tile + (h + head) * head_bytes + at) = *reinterpret_cast<const unsigned short*>(s_tile[turn] + head * T::bytes + at);
+            }
         }
     }
 }
@@ -135,27 +278,66 @@ struct Q4ReadProblem {
     int n_tokens, batch;
 };
 
-// One token per CTA, a lane per four dimensions.  Tokens without a page are read as zeros.
+// A tile of 16 tokens and up to eight KV heads per CTA: the tiles of the heads come in 16-byte pieces, eight values of a token go out in
+// one or two.  Tokens without a page are read as zeros.
+constexpr int kQ4ReadHeads = 8;
+
 template <int HD, bool kBf16>
-__global__ void __launch_bounds__(128) q4_read_kernel(const __grid_constant__ Q4ReadProblem P) {
+__global__ void __launch_bounds__(256) q4_read_kernel(const __grid_constant__ Q4ReadProblem P) {
     using T = Q4Layout<HD>;
+    __shared__ __align__(16) unsigned char s_tile[kQ4ReadHeads * T::bytes];
+    __shared__ Q4Span s_span;
     chain_begin();
-    const int token = blockIdx.x, b = packed_owner(P.ends, P.batch, token), kv = P.cache.kv_heads;
-    if (b < 0) return;
-    const int pos = (P.positions ? P.positions[b] : 0) + token - P.ends[b], in = pos & (kQ4Tile - 1);
-    for (int i = threadIdx.x; i < 2 * kv * (HD / 4); i += 128) {
-        const int which = i / (kv * (HD / 4)), rem = i - which * kv * (HD / 4), head = rem / (HD / 4), d4 = rem % (HD / 4), g = d4 >> 3;
-        const uint8_t* tile = q4_tile<HD>(P.cache, b, head, pos);
-        float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (threadIdx.x < 32) {
+        Q4Span S{-1, 0, 0, 0, 0};
+        if (!q4_span(P.ends, P.positions, P.batch, P.n_tokens, blockIdx.x, S)) S.b = -1;
+        if (threadIdx.x == 0) s_span = S;
+    }
+    __syncthreads();
+    const Q4Span S = s_span;
+    if (S.b < 0) return;
+    const int kv = P.cache.kv_heads, h0 = blockIdx.y * kQ4ReadHeads, heads = min(kQ4ReadHeads, kv - h0);
+    const uint8_t* tile = q4_tile<HD>(P.cache, S.b, h0, S.pos);
+    const size_t head_bytes = (size_t)(P.cache.page_size / kQ4Tile) * T::bytes;
+    if (tile) {
+        for (int i = threadIdx.x; i < heads * (T::bytes / 16); i += 256)
+            *reinterpret_cast<uint4*>(s_tile + i * 16) = *reinterpret_cast<const uint4*>(tile + i / (T::bytes / 16) * head_bytes + i % (T::bytes / 16) * 16);
+    } else if (threadIdx.x == 0) {
+        atomicExch(P.cache.status, 1);
+    }
+    __syncthreads();
+    const int tokens = S.to - S.from, eights = heads * (HD / 8);
+    for (int i = threadIdx.x; i < 2 * tokens * eights; i += 256) {
+        const int which = i / (tokens * eights), rem = i - which * tokens * eights, token = S.from + rem / eights, e = rem % eights;
+        const int head = e / (HD / 8), d8 = e % (HD / 8), g = d8 / 4, c = d8 % 4 * 2;
+        const unsigned char* from = s_tile + head * T::bytes;
+        float x[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) x[u] = 0.0f;
         if (tile) {
-            const unsigned w = *reinterpret_cast<const unsigned short*>(tile + (which ? T::value_at(in, g, d4 & 7) : T::key_at(in, g, d4 & 7)));
-            const unsigned meta = *reinterpret_cast<const unsigned*>(tile + (which ? T::value_meta : T::key_meta) + T::meta_at(in, g));
+            unsigned word;
+            if (which) word = *reinterpret_cast<const unsigned short*>(from + T::value_at(token, g, c)) | (unsigned)*reinterpret_cast<const unsigned short*>(from + T::value_at(token, g, c + 1)) << 16;
+            else word = *reinterpret_cast<const unsigned*>(from + T::key_at(token, g, c));
+            const unsigned meta = *reinterpret_cast<const unsigned*>(from + (which ? T::value_meta : T::key_meta) + T::meta_at(token, g));
             const float s = q4_scale(meta), m = q4_min(meta);
-            x = make_float4(fmaf((float)(w & 15), s, m), fmaf((float)(w >> 4 & 15), s, m), fmaf((float)(w >> 8 & 15), s, m), fmaf((float)(w >> 12), s, m));
-        } else {
-            atomicExch(P.cache.status, 1);
+#pragma unroll
+            for (int u = 0; u < 8; ++u) x[u] = fmaf((float)(word >> (4 * u) & 15u), s, m);
         }
-        q4_store4(which ? P.v : P.k, ((size_t)token * kv + head) * HD + d4 * 4, kBf16, x);
+        void* out = which ? P.v : P.k;
+        const size_t to = ((size_t)(S.row + token) * kv + h0 + head) * HD + d8 * 8;
+        if (kBf16) {
+            unsigned w[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const __nv_bfloat162 p = __floats2bfloat162_rn(x[2 * u], x[2 * u + 1]);
+                w[u] = *reinterpret_cast<const unsigned*>(&p);
+            }
+            *reinterpret_cast<uint4*>(reinterpret_cast<__nv_bfloat16*>(out) + to) = make_uint4(w[0], w[1], w[2], w[3]);
+        } else {
+            float4* f = reinterpret_cast<float4*>(reinterpret_cast<float*>(out) + to);
+            f[0] = make_float4(x[0], x[1], x[2], x[3]);
+            f[1] = make_float4(x[4], x[5], x[6], x[7]);
+        }
     }
 }
 
@@ -170,41 +352,55 @@ size_t ojasx_b200_q4kv_page_bytes(int kv_heads, int page_size, int head_dim) {
     return (size_t)kv_heads * (page_size / kQ4Tile) * (head_dim == 64 ? Q4Layout<64>::bytes : Q4Layout<128>::bytes);
 }
 
-int ojasx_b200_q4kv_append(const void* d_k, long long k_stride, const void* d_v, long long v_stride, const void* d_q, long long q_stride,
-                           void* d_q_out, void* d_pool, const int* d_block_table, const int* d_positions, const int* d_ends,
-                           const double* d_turns, int* d_status, int n_tokens, int batch, int max_pages, int num_pages, int page_size,
-                           int kv_heads, int q_heads, int head_dim, int io_dtype, void* stream) {
-    const int rc = q4_check(d_pool, d_block_table, max_pages, num_pages, page_size, kv_heads, head_dim, batch, io_dtype, d_status);
+int ojasx_b200_q4kv_append(const OjasxQ4Cache* cache, const void* d_k, long long k_stride, const void* d_v, long long v_stride, const void* d_q,
+                           long long q_stride, void* d_q_out, const int* d_block_table, int max_pages, const int* d_positions,
+                           const int* d_ends, int n_tokens, int batch, int io_dtype, void* stream) {
+    const int rc = q4_check(cache, d_block_table, max_pages, batch, io_dtype);
     if (rc != OJX_OK) return rc;
-    if (!d_k || !d_v || !d_positions || n_tokens < 0 || (d_q && (!d_q_out || q_heads <= 0)) || (!d_ends && n_tokens != batch)) return OJX_ERR_ARG;
+    if (!d_k || !d_v || !d_positions || n_tokens < 0 || (d_q && !d_q_out) || (!d_ends && n_tokens != batch)) return OJX_ERR_ARG;
     if (!q4_aligned(d_k) || !q4_aligned(d_v) || !q4_aligned(d_q) || !q4_aligned(d_q_out) || k_stride % 4 || v_stride % 4 || q_stride % 4) return OJX_ERR_ARG;
+    const int kv_heads = cache->kv_heads, q_heads = cache->q_heads, head_dim = cache->head_dim;
     if (n_tokens == 0) return OJX_OK;
     Q4AppendProblem P{};
-    P.cache = {static_cast<uint8_t*>(d_pool), d_block_table, d_status, max_pages, num_pages, page_size, kv_heads};
+    P.cache = q4_cache(cache, d_block_table, max_pages);
     P.k = d_k; P.v = d_v; P.q = d_q; P.q_out = d_q_out; P.k_stride = k_stride; P.v_stride = v_stride; P.q_stride = q_stride;
-    P.positions = d_positions; P.ends = d_ends; P.turns = d_turns; P.n_tokens = n_tokens; P.batch = batch; P.q_heads = q_heads;
+    P.positions = d_positions; P.ends = d_ends; P.turns = cache->turns; P.n_tokens = n_tokens; P.batch = batch; P.q_heads = q_heads;
     const bool bf = io_dtype == OJX_BF16;
-    auto kernel = head_dim == 64 ? (bf ? q4_append_kernel<64, true> : q4_append_kernel<64, false>)
-                                 : (bf ? q4_append_kernel<128, true> : q4_append_kernel<128, false>);
-    OJX_CUDA_TRY(launch_chained(kernel, n_tokens, 128, 0, static_cast<cudaStream_t>(stream), P));
+    const cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (d_ends && n_tokens >= 4LL * batch) {
+        const long long tiles = q4_spans(n_tokens, batch);
+        const int slices = (int)std::min<long long>(kv_heads, std::max<long long>(1, (4LL * num_sms() + tiles - 1) / tiles));   // some CTAs for every SM
+        if (tiles * slices > 0x7fffffffLL) return OJX_ERR_TOO_LARGE;
+        auto kernel = head_dim == 64 ? (bf ? q4_append_tile_kernel<64, true> : q4_append_tile_kernel<64, false>)
+                                     : (bf ? q4_append_tile_kernel<128, true> : q4_append_tile_kernel<128, false>);
+        OJX_CUDA_TRY(launch_chained(kernel, dim3((unsigned)(tiles * slices)), 256, 0, s, P, slices));
+    } else {
+        const int vectors = 1024 / head_dim, parts = (2 * kv_heads + (d_q ? q_heads : 0) + vectors - 1) / vectors;
+        if ((long long)n_tokens * parts > 0x7fffffffLL) return OJX_ERR_TOO_LARGE;
+        auto kernel = head_dim == 64 ? (bf ? q4_append_kernel<64, true> : q4_append_kernel<64, false>)
+                                     : (bf ? q4_append_kernel<128, true> : q4_append_kernel<128, false>);
+        OJX_CUDA_TRY(launch_chained(kernel, dim3((unsigned)(n_tokens * parts)), 128, 0, s, P));
+    }
     count_launch(1);
     return OJX_OK;
 }
 
-int ojasx_b200_q4kv_read(const void* d_pool, const int* d_block_table, const int* d_ends, const int* d_positions, void* d_k, void* d_v,
-                         int* d_status, int n_tokens, int batch, int max_pages, int num_pages, int page_size, int kv_heads, int head_dim,
-                         int io_dtype, void* stream) {
-    const int rc = q4_check(d_pool, d_block_table, max_pages, num_pages, page_size, kv_heads, head_dim, batch, io_dtype, d_status);
+int ojasx_b200_q4kv_read(const OjasxQ4Cache* cache, const int* d_block_table, int max_pages, const int* d_ends, const int* d_positions, void* d_k,
+                         void* d_v, int n_tokens, int batch, int io_dtype, void* stream) {
+    const int rc = q4_check(cache, d_block_table, max_pages, batch, io_dtype);
     if (rc != OJX_OK) return rc;
     if (!d_ends || !d_k || !d_v || n_tokens < 0 || !q4_aligned(d_k) || !q4_aligned(d_v)) return OJX_ERR_ARG;
+    const int kv_heads = cache->kv_heads, head_dim = cache->head_dim;
     if (n_tokens == 0) return OJX_OK;
     Q4ReadProblem P{};
-    P.cache = {static_cast<uint8_t*>(const_cast<void*>(d_pool)), d_block_table, d_status, max_pages, num_pages, page_size, kv_heads};
+    P.cache = q4_cache(cache, d_block_table, max_pages);
     P.k = d_k; P.v = d_v; P.ends = d_ends; P.positions = d_positions; P.n_tokens = n_tokens; P.batch = batch;
     const bool bf = io_dtype == OJX_BF16;
     auto kernel = head_dim == 64 ? (bf ? q4_read_kernel<64, true> : q4_read_kernel<64, false>)
                                  : (bf ? q4_read_kernel<128, true> : q4_read_kernel<128, false>);
-    OJX_CUDA_TRY(launch_chained(kernel, n_tokens, 128, 0, static_cast<cudaStream_t>(stream), P));
+    const long long tiles = q4_spans(n_tokens, batch);
+    if (tiles > 0x7fffffffLL || kv_heads > 65535 * kQ4ReadHeads) return OJX_ERR_TOO_LARGE;
+    OJX_CUDA_TRY(launch_chained(kernel, dim3((unsigned)tiles, (kv_heads + kQ4ReadHeads - 1) / kQ4ReadHeads), 256, 0, static_cast<cudaStream_t>(stream), P));
     count_launch(1);
     return OJX_OK;
 }

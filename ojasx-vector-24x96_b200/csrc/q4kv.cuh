@@ -15,6 +15,7 @@
 //   their    [token][g]: words, minimum << 16 | scale
 #pragma once
 #include "common.cuh"
+#include "../../include/ojasx_lut_b200.h"
 
 namespace ojx {
 
@@ -58,13 +59,16 @@ __device__ __forceinline__ float q4_scale(unsigned meta) { return __uint_as_floa
 __device__ __forceinline__ float q4_min(unsigned meta) { return __uint_as_float(meta & 0xffff0000u); }
 
 // What every entry point asks of a cache.
-inline int q4_check(const void* pool, const int* table, int max_pages, int num_pages, int page_size, int kv_heads, int head_dim, int batch,
-                    int dtype, int* status) {
-    if (!pool || !table || !status || max_pages <= 0 || num_pages <= 0 || kv_heads <= 0 || batch <= 0) return OJX_ERR_ARG;
+inline int q4_check(const OjasxQ4Cache* c, const int* table, int max_pages, int batch, int dtype) {
+    if (!c || !c->pool || !c->status || !table || max_pages <= 0 || c->num_pages <= 0 || c->kv_heads <= 0 || c->q_heads <= 0 || c->q_heads % c->kv_heads || batch <= 0)
+        return OJX_ERR_ARG;
     if (dtype != OJX_F32 && dtype != OJX_BF16) return OJX_ERR_ARG;
-    if (page_size <= 0 || page_size % kQ4Tile || (head_dim != 64 && head_dim != 128)) return OJX_ERR_UNSUPPORTED;
-    if ((long long)max_pages * page_size > 0x7fffffffLL) return OJX_ERR_TOO_LARGE;
-    return (reinterpret_cast<uintptr_t>(pool) & 15) ? OJX_ERR_ARG : OJX_OK;
+    if (c->page_size <= 0 || c->page_size % kQ4Tile || (c->head_dim != 64 && c->head_dim != 128)) return OJX_ERR_UNSUPPORTED;
+    if ((long long)max_pages * c->page_size > 0x7fffffffLL) return OJX_ERR_TOO_LARGE;
+    return (reinterpret_cast<uintptr_t>(c->pool) & 15) ? OJX_ERR_ARG : OJX_OK;
+}
+inline Q4Cache q4_cache(const OjasxQ4Cache* c, const int* table, int max_pages) {
+    return {static_cast<uint8_t*>(c->pool), table, c->status, max_pages, c->num_pages, c->page_size, c->kv_heads};
 }
 inline bool q4_aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 

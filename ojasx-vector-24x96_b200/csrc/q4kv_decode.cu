@@ -557,22 +557,22 @@ using namespace ojx;
 
 extern "C" {
 
-size_t ojasx_b200_q4kv_decode_workspace(int batch, int max_pages, int page_size, int kv_heads, int q_heads, int head_dim, int io_dtype) {
-    if (batch <= 0 || max_pages <= 0 || page_size <= 0 || kv_heads <= 0 || q_heads <= 0) return 0;
-    return q4_decode_bytes(q4_decode_ctas(batch, max_pages, page_size, kv_heads, q_heads / kv_heads, io_dtype), head_dim);
+size_t ojasx_b200_q4kv_decode_workspace(const OjasxQ4Cache* cache, int batch, int max_pages, int io_dtype) {
+    if (!cache || batch <= 0 || max_pages <= 0 || cache->page_size <= 0 || cache->kv_heads <= 0 || cache->q_heads <= 0) return 0;
+    return q4_decode_bytes(q4_decode_ctas(batch, max_pages, cache->page_size, cache->kv_heads, cache->q_heads / cache->kv_heads, io_dtype), cache->head_dim);
 }
 
-int ojasx_b200_q4kv_decode(const void* d_q, void* d_out, const void* d_pool, const int* d_block_table, const int* d_lengths, int* d_status,
-                           int batch, int max_pages, int num_pages, int page_size, int kv_heads, int q_heads, int head_dim, float scale,
-                           int io_dtype, void* workspace, size_t workspace_bytes, void* stream) {
-    const int rc = q4_check(d_pool, d_block_table, max_pages, num_pages, page_size, kv_heads, head_dim, batch, io_dtype, d_status);
+int ojasx_b200_q4kv_decode(const OjasxQ4Cache* cache, const void* d_q, void* d_out, const int* d_block_table, int max_pages, const int* d_lengths,
+                           int batch, float scale, int io_dtype, void* workspace, size_t workspace_bytes, void* stream) {
+    const int rc = q4_check(cache, d_block_table, max_pages, batch, io_dtype);
     if (rc != OJX_OK) return rc;
-    if (!d_q || !d_out || !d_lengths || q_heads <= 0 || q_heads % kv_heads || !q4_aligned(d_q) || !q4_aligned(d_out)) return OJX_ERR_ARG;
-    const int share = q_heads / kv_heads, ctas = q4_decode_ctas(batch, max_pages, page_size, kv_heads, share, io_dtype);
+    const int kv_heads = cache->kv_heads, q_heads = cache->q_heads, head_dim = cache->head_dim;
+    if (!d_q || !d_out || !d_lengths || !q4_aligned(d_q) || !q4_aligned(d_out)) return OJX_ERR_ARG;
+    const int share = q_heads / kv_heads, ctas = q4_decode_ctas(batch, max_pages, cache->page_size, kv_heads, share, io_dtype);
     if (!workspace || !q4_aligned(workspace) || workspace_bytes < q4_decode_bytes(ctas, head_dim)) return OJX_ERR_ARG;
     if ((long long)batch * q_heads > 0x7fffffffLL) return OJX_ERR_TOO_LARGE;
     Q4DecodeProblem P{};
-    P.cache = {static_cast<uint8_t*>(const_cast<void*>(d_pool)), d_block_table, d_status, max_pages, num_pages, page_size, kv_heads};
+    P.cache = q4_cache(cache, d_block_table, max_pages);
     P.q = d_q; P.out = d_out; P.lengths = d_lengths; P.batch = batch; P.q_heads = q_heads; P.share = share;
     P.blocks = (share + kQdHeads - 1) / kQdHeads;
     P.pieces = static_cast<int2*>(workspace);

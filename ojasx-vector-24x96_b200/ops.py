@@ -1,13 +1,14 @@
 """Device-tensor operators over the ojasx_b200_* entry points (torch supplies memory and streams only)."""
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 from typing import Optional, Sequence
 
 import numpy as np
 import torch
 
-from ._lib import OjasxB200Error, check, lib
+from ._lib import OjasxB200Error, Q4Cache, check, lib
 
 _vp = C.c_void_p
 F32, BF16 = 0, 1
@@ -437,38 +438,42 @@ class VQKVCache:
             pass
 
 
-def _index32(t: torch.Tensor, name: str, shape, device) -> torch.Tensor:
-    """An int32 tensor of a call: on the call's device, contiguous, of the given shape."""
-    _require_cuda(t, name)
-    if t.dtype is not torch.int32 or tuple(t.shape) != tuple(shape) or t.device != device or not t.is_contiguous():
+# The calls below are a few microseconds of GPU work for a single token, so what is checked is asked for once.
+_DTYPE_CODES = {torch.float32: F32, torch.bfloat16: BF16}
+
+
+def _on_device(device) -> "contextlib.AbstractContextManager":
+    """Makes the device of a call's tensors the current one where it is not."""
+    return _HERE if device.index == torch._C._cuda_getDevice() else torch.cuda.device(device)
+
+
+_HERE = contextlib.nullcontext()
+
+
+def _index32(t: torch.Tensor, name: str, shape, device) -> int:
+    """Address of an int32 tensor of a call: on the call's device, contiguous, of the given shape."""
+    if t.dtype is not torch.int32 or t.shape != shape or t.device != device or not t.is_contiguous():
+        _require_cuda(t, name)
         raise ValueError(f"{name} must be a contiguous int32 tensor of shape {tuple(shape)} on {device}")
-    return t
+    return t.data_ptr()
 
 
-def _heads(t: torch.Tensor, name: str, rows: int, heads: int, head_dim: int, like: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """Activations [rows, heads, head_dim] of a call, float32 or bfloat16 like the others."""
-    _require_cuda(t, name)
-    _dtype_code(t)
-    if tuple(t.shape) != (rows, heads, head_dim):
-        raise ValueError(f"{name} must have the shape {(rows, heads, head_dim)}, got {tuple(t.shape)}")
-    if like is not None and (t.dtype != like.dtype or t.device != like.device):
-        raise ValueError(f"{name} must have the dtype and the device of the other activations")
-    return t
-
-
-def _rows(t: torch.Tensor) -> torch.Tensor:
-    """``t`` itself where its heads lie behind one another in rows on 16-byte boundaries (a view into a fused projection does), a copy
-    else."""
-    unit = 16 // t.element_size()
-    fits = t.stride(2) == 1 and t.stride(1) == t.shape[2] and t.stride(0) % unit == 0 and t.stride(0) >= t.shape[1] * t.shape[2] and t.data_ptr() % 16 == 0
-    if t.numel() == 0 or fits:
+def _rows(t: torch.Tensor, name: str, shape, dtype, device) -> torch.Tensor:
+    """Activations of a call, ``shape`` [rows, heads, head_dim]: ``t`` itself where its heads lie behind one another in rows on 16-byte
+    boundaries (a view into a fused projection does), a copy else."""
+    if t.shape != shape or t.dtype is not dtype or t.device != device:
+        _require_cuda(t, name)
+        _dtype_code(t)
+        raise ValueError(f"{name} must be {dtype} of shape {tuple(shape)} on {device}, got {t.dtype} of {tuple(t.shape)} on {t.device}")
+    row, head, unit = t.stride()
+    if unit == 1 and head == shape[2] and row % (16 // t.element_size()) == 0 and row >= head * shape[1] and t.data_ptr() % 16 == 0:
         return t
-    return t.clone(memory_format=torch.contiguous_format)
+    return t.clone(memory_format=torch.contiguous_format) if t.numel() else t
 
 
 def _out(out: Optional[torch.Tensor], like: torch.Tensor) -> torch.Tensor:
     if out is None:
-        return torch.empty(like.shape, device=like.device, dtype=like.dtype)
+        return torch.empty_like(like, memory_format=torch.contiguous_format)
     if out.shape != like.shape or out.dtype != like.dtype or out.device != like.device or not out.is_contiguous() or out.data_ptr() % 16:
         raise ValueError("out must be contiguous, 16-byte aligned and of the shape, dtype and device of q")
     return out
@@ -504,6 +509,10 @@ class Q4PagedKVCache:
         if rope_theta is not None:
             j = np.arange(self.head_dim // 2, dtype=np.float64)
             self._turns = torch.from_numpy(float(rope_theta) ** (-2.0 * j / self.head_dim) / (2.0 * np.pi)).to(self.device)
+        self._c = Q4Cache(self.pool.data_ptr(), self._status.data_ptr(), 0 if self._turns is None else self._turns.data_ptr(), self.num_pages,
+                          self.page_size, self.kv_heads, self.q_heads, self.head_dim)
+        self._cache = C.addressof(self._c)
+        self._sizes = {}      # workspace of a decode by batch, pages per sequence and dtype
 
     @property
     def memory_bytes(self) -> int:
@@ -556,76 +565,83 @@ class Q4PagedKVCache:
                 "v_codes": split(halves, 4).reshape(*shape, -1), "v_scales": bf16((vm << 16) >> 16), "v_mins": bf16(vm >> 16)}
 
     # ------------------------------------------------------------------ the calls of a model
-    def _table(self, block_table: torch.Tensor, rows: Optional[int] = None) -> torch.Tensor:
-        if block_table.dim() != 2 or block_table.shape[1] == 0 or (rows is not None and block_table.shape[0] != rows):
-            raise ValueError("block_table must be [batch, pages per sequence], a row for every sequence")
-        return _index32(block_table, "block_table", block_table.shape, self.device)
+    def _table(self, block_table: torch.Tensor) -> int:
+        shape = block_table.shape
+        if len(shape) != 2 or shape[1] == 0:
+            raise ValueError("block_table must be [batch, pages per sequence]")
+        return _index32(block_table, "block_table", shape, self.device)
 
     def append(self, k: torch.Tensor, v: torch.Tensor, block_table: torch.Tensor, positions: torch.Tensor,
                q: Optional[torch.Tensor] = None, cu_seqlens: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
         """``k``, ``v`` [tokens, kv_heads, head_dim] behind the ``positions[b]`` tokens that sequence b has: one token per sequence, or
         with ``cu_seqlens`` int32 [batch + 1] the packed tokens ``cu_seqlens[b] .. cu_seqlens[b + 1]``.  ``q``
         [tokens, q_heads, head_dim] is turned as the keys are and returned (its rows behind the last sequence are not written)."""
+        table, dtype, dev = self._table(block_table), k.dtype, self.device
         B, n = block_table.shape[0], k.shape[0]
-        table = self._table(block_table)
-        _heads(k, "k", n, self.kv_heads, self.head_dim)
-        _heads(v, "v", n, self.kv_heads, self.head_dim, k)
-        if k.device != self.device:
-            raise ValueError(f"the cache is on {self.device}")
+        if dtype not in _DTYPE_CODES:
+            _dtype_code(k)
+        shape = (n, self.kv_heads, self.head_dim)
+        k, v = _rows(k, "k", shape, dtype, dev), _rows(v, "v", shape, dtype, dev)
         if cu_seqlens is None and n != B:
             raise ValueError("one token per sequence, or cu_seqlens")
-        positions = _index32(positions, "positions", (B,), self.device)
-        ends = None if cu_seqlens is None else _index32(cu_seqlens, "cu_seqlens", (B + 1,), self.device).data_ptr()
-        k, v, out = _rows(k), _rows(v), None
+        at = _index32(positions, "positions", (B,), dev)
+        ends = None if cu_seqlens is None else _index32(cu_seqlens, "cu_seqlens", (B + 1,), dev)
+        out, qp, qs, op = None, None, 0, None
         if q is not None:
-            q = _rows(_heads(q, "q", n, self.q_heads, self.head_dim, k))
-            out = torch.empty(q.shape, device=q.device, dtype=q.dtype)
+            q = _rows(q, "q", (n, self.q_heads, self.head_dim), dtype, dev)
+            out = torch.empty_like(q, memory_format=torch.contiguous_format)
+            qp, qs, op = q.data_ptr(), q.stride(0), out.data_ptr()
         if n and B:
-            with torch.cuda.device(self.device):
-                check(lib().ojasx_b200_q4kv_append(k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0), None if q is None else q.data_ptr(),
-                                                   0 if q is None else q.stride(0), None if q is None else out.data_ptr(), self.pool.data_ptr(),
-                                                   table.data_ptr(), positions.data_ptr(), ends, None if self._turns is None else self._turns.data_ptr(),
-                                                   self._status.data_ptr(), n, B, table.shape[1], self.num_pages, self.page_size, self.kv_heads,
-                                                   self.q_heads, self.head_dim, _dtype_code(k), _stream_ptr(self.device)), "ojasx_b200_q4kv_append")
+            with _on_device(dev):
+                rc = lib().ojasx_b200_q4kv_append(self._cache, k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0), qp, qs, op, table,
+                                                  block_table.shape[1], at, ends, n, B, _DTYPE_CODES[dtype], _stream_ptr(dev))
+            if rc:
+                check(rc, "ojasx_b200_q4kv_append")
         return out
 
     def read(self, block_table: torch.Tensor, cu_seqlens: torch.Tensor, tokens: int, positions: Optional[torch.Tensor] = None,
              dtype: torch.dtype = torch.bfloat16):
         """(k, v) [tokens, kv_heads, head_dim]: the values of ``cu_seqlens[b + 1] - cu_seqlens[b]`` tokens of every sequence, from
         ``positions[b]`` (default 0) on.  Rows behind the last sequence are not written."""
-        table, B = self._table(block_table), block_table.shape[0]
-        ends = _index32(cu_seqlens, "cu_seqlens", (B + 1,), self.device)
-        positions = None if positions is None else _index32(positions, "positions", (B,), self.device).data_ptr()
-        k = torch.empty((int(tokens), self.kv_heads, self.head_dim), device=self.device, dtype=dtype)
+        table, B, dev = self._table(block_table), block_table.shape[0], self.device
+        ends = _index32(cu_seqlens, "cu_seqlens", (B + 1,), dev)
+        at = None if positions is None else _index32(positions, "positions", (B,), dev)
+        if dtype not in _DTYPE_CODES:
+            raise TypeError(f"values are read as float32 or bfloat16, not {dtype}")
+        k = torch.empty((int(tokens), self.kv_heads, self.head_dim), device=dev, dtype=dtype)
         v = torch.empty_like(k)
         if tokens and B:
-            with torch.cuda.device(self.device):
-                check(lib().ojasx_b200_q4kv_read(self.pool.data_ptr(), table.data_ptr(), ends.data_ptr(), positions, k.data_ptr(), v.data_ptr(),
-                                                 self._status.data_ptr(), int(tokens), B, table.shape[1], self.num_pages, self.page_size,
-                                                 self.kv_heads, self.head_dim, _dtype_code(k), _stream_ptr(self.device)), "ojasx_b200_q4kv_read")
+            with _on_device(dev):
+                rc = lib().ojasx_b200_q4kv_read(self._cache, table, block_table.shape[1], ends, at, k.data_ptr(), v.data_ptr(), int(tokens), B,
+                                                _DTYPE_CODES[dtype], _stream_ptr(dev))
+            if rc:
+                check(rc, "ojasx_b200_q4kv_read")
         return k, v
 
     def decode(self, q: torch.Tensor, block_table: torch.Tensor, lengths: torch.Tensor, scale: float = -1.0,
                out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """One query per sequence, ``q`` [batch, q_heads, head_dim], over the first ``lengths[b]`` tokens of its sequence (zeros for an
         empty one); ``scale <= 0`` is 1/sqrt(head_dim)."""
-        B = q.shape[0]
-        table = self._table(block_table, B)
-        q = _heads(q, "q", B, self.q_heads, self.head_dim)
-        if q.device != self.device:
-            raise ValueError(f"the cache is on {self.device}")
-        q = q if q.is_contiguous() and q.data_ptr() % 16 == 0 else q.clone(memory_format=torch.contiguous_format)
-        lengths = _index32(lengths, "lengths", (B,), self.device)
+        table, dtype, dev = self._table(block_table), q.dtype, self.device
+        B, pages = block_table.shape
+        if dtype not in _DTYPE_CODES:
+            _dtype_code(q)
+        q = _rows(q, "q", (B, self.q_heads, self.head_dim), dtype, dev)
+        if not q.is_contiguous():
+            q = q.contiguous()
+        n = _index32(lengths, "lengths", (B,), dev)
         o = _out(out, q)
         if B:
-            size = lib().ojasx_b200_q4kv_decode_workspace(B, table.shape[1], self.page_size, self.kv_heads, self.q_heads, self.head_dim,
-                                                          _dtype_code(q))
-            ws = torch.empty(size, device=self.device, dtype=torch.uint8)     # of this call, so that calls on several streams do not share it
-            with torch.cuda.device(self.device):
-                check(lib().ojasx_b200_q4kv_decode(q.data_ptr(), o.data_ptr(), self.pool.data_ptr(), table.data_ptr(), lengths.data_ptr(),
-                                                   self._status.data_ptr(), B, table.shape[1], self.num_pages, self.page_size, self.kv_heads,
-                                                   self.q_heads, self.head_dim, float(scale), _dtype_code(q), ws.data_ptr(), size,
-                                                   _stream_ptr(self.device)), "ojasx_b200_q4kv_decode")
+            key = (B, pages, dtype)
+            size = self._sizes.get(key)
+            if size is None:
+                size = self._sizes[key] = lib().ojasx_b200_q4kv_decode_workspace(self._cache, B, pages, _DTYPE_CODES[dtype])
+            ws = torch.empty(size, device=dev, dtype=torch.uint8)     # of this call, so that calls on several streams do not share it
+            with _on_device(dev):
+                rc = lib().ojasx_b200_q4kv_decode(self._cache, q.data_ptr(), o.data_ptr(), table, pages, n, B, scale, _DTYPE_CODES[dtype],
+                                                  ws.data_ptr(), size, _stream_ptr(dev))
+            if rc:
+                check(rc, "ojasx_b200_q4kv_decode")
         return o
 
     def prefill(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, block_table: torch.Tensor, positions: torch.Tensor,
@@ -648,28 +664,34 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     if q.dim() != 3 or k.dim() != 3 or k.shape[1] == 0 or q.shape[1] % k.shape[1]:
         raise ValueError("q must be [tokens, q_heads, head_dim] and k [keys, kv_heads, head_dim], q_heads a multiple of kv_heads")
     T, Hq, hd = q.shape
+    M, Hkv, _ = k.shape
+    dtype, dev = q.dtype, q.device
     if hd not in (64, 128):
         raise ValueError("head_dim must be 64 or 128")
-    if Hq // k.shape[1] > 64:
+    if Hq // Hkv > 64:
         raise ValueError("at most 64 query heads share a KV head")
-    _heads(q, "q", T, Hq, hd)
-    _heads(k, "k", k.shape[0], k.shape[1], hd, q)
-    _heads(v, "v", k.shape[0], k.shape[1], hd, q)
+    _require_cuda(q, "q")
+    if dtype not in _DTYPE_CODES:
+        _dtype_code(q)
     if cu_seqlens.dim() != 1 or cu_seqlens.shape[0] < 1:
         raise ValueError("cu_seqlens must be [batch + 1]")
     B = cu_seqlens.shape[0] - 1
-    ends = _index32(cu_seqlens, "cu_seqlens", (B + 1,), q.device)
-    if cu_keys is None and k.shape[0] != T:
+    ends = _index32(cu_seqlens, "cu_seqlens", (B + 1,), dev)
+    if cu_keys is None and M != T:
         raise ValueError("as many keys as queries, or cu_keys")
-    key_ends = ends if cu_keys is None else _index32(cu_keys, "cu_keys", (B + 1,), q.device)
+    key_ends = ends if cu_keys is None else _index32(cu_keys, "cu_keys", (B + 1,), dev)
+    q = _rows(q, "q", (T, Hq, hd), dtype, dev)
+    k, v = _rows(k, "k", (M, Hkv, hd), dtype, dev), _rows(v, "v", (M, Hkv, hd), dtype, dev)
     o = _out(out, q)
-    q, k, v = _rows(q), _rows(k), _rows(v)
     if T and B:
-        size = lib().ojasx_b200_prompt_workspace(k.shape[0], k.shape[1], hd, _dtype_code(q))
-        ws = torch.empty(size, device=q.device, dtype=torch.uint8) if size else None
-        with torch.cuda.device(q.device):
-            check(lib().ojasx_b200_prompt_attention(q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(),
-                                                    v.stride(0), v.stride(1), o.data_ptr(), ends.data_ptr(), key_ends.data_ptr(), B, T, k.shape[0],
-                                                    Hq, k.shape[1], hd, float(scale), _dtype_code(q), None if ws is None else ws.data_ptr(), size,
-                                                    _stream_ptr(q.device)), "ojasx_b200_prompt_attention")
+        size, ws = 0, None
+        if dtype is torch.float32:
+            size = lib().ojasx_b200_prompt_workspace(M, Hkv, hd, F32)
+            ws = torch.empty(size, device=dev, dtype=torch.uint8)
+        with _on_device(dev):
+            rc = lib().ojasx_b200_prompt_attention(q.data_ptr(), q.stride(0), hd, k.data_ptr(), k.stride(0), hd, v.data_ptr(), v.stride(0), hd,
+                                                   o.data_ptr(), ends, key_ends, B, T, M, Hq, Hkv, hd, scale, _DTYPE_CODES[dtype],
+                                                   None if ws is None else ws.data_ptr(), size, _stream_ptr(dev))
+        if rc:
+            check(rc, "ojasx_b200_prompt_attention")
     return o

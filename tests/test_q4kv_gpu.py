@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from ojasx_b200 import ops
-from ojasx_b200._lib import OjasxB200Error, lib
+from ojasx_b200._lib import OjasxB200Error, Q4Cache, lib
 
 from q4_plain import attend, gather, quantize, random_pool, random_table, rotate, tolerance, values
 
@@ -32,23 +32,37 @@ def _randn(g, *shape, dtype=torch.float32):
 # ---------------------------------------------------------------------------------------------- refusals (no GPU)
 
 def test_c_entries_refuse_missing_and_unfit_arguments():
+    import ctypes as C
     L = lib()
     one = 4096   # an address that no call gets as far as using
-    append = lambda **kw: L.ojasx_b200_q4kv_append(*{**dict(k=one, ks=128, v=one, vs=128, q=None, qs=0, qo=None, pool=one, table=one, pos=one,
-             ends=None, turns=None, status=one, n=1, b=1, mp=1, np_=1, ps=16, kv=1, qh=1, hd=128, io=0, st=None), **kw}.values())  # noqa: E731
-    for bad in (dict(k=None), dict(v=None), dict(pool=None), dict(table=None), dict(pos=None), dict(status=None), dict(n=2), dict(n=-1), dict(b=0),
-                dict(mp=0), dict(np_=0), dict(kv=0), dict(io=7), dict(k=one + 4), dict(ks=2), dict(pool=one + 8), dict(q=one), dict(q=one, qo=one, qh=0)):
+    kept = []
+
+    def cache(**kw):
+        c = Q4Cache(**{**dict(pool=one, status=one, turns=None, num_pages=1, page_size=16, kv_heads=2, q_heads=4, head_dim=128), **kw})
+        kept.append(c)
+        return C.addressof(c)
+
+    bad_caches = [(None, -1)] + [(cache(**kw), -1) for kw in (dict(pool=None), dict(status=None), dict(num_pages=0), dict(kv_heads=0), dict(q_heads=3),
+                                 dict(q_heads=0), dict(pool=one + 8))]
+    bad_caches += [(cache(**kw), -4) for kw in (dict(page_size=8), dict(page_size=24), dict(page_size=0), dict(head_dim=96), dict(head_dim=0))]
+    good = cache()
+    append = lambda **kw: L.ojasx_b200_q4kv_append(*{**dict(c=good, k=one, ks=128, v=one, vs=128, q=None, qs=0, qo=None, table=one, mp=1, pos=one,
+             ends=None, n=1, b=1, io=0, st=None), **kw}.values())  # noqa: E731
+    decode = lambda **kw: L.ojasx_b200_q4kv_decode(*{**dict(c=good, q=one, o=one, table=one, mp=1, n=one, b=1, sc=-1.0, io=1, ws=one, size=1 << 30,
+             st=None), **kw}.values())  # noqa: E731
+    read = lambda **kw: L.ojasx_b200_q4kv_read(*{**dict(c=good, table=one, mp=1, ends=one, pos=None, k=one, v=one, n=1, b=1, io=0, st=None),
+                                               **kw}.values())  # noqa: E731
+    for call in (append, decode, read):
+        for c, code in bad_caches:
+            assert call(c=c) == code
+        for bad in (dict(table=None), dict(mp=0), dict(b=0), dict(io=7)):
+            assert call(**bad) == -1, bad
+        assert call(c=cache(page_size=4096), mp=1 << 20) == -5
+    for bad in (dict(k=None), dict(v=None), dict(pos=None), dict(n=2), dict(n=-1), dict(k=one + 4), dict(ks=2), dict(q=one), dict(q=one, qo=one + 8)):
         assert append(**bad) == -1, bad
-    for bad in (dict(ps=8), dict(ps=24), dict(ps=0), dict(hd=96), dict(hd=0)):
-        assert append(**bad) == -4, bad
-    assert append(mp=1 << 20, ps=4096) == -5
     assert append(n=0, ends=one) == 0
-    decode = lambda **kw: L.ojasx_b200_q4kv_decode(*{**dict(q=one, o=one, pool=one, table=one, n=one, status=one, b=1, mp=1, np_=1, ps=16, kv=2, qh=4,
-             hd=64, sc=-1.0, io=1, ws=one, size=1 << 30, st=None), **kw}.values())  # noqa: E731
-    for bad in (dict(q=None), dict(o=None), dict(n=None), dict(qh=3), dict(qh=0), dict(q=one + 2), dict(o=one + 8), dict(ws=None), dict(size=1000), dict(ws=one + 4)):
+    for bad in (dict(q=None), dict(o=None), dict(n=None), dict(q=one + 2), dict(o=one + 8), dict(ws=None), dict(size=1000), dict(ws=one + 4)):
         assert decode(**bad) == -1, bad
-    read = lambda **kw: L.ojasx_b200_q4kv_read(*{**dict(pool=one, table=one, ends=one, pos=None, k=one, v=one, status=one, n=1, b=1, mp=1, np_=1, ps=16,
-             kv=1, hd=64, io=0, st=None), **kw}.values())  # noqa: E731
     for bad in (dict(ends=None), dict(k=None), dict(v=one + 1), dict(n=-1)):
         assert read(**bad) == -1, bad
     assert read(n=0) == 0

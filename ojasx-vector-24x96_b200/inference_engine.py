@@ -1,5 +1,6 @@
 """Decode driver over the split-manifold kernels: a random-initialised decoder stack whose every linear
-(q, k, v, o, the 512-expert MoE, lm_head) is VQ-coded and whose KV cache is codebook-quantised, with the
+(q, k, v, o, the 512-expert MoE, lm_head) is VQ-coded and whose KV cache is codebook-quantised or, with
+``StackConfig(kv_format="q4")``, in 4-bit pages, with the
 method names of the reference engines (``OjasXInferenceEngine.prefill / decode_step / generate``,
 ``ojasx_24x96/engine.py:153-369``; greedy = arg-max of the logits, ``:213-214``; entry class
 ``UniversalInferenceEngine``, ``ojasx_24x96/inference_engine.py:149-389``).
@@ -21,7 +22,7 @@ import torch
 from torch import nn
 
 from . import synth
-from .ops import VQKVCache, VQLinear, VQLinearGroup, VQMoE, add_int_, rmsnorm, rope_qk_
+from .ops import Q4PagedKVCache, VQKVCache, VQLinear, VQLinearGroup, VQMoE, add_int_, rmsnorm, rope_qk_
 
 
 @dataclass
@@ -41,6 +42,8 @@ class StackConfig:
     outlier_frac: float = 0.0038
     max_seq_len: int = 1024
     distinct_layers: int = 1     # host weight sets generated; device copies cycle through them
+    kv_format: str = "vq"        # the KV caches: "vq" codebook codes (8 bits a block), "q4" pages of 4-bit codes
+    page_size: int = 64          # tokens of a page of a "q4" cache
 
 
 @dataclass
@@ -102,8 +105,12 @@ class _Layer:
             self.qkv = VQLinearGroup([self.q, self.k, self.v]) if batch == 1 else None
             self.moe = VQMoE(w.moe)
             self.moe.reserve(batch, cfg.top_k)
-            self.cache = VQKVCache(batch, cfg.kv_heads, cfg.q_heads, cfg.head_dim, cfg.block_dim, cfg.max_seq_len,
-                                   w.k_codebook, w.v_codebook)
+            if cfg.kv_format == "q4":
+                self.cache = Q4PagedKVCache(batch * -(-cfg.max_seq_len // cfg.page_size), cfg.page_size, cfg.kv_heads, cfg.q_heads, cfg.head_dim,
+                                            rope_theta=cfg.rope_theta, device=device)
+            else:
+                self.cache = VQKVCache(batch, cfg.kv_heads, cfg.q_heads, cfg.head_dim, cfg.block_dim, cfg.max_seq_len,
+                                       w.k_codebook, w.v_codebook)
             return
         # One rank of several: its KV heads with their query heads, its rows of o_proj, its experts.  The three
         # exchanges of a layer (attention outputs, o_proj outputs, expert outputs) are fused into the producing kernels.
@@ -145,8 +152,13 @@ class VQDecoderStack:
         """``segment``: a ``sharding.PeerSegment`` makes this the stack of ONE rank of several GPUs: KV heads (with the
         q/k/v rows of their heads), o_proj rows, experts and lm_head rows are split over the ranks; hidden states are
         replicated; every exchange goes through the segment.  Every rank must drive its stack with the same calls."""
+        if cfg.kv_format not in ("vq", "q4"):
+            raise ValueError(f"kv_format must be 'vq' or 'q4', got {cfg.kv_format!r}")
+        if cfg.kv_format == "q4" and segment is not None:
+            raise ValueError("a stack split over several ranks keeps codebook caches (kv_format 'vq')")
         self.cfg, self.batch, self.dtype, self.use_graph = cfg, batch, dtype, use_graph
         self.segment = segment
+        self.q4 = cfg.kv_format == "q4"
         self.device = device or torch.device("cuda", torch.cuda.current_device())
         self.embed = torch.from_numpy(weights.embed).to(self.device)
         self.final_norm = torch.from_numpy(weights.final_norm).to(self.device)
@@ -166,21 +178,31 @@ class VQDecoderStack:
             self._mine = torch.empty((batch, 2), dtype=torch.float32, device=self.device)
             self._next = None
         self.gather_logits = True
-        self.pos = torch.zeros(batch, dtype=torch.int32, device=self.device)
+        # positions of the next tokens, and the lengths with them
+        self._places = torch.arange(2, dtype=torch.int32, device=self.device).view(2, 1).repeat(1, batch)
+        self.pos, self.lengths = self._places[0], self._places[1]
         self.position = 0
+        # one block table for the caches of all layers: every sequence has the pages for max_seq_len tokens
+        pages = -(-cfg.max_seq_len // cfg.page_size) if self.q4 else 1
+        self.block_table = torch.arange(batch * pages, dtype=torch.int32, device=self.device).view(batch, pages)
         self._graph = None
         self._moe_rows = batch       # tokens the MoE scratch of the layers is reserved for
         self._ids = torch.zeros(batch, dtype=torch.int64, device=self.device)
         self._logits = None
-        if use_graph:
+        if use_graph and not self.q4:
             for l in self.layers:
                 l.cache.set_static_plan(True)
 
     def reset(self) -> None:
-        for l in self.layers:
-            l.cache.reset()
-        self.pos.zero_()
+        if not self.q4:
+            for l in self.layers:
+                l.cache.reset()
+        self._move_to(0)
         self.position = 0
+
+    def _move_to(self, position: int) -> None:
+        self.pos.fill_(position)
+        self.lengths.fill_(position + 1)
 
     def named_quantized_ops(self):
         """(name, operator) of every VQ-coded operator of the stack, for audits."""
@@ -227,14 +249,17 @@ class VQDecoderStack:
                 q = l.q(a).view(B, cfg.q_heads, cfg.head_dim)
                 k = l.k(a).view(B, cfg.kv_heads, cfg.head_dim)
                 v = l.v(a).view(B, cfg.kv_heads, cfg.head_dim)
-            rope_qk_(q, k, self.pos, cfg.rope_theta)
-            l.cache.append(k, v)
-            att = l.cache.decode(q)
+            if self.q4:
+                att = l.cache.decode(l.cache.append(k, v, self.block_table, self.pos, q=q), self.block_table, self.lengths)
+            else:
+                rope_qk_(q, k, self.pos, cfg.rope_theta)
+                l.cache.append(k, v)
+                att = l.cache.decode(q)
             o = l.o(att.view(B, cfg.q_heads * cfg.head_dim))
             m = rmsnorm(h, l.norm2, cfg.rms_eps, add=o)
             pending = l.moe.forward_routed(m, cfg.top_k)
         a = rmsnorm(h, self.final_norm, cfg.rms_eps, add=pending)
-        add_int_(self.pos, 1)
+        add_int_(self._places, 1)
         return self.lm_head(a).float()
 
     def _enqueue_step_sharded(self, h: torch.Tensor) -> torch.Tensor:
@@ -291,9 +316,10 @@ class VQDecoderStack:
             torch.cuda.current_stream().wait_stream(side)
             torch.cuda.synchronize()
             # ... whose token is dropped again before the capture; a capture records launches, it runs nothing
-            for l in self.layers:
-                l.cache.crop(cached)
-            self.pos.fill_(cached)
+            if not self.q4:
+                for l in self.layers:
+                    l.cache.crop(cached)
+            self._move_to(cached)
             self._graph = torch.cuda.CUDAGraph()
             with torch.cuda.graph(self._graph):
                 self._logits = self._enqueue_step(self._ids)
@@ -333,14 +359,20 @@ class VQDecoderStack:
 
     def _prefill_chunk(self, ids: torch.Tensor) -> torch.Tensor:
         """``ids [batch, Sc]``: rows are ordered position-major (row = s * batch + b), so that the q, k, v and attention
-        rows of one position are contiguous ``[batch, heads, head_dim]`` blocks for the cache calls."""
+        rows of one position are contiguous ``[batch, heads, head_dim]`` blocks for the cache calls; with 4-bit caches sequence after
+        sequence, as their calls take packed prompts."""
         cfg, B = self.cfg, self.batch
         Sc = ids.shape[1]
         rows = B * Sc
         if rows > self._moe_rows:    # the MoE scratch grows: a captured step would keep pointers to the old one
             self._moe_rows, self._graph = rows, None
-        h = self.embed[ids.t().reshape(-1)].to(self.dtype)
-        pos_rows = (self.pos.view(1, B) + torch.arange(Sc, device=self.device, dtype=torch.int32).view(Sc, 1)).reshape(-1).contiguous()
+        h = self.embed[(ids if self.q4 else ids.t()).reshape(-1)].to(self.dtype)
+        if self.q4:
+            context = self.position + Sc
+            sequences = torch.arange(B + 1, device=self.device, dtype=torch.int32)
+            ends, context_ends = sequences * Sc, sequences * context
+        else:
+            pos_rows = (self.pos.view(1, B) + torch.arange(Sc, device=self.device, dtype=torch.int32).view(Sc, 1)).reshape(-1).contiguous()
         pending = None
         for l in self.layers:
             l.moe.reserve(rows, cfg.top_k)
@@ -348,16 +380,20 @@ class VQDecoderStack:
             q = l.q(a).view(rows, cfg.q_heads, cfg.head_dim)
             k = l.k(a).view(rows, cfg.kv_heads, cfg.head_dim)
             v = l.v(a).view(rows, cfg.kv_heads, cfg.head_dim)
-            rope_qk_(q, k, pos_rows, cfg.rope_theta)
-            q4, k4, v4 = (t.view(Sc, B, t.shape[1], cfg.head_dim) for t in (q, k, v))
-            att = l.cache.prefill(k4, v4, q4)
+            if self.q4:
+                att = l.cache.prefill(q, k, v, self.block_table, self.pos, ends, context_ends, B * context)
+            else:
+                rope_qk_(q, k, pos_rows, cfg.rope_theta)
+                q4, k4, v4 = (t.view(Sc, B, t.shape[1], cfg.head_dim) for t in (q, k, v))
+                att = l.cache.prefill(k4, v4, q4)
             o = l.o(att.view(rows, cfg.q_heads * cfg.head_dim))
             m = rmsnorm(h, l.norm2, cfg.rms_eps, add=o)
             pending = l.moe.forward_routed(m, cfg.top_k)
         a = rmsnorm(h, self.final_norm, cfg.rms_eps, add=pending)
-        add_int_(self.pos, Sc)
+        add_int_(self._places, Sc)
         self.position += Sc
-        return self.lm_head(a[(Sc - 1) * B:].contiguous()).float()
+        last = a.view(B, Sc, -1)[:, -1] if self.q4 else a[(Sc - 1) * B:]
+        return self.lm_head(last.contiguous()).float()
 
     @torch.no_grad()
     def generate(self, prompt_ids: torch.Tensor, max_new_tokens: int) -> torch.Tensor:

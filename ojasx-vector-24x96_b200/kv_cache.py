@@ -5,7 +5,9 @@ The reference manager watches whatever a HuggingFace model returns as ``past_key
 and trims it.  Here the caches are the codebook-quantised ``ops.VQKVCache`` objects of this package (one
 per decoder layer): the manager admits a sequence length against ``max_context_length``, reports the bytes
 the code storage occupies, and ``crop`` / ``reset`` act on the device-side lengths, so a cropped cache
-decodes over the shorter context.  Plain tensor structures (``((k, v), ...)`` tuples, lists, dicts) are
+decodes over the shorter context; a 4-bit paged cache (``ops.Q4PagedKVCache``) is counted with its pages, the
+lengths of its sequences are the caller's (``update(..., sequence_length=n)``, and a crop is a smaller length in the
+next call).  Plain tensor structures (``((k, v), ...)`` tuples, lists, dicts) are
 still counted and cropped along their sequence axis, which keeps callers of the reference class working.
 """
 from __future__ import annotations
@@ -15,7 +17,9 @@ from typing import Any, Dict, Iterable, List, Optional, Union
 
 import torch
 
-from .ops import VQKVCache
+from .ops import Q4PagedKVCache, VQKVCache
+
+_CACHES = (VQKVCache, Q4PagedKVCache)
 
 
 @dataclass(frozen=True)
@@ -36,7 +40,7 @@ def _walk(obj: Any, depth: int = 0) -> Iterable[Any]:
     """Leaves (tensors and quantised caches) of a nested cache structure."""
     if obj is None or depth > 12:
         return
-    if isinstance(obj, (torch.Tensor, VQKVCache)):
+    if isinstance(obj, (torch.Tensor, *_CACHES)):
         yield obj
     elif isinstance(obj, dict):
         for v in obj.values():
@@ -44,7 +48,7 @@ def _walk(obj: Any, depth: int = 0) -> Iterable[Any]:
     elif isinstance(obj, (list, tuple)):
         for v in obj:
             yield from _walk(v, depth + 1)
-    elif hasattr(obj, "cache") and isinstance(getattr(obj, "cache"), VQKVCache):   # a decoder layer of this package
+    elif hasattr(obj, "cache") and isinstance(getattr(obj, "cache"), _CACHES):   # a decoder layer of this package
         yield obj.cache
     elif hasattr(obj, "layers"):
         yield from _walk(getattr(obj, "layers"), depth + 1)
@@ -90,7 +94,7 @@ class OjasXKVCacheManager:
 
     @property
     def allocated_bytes(self) -> int:
-        caches = [l for l in self._leaves() if isinstance(l, VQKVCache)]
+        caches = [l for l in self._leaves() if isinstance(l, _CACHES)]
         return sum(c.memory_bytes for c in caches) + sum(t.numel() * t.element_size() for t in self.extract_live_tensors())
 
     @property
@@ -102,13 +106,15 @@ class OjasXKVCacheManager:
             return len(getattr(pkv, "layers"))
         if isinstance(pkv, (list, tuple)):
             return len(pkv)
-        return len([l for l in self._leaves() if isinstance(l, VQKVCache)])
+        return len([l for l in self._leaves() if isinstance(l, _CACHES)])
 
     @property
     def dtype(self) -> str:
         for leaf in self._leaves():
             if isinstance(leaf, VQKVCache):
                 return "uint8_codebook_vq"
+            if isinstance(leaf, Q4PagedKVCache):
+                return "uint4_groups"
             if isinstance(leaf, torch.Tensor):
                 return str(leaf.dtype).replace("torch.", "")
         return str(self.default_dtype).replace("torch.", "")
@@ -145,6 +151,8 @@ class OjasXKVCacheManager:
         def trim(obj: Any) -> Any:
             if isinstance(obj, VQKVCache):
                 obj.crop(max_length)
+                return obj
+            if isinstance(obj, Q4PagedKVCache):
                 return obj
             if isinstance(obj, torch.Tensor):
                 return obj[..., :max_length, :] if obj.ndim >= 2 and obj.shape[-2] > max_length else obj

@@ -395,7 +395,7 @@ OJASX_API int ojasx_b200_paged_kv_decode(const void* d_q, void* d_out, const int
 
 /* ---- 4-bit paged KV cache and attention over whole prompts (no counterpart in the reference, whose paged cache holds int8 and
  * whose attention is over padded batches, ojasx_24x96/long_context.py:92-279).  Tensors are device pointers, 16-byte aligned; row
- * strides in elements, multiples of 4.
+ * strides in elements, whole multiples of 16 bytes.
  *
  * Format: 32 consecutive dimensions of a token's key or value share a bf16 minimum (the largest not above their own) and a bf16
  * scale (the smallest not below (max - minimum) / 15); a value is a code 0..15 and reads as code * scale + minimum, within half a

@@ -16,6 +16,16 @@ __device__ __forceinline__ float4 q4_load4(const void* p, size_t i, bool bf16) {
     const uint2 w = *reinterpret_cast<const uint2*>(reinterpret_cast<const __nv_bfloat16*>(p) + i);
     return make_float4(__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xffff0000u), __uint_as_float(w.y << 16), __uint_as_float(w.y & 0xffff0000u));
 }
+__device__ __forceinline__ void q4_load8(const void* p, size_t i, bool bf16, float4& a, float4& b) {
+    if (!bf16) {
+        a = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(p) + i)[0];
+        b = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(p) + i)[1];
+        return;
+    }
+    const uint4 w = *reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(p) + i);
+    a = make_float4(__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xffff0000u), __uint_as_float(w.y << 16), __uint_as_float(w.y & 0xffff0000u));
+    b = make_float4(__uint_as_float(w.z << 16), __uint_as_float(w.z & 0xffff0000u), __uint_as_float(w.w << 16), __uint_as_float(w.w & 0xffff0000u));
+}
 __device__ __forceinline__ void q4_store4(void* p, size_t i, bool bf16, float4 v) {
     if (!bf16) {
         *reinterpret_cast<float4*>(reinterpret_cast<float*>(p) + i) = v;
@@ -36,13 +46,15 @@ __device__ __forceinline__ float q4_more(float a, float b) {
     return a;
 }
 
-// Four values of a group whose other 28 are with the neighbouring seven lanes, as nibbles; `meta`: the group's minimum and scale.
+// Eight consecutive values of a group whose other 24 are with the lanes whose numbers differ in bits 1 and 2, as nibbles of a word;
+// `meta`: the group's minimum and scale.
 // Quotients are those of IEEE division: with the rounded reciprocal r of s, q = v r, and q + (v - q s) r is v / s rounded (Markstein's
 // theorem) where nothing leaves the range of fp32, which the branch sees to.  v - minimum is not negative and at most 15 scales.
-__device__ __forceinline__ unsigned q4_encode(float4 x, unsigned& meta) {
-    float lo = q4_less(q4_less(x.x, x.y), q4_less(x.z, x.w)), hi = q4_more(q4_more(x.x, x.y), q4_more(x.z, x.w));
+__device__ __forceinline__ unsigned q4_encode(const float (&x)[8], unsigned& meta) {
+    float lo = q4_less(q4_less(q4_less(x[0], x[1]), q4_less(x[2], x[3])), q4_less(q4_less(x[4], x[5]), q4_less(x[6], x[7])));
+    float hi = q4_more(q4_more(q4_more(x[0], x[1]), q4_more(x[2], x[3])), q4_more(q4_more(x[4], x[5]), q4_more(x[6], x[7])));
 #pragma unroll
-    for (int off = 1; off < 8; off <<= 1) {
+    for (int off = 2; off < 8; off <<= 1) {
         lo = q4_less(lo, __shfl_xor_sync(0xffffffffu, lo, off));
         hi = q4_more(hi, __shfl_xor_sync(0xffffffffu, hi, off));
     }
@@ -50,28 +62,63 @@ __device__ __forceinline__ unsigned q4_encode(float4 x, unsigned& meta) {
     const float m = __uint_as_float(mb), range = hi - m;
     unsigned sb = (__float_as_uint(__fdiv_rn(range, 15.0f)) + 0xffffu) & 0xffff0000u;                          // up
     float s = __uint_as_float(sb);
-    unsigned code;
+    unsigned code = 0;
     if (s > 0x1p-90f && s < 0x1p90f) {
         const float r = __frcp_rn(s);
-        auto step = [&](float v) {   // rounded by an addition: the code is in the lowest bits
-            const float d = v - m, q = d * r;
-            return __float_as_uint(fmaf(fmaf(-q, s, d), r, q) + 12582912.0f) & 15u;
-        };
-        code = step(x.x) | step(x.y) << 4 | step(x.z) << 8 | step(x.w) << 12;
+        // rounded by an addition, which leaves a code in the lowest bits; what is above them adds up to a constant
+        constexpr float round = 12582912.0f;
+        constexpr unsigned above = 0x4b400000u * 0x11111111u;
+#pragma unroll
+        for (int i = 7; i >= 0; --i) {
+            const float d = x[i] - m, q = d * r;
+            code = code * 16u + __float_as_uint(fmaf(fmaf(-q, s, d), r, q) + round);
+        }
+        code -= above;
     } else {
-        const bool wide = isinf(range);   // beyond fp32: quotients first, then their difference
-        if (wide) sb = (__float_as_uint(hi / 15.0f - m / 15.0f) + 0xffffu) & 0xffff0000u;
-        s = __uint_as_float(sb);
-        const float d = s > 0.0f ? s : 1.0f;   // a group of one value that bf16 holds has no steps
-        auto step = [&](float v) { return (unsigned)fminf(fmaxf(rintf(wide ? v / d - m / d : __fdiv_rn(v - m, d)), 0.0f), 15.0f); };
-        code = step(x.x) | step(x.y) << 4 | step(x.z) << 8 | step(x.w) << 12;
-        if (!isfinite(lo) || !isfinite(hi) || isinf(m) || isinf(s)) {
+        if (!isfinite(lo) || !isfinite(hi)) {
             meta = 0x7fff0000u;
             return 0u;
         }
+        const bool wide = isinf(range);   // beyond fp32: quotients first, then their difference
+        if (wide) sb = (__float_as_uint(hi / 15.0f - m / 15.0f) + 0xffffu) & 0xffff0000u;
+        s = __uint_as_float(sb);
+        if (isinf(m) || isinf(s)) {
+            meta = 0x7fff0000u;
+            return 0u;
+        }
+        const float d = s > 0.0f ? s : 1.0f;   // a group of one value that bf16 holds has no steps
+#pragma unroll
+        for (int i = 7; i >= 0; --i) code = code << 4 | (unsigned)fminf(fmaxf(rintf(wide ? x[i] / d - m / d : __fdiv_rn(x[i] - m, d)), 0.0f), 15.0f);
     }
     meta = mb | sb >> 16;
     return code;
+}
+// From four values of either half of a vector (as the rotation has them) to eight consecutive ones: even lanes get the first half's.
+template <int HD>
+__device__ __forceinline__ void q4_gather(float4 a, float4 d, int l, float (&x)[8]) {
+    const bool odd = l & 1;
+    const float4 give = odd ? a : d;
+    const float4 got = make_float4(__shfl_xor_sync(0xffffffffu, give.x, 1), __shfl_xor_sync(0xffffffffu, give.y, 1), __shfl_xor_sync(0xffffffffu, give.z, 1),
+                                   __shfl_xor_sync(0xffffffffu, give.w, 1));
+    const float4 u = odd ? got : a, v = odd ? d : got;
+    x[0] = u.x; x[1] = u.y; x[2] = u.z; x[3] = u.w; x[4] = v.x; x[5] = v.y; x[6] = v.z; x[7] = v.w;
+}
+// The dimensions that lane l has then begin at this one.
+template <int HD>
+__device__ __forceinline__ int q4_first(int l) { return (l & 1) * (HD / 2) + (l >> 1) * 8; }
+
+// A token's eight dimensions from `d0` on, and their group's scale and minimum, into its tile.
+template <int HD>
+__device__ __forceinline__ void q4_put(unsigned char* tile, bool value, int in, int d0, unsigned code, unsigned meta) {
+    using T = Q4Layout<HD>;
+    const int g = d0 / 32, c = d0 % 32 / 4;
+    if (value) {
+        *reinterpret_cast<unsigned short*>(tile + T::value_at(in, g, c)) = (unsigned short)code;
+        *reinterpret_cast<unsigned short*>(tile + T::value_at(in, g, c + 1)) = (unsigned short)(code >> 16);
+    } else {
+        *reinterpret_cast<unsigned*>(tile + T::key_at(in, g, c)) = code;
+    }
+    if (c == 0) *reinterpret_cast<unsigned*>(tile + (value ? T::value_meta : T::key_meta) + T::meta_at(in, g)) = meta;
 }
 
 struct Q4AppendProblem {
@@ -105,8 +152,7 @@ __device__ __forceinline__ void q4_rotate(float4& a, float4& d, const float (&c)
 // position is asked for before it, the page while the angles are made.
 template <int HD, bool kBf16>
 __global__ void __launch_bounds__(128) q4_append_kernel(const __grid_constant__ Q4AppendProblem P) {
-    constexpr int L = HD / 8, G = HD / 32, V = 128 / L;
-    using T = Q4Layout<HD>;
+    constexpr int L = HD / 8, V = 128 / L;
     chain_begin();
     const int kv = P.cache.kv_heads, tasks = 2 * kv + (P.q ? P.q_heads : 0), parts = (tasks + V - 1) / V;
     const int token = blockIdx.x / parts, l = threadIdx.x % L, first = blockIdx.x % parts * V + threadIdx.x / L;
@@ -129,25 +175,19 @@ __global__ void __launch_bounds__(128) q4_append_kernel(const __grid_constant__ 
         q4_angles(P.turns, 4 * l, pos, c, s);
         q4_rotate(a, d, c, s);
     }
-    unsigned meta[2];
-    const unsigned code[2] = {q4_encode(a, meta[0]), q4_encode(d, meta[1])};
+    float x[8];
+    q4_gather<HD>(a, d, l, x);
+    unsigned meta;
+    const unsigned code = q4_encode(x, meta);
     if (first >= tasks) return;
     if (kind == 2) {
         const size_t to = ((size_t)token * P.q_heads + head) * HD + 4 * l;
         q4_store4(P.q_out, to, kBf16, a);
         q4_store4(P.q_out, to + HD / 2, kBf16, d);
-        return;
-    }
-    if (!tile) {
-        if (l == 0) atomicExch(P.cache.status, 1);
-        return;
-    }
-    const int in = pos % kQ4Tile;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        const int g = h * (G / 2) + l / 8;
-        *reinterpret_cast<unsigned short*>(tile + (kind ? T::value_at(in, g, l % 8) : T::key_at(in, g, l % 8))) = (unsigned short)code[h];
-        if (l % 8 == 0) *reinterpret_cast<unsigned*>(tile + (kind ? T::value_meta : T::key_meta) + T::meta_at(in, g)) = meta[h];
+    } else if (tile) {
+        q4_put<HD>(tile, kind == 1, pos % kQ4Tile, q4_first<HD>(l), code, meta);
+    } else if (l == 0) {
+        atomicExch(P.cache.status, 1);
     }
 }
 
@@ -178,7 +218,7 @@ static long long q4_spans(int rows, int batch) { return rows / kQ4Tile + 2LL * s
 // Prompts: a tile of 16 tokens per CTA and some of the heads, a token to HD / 8 lanes (or two of them at head_dim 64), which make its
 // angles once.  A head's tile is put together in shared memory and written in 16-byte pieces: its words hold two tokens each.
 template <int HD, bool kBf16>
-__global__ void __launch_bounds__(256) q4_append_tile_kernel(const __grid_constant__ Q4AppendProblem P, int slices) {
+__global__ void __launch_bounds__(256, 4) q4_append_tile_kernel(const __grid_constant__ Q4AppendProblem P, int slices) {
     constexpr int L = HD / 8, G = HD / 32, W = 256 / (kQ4Tile * L);   // W: vectors of a token at a time
     using T = Q4Layout<HD>;
     __shared__ __align__(16) unsigned char s_tile[2][W * T::bytes];
@@ -223,34 +263,30 @@ __global__ void __launch_bounds__(256) q4_append_tile_kernel(const __grid_consta
     }
     const int h0 = (int)((long long)kv * slice / slices), h1 = (int)((long long)kv * (slice + 1) / slices);
     if (!tile || h0 >= h1) return;
-    float4 x[2][2];   // [keys, values][halves]
+    // keys as the rotation wants them, values as they are encoded
+    const int d0 = q4_first<HD>(l);
+    float4 x[4];
     auto load = [&](int h) {
-#pragma unroll
-        for (int which = 0; which < 2; ++which) {
-            const size_t at = row * (which ? P.v_stride : P.k_stride) + (size_t)min(h, h1 - 1) * HD + 4 * l;
-            x[which][0] = q4_load4(which ? P.v : P.k, at, kBf16);
-            x[which][1] = q4_load4(which ? P.v : P.k, at + HD / 2, kBf16);
-        }
+        const size_t key = row * P.k_stride + (size_t)min(h, h1 - 1) * HD + 4 * l, value = row * P.v_stride + (size_t)min(h, h1 - 1) * HD + d0;
+        x[0] = q4_load4(P.k, key, kBf16);
+        x[1] = q4_load4(P.k, key + HD / 2, kBf16);
+        q4_load8(P.v, value, kBf16, x[2], x[3]);
     };
     load(h0 + w);
     int turn = 0;
     for (int h = h0; h < h1; h += W, turn ^= 1) {
         unsigned char* to = s_tile[turn] + w * T::bytes;
-        float4 y[2][2];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) y[i >> 1][i & 1] = x[i >> 1][i & 1];
+        float4 a = x[0], d = x[1];
+        const float values[8] = {x[2].x, x[2].y, x[2].z, x[2].w, x[3].x, x[3].y, x[3].z, x[3].w};
         if (h + W < h1) load(h + W + w);
-        if (P.turns) q4_rotate(y[0][0], y[0][1], c, s);
-#pragma unroll
-        for (int which = 0; which < 2; ++which)
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                const int g = half * (G / 2) + l / 8;
-                unsigned meta;
-                const unsigned code = q4_encode(y[which][half], meta);
-                *reinterpret_cast<unsigned short*>(to + (which ? T::value_at(in, g, l % 8) : T::key_at(in, g, l % 8))) = (unsigned short)code;
-                if (l % 8 == 0) *reinterpret_cast<unsigned*>(to + (which ? T::value_meta : T::key_meta) + T::meta_at(in, g)) = meta;
-            }
+        if (P.turns) q4_rotate(a, d, c, s);
+        float keys[8];
+        q4_gather<HD>(a, d, l, keys);
+        unsigned meta;
+        unsigned code = q4_encode(keys, meta);
+        q4_put<HD>(to, false, in, d0, code, meta);
+        code = q4_encode(values, meta);
+        q4_put<HD>(to, true, in, d0, code, meta);
         __syncthreads();   // (the other buffer's pieces were read before the barrier of the turn before)
         const int heads = min(W, h1 - h);
         if (S.from == 0 && S.to == kQ4Tile) {
@@ -306,14 +342,14 @@ __global__ void __launch_bounds__(256) q4_read_kernel(const __grid_constant__ Q4
         atomicExch(P.cache.status, 1);
     }
     __syncthreads();
-    const int tokens = S.to - S.from, eights = heads * (HD / 8);
-    for (int i = threadIdx.x; i < 2 * tokens * eights; i += 256) {
-        const int which = i / (tokens * eights), rem = i - which * tokens * eights, token = S.from + rem / eights, e = rem % eights;
-        const int head = e / (HD / 8), d8 = e % (HD / 8), g = d8 / 4, c = d8 % 4 * 2;
-        const unsigned char* from = s_tile + head * T::bytes;
+    // eight dimensions of a token and head per thread
+    constexpr int E = HD / 8, R = 256 / (2 * kQ4ReadHeads * E);   // R: tokens at a time
+    const int d8 = threadIdx.x % E, head = threadIdx.x / E % kQ4ReadHeads, which = threadIdx.x / (E * kQ4ReadHeads) % 2, g = d8 / 4, c = d8 % 4 * 2;
+    if (head >= heads) return;
+    const unsigned char* from = s_tile + head * T::bytes;
+    const size_t to0 = ((size_t)S.row * kv + h0 + head) * HD + d8 * 8;
+    for (int token = S.from + threadIdx.x / (E * kQ4ReadHeads * 2); token < S.to; token += R) {
         float x[8];
-#pragma unroll
-        for (int u = 0; u < 8; ++u) x[u] = 0.0f;
         if (tile) {
             unsigned word;
             if (which) word = *reinterpret_cast<const unsigned short*>(from + T::value_at(token, g, c)) | (unsigned)*reinterpret_cast<const unsigned short*>(from + T::value_at(token, g, c + 1)) << 16;
@@ -321,10 +357,13 @@ __global__ void __launch_bounds__(256) q4_read_kernel(const __grid_constant__ Q4
             const unsigned meta = *reinterpret_cast<const unsigned*>(from + (which ? T::value_meta : T::key_meta) + T::meta_at(token, g));
             const float s = q4_scale(meta), m = q4_min(meta);
 #pragma unroll
-            for (int u = 0; u < 8; ++u) x[u] = fmaf((float)(word >> (4 * u) & 15u), s, m);
+            for (int u = 0; u < 8; ++u) x[u] = fmaf(__uint_as_float(0x4b000000u | (word >> (4 * u) & 15u)) - 8388608.0f, s, m);
+        } else {
+#pragma unroll
+            for (int u = 0; u < 8; ++u) x[u] = 0.0f;
         }
         void* out = which ? P.v : P.k;
-        const size_t to = ((size_t)(S.row + token) * kv + h0 + head) * HD + d8 * 8;
+        const size_t to = to0 + (size_t)token * kv * HD;
         if (kBf16) {
             unsigned w[4];
 #pragma unroll
@@ -358,7 +397,7 @@ int ojasx_b200_q4kv_append(const OjasxQ4Cache* cache, const void* d_k, long long
     const int rc = q4_check(cache, d_block_table, max_pages, batch, io_dtype);
     if (rc != OJX_OK) return rc;
     if (!d_k || !d_v || !d_positions || n_tokens < 0 || (d_q && !d_q_out) || (!d_ends && n_tokens != batch)) return OJX_ERR_ARG;
-    if (!q4_aligned(d_k) || !q4_aligned(d_v) || !q4_aligned(d_q) || !q4_aligned(d_q_out) || k_stride % 4 || v_stride % 4 || q_stride % 4) return OJX_ERR_ARG;
+    if (!q4_aligned(d_k) || !q4_aligned(d_v) || !q4_aligned(d_q) || !q4_aligned(d_q_out) || (k_stride | v_stride | q_stride) % (io_dtype == OJX_BF16 ? 8 : 4)) return OJX_ERR_ARG;
     const int kv_heads = cache->kv_heads, q_heads = cache->q_heads, head_dim = cache->head_dim;
     if (n_tokens == 0) return OJX_OK;
     Q4AppendProblem P{};
@@ -369,7 +408,7 @@ int ojasx_b200_q4kv_append(const OjasxQ4Cache* cache, const void* d_k, long long
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (d_ends && n_tokens >= 4LL * batch) {
         const long long tiles = q4_spans(n_tokens, batch);
-        const int slices = (int)std::min<long long>(kv_heads, std::max<long long>(1, (4LL * num_sms() + tiles - 1) / tiles));   // some CTAs for every SM
+        const int slices = (int)std::min<long long>(kv_heads, std::max<long long>(1, (8LL * num_sms() + tiles - 1) / tiles));   // twice what the GPU holds
         if (tiles * slices > 0x7fffffffLL) return OJX_ERR_TOO_LARGE;
         auto kernel = head_dim == 64 ? (bf ? q4_append_tile_kernel<64, true> : q4_append_tile_kernel<64, false>)
                                      : (bf ? q4_append_tile_kernel<128, true> : q4_append_tile_kernel<128, false>);

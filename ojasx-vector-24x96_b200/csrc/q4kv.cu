@@ -118,7 +118,10 @@ __device__ __forceinline__ void q4_put(unsigned char* tile, bool value, int in, 
     } else {
         *reinterpret_cast<unsigned*>(tile + T::key_at(in, g, c)) = code;
     }
-    if (c == 0) *reinterpret_cast<unsigned*>(tile + (value ? T::value_meta : T::key_meta) + T::meta_at(in, g)) = meta;
+    if (c == 0) {
+        *reinterpret_cast<unsigned short*>(tile + (value ? T::value_scales : T::key_scales) + T::meta_at(in, g)) = (unsigned short)meta;
+        *reinterpret_cast<unsigned short*>(tile + (value ? T::value_mins : T::key_mins) + T::meta_at(in, g)) = (unsigned short)(meta >> 16);
+    }
 }
 
 struct Q4AppendProblem {
@@ -300,7 +303,7 @@ __global__ void __launch_bounds__(256, 4) q4_append_tile_kernel(const __grid_con
                 const int head = i / (kQ4Tile * pieces), token = i / pieces % kQ4Tile, piece = i % pieces, which = piece / (10 * G), p = piece % (10 * G);
                 if (token < S.from || token >= S.to) continue;
                 const int at = p < 8 * G ? (which ? T::value_at(token, p / 8, p % 8) : T::key_at(token, p / 8, p % 8))
-                                         : (which ? T::value_meta : T::key_meta) + T::meta_at(token, 0) + (p - 8 * G) * 2;
+                                         : (p < 9 * G ? (which ? T::value_scales : T::key_scales) - 8 * G * 2 : (which ? T::value_mins : T::key_mins) - 9 * G * 2) + T::meta_at(token, 0) + p * 2;
                 *reinterpret_cast<unsigned short*>(tile + (h + head) * head_bytes + at) = *reinterpret_cast<const unsigned short*>(s_tile[turn] + head * T::bytes + at);
             }
         }
@@ -354,8 +357,8 @@ __global__ void __launch_bounds__(256) q4_read_kernel(const __grid_constant__ Q4
             unsigned word;
             if (which) word = *reinterpret_cast<const unsigned short*>(from + T::value_at(token, g, c)) | (unsigned)*reinterpret_cast<const unsigned short*>(from + T::value_at(token, g, c + 1)) << 16;
             else word = *reinterpret_cast<const unsigned*>(from + T::key_at(token, g, c));
-            const unsigned meta = *reinterpret_cast<const unsigned*>(from + (which ? T::value_meta : T::key_meta) + T::meta_at(token, g));
-            const float s = q4_scale(meta), m = q4_min(meta);
+            const float s = q4_bf16(*reinterpret_cast<const unsigned short*>(from + (which ? T::value_scales : T::key_scales) + T::meta_at(token, g)));
+            const float m = q4_bf16(*reinterpret_cast<const unsigned short*>(from + (which ? T::value_mins : T::key_mins) + T::meta_at(token, g)));
 #pragma unroll
             for (int u = 0; u < 8; ++u) x[u] = fmaf(__uint_as_float(0x4b000000u | (word >> (4 * u) & 15u)) - 8388608.0f, s, m);
         } else {

@@ -9,10 +9,10 @@
 // [pages][kv_heads][tiles].  A tile is laid out as the operands of mma.sync m16n8k16 that the decode kernel makes of it, so that
 // every lane reads whole 8- or 16-byte pieces, G = head_dim / 32 groups:
 //   keys     [token][t = 0..3][g]: words; word (t, g) holds dimensions 32 g + 8 t + j in nibble j
-//   their    [token][g]: words, minimum << 16 | scale
+//   their    scales, minima [token][g]
 //   values   [half][c = 0..7][pair = 0..3][g]: words; tokens 8 half + 2 pair (low 16 bits) and + 1 (high 16 bits), dimensions
 //            32 g + 4 c + i in nibble i of either
-//   their    [token][g]: words, minimum << 16 | scale
+//   their    scales, minima [token][g]
 #pragma once
 #include "common.cuh"
 #include "../../include/ojasx_lut_b200.h"
@@ -25,16 +25,17 @@ constexpr int kQ4Tile = 16;    // tokens of a tile
 template <int HD>
 struct Q4Layout {
     static constexpr int G = HD / kQ4Group;
-    static constexpr int key_meta = kQ4Tile * HD / 2;
-    static constexpr int values = key_meta + kQ4Tile * G * 4;
-    static constexpr int value_meta = values + kQ4Tile * HD / 2;
-    static constexpr int bytes = value_meta + kQ4Tile * G * 4;
+    static constexpr int codes = kQ4Tile * HD / 2, metas = kQ4Tile * G * 2;
+    static constexpr int key_scales = codes, key_mins = key_scales + metas;
+    static constexpr int values = key_mins + metas;
+    static constexpr int value_scales = values + codes, value_mins = value_scales + metas;
+    static constexpr int bytes = value_mins + metas;
     // dimensions 32 g + 4 c .. + 3 of a token, as 16 bits
     __host__ __device__ static constexpr int key_at(int token, int g, int c) { return ((token * 4 + (c >> 1)) * G + g) * 4 + (c & 1) * 2; }
     __host__ __device__ static constexpr int value_at(int token, int g, int c) {
         return values + ((((token >> 3) * 8 + c) * 4 + ((token >> 1) & 3)) * G + g) * 4 + (token & 1) * 2;
     }
-    __host__ __device__ static constexpr int meta_at(int token, int g) { return (token * G + g) * 4; }   // from key_meta or value_meta
+    __host__ __device__ static constexpr int meta_at(int token, int g) { return (token * G + g) * 2; }   // from any of the four
 };
 
 struct Q4Cache {
@@ -55,8 +56,10 @@ __device__ __forceinline__ uint8_t* q4_tile(const Q4Cache& C, int b, int head, i
     return C.pool + (((size_t)id * C.kv_heads + head) * tiles + (token - p * C.page_size) / kQ4Tile) * Q4Layout<HD>::bytes;
 }
 
-__device__ __forceinline__ float q4_scale(unsigned meta) { return __uint_as_float(meta << 16); }
-__device__ __forceinline__ float q4_min(unsigned meta) { return __uint_as_float(meta & 0xffff0000u); }
+// A scale or minimum, and the two in a word.
+__device__ __forceinline__ float q4_bf16(unsigned short b) { return __uint_as_float((unsigned)b << 16); }
+__device__ __forceinline__ float q4_low(unsigned w) { return __uint_as_float(w << 16); }
+__device__ __forceinline__ float q4_high(unsigned w) { return __uint_as_float(w & 0xffff0000u); }
 
 // What every entry point asks of a cache.
 inline int q4_check(const OjasxQ4Cache* c, const int* table, int max_pages, int batch, int dtype) {

@@ -11,7 +11,7 @@
 //   O[dim][head]   += codes of V, transposed (16 x 16) x p * s_g (16 x 8)    p * s_g turned by movmatrix
 // A bf16 query is one fp16 number where a power of two brings the head's largest to 2^15 (what is 2^29 below it loses bits), an fp32
 // one two of them (22 bits); so is p * s, one with bf16 activations (11 bits, below the rounding of the result), two with fp32.  The
-// reference of the weights is the largest score plus the exponent of its token's largest scale, so that p * s is in the range of fp16
+// reference of the weights is the largest score plus the exponent of the largest scale so far, so that p * s is in the range of fp16
 // whatever the scales are.
 //
 // Work: units of 128 tokens of a (sequence, KV head, eight query heads), all of them in a row, in equal shares for the CTAs whatever the
@@ -49,6 +49,7 @@ struct Q4DecodeProblem {
 };
 
 template <int N> struct Q4Words;
+template <> struct Q4Words<1> { using type = unsigned; };
 template <> struct Q4Words<2> { using type = uint2; };
 template <> struct Q4Words<4> { using type = uint4; };
 
@@ -81,11 +82,27 @@ __device__ __forceinline__ unsigned q4_part(float& a, float& b) {
     b -= __high2float(h);
     return *reinterpret_cast<const unsigned*>(&h);
 }
-// Exponent of a positive fp32 number, kept in -20..100.
-__device__ __forceinline__ float q4_exponent(float s) {
-    const unsigned e = min(max(__float_as_uint(s) >> 23, 107u), 227u);
-    return __uint_as_float(0x4b000000u | e) - (8388608.0f + 127.0f);
+// Exponent of a positive bf16 number, kept in -20..100.
+__device__ __forceinline__ float q4_exponent(unsigned bits) { return (float)(min(max((int)(bits >> 7), 107), 227) - 127); }
+
+// Quotient of numbers that are not negative (64-bit division takes some hundred instructions).
+__device__ __forceinline__ long long q4_quotient(long long a, long long b) {
+    return (unsigned long long)a >> 32 ? a / b : (long long)((unsigned)a / (unsigned)b);
 }
+// All units in shares that differ by one at most, none of them empty.
+struct Q4Shares {
+    long long least, more;   // units of a share; shares with one more, the first ones
+    int n;
+    __device__ __forceinline__ Q4Shares(long long all, int ctas) : n((int)min((long long)ctas, all)) {
+        least = n ? q4_quotient(all, n) : 0;
+        more = all - least * n;
+    }
+    __device__ __forceinline__ long long first(int cta) const { return least * min(cta, n) + min((long long)min(cta, n), more); }
+    __device__ __forceinline__ int owner(long long unit) const {
+        const long long big = more * (least + 1);
+        return (int)(unit < big ? q4_quotient(unit, least + 1) : more + q4_quotient(unit - big, least));
+    }
+};
 
 // A place in the row of units: unit `u` of the `units` of sequence b for (KV head, block of query heads) `hh`.
 struct Q4Place {
@@ -111,7 +128,7 @@ struct QdSmem {
     static constexpr int bytes(int heads) { return kQdWarps * (ring + heads * row * 4); }
 };
 
-constexpr int kQdCtas(bool bf16) { return bf16 ? 4 : 3; }   // per SM
+constexpr int kQdCtas(bool) { return 3; }   // per SM
 
 template <int HD, bool kBf16>
 __global__ void __launch_bounds__(kQdThreads, kQdCtas(kBf16)) q4_decode_kernel(const __grid_constant__ Q4DecodeProblem P) {
@@ -119,6 +136,7 @@ __global__ void __launch_bounds__(kQdThreads, kQdCtas(kBf16)) q4_decode_kernel(c
     using T = Q4Layout<HD>;
     using M = QdSmem<HD>;
     using Words = typename Q4Words<G>::type;
+    using Metas = typename Q4Words<G / 2>::type;   // a token's scales or minima
     extern __shared__ __align__(128) unsigned char qd_smem[];
     __shared__ float s_m[kQdWarps][kQdHeads], s_l[kQdWarps][kQdHeads];
     __shared__ __align__(8) unsigned long long s_bar[kQdWarps][kQdStages];
@@ -135,12 +153,16 @@ __global__ void __launch_bounds__(kQdThreads, kQdCtas(kBf16)) q4_decode_kernel(c
 
     // this CTA's share of all units, and the place where it begins
     long long total = 0;
+    int mine = 0, upto = 0;   // units of the lane's sequence (of the last 32), and with those before it
     for (int b0 = 0; b0 < P.batch; b0 += 32) {
-        int n = b0 + lane < P.batch ? Q4Place::length_units(P, b0 + lane) : 0;
-        total += __reduce_add_sync(0xffffffffu, (unsigned)n);
+        mine = upto = b0 + lane < P.batch ? Q4Place::length_units(P, b0 + lane) : 0;
+#pragma unroll
+        for (int off = 1; off < 32; off <<= 1) {
+            const int o = __shfl_up_sync(0xffffffffu, upto, off);
+            if (lane >= off) upto += o;
+        }
+        total += __shfl_sync(0xffffffffu, upto, 31);
     }
-    const long long all = total * heads, n_ctas = min((long long)gridDim.x, all), cta = min((long long)blockIdx.x, n_ctas);
-    const long long first = cta < n_ctas ? all * cta / n_ctas : all, last = cta < n_ctas ? all * (cta + 1) / n_ctas : all;
     // an empty sequence has no units: its zeros come from here
     for (int b = blockIdx.x; b < P.batch; b += gridDim.x) {
         if (Q4Place::length(P, b) > 0) continue;
@@ -150,29 +172,32 @@ __global__ void __launch_bounds__(kQdThreads, kQdCtas(kBf16)) q4_decode_kernel(c
         }
     }
     if (tid == 0) P.pieces[blockIdx.x] = make_int2(-1, 0);
+    const Q4Shares shares(total * heads, gridDim.x);
+    const long long first = shares.first(blockIdx.x), last = shares.first(blockIdx.x + 1);
     if (first >= last) return;
     Q4Place at{0, 0, 0, 0};
     {
         long long before = 0;
         for (int b0 = 0; b0 < P.batch; b0 += 32) {
-            const int n = b0 + lane < P.batch ? Q4Place::length_units(P, b0 + lane) : 0;
-            int sum = n;
+            if (P.batch > 32) {   // (else they are there still)
+                mine = upto = b0 + lane < P.batch ? Q4Place::length_units(P, b0 + lane) : 0;
 #pragma unroll
-            for (int off = 1; off < 32; off <<= 1) {
-                const int o = __shfl_up_sync(0xffffffffu, sum, off);
-                if (lane >= off) sum += o;
+                for (int off = 1; off < 32; off <<= 1) {
+                    const int o = __shfl_up_sync(0xffffffffu, upto, off);
+                    if (lane >= off) upto += o;
+                }
             }
-            const unsigned in = __ballot_sync(0xffffffffu, first < (before + sum) * heads);
+            const unsigned in = __ballot_sync(0xffffffffu, first < (before + upto) * heads);
             if (in) {
                 const int src = __ffs(in) - 1;
                 at.b = b0 + src;
-                at.units = __shfl_sync(0xffffffffu, n, src);
-                const long long rest = first - (before + __shfl_sync(0xffffffffu, sum - n, src)) * heads;
-                at.hh = (int)(rest / at.units);
+                at.units = __shfl_sync(0xffffffffu, mine, src);
+                const long long rest = first - (before + __shfl_sync(0xffffffffu, upto - mine, src)) * heads;
+                at.hh = (int)q4_quotient(rest, at.units);
                 at.u = (int)(rest - (long long)at.hh * at.units);
                 break;
             }
-            before += __shfl_sync(0xffffffffu, sum, 31);
+            before += __shfl_sync(0xffffffffu, upto, 31);
         }
     }
     __syncwarp();
@@ -232,6 +257,13 @@ __global__ void __launch_bounds__(kQdThreads, kQdCtas(kBf16)) q4_decode_kernel(c
         return true;
     };
     int filled = 0, taken = 0;
+    {   // the first item's queries come while the pages are looked up
+        const int h0 = (at.hh % P.blocks) * kQdHeads;
+        const char* q = reinterpret_cast<const char*>(P.q) + (((size_t)at.b * P.q_heads + at.hh / P.blocks * P.share + h0 + gq) * HD + 8 * t) * (kBf16 ? 2 : 4);
+        if (h0 + gq < P.share)
+#pragma unroll
+            for (int g = 0; g < G; ++g) asm volatile("prefetch.global.L1 [%0];" ::"l"(q + g * 32 * (kBf16 ? 2 : 4)));
+    }
     enter();
     for (int i = 0; i < kQdStages; ++i) filled += fill(i);
 
@@ -312,6 +344,8 @@ __global__ void __launch_bounds__(kQdThreads, kQdCtas(kBf16)) q4_decode_kernel(c
 #pragma unroll
         for (int g = 0; g < G; ++g) mins[g][0] = mins[g][1] = 0.0f;
 
+        unsigned most = 0, bound = 0;                  // largest scales of the values, two at a time: seen by the lane, and in use
+        float above = -kQdSlack - kQdRoom;             // the exponent in use, less what p * s may be above the reference
         const int u0 = at.u, u1 = (int)min((long long)at.units, at.u + (last - unit));
         for (int u = u0; u < u1 && ok; ++u) {
             const int token = (u * kQdWarps + warp) * kQdPair * kQ4Tile;
@@ -324,21 +358,19 @@ __global__ void __launch_bounds__(kQdThreads, kQdCtas(kBf16)) q4_decode_kernel(c
             const int seen[2] = {none & 1 ? 0 : length - token, none & 2 ? 0 : length - token - kQ4Tile};
             const bool part = min(seen[0], seen[1]) < kQ4Tile;
             float x[kQdPair][4];
-            float now[2] = {kQdLowest, kQdLowest};
+            float now[2] = {-INFINITY, -INFINITY};
 #pragma unroll
             for (int i = 0; i < kQdPair; ++i) {
                 const unsigned char* tile = stage + i * T::bytes;
                 const Words ka = *reinterpret_cast<const Words*>(tile + (gq * 4 + t) * (4 * G)), kb = *reinterpret_cast<const Words*>(tile + ((gq + 8) * 4 + t) * (4 * G));
-                const Words ma = *reinterpret_cast<const Words*>(tile + T::key_meta + gq * (4 * G)), mb = *reinterpret_cast<const Words*>(tile + T::key_meta + (gq + 8) * (4 * G));
-                const Words va = *reinterpret_cast<const Words*>(tile + T::value_meta + gq * (4 * G)), vb = *reinterpret_cast<const Words*>(tile + T::value_meta + (gq + 8) * (4 * G));
+                const Metas ma = *reinterpret_cast<const Metas*>(tile + T::key_scales + T::meta_at(gq, 0)), mb = *reinterpret_cast<const Metas*>(tile + T::key_scales + T::meta_at(gq + 8, 0));
                 const unsigned *wa = reinterpret_cast<const unsigned*>(&ka), *wb = reinterpret_cast<const unsigned*>(&kb);
                 const unsigned *ca = reinterpret_cast<const unsigned*>(&ma), *cb = reinterpret_cast<const unsigned*>(&mb);
-                const unsigned *ua = reinterpret_cast<const unsigned*>(&va), *ub = reinterpret_cast<const unsigned*>(&vb);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) x[i][e] = 0.0f;
                 {   // sum_g m_g sum(q_g): the minima, bf16 as they are, times the sums in three parts
-                    const bool odd = G == 4 && (t & 1);
-                    const unsigned a = __byte_perm(odd ? ca[G - 2] : ca[0], odd ? ca[G - 1] : ca[1], 0x7632), b = __byte_perm(odd ? cb[G - 2] : cb[0], odd ? cb[G - 1] : cb[1], 0x7632);
+                    const int pair = G == 4 ? (t & 1) * 2 : 0;
+                    const unsigned a = *reinterpret_cast<const unsigned*>(tile + T::key_mins + T::meta_at(gq, pair)), b = *reinterpret_cast<const unsigned*>(tile + T::key_mins + T::meta_at(gq + 8, pair));
                     q4_mma(x[i], a, b, a, b, qs[0], qs[1]);
                 }
 #pragma unroll
@@ -352,28 +384,28 @@ __global__ void __launch_bounds__(kQdThreads, kQdCtas(kBf16)) q4_decode_kernel(c
                         gm_mma(c, {a[0], b[0], a[1], b[1]}, qf[p][g][0], qf[p][g][1]);
                         gm_mma(c, {a[2], b[2], a[3], b[3]}, qf[p][g][2], qf[p][g][3]);
                     }
-                    x[i][0] = fmaf(q4_scale(ca[g]), c[0], x[i][0]);
-                    x[i][1] = fmaf(q4_scale(ca[g]), c[1], x[i][1]);
-                    x[i][2] = fmaf(q4_scale(cb[g]), c[2], x[i][2]);
-                    x[i][3] = fmaf(q4_scale(cb[g]), c[3], x[i][3]);
+                    const float low = g & 1 ? q4_high(ca[g / 2]) : q4_low(ca[g / 2]), high = g & 1 ? q4_high(cb[g / 2]) : q4_low(cb[g / 2]);
+                    x[i][0] = fmaf(low, c[0], x[i][0]);
+                    x[i][1] = fmaf(low, c[1], x[i][1]);
+                    x[i][2] = fmaf(high, c[2], x[i][2]);
+                    x[i][3] = fmaf(high, c[3], x[i][3]);
                 }
+                Metas va = *reinterpret_cast<const Metas*>(tile + T::value_scales + T::meta_at(gq, 0)), vb = *reinterpret_cast<const Metas*>(tile + T::value_scales + T::meta_at(gq + 8, 0));
                 if (part) {   // what is behind the last token may be anything
-                    if (gq >= seen[i]) x[i][0] = x[i][1] = -INFINITY;
-                    if (gq + 8 >= seen[i]) x[i][2] = x[i][3] = -INFINITY;
+                    if (gq >= seen[i]) { x[i][0] = x[i][1] = -INFINITY; va = Metas{}; }
+                    if (gq + 8 >= seen[i]) { x[i][2] = x[i][3] = -INFINITY; vb = Metas{}; }
                 }
-                float ba = 0.0f, bb = 0.0f;
+                const unsigned *ua = reinterpret_cast<const unsigned*>(&va), *ub = reinterpret_cast<const unsigned*>(&vb);
 #pragma unroll
-                for (int g = 0; g < G; ++g) {
-                    ba = fmaxf(ba, q4_scale(ua[g]));
-                    bb = fmaxf(bb, q4_scale(ub[g]));
-                }
-                ba = q4_exponent(ba);
-                bb = q4_exponent(bb);
-                now[0] = fmaxf(now[0], fmaxf(fmaf(x[i][0], unscale[0], ba), fmaf(x[i][2], unscale[0], bb)));
-                now[1] = fmaxf(now[1], fmaxf(fmaf(x[i][1], unscale[1], ba), fmaf(x[i][3], unscale[1], bb)));
+                for (int g = 0; g < G / 2; ++g) most = __vmaxu2(most, __vmaxu2(ua[g], ub[g]));
+                now[0] = fmaxf(now[0], fmaxf(x[i][0], x[i][2]));
+                now[1] = fmaxf(now[1], fmaxf(x[i][1], x[i][3]));
             }
-            // (the reference has to move for a row only where one of its lanes sees a score too far above it)
-            if (__any_sync(0xffffffffu, now[0] > top[0] + (kQdSlack + kQdRoom) || now[1] > top[1] + (kQdSlack + kQdRoom))) {
+            // the reference moves where a lane sees a score too far above it, or scales larger than those before
+            if (__any_sync(0xffffffffu, most != bound || fmaf(now[0], unscale[0], above) > top[0] || fmaf(now[1], unscale[1], above) > top[1])) {
+                const unsigned both = __reduce_max_sync(0xffffffffu, max(most & 0xffffu, most >> 16));
+                most = bound = both | both << 16;
+                above = q4_exponent(both) - (kQdSlack + kQdRoom);
 #pragma unroll
                 for (int off = 4; off < 32; off <<= 1) {
                     now[0] = fmaxf(now[0], __shfl_xor_sync(0xffffffffu, now[0], off));
@@ -381,8 +413,9 @@ __global__ void __launch_bounds__(kQdThreads, kQdCtas(kBf16)) q4_decode_kernel(c
                 }
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    const bool up = now[h] > top[h] + (kQdSlack + kQdRoom);
-                    const float to = up ? now[h] - kQdRoom : top[h], keep = up ? q4_exp2(top[h] - to) : 1.0f;
+                    const float score = fmaf(now[h], unscale[h], above);
+                    const bool up = score > top[h];
+                    const float to = up ? score + kQdSlack : top[h], keep = up ? q4_exp2(top[h] - to) : 1.0f;
                     top[h] = to;
                     l[h] *= keep;
 #pragma unroll
@@ -396,12 +429,14 @@ __global__ void __launch_bounds__(kQdThreads, kQdCtas(kBf16)) q4_decode_kernel(c
                 const unsigned char* tile = stage + i * T::bytes;
                 const Words va = *reinterpret_cast<const Words*>(tile + T::values + (gq * 4 + t) * (4 * G)),
                             vb = *reinterpret_cast<const Words*>(tile + T::values + (32 + gq * 4 + t) * (4 * G));
-                Words ma = *reinterpret_cast<const Words*>(tile + T::value_meta + gq * (4 * G)), mb = *reinterpret_cast<const Words*>(tile + T::value_meta + (gq + 8) * (4 * G));
+                Metas ma = *reinterpret_cast<const Metas*>(tile + T::value_scales + T::meta_at(gq, 0)), mb = *reinterpret_cast<const Metas*>(tile + T::value_scales + T::meta_at(gq + 8, 0));
+                Metas la = *reinterpret_cast<const Metas*>(tile + T::value_mins + T::meta_at(gq, 0)), lb = *reinterpret_cast<const Metas*>(tile + T::value_mins + T::meta_at(gq + 8, 0));
                 if (part) {
-                    if (gq >= seen[i]) ma = Words{};
-                    if (gq + 8 >= seen[i]) mb = Words{};
+                    if (gq >= seen[i]) ma = la = Metas{};
+                    if (gq + 8 >= seen[i]) mb = lb = Metas{};
                 }
                 const unsigned *na = reinterpret_cast<const unsigned*>(&ma), *nb = reinterpret_cast<const unsigned*>(&mb);
+                const unsigned *oa = reinterpret_cast<const unsigned*>(&la), *ob = reinterpret_cast<const unsigned*>(&lb);
                 const unsigned *wa = reinterpret_cast<const unsigned*>(&va), *wb = reinterpret_cast<const unsigned*>(&vb);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) x[i][e] = q4_exp2(fmaf(x[i][e], unscale[e & 1], -top[e & 1]));
@@ -409,7 +444,8 @@ __global__ void __launch_bounds__(kQdThreads, kQdCtas(kBf16)) q4_decode_kernel(c
                 l[1] += x[i][1] + x[i][3];
 #pragma unroll
                 for (int g = 0; g < G; ++g) {
-                    const float low = q4_min(na[g]), high = q4_min(nb[g]), sa = q4_scale(na[g]), sb = q4_scale(nb[g]);
+                    const float low = g & 1 ? q4_high(oa[g / 2]) : q4_low(oa[g / 2]), high = g & 1 ? q4_high(ob[g / 2]) : q4_low(ob[g / 2]);
+                    const float sa = g & 1 ? q4_high(na[g / 2]) : q4_low(na[g / 2]), sb = g & 1 ? q4_high(nb[g / 2]) : q4_low(nb[g / 2]);
                     mins[g][0] = fmaf(x[i][0], low, fmaf(x[i][2], high, mins[g][0]));
                     mins[g][1] = fmaf(x[i][1], low, fmaf(x[i][3], high, mins[g][1]));
                     float y[4] = {x[i][0] * sa, x[i][1] * sa, x[i][2] * sb, x[i][3] * sb};
@@ -483,9 +519,7 @@ __global__ void __launch_bounds__(kQdThreads, kQdCtas(kBf16)) q4_decode_kernel(c
             }
         }
         if (begins && !ends && tid == 0) {
-            // the CTA of the item's last unit: unit v is in share i of n where i all / n <= v < (i + 1) all / n, rounded down
-            const long long end = unit + (at.units - u1) - 1;
-            P.pieces[blockIdx.x] = make_int2(at.b * heads + at.hh, (int)(((end + 1) * n_ctas - 1) / all));
+            P.pieces[blockIdx.x] = make_int2(at.b * heads + at.hh, shares.owner(unit + (at.units - u1) - 1));
         }
         __syncthreads();   // the sums have been read
         at.u = u1 - 1;
@@ -497,25 +531,45 @@ __global__ void __launch_bounds__(kQdThreads, kQdCtas(kBf16)) q4_decode_kernel(c
     }
 }
 
-// Items that several CTAs have parts of; a CTA per CTA of the decode.
+// Items that several CTAs have parts of; a CTA per CTA of the decode, a thread per result.  Bound by latency: eight parts are asked for
+// at a time.
+constexpr int kQcThreads = 256;
+
 template <int HD, bool kBf16>
-__global__ void __launch_bounds__(kQdThreads) q4_combine_kernel(const __grid_constant__ Q4DecodeProblem P) {
+__global__ void __launch_bounds__(kQcThreads) q4_combine_kernel(const __grid_constant__ Q4DecodeProblem P) {
     chain_begin();
     const int2 piece = P.pieces[blockIdx.x];
     if (piece.x < 0) return;
     const int heads = P.cache.kv_heads * P.blocks, b = piece.x / heads, hh = piece.x % heads, h0 = (hh % P.blocks) * kQdHeads;
-    const int n_heads = min(kQdHeads, P.share - h0);
+    const int n_heads = min(kQdHeads, P.share - h0), first = blockIdx.x;
     const size_t row0 = ((size_t)b * P.q_heads + hh / P.blocks * P.share + h0) * HD;
-    auto part = [&](int c) { return P.partials + ((size_t)c * 2 + (c == (int)blockIdx.x ? 1 : 0)) * kQdHeads * (HD + 2); };
-    for (int i = threadIdx.x; i < n_heads * HD; i += kQdThreads) {
+    for (int i = threadIdx.x; i < n_heads * HD; i += kQcThreads) {
         const int h = i / HD, d = i % HD;
         float most = kQdLowest, acc = 0.0f, weight = 0.0f;
-        for (int c = blockIdx.x; c <= piece.y; ++c) most = fmaxf(most, part(c)[h * (HD + 2)]);
-        for (int c = blockIdx.x; c <= piece.y; ++c) {
-            const float* p = part(c) + h * (HD + 2);
-            const float keep = q4_exp2(p[0] - most);
-            acc = fmaf(p[2 + d], keep, acc);
-            weight = fmaf(p[1], keep, weight);
+        for (int c0 = first; c0 <= piece.y; c0 += 8) {
+            float m[8], w[8], v[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                const int c = min(c0 + u, piece.y);
+                const float* p = P.partials + (((size_t)c * 2 + (c == first ? 1 : 0)) * kQdHeads + h) * (HD + 2);
+                m[u] = p[0];
+                w[u] = p[1];
+                v[u] = p[2 + d];
+            }
+            float top = most;
+#pragma unroll
+            for (int u = 0; u < 8; ++u) top = fmaxf(top, m[u]);
+            const float keep = q4_exp2(most - top);
+            acc *= keep;
+            weight *= keep;
+            most = top;
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                if (c0 + u > piece.y) continue;
+                const float k = q4_exp2(m[u] - top);
+                acc = fmaf(v[u], k, acc);
+                weight = fmaf(w[u], k, weight);
+            }
         }
         acc = weight == 0.0f ? 0.0f : acc / weight;
         if (kBf16) reinterpret_cast<__nv_bfloat16*>(P.out)[row0 + i] = __float2bfloat16_rn(acc);
@@ -538,7 +592,7 @@ static int launch_q4_decode(const Q4DecodeProblem& P, int ctas, cudaStream_t s) 
     static std::atomic<bool> opted[64];
     OJX_CUDA_TRY(opt_in_smem(reinterpret_cast<const void*>(q4_decode_kernel<HD, kBf16>), QdSmem<HD>::bytes(kQdHeads), opted));
     OJX_CUDA_TRY(launch_chained(q4_decode_kernel<HD, kBf16>, ctas, kQdThreads, QdSmem<HD>::bytes(std::min(P.share, kQdHeads)), s, P));
-    OJX_CUDA_TRY(launch_chained(q4_combine_kernel<HD, kBf16>, ctas, kQdThreads, 0, s, P));
+    OJX_CUDA_TRY(launch_chained(q4_combine_kernel<HD, kBf16>, ctas, kQcThreads, 0, s, P));
     count_launch(2);
     return OJX_OK;
 }

@@ -526,13 +526,13 @@ class Q4PagedKVCache:
 
     # ------------------------------------------------------------------ codes in and out
     def _tiles(self):
-        """The pool as (key codes, key metas, value codes, value metas) by the layout of csrc/q4kv.cuh, views of int32 words."""
+        """Views of the pool by the layout of csrc/q4kv.cuh: key codes, their scales and minima, value codes, theirs."""
         G, T = self.head_dim // 32, self.page_size // 16
-        words = self.pool.view(torch.int32).view(self.num_pages, self.kv_heads, T, -1)
-        cuts = [16 * 4 * G, 16 * G, 16 * 4 * G, 16 * G]
-        k, km, v, vm = words.split(cuts, dim=-1)
         lead = (self.num_pages, self.kv_heads, T)
-        return k.view(*lead, 16, 4, G), km.view(*lead, 16, G), v.view(*lead, 2, 8, 4, G), vm.view(*lead, 16, G)
+        k, ks, km, v, vs, vm = self.pool.view(torch.int32).view(*lead, -1).split([64 * G, 8 * G, 8 * G] * 2, dim=-1)
+        metas = (t.view(torch.bfloat16) for t in (ks, km, vs, vm))
+        ks, km, vs, vm = (t.view(*lead, 16, G) for t in metas)
+        return k.view(*lead, 16, 4, G), ks, km, v.view(*lead, 2, 8, 4, G), vs, vm
 
     def load(self, k_codes, k_scales, k_mins, v_codes, v_scales, v_mins) -> None:
         """Fills the pool: codes uint8 0..15 [num_pages, kv_heads, page_size, head_dim], scales and minima bf16
@@ -544,25 +544,27 @@ class Q4PagedKVCache:
                                      ("v_scales", v_scales, G, torch.bfloat16), ("v_mins", v_mins, G, torch.bfloat16)):
             if tuple(t.shape) != (self.num_pages, self.kv_heads, self.page_size, last) or t.dtype != dtype:
                 raise ValueError(f"{name} must be {dtype} of shape {(self.num_pages, self.kv_heads, self.page_size, last)}")
-        k, km, v, vm = self._tiles()
-        nibbles = lambda c, n: sum((c[..., i].to(torch.int32) & 15) << (4 * i) for i in range(n))  # noqa: E731
-        word16 = lambda t: t.contiguous().view(torch.int16).to(torch.int32)  # noqa: E731
-        meta = lambda mins, scales: ((word16(mins) << 16) | (word16(scales) & 0xffff)).view(*lead, 16, G)  # noqa: E731
-        k.copy_(nibbles(k_codes.to(self.device).view(*lead, 16, G, 4, 8), 8).transpose(-1, -2))
-        halves = nibbles(v_codes.to(self.device).view(*lead, 2, 4, 2, G, 8, 4), 4)     # [half, pair, odd, g, c]
-        v.copy_(((halves[..., 1, :, :] << 16) | halves[..., 0, :, :]).permute(0, 1, 2, 3, 6, 4, 5))
-        km.copy_(meta(k_mins.to(self.device), k_scales.to(self.device)))
-        vm.copy_(meta(v_mins.to(self.device), v_scales.to(self.device)))
+        k, ks, km, v, vs, vm = self._tiles()
+
+        def bytes_of(codes):    # two codes to a byte: [..., head_dim / 2]
+            pairs = codes.to(self.device).contiguous().view(torch.int16)
+            return ((pairs & 15) | ((pairs >> 4) & 240)).to(torch.uint8)
+
+        k.copy_(bytes_of(k_codes).view(torch.int32).view(*lead, 16, G, 4).transpose(-1, -2))
+        halves = bytes_of(v_codes).view(torch.int16).view(*lead, 2, 4, 2, G, 8)     # [half, pair, odd, g, c]
+        v.view(torch.int16).view(*lead, 2, 8, 4, G, 2).copy_(halves.permute(0, 1, 2, 3, 7, 4, 6, 5))
+        for to, t in ((ks, k_scales), (km, k_mins), (vs, v_scales), (vm, v_mins)):
+            to.copy_(t.view(*lead, 16, G) if t.is_contiguous() else t.contiguous().view(*lead, 16, G))
 
     def unload(self) -> dict:
         """The pool as ``load`` takes it."""
-        k, km, v, vm = self._tiles()
+        k, ks, km, v, vs, vm = self._tiles()
         shape = (self.num_pages, self.kv_heads, self.page_size)
-        bf16 = lambda w: w.to(torch.int16).view(torch.bfloat16).reshape(*shape, -1)  # noqa: E731
-        split = lambda w, n: torch.stack([(w >> (4 * i)) & 15 for i in range(n)], -1).to(torch.uint8)  # noqa: E731
-        halves = torch.stack([v & 0xffff, (v >> 16) & 0xffff], -1).permute(0, 1, 2, 3, 5, 7, 6, 4)   # [half, pair, odd, g, c]
-        return {"k_codes": split(k.transpose(-1, -2), 8).reshape(*shape, -1), "k_scales": bf16((km << 16) >> 16), "k_mins": bf16(km >> 16),
-                "v_codes": split(halves, 4).reshape(*shape, -1), "v_scales": bf16((vm << 16) >> 16), "v_mins": bf16(vm >> 16)}
+        split = lambda b: torch.stack([b & 15, b >> 4], -1).reshape(*shape, -1)  # noqa: E731
+        k = k.transpose(-1, -2).contiguous().view(torch.uint8)
+        v = v.view(torch.int16).unflatten(-1, (-1, 2)).permute(0, 1, 2, 3, 5, 7, 6, 4).contiguous().view(torch.uint8)    # [half, pair, odd, g, c]
+        metas = {n: t.reshape(*shape, -1) for n, t in (("k_scales", ks), ("k_mins", km), ("v_scales", vs), ("v_mins", vm))}
+        return {"k_codes": split(k), "v_codes": split(v), **metas}
 
     # ------------------------------------------------------------------ the calls of a model
     def _table(self, block_table: torch.Tensor) -> int:

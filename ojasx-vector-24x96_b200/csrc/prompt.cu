@@ -30,7 +30,8 @@ struct PromptProblem {
 // the weights back over S as bf16, O += P V with P read from tensor memory.  The two tiles take turns: while the tensor cores are at
 // one, 128 threads are at the other's exponentials.
 //   warps 0..3, 4..7: the rows of the two tiles; warp 8: issues the products; warp 9: the copies of Q, K and V (K and V in a ring);
-//   warps 10, 11: none, but for the keys' factors of fp32 (registers are moved between groups of four warps: 384 * 168 = 64512 are 2 * 128 * 216 + 128 * 64 and some)
+//   warp 11: what to do next, so that a CTA's copies and products for one part of the prompts begin while it is at the last results of
+//   another; warp 10: nothing here, the keys' factors of fp32 (registers are moved between groups of four warps: 384 * 168 = 64512 are 2 * 128 * 216 + 128 * 64 and some)
 // Maxima are left behind: a row's sums are relative to the maximum it had when a score was last more than 2^8 above it, so that
 // O is rescaled a few times per row and not once per step (weights up to 2^8 cost nothing in bf16 or in fp32 sums).
 constexpr int kPaRows = 128, kPaKeys = 128, kPaThreads = 384;
@@ -41,7 +42,7 @@ struct PaSmem {
     static constexpr int tile = 128 * HD * 2;                     // 128 rows or keys
     static constexpr int slots = HD == 128 ? 5 : 8;
     static constexpr int ring = 2 * tile, bars = ring + slots * tile;
-    static constexpr int bytes = bars + 256 + 1024;               // (swizzled tiles begin on 1024 bytes)
+    static constexpr int bytes = bars + 384 + 1024;               // (swizzled tiles begin on 1024 bytes)
 };
 
 // Two fp32 numbers in one register pair: half the instructions for what is done to all scores.
@@ -81,13 +82,16 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_tc_kernel(const __grid_c
     constexpr int NS = M::slots, C = HD / 64;
     extern __shared__ unsigned char pa_raw[];
     unsigned char* smem = pa_raw + ((1024u - (tc_smem(pa_raw) & 1023u)) & 1023u);
-    __shared__ int s_seq, s_part, s_gone, s_odd[2];
+    __shared__ int s_gone, s_odd[2];
     __shared__ unsigned s_tmem;
+    __shared__ __align__(16) int s_item[2][8];
+    __shared__ __align__(16) int s_stolen[4];
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;   // (the same for a warp, as the compiler sees)
     const unsigned base = tc_smem(smem), bars = base + M::bars;
     const unsigned full = bars, empty = bars + 8 * NS, q_full = empty + 8 * NS, s_full = q_full + 16, p_full = s_full + 16, o_full = p_full + 16,
-                   checked = o_full + 16, p_half = checked + 16, ended = p_half + 16, gone = tc_smem(&s_gone);
-    const int head = blockIdx.x % P.kv_heads, per = kPaRows / P.share;
+                   checked = o_full + 16, p_half = checked + 16, q_empty = p_half + 16, item_full = q_empty + 16, item_empty = item_full + 16,
+                   want = item_empty + 16, steal = want + 8, ended = steal + 8, gone = tc_smem(&s_gone);
+    const int per = kPaRows / P.share;
     if (tid == 0) {
         for (int i = 0; i < NS; ++i) { tc_bar_init(full + 8 * i, 1); tc_bar_init(empty + 8 * i, 1); }
         for (int i = 0; i < 2; ++i) {
@@ -97,22 +101,19 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_tc_kernel(const __grid_c
             tc_bar_init(p_full + 8 * i, 4);
             tc_bar_init(o_full + 8 * i, 1);
             tc_bar_init(checked + 8 * i, 4);
+            tc_bar_init(q_empty + 8 * i, 1);
+            tc_bar_init(item_full + 8 * i, 1);
+            tc_bar_init(item_empty + 8 * i, 10);
             s_odd[i] = 0;
         }
+        tc_bar_init(want, 1);
+        tc_bar_init(steal, 1);
         tc_bar_init(ended, 1);
         s_gone = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     chain_begin();
-    if (warp == 0) {
-        // the last parts of a sequence, which see the most keys, first
-        int seq = -1, part = 0;
-        const bool in = packed_part(P.batch, (int)(gridDim.x / P.kv_heads) - 1 - (int)blockIdx.x / P.kv_heads,
-                                    [&](int b) { return (packed_range(P.ends, b, P.n_rows).count + 2 * per - 1) / (2 * per); }, seq, part);
-        if (lane == 0) { s_seq = in ? seq : -1; s_part = part; }
-    }
     __syncthreads();
-    if (s_seq < 0) return;
     if (warp == 8) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(tc_smem(&s_tmem)) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -121,38 +122,107 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_tc_kernel(const __grid_c
     __syncthreads();
     tc_after();
     const unsigned tmem = __shfl_sync(0xffffffffu, s_tmem, 0);
-    const PackedRange rows = packed_range(P.ends, s_seq, P.n_rows), keys = packed_range(P.key_ends, s_seq, P.n_keys);
-    const int ahead = keys.count - rows.count;
-    int pos[2], live[2], steps[2];   // first position, positions and steps of the tiles
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        pos[i] = (s_part * 2 + i) * per;
-        live[i] = max(0, min(per, rows.count - pos[i]));
-        steps[i] = live[i] > 0 ? max(0, pos[i] + live[i] + ahead + kPaKeys - 1) / kPaKeys : 0;
-    }
-    const int n = max(steps[0], steps[1]);
     bool ok = true;
     auto wait = [&](unsigned bar, unsigned parity) { return tc_wait(bar, parity, gone); };
+    // Item `number` of the CTA, as warp 11 has put it down; false behind the last one (or where a wait ran out).
+    struct { int row, key, ahead, head, pos[2], live[2], steps[2], n; } item;   // first row and key; first position, positions and steps of the tiles
+    auto take = [&](int number) {
+        if (!(ok = wait(item_full + 8 * (number & 1), (number >> 1) & 1))) return false;
+        const int4 a = *reinterpret_cast<const int4*>(s_item[number & 1]), b = *reinterpret_cast<const int4*>(s_item[number & 1] + 4);
+        __syncwarp();
+        if (lane == 0) tc_bar_arrive(item_empty + 8 * (number & 1));
+        item.row = a.x; item.key = a.y; item.ahead = a.z; item.head = a.w;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            item.pos[i] = b.x + i * per;
+            item.live[i] = i ? b.z : b.y;
+            item.steps[i] = item.live[i] > 0 ? max(0, item.pos[i] + item.live[i] + item.ahead + kPaKeys - 1) / kPaKeys : 0;
+        }
+        item.n = max(item.steps[0], item.steps[1]);
+        return item.row >= 0;
+    };
 
     if (warp >= 8) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
-        if (warp == 9 && lane == 0) {
-            for (int i = 0; i < 2; ++i) {
-                if (!steps[i]) continue;
-                tc_bar_expect(q_full + 8 * i, per * P.share * HD * 2);
-                for (int c = 0; c < C; ++c) tc_load3(base + i * M::tile + c * (M::tile / C), &q_map, 64 * c, head * P.share, rows.first + pos[i], q_full + 8 * i);
+        if (warp == 11) {
+            // Work: the CTA's own part of the prompts, and then those of CTAs that have not begun, asked for when the copies of the last one
+            // have been issued.  The last parts of a sequence, which see the most keys, come first.
+            int cta = blockIdx.x, number = 0;
+            unsigned asked = 0;
+            while (ok) {
+                int seq = -1, part = 0;
+                const bool in = cta >= 0 && packed_part(P.batch, (int)(gridDim.x / P.kv_heads) - 1 - cta / P.kv_heads,
+                                                        [&](int b) { return (packed_range(P.ends, b, P.n_rows).count + 2 * per - 1) / (2 * per); }, seq, part);
+                if (in || cta < 0) {
+                    if (number >= 2 && !(ok = wait(item_empty + 8 * (number & 1), ((number >> 1) - 1) & 1))) break;
+                    if (lane == 0) {
+                        int4 a = make_int4(-1, 0, 0, 0), b = make_int4(0, 0, 0, 0);
+                        if (in) {
+                            const PackedRange rows = packed_range(P.ends, seq, P.n_rows), keys = packed_range(P.key_ends, seq, P.n_keys);
+                            const int pos = part * 2 * per;
+                            a = make_int4(rows.first, keys.first, keys.count - rows.count, cta % P.kv_heads);
+                            b = make_int4(pos, min(per, rows.count - pos), max(0, min(per, rows.count - pos - per)), 0);
+                        }
+                        *reinterpret_cast<int4*>(s_item[number & 1]) = a;
+                        *reinterpret_cast<int4*>(s_item[number & 1] + 4) = b;
+                        tc_bar_arrive(item_full + 8 * (number & 1));
+                    }
+                    __syncwarp();
+                    if (cta < 0 || !(ok = wait(want, number & 1))) break;
+                    ++number;
+                }
+                if (lane == 0) {
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    tc_bar_expect(steal, 16);
+                    tc_steal(tc_smem(s_stolen), steal);
+                }
+                __syncwarp();
+                if (!(ok = wait(steal, asked & 1))) {   // nothing may land after the CTA has left
+                    bar_wait(steal, asked & 1);
+                    break;
+                }
+                ++asked;
+                cta = tc_stolen(tc_smem(s_stolen));
+                __syncwarp();
             }
-            int s = 0;
-            for (; s < 2 * n; ++s) {   // K of step 0, V of step 0, K of step 1, ...
-                const int slot = s % NS;
-                if (s >= NS && !(ok = bar_wait(empty + 8 * slot, (s / NS - 1) & 1, gone))) break;
-                tc_bar_expect(full + 8 * slot, M::tile);
-                for (int c = 0; c < C; ++c)
-                    tc_load3(base + M::ring + slot * M::tile + c * (M::tile / C), s & 1 ? &v_map : &k_map, 64 * c, head, keys.first + (s >> 1) * kPaKeys, full + 8 * slot);
+        }
+        if (warp == 9) {
+            TcRing<NS> ring{0, 1};   // (of the phases that free the slots: none is waited for the first time round)
+            int quota = NS, loads[2] = {0, 0};
+            for (int number = 0; take(number); ++number) {
+                auto stage = [&](bool value, int j) {
+                    if (quota > 0) --quota;
+                    else if (!(ok = wait(empty + 8 * ring.slot, ring.parity))) return;
+                    if (lane == 0) {
+                        tc_bar_expect(full + 8 * ring.slot, M::tile);
+                        for (int c = 0; c < C; ++c)
+                            tc_load3(base + M::ring + ring.slot * M::tile + c * (M::tile / C), value ? &v_map : &k_map, 64 * c, item.head, item.key + j * kPaKeys,
+                                     full + 8 * ring.slot);
+                    }
+                    __syncwarp();
+                    ring.next(1);
+                };
+                for (int j = 0; j < item.n && ok; ++j) {   // K of step 0, Q, V of step 0, K of step 1, ...
+                    stage(false, j);
+                    for (int i = 0; i < 2 && j == 0 && ok; ++i) {
+                        if (!item.steps[i]) continue;
+                        if (loads[i] > 0 && !(ok = wait(q_empty + 8 * i, (loads[i] - 1) & 1))) break;
+                        ++loads[i];
+                        if (lane == 0) {
+                            tc_bar_expect(q_full + 8 * i, per * P.share * HD * 2);
+                            for (int c = 0; c < C; ++c)
+                                tc_load3(base + i * M::tile + c * (M::tile / C), &q_map, 64 * c, item.head * P.share, item.row + item.pos[i], q_full + 8 * i);
+                        }
+                        __syncwarp();
+                    }
+                    if (ok) stage(true, j);
+                }
+                if (!ok) break;
+                if (lane == 0) tc_bar_arrive(want);
             }
             if (!ok) {   // nothing may land after the CTA has left
-                for (int u = max(0, s - NS); u < s; ++u) bar_wait(full + 8 * (u % NS), (u / NS) & 1);
-                for (int i = 0; i < 2; ++i) if (steps[i]) bar_wait(q_full + 8 * i, 0);
+                for (int u = 0; u < NS; ++u) { bar_wait(full + 8 * u, 0); bar_wait(full + 8 * u, 1); }
+                for (int i = 0; i < 2; ++i) { bar_wait(q_full + 8 * i, 0); bar_wait(q_full + 8 * i, 1); }
             }
         }
         if (warp == 8) {
@@ -169,46 +239,58 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_tc_kernel(const __grid_c
                 tc_commit(lead, s_full + 8 * i);
             };
             TcRing<NS> kr{0, 0}, vr{1, 0};
-            if (n > 0) ok = wait(full, 0);
+            unsigned done[2] = {0, 0}, items[2] = {0, 0};   // steps of the tiles so far, and items
+            for (int number = 0; take(number); ++number) {
+                const int n = item.n;
+                if (n == 0) continue;
+                ok = wait(full + 8 * kr.slot, kr.parity);
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
-                if (ok && steps[i]) {
-                    ok = wait(q_full + 8 * i, 0);
-                    if (ok) scores(i, 0);
-                }
-            if (n > 0 && ok) tc_commit(lead, empty);
-            for (int j = 0; j < n && ok; ++j) {
-                kr.next(2);
-                bool loaded = false;   // K of the next step
-                ok = wait(full + 8 * vr.slot, vr.parity);
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    if (j >= steps[i] || !ok) continue;
-                    // the first 64 keys' weights come earlier, so that their product runs beside the other half's exponentials
-                    const unsigned long long b = tc_at(ring_v, vr.slot * M::tile);
-                    const bool maybe = (j + 1) * kPaKeys - 1 > pos[i] + ahead;
-#pragma unroll
-                    for (int half = 0; half < 2; ++half) {
-                        if (!(ok = wait((half ? p_full : p_half) + 8 * i, j & 1))) break;
+                for (int i = 0; i < 2; ++i)
+                    if (ok && item.steps[i]) {
+                        ok = wait(q_full + 8 * i, items[i]++ & 1);
+                        if (!ok) continue;
                         tc_after();
-                        if (maybe && *reinterpret_cast<volatile int*>(&s_odd[i]) == j + 1) continue;   // (the rows have added their products themselves)
+                        scores(i, kr.slot);
+                        if (item.steps[i] == 1) tc_commit(lead, q_empty + 8 * i);
+                    }
+                if (!ok) break;
+                tc_commit(lead, empty + 8 * kr.slot);
+                for (int j = 0; j < n && ok; ++j) {
+                    kr.next(2);
+                    bool loaded = false;   // K of the next step
+                    ok = wait(full + 8 * vr.slot, vr.parity);
 #pragma unroll
-                        for (int k = half * kPaKeys / 32; k < (half + 1) * kPaKeys / 32; ++k)
-                            tc_mma_ts(lead, tmem + 256 + i * 128, tmem + i * 128 + k * 8, tc_at(b, k * 2048), iv, j > 0 || k > 0);
+                    for (int i = 0; i < 2; ++i) {
+                        if (j >= item.steps[i] || !ok) continue;
+                        const unsigned step = ++done[i];
+                        // the first 64 keys' weights come earlier, so that their product runs beside the other half's exponentials
+                        const unsigned long long b = tc_at(ring_v, vr.slot * M::tile);
+                        const bool maybe = (j + 1) * kPaKeys - 1 > item.pos[i] + item.ahead;
+#pragma unroll
+                        for (int half = 0; half < 2; ++half) {
+                            if (!(ok = wait((half ? p_full : p_half) + 8 * i, (step - 1) & 1))) break;
+                            tc_after();
+                            if (maybe && *reinterpret_cast<volatile int*>(&s_odd[i]) == (int)step) continue;   // (the rows have added their products themselves)
+#pragma unroll
+                            for (int k = half * kPaKeys / 32; k < (half + 1) * kPaKeys / 32; ++k)
+                                tc_mma_ts(lead, tmem + 256 + i * 128, tmem + i * 128 + k * 8, tc_at(b, k * 2048), iv, j > 0 || k > 0);
+                        }
+                        if (!ok) continue;
+                        if (j + 1 < item.steps[i]) {
+                            if (!loaded && !(ok = wait(full + 8 * kr.slot, kr.parity))) continue;
+                            loaded = true;
+                            scores(i, kr.slot);   // (in order: its commit says that O is up to date, too)
+                            if (j + 2 == item.steps[i]) tc_commit(lead, q_empty + 8 * i);
+                        } else {
+                            tc_commit(lead, o_full + 8 * i);
+                        }
                     }
-                    if (!ok) continue;
-                    if (j + 1 < steps[i]) {
-                        if (!loaded && !(ok = wait(full + 8 * kr.slot, kr.parity))) continue;
-                        loaded = true;
-                        scores(i, kr.slot);   // (in order: its commit says that O is up to date, too)
-                    } else {
-                        tc_commit(lead, o_full + 8 * i);
-                    }
+                    if (!ok) break;
+                    tc_commit(lead, empty + 8 * vr.slot);
+                    if (j + 1 < n) tc_commit(lead, empty + 8 * kr.slot);
+                    vr.next(2);
                 }
                 if (!ok) break;
-                tc_commit(lead, empty + 8 * vr.slot);
-                if (j + 1 < n) tc_commit(lead, empty + 8 * kr.slot);
-                vr.next(2);
             }
             if (!ok) {
                 tc_commit(lead, ended);
@@ -218,12 +300,10 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_tc_kernel(const __grid_c
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
         const int i = warp >> 2, row = tid & 127;   // the row's lane of tensor memory is its place in the tile
-        const int at = min(row, max(live[i] * P.share - 1, 0)), last = pos[i] + at / P.share + ahead;   // last key that the row sees
         const unsigned lanes = (unsigned)((warp & 3) * 32) << 16, st = tmem + i * 128 + lanes, ot = tmem + 256 + i * 128 + lanes;
         const float scale = P.scale * 1.4426950408889634f;
-        float top = 0.0f;
-        unsigned long long sum2[2] = {0, 0};
         int checks = 0;
+        unsigned done = 0, items = 0, before = 0;   // steps of the tile so far, its items, and the steps of the CTA
         auto rescale = [&](float by) {   // the warp's rows of O
             for (int c = 0; c < HD; c += 32) {
                 unsigned o[32];
@@ -235,154 +315,164 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_tc_kernel(const __grid_c
                 tc_st32(ot + c, o);
             }
         };
-        for (int j = 0; j < steps[i]; ++j) {
-            if (!(ok = wait(s_full + 8 * i, j & 1))) break;
-            tc_after();
-            unsigned s[128];
+        for (int number = 0; take(number); ++number) {
+            const int pos = i ? item.pos[1] : item.pos[0], live = i ? item.live[1] : item.live[0], steps = i ? item.steps[1] : item.steps[0];
+            const int last = pos + min(row, max(live * P.share - 1, 0)) / P.share + item.ahead;   // last key that the row sees
+            float top = 0.0f;
+            unsigned long long sum2[2] = {0, 0};
+            for (int j = 0; j < steps; ++j) {
+                const unsigned step = ++done;
+                if (!(ok = wait(s_full + 8 * i, (step - 1) & 1))) break;
+                tc_after();
+                unsigned s[128];
 #pragma unroll
-            for (int c = 0; c < 4; ++c) tc_ld32(st + 32 * c, s + 32 * c);
-            tc_wait_ld();
+                for (int c = 0; c < 4; ++c) tc_ld32(st + 32 * c, s + 32 * c);
+                tc_wait_ld();
 #pragma unroll
-            for (int c = 0; c < 4; ++c) tc_pin32(s + 32 * c);
-            const bool masked = (j + 1) * kPaKeys - 1 > pos[i] + ahead;   // some row does not see all of these keys
-            if (masked) {
-                const int see = last - j * kPaKeys;
+                for (int c = 0; c < 4; ++c) tc_pin32(s + 32 * c);
+                const bool masked = (j + 1) * kPaKeys - 1 > pos + item.ahead;   // some row does not see all of these keys
+                if (masked) {
+                    const int see = last - j * kPaKeys;
 #pragma unroll
-                for (int e = 0; e < 128; ++e) s[e] = e > see ? 0xff800000u : s[e];
-            }
-            float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-            for (int e = 0; e < 128; e += 8)
-#pragma unroll
-                for (int u = 0; u < 4; ++u) m[u] = pa_max3(m[u], __uint_as_float(s[e + 2 * u]), __uint_as_float(s[e + 2 * u + 1]));
-            const float now = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
-            const bool up = (now - top) * scale > kPaSlack;   // (by the row's own scores: its result does not depend on its neighbours)
-            if (j == 0) {
-                top = now;
-            } else if (__any_sync(0xffffffffu, up)) {
-                const float to = up ? now : top, by = up ? exp2f((top - now) * scale) : 1.0f;
-                rescale(by);
-                sum2[0] = pa_mul2(sum2[0], pa_pair(by, by));
-                sum2[1] = pa_mul2(sum2[1], pa_pair(by, by));
-                top = to;
-            }
-            const float off = top == -INFINITY ? 0.0f : top * scale;   // (a row that has seen nothing: its weights are exp(-inf))
-            const unsigned long long scale2 = pa_pair(scale, scale), off2 = pa_pair(-off, -off);
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                unsigned w[32];
-#pragma unroll
-                for (int e = 0; e < 32; ++e) {
-                    unsigned long long x = pa_fma2((unsigned long long)s[64 * c + 2 * e + 1] << 32 | s[64 * c + 2 * e], scale2, off2);
-                    x = pa_exp2(x);
-                    sum2[e & 1] = pa_add2(sum2[e & 1], x);
-                    const __nv_bfloat162 h = __floats2bfloat162_rn(__uint_as_float((unsigned)x), __uint_as_float((unsigned)(x >> 32)));
-                    w[e] = *reinterpret_cast<const unsigned*>(&h);
+                    for (int e = 0; e < 128; ++e) s[e] = e > see ? 0xff800000u : s[e];
                 }
-                tc_st32(st + 32 * c, w);
-                if (c == 0 && !masked) {
-                    tc_wait_st();
-                    tc_before();
-                    __syncwarp();
-                    if (lane == 0) tc_bar_arrive(p_half + 8 * i);
-                }
-            }
-            if (masked) {
-                // A weight of zero times an infinity is a NaN, and the products take all keys of the step.  Where a value among them is
-                // not finite (padding behind a sequence, another sequence's rows) each row adds the values that it sees itself.
-                if (!(ok = wait(full + 8 * ((2 * j + 1) % NS), ((2 * j + 1) / NS) & 1))) break;
-                const unsigned char* v = smem + M::ring + ((2 * j + 1) % NS) * M::tile;
-                unsigned odd = 0;
-                for (int e = row; e < M::tile / 16; e += 128) {
-                    const uint4 x = reinterpret_cast<const uint4*>(v)[e];   // an exponent of all ones carries into the sign's place
-                    odd |= (((x.x & 0x7f807f80u) + 0x00800080u) | ((x.y & 0x7f807f80u) + 0x00800080u) | ((x.z & 0x7f807f80u) + 0x00800080u) |
-                            ((x.w & 0x7f807f80u) + 0x00800080u)) & 0x80008000u;
-                }
-                odd = __reduce_or_sync(0xffffffffu, odd);
-                if (lane == 0) {
-                    if (odd) *reinterpret_cast<volatile int*>(&s_odd[i]) = j + 1;
-                    tc_bar_arrive(checked + 8 * i);
-                }
-                if (!(ok = wait(checked + 8 * i, checks++ & 1))) break;
-                if (*reinterpret_cast<volatile int*>(&s_odd[i]) == j + 1) {
-                    tc_wait_st();
-                    const int see = min(last - j * kPaKeys, kPaKeys - 1);
-                    for (int c = 0; c < HD; c += 32) {
-                        float o[32];
+                float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                        for (int e = 0; e < 32; ++e) o[e] = 0.0f;
-                        for (int k = 0; k < kPaKeys; ++k) {
-                            unsigned w = tc_ld1(st + (k >> 1));
-                            tc_wait_ld();
-                            asm volatile("" : "+r"(w));
-                            if (k <= see) {
-                                const float p = __uint_as_float(k & 1 ? w & 0xffff0000u : w << 16);
-                                const unsigned char* line = v + (c / 64) * (M::tile / C) + k * 128;
+                for (int e = 0; e < 128; e += 8)
 #pragma unroll
-                                for (int e = 0; e < 4; ++e) {
-                                    const uint4 x = *reinterpret_cast<const uint4*>(line + (((c % 64) / 8 + e) ^ (k & 7)) * 16);
-                                    const unsigned xs[4] = {x.x, x.y, x.z, x.w};
+                    for (int u = 0; u < 4; ++u) m[u] = pa_max3(m[u], __uint_as_float(s[e + 2 * u]), __uint_as_float(s[e + 2 * u + 1]));
+                const float now = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+                const bool up = (now - top) * scale > kPaSlack;   // (by the row's own scores: its result does not depend on its neighbours)
+                if (j == 0) {
+                    top = now;
+                } else if (__any_sync(0xffffffffu, up)) {
+                    const float to = up ? now : top, by = up ? exp2f((top - now) * scale) : 1.0f;
+                    rescale(by);
+                    sum2[0] = pa_mul2(sum2[0], pa_pair(by, by));
+                    sum2[1] = pa_mul2(sum2[1], pa_pair(by, by));
+                    top = to;
+                }
+                const float off = top == -INFINITY ? 0.0f : top * scale;   // (a row that has seen nothing: its weights are exp(-inf))
+                const unsigned long long scale2 = pa_pair(scale, scale), off2 = pa_pair(-off, -off);
 #pragma unroll
-                                    for (int h = 0; h < 4; ++h) {
-                                        o[8 * e + 2 * h] = fmaf(p, __uint_as_float(xs[h] << 16), o[8 * e + 2 * h]);
-                                        o[8 * e + 2 * h + 1] = fmaf(p, __uint_as_float(xs[h] & 0xffff0000u), o[8 * e + 2 * h + 1]);
+                for (int c = 0; c < 2; ++c) {
+                    unsigned w[32];
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) {
+                        unsigned long long x = pa_fma2((unsigned long long)s[64 * c + 2 * e + 1] << 32 | s[64 * c + 2 * e], scale2, off2);
+                        x = pa_exp2(x);
+                        sum2[e & 1] = pa_add2(sum2[e & 1], x);
+                        const __nv_bfloat162 h = __floats2bfloat162_rn(__uint_as_float((unsigned)x), __uint_as_float((unsigned)(x >> 32)));
+                        w[e] = *reinterpret_cast<const unsigned*>(&h);
+                    }
+                    tc_st32(st + 32 * c, w);
+                    if (c == 0 && !masked) {
+                        tc_wait_st();
+                        tc_before();
+                        __syncwarp();
+                        if (lane == 0) tc_bar_arrive(p_half + 8 * i);
+                    }
+                }
+                if (masked) {
+                    // A weight of zero times an infinity is a NaN, and the products take all keys of the step.  Where a value among them is
+                    // not finite (padding behind a sequence, another sequence's rows) each row adds the values that it sees itself.
+                    const unsigned place = 2 * (before + j) + 1;
+                    if (!(ok = wait(full + 8 * (place % NS), place / NS & 1))) break;
+                    const unsigned char* v = smem + M::ring + place % NS * M::tile;
+                    unsigned odd = 0;
+                    for (int e = row; e < M::tile / 16; e += 128) {
+                        const uint4 x = reinterpret_cast<const uint4*>(v)[e];   // an exponent of all ones carries into the sign's place
+                        odd |= (((x.x & 0x7f807f80u) + 0x00800080u) | ((x.y & 0x7f807f80u) + 0x00800080u) | ((x.z & 0x7f807f80u) + 0x00800080u) |
+                                ((x.w & 0x7f807f80u) + 0x00800080u)) & 0x80008000u;
+                    }
+                    odd = __reduce_or_sync(0xffffffffu, odd);
+                    if (lane == 0) {
+                        if (odd) *reinterpret_cast<volatile int*>(&s_odd[i]) = (int)step;
+                        tc_bar_arrive(checked + 8 * i);
+                    }
+                    if (!(ok = wait(checked + 8 * i, checks++ & 1))) break;
+                    if (*reinterpret_cast<volatile int*>(&s_odd[i]) == (int)step) {
+                        tc_wait_st();
+                        const int see = min(last - j * kPaKeys, kPaKeys - 1);
+                        for (int c = 0; c < HD; c += 32) {
+                            float o[32];
+#pragma unroll
+                            for (int e = 0; e < 32; ++e) o[e] = 0.0f;
+                            for (int k = 0; k < kPaKeys; ++k) {
+                                unsigned w = tc_ld1(st + (k >> 1));
+                                tc_wait_ld();
+                                asm volatile("" : "+r"(w));
+                                if (k <= see) {
+                                    const float p = __uint_as_float(k & 1 ? w & 0xffff0000u : w << 16);
+                                    const unsigned char* line = v + (c / 64) * (M::tile / C) + k * 128;
+#pragma unroll
+                                    for (int e = 0; e < 4; ++e) {
+                                        const uint4 x = *reinterpret_cast<const uint4*>(line + (((c % 64) / 8 + e) ^ (k & 7)) * 16);
+                                        const unsigned xs[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                                        for (int h = 0; h < 4; ++h) {
+                                            o[8 * e + 2 * h] = fmaf(p, __uint_as_float(xs[h] << 16), o[8 * e + 2 * h]);
+                                            o[8 * e + 2 * h + 1] = fmaf(p, __uint_as_float(xs[h] & 0xffff0000u), o[8 * e + 2 * h + 1]);
+                                        }
                                     }
                                 }
+                                __syncwarp();
                             }
-                            __syncwarp();
-                        }
-                        unsigned r[32];
-                        if (j > 0) {
-                            tc_ld32(ot + c, r);
-                            tc_wait_ld();
-                            tc_pin32(r);
-                        }
+                            unsigned r[32];
+                            if (j > 0) {
+                                tc_ld32(ot + c, r);
+                                tc_wait_ld();
+                                tc_pin32(r);
+                            }
 #pragma unroll
-                        for (int e = 0; e < 32; ++e) r[e] = __float_as_uint(o[e] + (j > 0 ? __uint_as_float(r[e]) : 0.0f));
-                        tc_st32(ot + c, r);
+                            for (int e = 0; e < 32; ++e) r[e] = __float_as_uint(o[e] + (j > 0 ? __uint_as_float(r[e]) : 0.0f));
+                            tc_st32(ot + c, r);
+                        }
+                    }
+                }
+                tc_wait_st();
+                tc_before();
+                __syncwarp();
+                if (lane == 0) {
+                    if (masked) tc_bar_arrive(p_half + 8 * i);
+                    tc_bar_arrive(p_full + 8 * i);
+                }
+            }
+            if (ok && live > 0) {
+                const int position = row / P.share;
+                const bool out = position < live && row < per * P.share;
+                sum2[0] = pa_add2(sum2[0], sum2[1]);
+                const float total = __uint_as_float((unsigned)sum2[0]) + __uint_as_float((unsigned)(sum2[0] >> 32)), inv = total == 0.0f ? 0.0f : 1.0f / total;
+                uint4* to = reinterpret_cast<uint4*>(reinterpret_cast<__nv_bfloat16*>(P.out) +
+                                                     ((size_t)(item.row + pos + (out ? position : 0)) * P.q_heads + item.head * P.share + (out ? row % P.share : 0)) * HD);
+                if (steps) {
+                    ok = wait(o_full + 8 * i, items++ & 1);
+                    tc_after();
+                }
+                for (int c = 0; c < HD && ok; c += 32) {
+                    unsigned o[32];
+                    if (steps) {
+                        tc_ld32(ot + c, o);
+                        tc_wait_ld();
+                        tc_pin32(o);
+                    }
+                    if (!out) continue;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        unsigned w[4];
+#pragma unroll
+                        for (int h = 0; h < 4; ++h) {
+                            // (a row whose weights are all zero has a sum of zero: nothing it saw, or scores of -inf)
+                            const float x = steps ? __uint_as_float(o[8 * e + 2 * h]) * inv : 0.0f, y = steps ? __uint_as_float(o[8 * e + 2 * h + 1]) * inv : 0.0f;
+                            const __nv_bfloat162 p = __floats2bfloat162_rn(x, y);
+                            w[h] = *reinterpret_cast<const unsigned*>(&p);
+                        }
+                        to[c / 8 + e] = make_uint4(w[0], w[1], w[2], w[3]);
                     }
                 }
             }
-            tc_wait_st();
-            tc_before();
-            __syncwarp();
-            if (lane == 0) {
-                if (masked) tc_bar_arrive(p_half + 8 * i);
-                tc_bar_arrive(p_full + 8 * i);
-            }
-        }
-        if (ok && live[i] > 0) {
-            const int position = row / P.share;
-            const bool out = position < live[i] && row < per * P.share;
-            sum2[0] = pa_add2(sum2[0], sum2[1]);
-            const float total = __uint_as_float((unsigned)sum2[0]) + __uint_as_float((unsigned)(sum2[0] >> 32)), inv = total == 0.0f ? 0.0f : 1.0f / total;
-            uint4* to = reinterpret_cast<uint4*>(reinterpret_cast<__nv_bfloat16*>(P.out) +
-                                                 ((size_t)(rows.first + pos[i] + (out ? position : 0)) * P.q_heads + head * P.share + (out ? row % P.share : 0)) * HD);
-            if (steps[i]) {
-                ok = wait(o_full + 8 * i, 0);
-                tc_after();
-            }
-            for (int c = 0; c < HD && ok; c += 32) {
-                unsigned o[32];
-                if (steps[i]) {
-                    tc_ld32(ot + c, o);
-                    tc_wait_ld();
-                    tc_pin32(o);
-                }
-                if (!out) continue;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    unsigned w[4];
-#pragma unroll
-                    for (int h = 0; h < 4; ++h) {
-                        // (a row whose weights are all zero has a sum of zero: nothing it saw, or scores of -inf)
-                        const float x = steps[i] ? __uint_as_float(o[8 * e + 2 * h]) * inv : 0.0f, y = steps[i] ? __uint_as_float(o[8 * e + 2 * h + 1]) * inv : 0.0f;
-                        const __nv_bfloat162 p = __floats2bfloat162_rn(x, y);
-                        w[h] = *reinterpret_cast<const unsigned*>(&p);
-                    }
-                    to[c / 8 + e] = make_uint4(w[0], w[1], w[2], w[3]);
-                }
-            }
+            before += item.n;
+            if (!ok) break;
         }
     }
     if (!ok) atomicExch(&g_prompt_error, 1);

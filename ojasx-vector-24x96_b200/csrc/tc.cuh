@@ -23,6 +23,22 @@ __device__ __forceinline__ bool tc_wait(unsigned bar, unsigned parity, unsigned 
     asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(done) : "r"(bar), "r"(parity) : "memory");
     return __all_sync(0xffffffffu, done) || __all_sync(0xffffffffu, bar_wait(bar, parity, gone));
 }
+// Asks for a CTA of the grid that has not begun, to do its work in its place: 16 bytes at `to` and on `bar` (whose transaction count
+// the caller raises); then its number, or -1 where there is none any more (after which nothing may be asked again).
+__device__ __forceinline__ void tc_steal(unsigned to, unsigned bar) {
+    asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(to), "r"(bar) : "memory");
+}
+__device__ __forceinline__ int tc_stolen(unsigned from) {
+    int cta;
+    asm volatile(
+        "{\n\t.reg .b128 h;\n\t.reg .pred p;\n\tld.shared.b128 h, [%1];\n\tmov.u32 %0, -1;\n\t"
+        "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, h;\n\t"
+        "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %0, h;\n\t}"
+        : "=r"(cta)
+        : "r"(from)
+        : "memory");
+    return cta;
+}
 // A place in a ring of N stages and the parity of its next phase.
 template <int N>
 struct TcRing {

@@ -31,7 +31,8 @@ struct PromptProblem {
 // one, 128 threads are at the other's exponentials.
 //   warps 0..3, 4..7: the rows of the two tiles; warp 8: issues the products; warp 9: the copies of Q, K and V (K and V in a ring);
 //   warp 11: what to do next, so that a CTA's copies and products for one part of the prompts begin while it is at the last results of
-//   another; warp 10: nothing here, the keys' factors of fp32 (registers are moved between groups of four warps: 384 * 168 = 64512 are 2 * 128 * 216 + 128 * 64 and some)
+//   another; warp 10: nothing here, the keys' factors of fp32 (registers are moved between groups of four
+//   warps: 384 * 168 = 64512 are 2 * 128 * 232 + 128 * 40; with 216 for a row 561 us at 8192 positions, 152 packed, against 517 and 139)
 // Maxima are left behind: a row's sums are relative to the maximum it had when a score was last more than 2^8 above it, so that
 // O is rescaled a few times per row and not once per step (weights up to 2^8 cost nothing in bf16 or in fp32 sums).
 constexpr int kPaRows = 128, kPaKeys = 128, kPaThreads = 384;
@@ -143,7 +144,7 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_tc_kernel(const __grid_c
     };
 
     if (warp >= 8) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
         if (warp == 11) {
             // Work: the CTA's own part of the prompts, and then those of CTAs that have not begun, asked for when the copies of the last one
             // have been issued.  The last parts of a sequence, which see the most keys, come first.
@@ -298,7 +299,7 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_tc_kernel(const __grid_c
             }
         }
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
         const int i = warp >> 2, row = tid & 127;   // the row's lane of tensor memory is its place in the tile
         const unsigned lanes = (unsigned)((warp & 3) * 32) << 16, st = tmem + i * 128 + lanes, ot = tmem + 256 + i * 128 + lanes;
         const float scale = P.scale * 1.4426950408889634f;
@@ -315,9 +316,19 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_tc_kernel(const __grid_c
                 tc_st32(ot + c, o);
             }
         };
-        for (int number = 0; take(number); ++number) {
-            const int pos = i ? item.pos[1] : item.pos[0], live = i ? item.live[1] : item.live[0], steps = i ? item.steps[1] : item.steps[0];
-            const int last = pos + min(row, max(live * P.share - 1, 0)) / P.share + item.ahead;   // last key that the row sees
+        for (int number = 0;; ++number) {
+            // (read again where it is needed: registers are short between)
+            const volatile int* const what = s_item[number & 1];
+            if (!(ok = wait(item_full + 8 * (number & 1), (number >> 1) & 1)) || what[0] < 0) break;
+            int steps, last, first, n;   // of the tile; last key that the row sees, and that the tile's first row sees; steps of both tiles
+            {
+                const int pos = what[4] + i * per, live = what[5 + i], ahead = what[2], end = pos + live + ahead;
+                steps = live > 0 ? max(0, end + kPaKeys - 1) / kPaKeys : 0;
+                first = pos + ahead;
+                last = first + min(row, max(live * P.share - 1, 0)) / P.share;
+                const int other = what[6 - i], to = what[4] + (1 - i) * per + other + ahead;
+                n = max(steps, other > 0 ? max(0, to + kPaKeys - 1) / kPaKeys : 0);
+            }
             float top = 0.0f;
             unsigned long long sum2[2] = {0, 0};
             for (int j = 0; j < steps; ++j) {
@@ -330,7 +341,7 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_tc_kernel(const __grid_c
                 tc_wait_ld();
 #pragma unroll
                 for (int c = 0; c < 4; ++c) tc_pin32(s + 32 * c);
-                const bool masked = (j + 1) * kPaKeys - 1 > pos + item.ahead;   // some row does not see all of these keys
+                const bool masked = (j + 1) * kPaKeys - 1 > first;   // some row does not see all of these keys
                 if (masked) {
                     const int see = last - j * kPaKeys;
 #pragma unroll
@@ -438,13 +449,14 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_tc_kernel(const __grid_c
                     tc_bar_arrive(p_full + 8 * i);
                 }
             }
+            const int live = what[5 + i];
             if (ok && live > 0) {
                 const int position = row / P.share;
                 const bool out = position < live && row < per * P.share;
                 sum2[0] = pa_add2(sum2[0], sum2[1]);
                 const float total = __uint_as_float((unsigned)sum2[0]) + __uint_as_float((unsigned)(sum2[0] >> 32)), inv = total == 0.0f ? 0.0f : 1.0f / total;
                 uint4* to = reinterpret_cast<uint4*>(reinterpret_cast<__nv_bfloat16*>(P.out) +
-                                                     ((size_t)(item.row + pos + (out ? position : 0)) * P.q_heads + item.head * P.share + (out ? row % P.share : 0)) * HD);
+                                                     ((size_t)(what[0] + what[4] + i * per + (out ? position : 0)) * P.q_heads + what[3] * P.share + (out ? row % P.share : 0)) * HD);
                 if (steps) {
                     ok = wait(o_full + 8 * i, items++ & 1);
                     tc_after();
@@ -471,8 +483,10 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_tc_kernel(const __grid_c
                     }
                 }
             }
-            before += item.n;
             if (!ok) break;
+            before += n;
+            __syncwarp();
+            if (lane == 0) tc_bar_arrive(item_empty + 8 * (number & 1));
         }
     }
     if (!ok) atomicExch(&g_prompt_error, 1);

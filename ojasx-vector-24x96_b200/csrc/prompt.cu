@@ -526,17 +526,18 @@ static int launch_prompt_tc(const PromptProblem& P, cudaStream_t s) {
 //   those of Q and K are taken out of the scores (a factor per row, a factor per key);
 //   those of V go into the weights, y = 2^(x + e - reference) with e the exponent of the key's largest value, so that a weight times its
 //   value is what it is, and the sum of weights takes y * 2^-e.  e stays in -20..100: the values of a smaller row keep fewer bits.
-// Steps are of 48 keys (two tiles' Q take 128 KB, two steps' K and V 96).  The tensor cores cut what they add to a sum, so a step's
-// products with V are summed on their own and join the row's fp32 sums, which are in its thread's registers.
-constexpr int kPpKeys = 48;
+// The high parts of Q are in tensor memory, where products take them without the shared memory's bandwidth; the low ones, and K and V
+// in steps of 64 keys, are in shared memory.  The tensor cores cut what they add to a sum, so a step's products with V are summed on
+// their own and join the row's fp32 sums, which are in its thread's registers.
+constexpr int kPpKeys = 64;
 constexpr float kPpRoom = 5.0f;   // y is 2^5 at most when the reference is set, 2^13 later on
 
 template <int HD>
 struct PpSmem {
-    static constexpr int plane = 128 * HD * 2, tile = 2 * plane;              // of Q
+    static constexpr int tile = 128 * HD * 2;                                 // of Q: the low parts
     static constexpr int part = kPpKeys * HD * 2, slot = 2 * part;            // of K or V: two planes
     static constexpr int slots = HD == 128 ? 4 : 8;
-    static constexpr int ring = 2 * tile, factors = ring + slots * slot;      // [2][3][48]: of K, e, 2^-e
+    static constexpr int ring = 2 * tile, factors = ring + slots * slot;      // [2][3][64]: of K, e, 2^-e
     static constexpr int bars = factors + 2 * 3 * kPpKeys * 4;
     static constexpr int bytes = bars + 256 + 1024;
 };
@@ -643,7 +644,8 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_pair_kernel(const __grid
     tc_before();
     __syncthreads();
     tc_after();
-    const unsigned tmem = __shfl_sync(0xffffffffu, s_tmem, 0);   // S and then the weights of tile i at 64 i (hi 24 columns, lo 24), a step's O at 256 + 128 i
+    // S and then the weights of tile i at 64 i (hi 32 columns, lo 32), Q's high parts at 128 + 64 i, a step's O at 256 + 128 i
+    const unsigned tmem = __shfl_sync(0xffffffffu, s_tmem, 0);
     const PackedRange rows = packed_range(P.ends, s_seq, P.n_rows), keys = packed_range(P.key_ends, s_seq, P.n_keys);
     const int ahead = keys.count - rows.count;
     int pos[2], live[2], steps[2];
@@ -658,7 +660,7 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_pair_kernel(const __grid
     auto wait = [&](unsigned bar, unsigned parity) { return tc_wait(bar, parity, gone); };
 
     if (warp >= 8) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
         if (warp == 9 && lane == 0) {
             int s = 0;
             for (; s < 2 * n; ++s) {   // K of step 0, V of step 0, K of step 1, ...
@@ -694,12 +696,13 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_pair_kernel(const __grid
             auto scores = [&](int i, int slot) {
                 const unsigned long long a = tc_at(q_desc, i * M::tile), b = tc_at(ring_k, slot * M::slot);
 #pragma unroll
-                for (int p = 0; p < 3; ++p) {   // lo hi, hi lo, hi hi
+                for (int k = 0; k < HD / 16; ++k)   // lo hi
+                    tc_mma(lead, tmem + i * 64, tc_at(a, (k / 4) * (M::tile / C) + (k % 4) * 32), tc_at(b, (k / 4) * (M::part / C) + (k % 4) * 32), iq, k > 0);
+#pragma unroll
+                for (int p = 1; p >= 0; --p)        // hi lo, hi hi
 #pragma unroll
                     for (int k = 0; k < HD / 16; ++k)
-                        tc_mma(lead, tmem + i * 64, tc_at(a, (p == 0) * M::plane + (k / 4) * (M::plane / C) + (k % 4) * 32),
-                               tc_at(b, (p == 1) * M::part + (k / 4) * (M::part / C) + (k % 4) * 32), iq, p > 0 || k > 0);
-                }
+                        tc_mma_ts(lead, tmem + i * 64, tmem + 128 + i * 64 + k * 8, tc_at(b, p * M::part + (k / 4) * (M::part / C) + (k % 4) * 32), iq, true);
                 tc_commit(lead, s_full + 8 * i);
             };
             TcRing<NS> kr{0, 0}, vr{1, 0};
@@ -748,7 +751,7 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_pair_kernel(const __grid
             }
         }
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
         const int i = warp >> 2, row = tid & 127;
         const int at = min(row, max(live[i] * P.share - 1, 0)), last = pos[i] + at / P.share + ahead;
         const bool out = row < live[i] * P.share;
@@ -757,38 +760,61 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_pair_kernel(const __grid
         const int q_head = head * P.share + (out ? row % P.share : 0);
         int checks = 0;
         float unscale = 0.0f;
-        if (steps[i]) {   // the warp's rows of Q, HD / 4 lanes to a row
+        if (steps[i]) {   // the warp's rows of Q, HD / 4 lanes to a row: the high parts through shared memory to tensor memory, then the low ones
             constexpr int L = HD / 4, R = 32 / L;
-            const int r0 = (warp & 3) * 32 + lane / L, l = lane % L;
-#pragma unroll 4
-            for (int r = 0; r < 32; r += R) {
-                const int mine = r0 + r;
-                float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                if (mine < live[i] * P.share)
-                    x = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(P.q) + (size_t)(rows.first + pos[i] + mine / P.share) * P.q_row +
-                                                         (size_t)(head * P.share + mine % P.share) * P.q_head + 4 * l);
-                unsigned most = max(max(__float_as_uint(x.x) & 0x7fffffffu, __float_as_uint(x.y) & 0x7fffffffu),
-                                    max(__float_as_uint(x.z) & 0x7fffffffu, __float_as_uint(x.w) & 0x7fffffffu));
+            const int l = lane % L, sub = lane / L;
+            const long long from = out ? (long long)where * P.q_row + (long long)q_head * P.q_head : -1;   // of the thread's own row
+            float4 x[32 / R];
+#pragma unroll
+            for (int r = 0; r < 32 / R; ++r) {   // (all loads before the first is waited for)
+                const long long at_row = __shfl_sync(0xffffffffu, from, r * R + sub);
+                x[r] = at_row >= 0 ? *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(P.q) + at_row + 4 * l) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            }
+#pragma unroll
+            for (int r = 0; r < 32 / R; ++r) {
+                unsigned most = max(max(__float_as_uint(x[r].x) & 0x7fffffffu, __float_as_uint(x[r].y) & 0x7fffffffu),
+                                    max(__float_as_uint(x[r].z) & 0x7fffffffu, __float_as_uint(x[r].w) & 0x7fffffffu));
 #pragma unroll
                 for (int off = L / 2; off >= 1; off >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, off));
                 float up, down;
                 gm_scale(most, up, down);
-                const float a = x.x * up, b = x.y * up, c = x.z * up, d = x.w * up;
-                const __half2 h0 = __floats2half2_rn(a, b), h1 = __floats2half2_rn(c, d);
-                unsigned char* to = smem + i * M::tile + (4 * l / 64) * (M::plane / C) + mine * 128 + (((l % 16) / 2 ^ (mine & 7)) << 4) + (l & 1) * 8;
-                *reinterpret_cast<uint2*>(to) = make_uint2(*reinterpret_cast<const unsigned*>(&h0), *reinterpret_cast<const unsigned*>(&h1));
-                *reinterpret_cast<uint2*>(to + M::plane) = make_uint2(gm_pack(a - __low2float(h0), b - __high2float(h0)), gm_pack(c - __low2float(h1), d - __high2float(h1)));
-                const float back = __shfl_sync(0xffffffffu, down, (lane - r) * L & 31);   // lane r + k takes that of the k-th row of these
-                if (lane >= r && lane < r + R) unscale = back;
+                x[r] = make_float4(x[r].x * up, x[r].y * up, x[r].z * up, x[r].w * up);
+                const float back = __shfl_sync(0xffffffffu, down, (lane % R) * L);   // lane r * R + k takes that of the k-th row of these
+                if (lane / R == r) unscale = back;
+            }
+#pragma unroll
+            for (int low = 0; low < 2; ++low) {
+#pragma unroll
+                for (int r = 0; r < 32 / R; ++r) {
+                    const int mine = (warp & 3) * 32 + r * R + sub;
+                    const __half2 h0 = __floats2half2_rn(x[r].x, x[r].y), h1 = __floats2half2_rn(x[r].z, x[r].w);
+                    *reinterpret_cast<uint2*>(smem + i * M::tile + (4 * l / 64) * (M::tile / C) + mine * 128 + (((l % 16) / 2 ^ (mine & 7)) << 4) + (l & 1) * 8) =
+                        make_uint2(*reinterpret_cast<const unsigned*>(&h0), *reinterpret_cast<const unsigned*>(&h1));
+                    x[r] = make_float4(x[r].x - __low2float(h0), x[r].y - __high2float(h0), x[r].z - __low2float(h1), x[r].w - __high2float(h1));
+                }
+                __syncwarp();
+                if (low) break;
+#pragma unroll
+                for (int c = 0; c < C; ++c) {
+                    unsigned w[32];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        *reinterpret_cast<uint4*>(w + 4 * e) = *reinterpret_cast<const uint4*>(smem + i * M::tile + c * (M::tile / C) + row * 128 + ((e ^ (row & 7)) << 4));
+                    tc_st32(tmem + 128 + i * 64 + lanes + 32 * c, w);
+                }
+                tc_wait_st();
+                __syncwarp();
             }
             unscale *= P.scale * 1.4426950408889634f;
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            tc_before();
             __syncwarp();
             if (lane == 0) tc_bar_arrive(q_full + 8 * i);
         }
-        float top = -INFINITY, sum[2] = {0.0f, 0.0f}, o[HD];
+        float top = -INFINITY;
+        unsigned long long sum = 0, o[HD / 2];
 #pragma unroll
-        for (int d = 0; d < HD; ++d) o[d] = 0.0f;
+        for (int d = 0; d < HD / 2; ++d) o[d] = 0;
         bool parted = false;   // a step's O is in tensor memory
         auto join = [&]() {
 #pragma unroll
@@ -798,7 +824,7 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_pair_kernel(const __grid
                 tc_wait_ld();
                 tc_pin32(x);
 #pragma unroll
-                for (int e = 0; e < 32; ++e) o[c + e] += __uint_as_float(x[e]);
+                for (int e = 0; e < 16; ++e) o[c / 2 + e] = pa_add2(o[c / 2 + e], (unsigned long long)x[2 * e + 1] << 32 | x[2 * e]);
             }
         };
         for (int j = 0; j < n; ++j) {
@@ -813,63 +839,63 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_pair_kernel(const __grid
             if (parted) join();
             unsigned s[N];
             tc_ld32(st, s);
-            tc_ld16(st + 32, s + 32);
+            tc_ld32(st + 32, s + 32);
             if (!(ok = wait(f_full + 8 * (j & 1), (j / 2) & 1))) break;
             tc_wait_ld();
             tc_pin32(s);
-            tc_pin16(s + 32);
+            tc_pin32(s + 32);
             const float* f = reinterpret_cast<const float*>(smem + M::factors) + (j & 1) * 3 * N;
             const bool masked = (j + 1) * N - 1 > pos[i] + ahead;
             const int see = last - j * N;
-            float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+            const unsigned long long unscale2 = pa_pair(unscale, unscale);
+            float m[2] = {-INFINITY, -INFINITY};
 #pragma unroll
             for (int e = 0; e < N; e += 4) {
-                const float4 kf = *reinterpret_cast<const float4*>(f + e), ex = *reinterpret_cast<const float4*>(f + N + e);
-                const float kfs[4] = {kf.x, kf.y, kf.z, kf.w}, exs[4] = {ex.x, ex.y, ex.z, ex.w};
+                const ulonglong2 kf = *reinterpret_cast<const ulonglong2*>(f + e), ex = *reinterpret_cast<const ulonglong2*>(f + N + e);
+                const unsigned long long x = pa_fma2(pa_mul2((unsigned long long)s[e + 1] << 32 | s[e], kf.x), unscale2, ex.x);
+                const unsigned long long y = pa_fma2(pa_mul2((unsigned long long)s[e + 3] << 32 | s[e + 2], kf.y), unscale2, ex.y);
+                s[e] = (unsigned)x; s[e + 1] = (unsigned)(x >> 32); s[e + 2] = (unsigned)y; s[e + 3] = (unsigned)(y >> 32);
+                if (masked) {
 #pragma unroll
-                for (int u = 0; u < 4; ++u) {
-                    float x = fmaf(__uint_as_float(s[e + u]) * kfs[u], unscale, exs[u]);
-                    if (masked) x = e + u > see ? -INFINITY : x;
-                    s[e + u] = __float_as_uint(x);
-                    m[u] = fmaxf(m[u], x);
+                    for (int u = 0; u < 4; ++u) s[e + u] = e + u > see ? 0xff800000u : s[e + u];
                 }
+                m[0] = pa_max3(m[0], __uint_as_float(s[e]), __uint_as_float(s[e + 1]));
+                m[1] = pa_max3(m[1], __uint_as_float(s[e + 2]), __uint_as_float(s[e + 3]));
             }
-            const float now = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])) - kPpRoom;
+            const float now = fmaxf(m[0], m[1]) - kPpRoom;
             const bool up = now > top + kPaSlack;
             if (j == 0) {
                 top = now;
             } else if (__any_sync(0xffffffffu, up)) {
                 const float by = up ? exp2f(top - now) : 1.0f;
+                const unsigned long long by2 = pa_pair(by, by);
                 top = up ? now : top;
-                sum[0] *= by;
-                sum[1] *= by;
+                sum = pa_mul2(sum, by2);
 #pragma unroll
-                for (int d = 0; d < HD; ++d) o[d] *= by;
+                for (int d = 0; d < HD / 2; ++d) o[d] = pa_mul2(o[d], by2);
             }
             const float off = top == -INFINITY ? 0.0f : top;
-            unsigned w[N / 2];   // low parts; the high ones take the scores' place
+            const unsigned long long off2 = pa_pair(-off, -off);
 #pragma unroll
-            for (int e = 0; e < N; e += 4) {
-                const float4 vf = *reinterpret_cast<const float4*>(f + 2 * N + e);
-                const float vfs[4] = {vf.x, vf.y, vf.z, vf.w};
-                float y[4];
+            for (int c = 0; c < N; c += 32) {
+                unsigned hi[16], lo[16];
 #pragma unroll
-                for (int u = 0; u < 4; ++u) {
-                    y[u] = __uint_as_float(s[e + u]) - off;
-                    asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(y[u]));
-                    sum[u & 1] = fmaf(y[u], vfs[u], sum[u & 1]);
+                for (int e = 0; e < 32; e += 4) {
+                    const ulonglong2 vf = *reinterpret_cast<const ulonglong2*>(f + 2 * N + c + e);
+                    const unsigned long long vfs[2] = {vf.x, vf.y};
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        const unsigned long long y = pa_exp2(pa_add2((unsigned long long)s[c + e + 2 * u + 1] << 32 | s[c + e + 2 * u], off2));
+                        sum = pa_fma2(y, vfs[u], sum);
+                        const __half2 h = __floats2half2_rn(__uint_as_float((unsigned)y), __uint_as_float((unsigned)(y >> 32)));
+                        const unsigned long long rest = pa_add2(y, pa_pair(-__low2float(h), -__high2float(h)));
+                        hi[e / 2 + u] = *reinterpret_cast<const unsigned*>(&h);
+                        lo[e / 2 + u] = gm_pack(__uint_as_float((unsigned)rest), __uint_as_float((unsigned)(rest >> 32)));
+                    }
                 }
-#pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    const __half2 h = __floats2half2_rn(y[2 * u], y[2 * u + 1]);
-                    s[e / 2 + u] = *reinterpret_cast<const unsigned*>(&h);
-                    w[e / 2 + u] = gm_pack(y[2 * u] - __low2float(h), y[2 * u + 1] - __high2float(h));
-                }
+                tc_st16(st + c / 2, hi);
+                tc_st16(st + N / 2 + c / 2, lo);
             }
-            tc_st16(st, s);
-            tc_st8(st + 16, s + 16);
-            tc_st16(st + N / 2, w);
-            tc_st8(st + N / 2 + 16, w + 16);
             parted = true;
             if (masked) {   // (as in the bf16 kernel: values that are not finite among those that are not seen)
                 if (!(ok = wait(full + 8 * ((2 * j + 1) % NS), ((2 * j + 1) / NS) & 1))) break;
@@ -908,8 +934,7 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_pair_kernel(const __grid
 #pragma unroll
                                     for (int h = 0; h < 4; ++h) {
                                         const __half2 vh = *reinterpret_cast<const __half2*>(&hs[h]), vl = *reinterpret_cast<const __half2*>(&ls[h]);
-                                        o[c + 8 * e + 2 * h] = fmaf(y, __low2float(vh) + __low2float(vl), o[c + 8 * e + 2 * h]);
-                                        o[c + 8 * e + 2 * h + 1] = fmaf(y, __high2float(vh) + __high2float(vl), o[c + 8 * e + 2 * h + 1]);
+                                        o[c / 2 + 4 * e + h] = pa_fma2(pa_pair(y, y), pa_pair(__low2float(vh) + __low2float(vl), __high2float(vh) + __high2float(vl)), o[c / 2 + 4 * e + h]);
                                     }
                                 }
                             }
@@ -931,11 +956,13 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_pair_kernel(const __grid
                 tc_after();
                 if (ok && parted) join();
             }
-            const float total = sum[0] + sum[1], inv = total == 0.0f ? 0.0f : 1.0f / (total * 16384.0f);   // (values are 2^14 times as large as their exponents say)
+            const float total = __uint_as_float((unsigned)sum) + __uint_as_float((unsigned)(sum >> 32)), inv = total == 0.0f ? 0.0f : 1.0f / (total * 16384.0f);   // (values are 2^14 times as large as their exponents say)
             if (ok && out) {
                 float4* to = reinterpret_cast<float4*>(reinterpret_cast<float*>(P.out) + (where * P.q_heads + q_head) * HD);
 #pragma unroll
-                for (int d = 0; d < HD; d += 4) to[d / 4] = make_float4(o[d] * inv, o[d + 1] * inv, o[d + 2] * inv, o[d + 3] * inv);
+                for (int d = 0; d < HD / 2; d += 2)
+                    to[d / 2] = make_float4(__uint_as_float((unsigned)o[d]) * inv, __uint_as_float((unsigned)(o[d] >> 32)) * inv,
+                                            __uint_as_float((unsigned)o[d + 1]) * inv, __uint_as_float((unsigned)(o[d + 1] >> 32)) * inv);
             }
         }
     }

@@ -130,6 +130,34 @@ def test_what_is_not_seen_has_no_part(cuda, dtype, hd, bad):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_many_short_sequences(cuda, dtype, hd):
+    """More parts than the GPU has SMs, of all kinds in turn: without queries, without keys, with values that are not finite behind what
+    is seen, with queries that see nothing."""
+    g = _gen(hd + 1)
+    lengths = [(7 * i) % 41 for i in range(300)] + [300, 0, 257]
+    key_lengths = [0 if i % 9 == 4 else n + (i % 5) * 30 if i % 3 else max(0, n - 5) for i, n in enumerate(lengths)]
+    n, m = sum(lengths), sum(key_lengths)
+    q, k, v = _randn(g, n, 6, hd, dtype=dtype), _randn(g, m, 2, hd, dtype=dtype), _randn(g, m, 2, hd, dtype=dtype)
+    want = ops.prompt_attention(q, k, v, _ends(lengths), _ends(key_lengths))
+    _check(q, k, v, lengths, key_lengths, want)
+    odd, at, e = v.clone(), 0, 0
+    keep = torch.ones(n, dtype=torch.bool, device=cuda)
+    for i, (a, b) in enumerate(zip(lengths, key_lengths)):
+        if i % 4 == 1 and a > 3 and b > 3:      # the last three keys: the last three queries alone see one of them
+            odd[e + b - 3:e + b] = math.inf
+            keep[at + a - 3:at + a] = False
+        at, e = at + a, e + b
+    got = ops.prompt_attention(q, k, odd, _ends(lengths), _ends(key_lengths))
+    # a part whose values are added one by one adds them in another order: both are within the tolerance of the 64-bit result, and
+    # rounded to bf16 (2^-8 of values up to 5)
+    bound = 2.0 ** -16 if dtype == torch.float32 else 2.0 ** -8 * 5
+    assert float((got[keep].float() - want[keep].float()).abs().max()) <= bound
+    assert not torch.isfinite(got[~keep].float()).any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_views_and_odd_layouts(cuda, dtype):
     g, n = _gen(3), 90
     x = _randn(g, n, 8 * 64 + 16, dtype=dtype)

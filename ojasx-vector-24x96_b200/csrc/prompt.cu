@@ -25,24 +25,25 @@ struct PromptProblem {
 
 // ------------------------------------------------------------------------------------ bf16 on the 5th-generation tensor cores
 //
-// A CTA has two tiles of 128 rows of one sequence and KV head (rows are (position, head of the KV head)) and walks the keys 128 at a
+// A CTA has two tiles of 128 rows of one sequence and KV head (rows are (position, head of the KV head)) and walks the keys 64 at a
 // time.  Per tile and step: S = Q K^T into tensor memory, one thread per row takes the maximum, the exponentials and their sum, writes
-// the weights back over S as bf16, O += P V with P read from tensor memory.  The two tiles take turns: while the tensor cores are at
-// one, 128 threads are at the other's exponentials.
+// the weights back over S as bf16, O += P V with P read from tensor memory.  A tile has S twice: the products of a step are made while
+// the row's threads are at the step before, and those of the tiles go on in turn.  (With one S of 128 keys a tile, whose products wait
+// for its weights: 526 us at 8192 positions, 139 packed.)
 //   warps 0..3, 4..7: the rows of the two tiles; warp 8: issues the products; warp 9: the copies of Q, K and V (K and V in a ring);
 //   warp 11: what to do next, so that a CTA's copies and products for one part of the prompts begin while it is at the last results of
-//   another; warp 10: nothing here, the keys' factors of fp32 (registers are moved between groups of four
-//   warps: 384 * 168 = 64512 are 2 * 128 * 232 + 128 * 40; with 216 for a row 561 us at 8192 positions, 152 packed, against 517 and 139)
+//   another (packed prompts 171 us without, 150 with it); warp 10: none.  Registers move between groups of four warps: 384 * 168 are
+//   2 * 128 * 200 + 128 * 96 and some.
 // Maxima are left behind: a row's sums are relative to the maximum it had when a score was last more than 2^8 above it, so that
 // O is rescaled a few times per row and not once per step (weights up to 2^8 cost nothing in bf16 or in fp32 sums).
-constexpr int kPaRows = 128, kPaKeys = 128, kPaThreads = 384;
+constexpr int kPaRows = 128, kPaKeys = 64, kPaThreads = 384;
 constexpr float kPaSlack = 8.0f;
 
 template <int HD>
 struct PaSmem {
-    static constexpr int tile = 128 * HD * 2;                     // 128 rows or keys
-    static constexpr int slots = HD == 128 ? 5 : 8;
-    static constexpr int ring = 2 * tile, bars = ring + slots * tile;
+    static constexpr int tile = 128 * HD * 2, part = kPaKeys * HD * 2;     // of Q, and of K or V
+    static constexpr int slots = 10;
+    static constexpr int ring = 2 * tile, bars = ring + slots * part;
     static constexpr int bytes = bars + 384 + 1024;               // (swizzled tiles begin on 1024 bytes)
 };
 
@@ -89,17 +90,18 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_tc_kernel(const __grid_c
     __shared__ __align__(16) int s_stolen[4];
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;   // (the same for a warp, as the compiler sees)
     const unsigned base = tc_smem(smem), bars = base + M::bars;
-    const unsigned full = bars, empty = bars + 8 * NS, q_full = empty + 8 * NS, s_full = q_full + 16, p_full = s_full + 16, o_full = p_full + 16,
-                   checked = o_full + 16, p_half = checked + 16, q_empty = p_half + 16, item_full = q_empty + 16, item_empty = item_full + 16,
+    const unsigned full = bars, empty = bars + 8 * NS, q_full = empty + 8 * NS, s_full = q_full + 16, p_full = s_full + 32, o_full = p_full + 32,
+                   checked = o_full + 16, q_empty = checked + 16, item_full = q_empty + 16, item_empty = item_full + 16,
                    want = item_empty + 16, steal = want + 8, ended = steal + 8, gone = tc_smem(&s_gone);
     const int per = kPaRows / P.share;
     if (tid == 0) {
         for (int i = 0; i < NS; ++i) { tc_bar_init(full + 8 * i, 1); tc_bar_init(empty + 8 * i, 1); }
         for (int i = 0; i < 2; ++i) {
             tc_bar_init(q_full + 8 * i, 1);
-            tc_bar_init(s_full + 8 * i, 1);
-            tc_bar_init(p_half + 8 * i, 4);
-            tc_bar_init(p_full + 8 * i, 4);
+            tc_bar_init(s_full + 16 * i, 1);
+            tc_bar_init(s_full + 16 * i + 8, 1);
+            tc_bar_init(p_full + 16 * i, 4);
+            tc_bar_init(p_full + 16 * i + 8, 4);
             tc_bar_init(o_full + 8 * i, 1);
             tc_bar_init(checked + 8 * i, 4);
             tc_bar_init(q_empty + 8 * i, 1);
@@ -144,7 +146,7 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_tc_kernel(const __grid_c
     };
 
     if (warp >= 8) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
         if (warp == 11) {
             // Work: the CTA's own part of the prompts, and then those of CTAs that have not begun, asked for when the copies of the last one
             // have been issued.  The last parts of a sequence, which see the most keys, come first.
@@ -195,9 +197,9 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_tc_kernel(const __grid_c
                     if (quota > 0) --quota;
                     else if (!(ok = wait(empty + 8 * ring.slot, ring.parity))) return;
                     if (lane == 0) {
-                        tc_bar_expect(full + 8 * ring.slot, M::tile);
+                        tc_bar_expect(full + 8 * ring.slot, M::part);
                         for (int c = 0; c < C; ++c)
-                            tc_load3(base + M::ring + ring.slot * M::tile + c * (M::tile / C), value ? &v_map : &k_map, 64 * c, item.head, item.key + j * kPaKeys,
+                            tc_load3(base + M::ring + ring.slot * M::part + c * (M::part / C), value ? &v_map : &k_map, 64 * c, item.head, item.key + j * kPaKeys,
                                      full + 8 * ring.slot);
                     }
                     __syncwarp();
@@ -229,67 +231,67 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_tc_kernel(const __grid_c
         if (warp == 8) {
             const unsigned lead = tc_lead();
             constexpr unsigned iq = tc_idesc<true, false>(kPaKeys), iv = tc_idesc<true, true>(HD);
-            const unsigned long long ring_k = tc_desc(base + M::ring), ring_v = tc_desc(base + M::ring, M::tile / C), q_desc = tc_desc(base);
-            auto scores = [&](int i, int slot) {
-                const unsigned long long a = tc_at(q_desc, i * M::tile), b = tc_at(ring_k, slot * M::tile);
+            const unsigned long long ring_k = tc_desc(base + M::ring), ring_v = tc_desc(base + M::ring, M::part / C), q_desc = tc_desc(base);
+            auto scores = [&](int i, int half, int slot) {
+                const unsigned long long a = tc_at(q_desc, i * M::tile), b = tc_at(ring_k, slot * M::part);
 #pragma unroll
-                for (int k = 0; k < HD / 16; ++k) {
-                    const int off = (k / 4) * (M::tile / C) + (k % 4) * 32;
-                    tc_mma(lead, tmem + i * 128, tc_at(a, off), tc_at(b, off), iq, k > 0);
-                }
-                tc_commit(lead, s_full + 8 * i);
+                for (int k = 0; k < HD / 16; ++k)
+                    tc_mma(lead, tmem + i * 128 + half * 64, tc_at(a, (k / 4) * (M::tile / C) + (k % 4) * 32), tc_at(b, (k / 4) * (M::part / C) + (k % 4) * 32), iq, k > 0);
+                tc_commit(lead, s_full + 16 * i + 8 * half);
             };
             TcRing<NS> kr{0, 0}, vr{1, 0};
-            unsigned done[2] = {0, 0}, items[2] = {0, 0};   // steps of the tiles so far, and items
+            unsigned done[2] = {0, 0}, halves[2] = {0, 0}, items[2] = {0, 0};   // steps of the tiles so far, those with either S (a bit each), and items
             for (int number = 0; take(number); ++number) {
                 const int n = item.n;
-                if (n == 0) continue;
-                ok = wait(full + 8 * kr.slot, kr.parity);
 #pragma unroll
-                for (int i = 0; i < 2; ++i)
-                    if (ok && item.steps[i]) {
-                        ok = wait(q_full + 8 * i, items[i]++ & 1);
-                        if (!ok) continue;
-                        tc_after();
-                        scores(i, kr.slot);
-                        if (item.steps[i] == 1) tc_commit(lead, q_empty + 8 * i);
+                for (int j = 0; j < 2; ++j) {   // the scores of two steps ahead
+                    if (j >= n || !ok) continue;
+                    ok = wait(full + 8 * kr.slot, kr.parity);
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        if (j >= item.steps[i] || !ok) continue;
+                        if (j == 0) {
+                            if (!(ok = wait(q_full + 8 * i, items[i]++ & 1))) continue;
+                            tc_after();
+                        }
+                        scores(i, j, kr.slot);
+                        if (j + 1 == item.steps[i]) tc_commit(lead, q_empty + 8 * i);
                     }
-                if (!ok) break;
-                tc_commit(lead, empty + 8 * kr.slot);
-                for (int j = 0; j < n && ok; ++j) {
+                    tc_commit(lead, empty + 8 * kr.slot);
                     kr.next(2);
-                    bool loaded = false;   // K of the next step
+                }
+                for (int j = 0; j < n && ok; ++j) {
+                    bool loaded = false;   // K of the step after the next
                     ok = wait(full + 8 * vr.slot, vr.parity);
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
                         if (j >= item.steps[i] || !ok) continue;
                         const unsigned step = ++done[i];
-                        // the first 64 keys' weights come earlier, so that their product runs beside the other half's exponentials
-                        const unsigned long long b = tc_at(ring_v, vr.slot * M::tile);
-                        const bool maybe = (j + 1) * kPaKeys - 1 > item.pos[i] + item.ahead;
+                        if (!(ok = wait(p_full + 16 * i + 8 * (j & 1), halves[i] >> (j & 1) & 1))) continue;
+                        halves[i] ^= 1u << (j & 1);
+                        tc_after();
+                        // (values that are not finite behind what is seen: the rows have added their products themselves)
+                        if (!((j + 1) * kPaKeys - 1 > item.pos[i] + item.ahead && *reinterpret_cast<volatile int*>(&s_odd[i]) == (int)step)) {
+                            const unsigned long long b = tc_at(ring_v, vr.slot * M::part);
 #pragma unroll
-                        for (int half = 0; half < 2; ++half) {
-                            if (!(ok = wait((half ? p_full : p_half) + 8 * i, (step - 1) & 1))) break;
-                            tc_after();
-                            if (maybe && *reinterpret_cast<volatile int*>(&s_odd[i]) == (int)step) continue;   // (the rows have added their products themselves)
-#pragma unroll
-                            for (int k = half * kPaKeys / 32; k < (half + 1) * kPaKeys / 32; ++k)
-                                tc_mma_ts(lead, tmem + 256 + i * 128, tmem + i * 128 + k * 8, tc_at(b, k * 2048), iv, j > 0 || k > 0);
+                            for (int k = 0; k < kPaKeys / 16; ++k)
+                                tc_mma_ts(lead, tmem + 256 + i * 128, tmem + i * 128 + (j & 1) * 64 + k * 8, tc_at(b, k * 2048), iv, j > 0 || k > 0);
                         }
-                        if (!ok) continue;
-                        if (j + 1 < item.steps[i]) {
+                        tc_commit(lead, o_full + 8 * i);
+                        if (j + 2 < item.steps[i]) {
                             if (!loaded && !(ok = wait(full + 8 * kr.slot, kr.parity))) continue;
                             loaded = true;
-                            scores(i, kr.slot);   // (in order: its commit says that O is up to date, too)
-                            if (j + 2 == item.steps[i]) tc_commit(lead, q_empty + 8 * i);
-                        } else {
-                            tc_commit(lead, o_full + 8 * i);
+                            scores(i, j & 1, kr.slot);   // (behind the products that read the weights in their place)
+                            if (j + 3 == item.steps[i]) tc_commit(lead, q_empty + 8 * i);
                         }
                     }
                     if (!ok) break;
                     tc_commit(lead, empty + 8 * vr.slot);
-                    if (j + 1 < n) tc_commit(lead, empty + 8 * kr.slot);
                     vr.next(2);
+                    if (j + 2 < n) {
+                        tc_commit(lead, empty + 8 * kr.slot);
+                        kr.next(2);
+                    }
                 }
                 if (!ok) break;
             }
@@ -299,12 +301,12 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_tc_kernel(const __grid_c
             }
         }
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
         const int i = warp >> 2, row = tid & 127;   // the row's lane of tensor memory is its place in the tile
         const unsigned lanes = (unsigned)((warp & 3) * 32) << 16, st = tmem + i * 128 + lanes, ot = tmem + 256 + i * 128 + lanes;
         const float scale = P.scale * 1.4426950408889634f;
         int checks = 0;
-        unsigned done = 0, items = 0, before = 0;   // steps of the tile so far, its items, and the steps of the CTA
+        unsigned done = 0, halves = 0, before = 0;   // steps of the tile so far, those with either S (a bit each), and the CTA's
         auto rescale = [&](float by) {   // the warp's rows of O
             for (int c = 0; c < HD; c += 32) {
                 unsigned o[32];
@@ -333,23 +335,25 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_tc_kernel(const __grid_c
             unsigned long long sum2[2] = {0, 0};
             for (int j = 0; j < steps; ++j) {
                 const unsigned step = ++done;
-                if (!(ok = wait(s_full + 8 * i, (step - 1) & 1))) break;
+                const unsigned at = st + (j & 1) * 64;
+                if (!(ok = wait(s_full + 16 * i + 8 * (j & 1), halves >> (j & 1) & 1))) break;
+                halves ^= 1u << (j & 1);
                 tc_after();
-                unsigned s[128];
-#pragma unroll
-                for (int c = 0; c < 4; ++c) tc_ld32(st + 32 * c, s + 32 * c);
+                unsigned s[64];
+                tc_ld32(at, s);
+                tc_ld32(at + 32, s + 32);
                 tc_wait_ld();
-#pragma unroll
-                for (int c = 0; c < 4; ++c) tc_pin32(s + 32 * c);
+                tc_pin32(s);
+                tc_pin32(s + 32);
                 const bool masked = (j + 1) * kPaKeys - 1 > first;   // some row does not see all of these keys
                 if (masked) {
                     const int see = last - j * kPaKeys;
 #pragma unroll
-                    for (int e = 0; e < 128; ++e) s[e] = e > see ? 0xff800000u : s[e];
+                    for (int e = 0; e < 64; ++e) s[e] = e > see ? 0xff800000u : s[e];
                 }
                 float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                for (int e = 0; e < 128; e += 8)
+                for (int e = 0; e < 64; e += 8)
 #pragma unroll
                     for (int u = 0; u < 4; ++u) m[u] = pa_max3(m[u], __uint_as_float(s[e + 2 * u]), __uint_as_float(s[e + 2 * u + 1]));
                 const float now = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
@@ -357,6 +361,8 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_tc_kernel(const __grid_c
                 if (j == 0) {
                     top = now;
                 } else if (__any_sync(0xffffffffu, up)) {
+                    if (!(ok = wait(o_full + 8 * i, (step - 2) & 1))) break;   // the products of the step before
+                    tc_after();
                     const float to = up ? now : top, by = up ? exp2f((top - now) * scale) : 1.0f;
                     rescale(by);
                     sum2[0] = pa_mul2(sum2[0], pa_pair(by, by));
@@ -365,33 +371,23 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_tc_kernel(const __grid_c
                 }
                 const float off = top == -INFINITY ? 0.0f : top * scale;   // (a row that has seen nothing: its weights are exp(-inf))
                 const unsigned long long scale2 = pa_pair(scale, scale), off2 = pa_pair(-off, -off);
+                unsigned w[32];
 #pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    unsigned w[32];
-#pragma unroll
-                    for (int e = 0; e < 32; ++e) {
-                        unsigned long long x = pa_fma2((unsigned long long)s[64 * c + 2 * e + 1] << 32 | s[64 * c + 2 * e], scale2, off2);
-                        x = pa_exp2(x);
-                        sum2[e & 1] = pa_add2(sum2[e & 1], x);
-                        const __nv_bfloat162 h = __floats2bfloat162_rn(__uint_as_float((unsigned)x), __uint_as_float((unsigned)(x >> 32)));
-                        w[e] = *reinterpret_cast<const unsigned*>(&h);
-                    }
-                    tc_st32(st + 32 * c, w);
-                    if (c == 0 && !masked) {
-                        tc_wait_st();
-                        tc_before();
-                        __syncwarp();
-                        if (lane == 0) tc_bar_arrive(p_half + 8 * i);
-                    }
+                for (int e = 0; e < 32; ++e) {
+                    const unsigned long long x = pa_exp2(pa_fma2((unsigned long long)s[2 * e + 1] << 32 | s[2 * e], scale2, off2));
+                    sum2[e & 1] = pa_add2(sum2[e & 1], x);
+                    const __nv_bfloat162 h = __floats2bfloat162_rn(__uint_as_float((unsigned)x), __uint_as_float((unsigned)(x >> 32)));
+                    w[e] = *reinterpret_cast<const unsigned*>(&h);
                 }
+                tc_st32(at, w);
                 if (masked) {
                     // A weight of zero times an infinity is a NaN, and the products take all keys of the step.  Where a value among them is
                     // not finite (padding behind a sequence, another sequence's rows) each row adds the values that it sees itself.
                     const unsigned place = 2 * (before + j) + 1;
                     if (!(ok = wait(full + 8 * (place % NS), place / NS & 1))) break;
-                    const unsigned char* v = smem + M::ring + place % NS * M::tile;
+                    const unsigned char* v = smem + M::ring + place % NS * M::part;
                     unsigned odd = 0;
-                    for (int e = row; e < M::tile / 16; e += 128) {
+                    for (int e = row; e < M::part / 16; e += 128) {
                         const uint4 x = reinterpret_cast<const uint4*>(v)[e];   // an exponent of all ones carries into the sign's place
                         odd |= (((x.x & 0x7f807f80u) + 0x00800080u) | ((x.y & 0x7f807f80u) + 0x00800080u) | ((x.z & 0x7f807f80u) + 0x00800080u) |
                                 ((x.w & 0x7f807f80u) + 0x00800080u)) & 0x80008000u;
@@ -403,6 +399,8 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_tc_kernel(const __grid_c
                     }
                     if (!(ok = wait(checked + 8 * i, checks++ & 1))) break;
                     if (*reinterpret_cast<volatile int*>(&s_odd[i]) == (int)step) {
+                        if (j > 0 && !(ok = wait(o_full + 8 * i, (step - 2) & 1))) break;
+                        tc_after();
                         tc_wait_st();
                         const int see = min(last - j * kPaKeys, kPaKeys - 1);
                         for (int c = 0; c < HD; c += 32) {
@@ -410,12 +408,12 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_tc_kernel(const __grid_c
 #pragma unroll
                             for (int e = 0; e < 32; ++e) o[e] = 0.0f;
                             for (int k = 0; k < kPaKeys; ++k) {
-                                unsigned w = tc_ld1(st + (k >> 1));
+                                unsigned w = tc_ld1(at + (k >> 1));
                                 tc_wait_ld();
                                 asm volatile("" : "+r"(w));
                                 if (k <= see) {
                                     const float p = __uint_as_float(k & 1 ? w & 0xffff0000u : w << 16);
-                                    const unsigned char* line = v + (c / 64) * (M::tile / C) + k * 128;
+                                    const unsigned char* line = v + (c / 64) * (M::part / C) + k * 128;
 #pragma unroll
                                     for (int e = 0; e < 4; ++e) {
                                         const uint4 x = *reinterpret_cast<const uint4*>(line + (((c % 64) / 8 + e) ^ (k & 7)) * 16);
@@ -444,10 +442,7 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_tc_kernel(const __grid_c
                 tc_wait_st();
                 tc_before();
                 __syncwarp();
-                if (lane == 0) {
-                    if (masked) tc_bar_arrive(p_half + 8 * i);
-                    tc_bar_arrive(p_full + 8 * i);
-                }
+                if (lane == 0) tc_bar_arrive(p_full + 16 * i + 8 * (j & 1));
             }
             const int live = what[5 + i];
             if (ok && live > 0) {
@@ -458,7 +453,7 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_tc_kernel(const __grid_c
                 uint4* to = reinterpret_cast<uint4*>(reinterpret_cast<__nv_bfloat16*>(P.out) +
                                                      ((size_t)(what[0] + what[4] + i * per + (out ? position : 0)) * P.q_heads + what[3] * P.share + (out ? row % P.share : 0)) * HD);
                 if (steps) {
-                    ok = wait(o_full + 8 * i, items++ & 1);
+                    ok = wait(o_full + 8 * i, (done - 1) & 1);
                     tc_after();
                 }
                 for (int c = 0; c < HD && ok; c += 32) {

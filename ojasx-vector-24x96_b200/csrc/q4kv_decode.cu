@@ -3,9 +3,12 @@
 // With the codes c, scales s and minima m of a token's groups of 32 dimensions, a score is sum_g (s_g (q_g . c_g) + m_g sum(q_g)) and
 // the result sum_t p_t (s_tg c_t + m_tg) per dimension of group g: both products take the codes as they are on mma.sync m16n8k16, and
 // the scales join in fp32 (those of the values before their product, as p * s).  A nibble in the lowest bits of an fp16 number is the
-// subnormal c * 2^-24, in the next ones 16 times that, exact in the tensor cores: a word of eight codes becomes operands with five
-// integer instructions, and the powers of two are taken out of the queries and the results (12 for bf16 numbers, which need an
-// exponent and its subtraction: 295 against XXX us at 16 sequences of 32768 tokens, 8 KV heads of 4 query heads of 128).
+// subnormal c * 2^-24, in the next ones 16 times that: a word of eight codes becomes operands with five integer instructions, and the
+// powers of two are taken out of the queries and the results (12 instructions for bf16 numbers, which need an exponent and its
+// subtraction: 295 against 211 us at 16 sequences of 32768 tokens, 8 KV heads of 4 query heads of 128).  The tensor cores line up what
+// they add by exponents that a subnormal does not have: sums of them keep 16 bits, enough for bf16 activations.  For fp32 ones the
+// codes are made whole numbers around zero, 1024 + c less 1032, and the minima m + 8 s: the two parts of a result are then of its own
+// size and do not cancel (2e-5 off 64 bits with subnormals, 8e-7 with c itself, 2e-7 so).
 // A warp takes tiles of 16 tokens:
 //   S[token][head]  = codes of K (16 x 16 a step) x q (16 x 8)           a group's steps have sums of their own
 //   O[dim][head]   += codes of V, transposed (16 x 16) x p * s_g (16 x 8)    p * s_g turned by movmatrix
@@ -33,7 +36,6 @@ constexpr int kQdUnit = kQdWarps * kQdPair * kQ4Tile;   // tokens
 constexpr float kQdLowest = -3.0e38f;         // finite: scores of -inf weigh nothing, a NaN makes its head's result one
 constexpr float kQdSlack = 8.0f;              // sums are relative to a reference, until a score is 2^8 above it ...
 constexpr float kQdRoom = 5.0f;               // ... and the largest p * s is 2^5 then: 2^14 at most
-constexpr float kQdCode = 16777216.0f;        // 2^24: a code is a subnormal of fp16
 
 static __device__ int g_q4_error;   // raised when a bounded wait inside a kernel ran out
 
@@ -63,13 +65,22 @@ __device__ __forceinline__ unsigned q4_turn(unsigned v) {   // an 8 x 8 matrix o
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
     return r;
 }
-// Nibbles i and i + 4 of a word as fp16 numbers, c * 2^-24 for even i and 16 c * 2^-24 for odd i.
+// Nibbles i and i + 4 of a word as fp16 numbers, 16 times as large for odd i: c * 2^-24 (kSub) or c - 8.
+template <bool kSub>
 __device__ __forceinline__ void q4_codes(unsigned w, unsigned (&c)[4]) {
-    const unsigned v = w >> 8;
-    c[0] = w & 0x000f000fu;
-    c[1] = w & 0x00f000f0u;
-    c[2] = v & 0x000f000fu;
-    c[3] = v & 0x00f000f0u;
+    const unsigned v = w >> 8, one = kSub ? 0u : 0x64006400u;   // 1024
+    c[0] = (w & 0x000f000fu) | one;
+    c[1] = (w & 0x00f000f0u) | one;
+    c[2] = (v & 0x000f000fu) | one;
+    c[3] = (v & 0x00f000f0u) | one;
+    if (!kSub) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float zero = i & 1 ? 1024.0f + 16 * 8.0f : 1024.0f + 8.0f;
+            const __half2 h = __hsub2(*reinterpret_cast<const __half2*>(&c[i]), __floats2half2_rn(zero, zero));
+            c[i] = *reinterpret_cast<const unsigned*>(&h);
+        }
+    }
 }
 __device__ __forceinline__ float q4_exp2(float x) {
     asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(x));
@@ -133,6 +144,7 @@ constexpr int kQdCtas(bool) { return 3; }   // per SM
 template <int HD, bool kBf16>
 __global__ void __launch_bounds__(kQdThreads, kQdCtas(kBf16)) q4_decode_kernel(const __grid_constant__ Q4DecodeProblem P) {
     constexpr int G = HD / 32, NP = kBf16 ? 1 : 2;
+    constexpr float kCode = kBf16 ? 16777216.0f : 1.0f;   // what the operands are less than their codes
     using T = Q4Layout<HD>;
     using M = QdSmem<HD>;
     using Words = typename Q4Words<G>::type;
@@ -274,7 +286,8 @@ __global__ void __launch_bounds__(kQdThreads, kQdCtas(kBf16)) q4_decode_kernel(c
         const bool begins = at.u == 0;
         // the queries as the second operand: lane (head gq, t) has the dimensions 32 g + 8 t + 0..7, pairs i and i + 4
         unsigned qf[NP][G][4];
-        unsigned qs[2];       // sums over the groups in three bf16 parts, as an operand: k = 4 part + group
+        unsigned qs[2];       // bf16: sums over the groups in three bf16 parts, as an operand: k = 4 part + group
+        float qsum[G][2];     // fp32: sums for the heads 2 t and 2 t + 1
         float unscale[2];
         {
             float x[G][8];
@@ -303,8 +316,8 @@ __global__ void __launch_bounds__(kQdThreads, kQdCtas(kBf16)) q4_decode_kernel(c
             most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
             float up, down;
             gm_scale(most, up, down);
-            // a score comes out of the products with 2^24 too little and this factor too much
-            const float back = fminf(down * (P.scale * kQdCode), 3.0e38f);
+            // what a score comes out of the products with
+            const float back = fminf(down * (P.scale * kCode), 3.0e38f);
             unscale[0] = __shfl_sync(0xffffffffu, back, 8 * t);        // heads 2 t and 2 t + 1
             unscale[1] = __shfl_sync(0xffffffffu, back, 8 * t + 4);
             float total[4] = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -315,8 +328,12 @@ __global__ void __launch_bounds__(kQdThreads, kQdCtas(kBf16)) q4_decode_kernel(c
                 float sum = ((x[g][0] + x[g][1]) + (x[g][2] + x[g][3])) + ((x[g][4] + x[g][5]) + (x[g][6] + x[g][7]));
                 sum += __shfl_xor_sync(0xffffffffu, sum, 1);
                 sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-                sum *= 1.0f / kQdCode;
+                sum *= 1.0f / kCode;
                 total[g] = sum;
+                if (!kBf16) {
+                    qsum[g][0] = __shfl_sync(0xffffffffu, sum, 8 * t);
+                    qsum[g][1] = __shfl_sync(0xffffffffu, sum, 8 * t + 4);
+                }
 #pragma unroll
                 for (int i = 1; i < 8; i += 2) x[g][i] *= 0.0625f;     // (the codes of odd nibbles are 16 times as large)
 #pragma unroll
@@ -368,16 +385,22 @@ __global__ void __launch_bounds__(kQdThreads, kQdCtas(kBf16)) q4_decode_kernel(c
                 const unsigned *ca = reinterpret_cast<const unsigned*>(&ma), *cb = reinterpret_cast<const unsigned*>(&mb);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) x[i][e] = 0.0f;
-                {   // sum_g m_g sum(q_g): the minima, bf16 as they are, times the sums in three parts
+                if (kBf16) {   // sum_g m_g sum(q_g): the minima, bf16 as they are, times the sums in three parts
                     const int pair = G == 4 ? (t & 1) * 2 : 0;
                     const unsigned a = *reinterpret_cast<const unsigned*>(tile + T::key_mins + T::meta_at(gq, pair)), b = *reinterpret_cast<const unsigned*>(tile + T::key_mins + T::meta_at(gq + 8, pair));
                     q4_mma(x[i], a, b, a, b, qs[0], qs[1]);
                 }
+                Metas la{}, lb{};
+                if (!kBf16) {
+                    la = *reinterpret_cast<const Metas*>(tile + T::key_mins + T::meta_at(gq, 0));
+                    lb = *reinterpret_cast<const Metas*>(tile + T::key_mins + T::meta_at(gq + 8, 0));
+                }
+                const unsigned *oa = reinterpret_cast<const unsigned*>(&la), *ob = reinterpret_cast<const unsigned*>(&lb);
 #pragma unroll
                 for (int g = 0; g < G; ++g) {
                     unsigned a[4], b[4];
-                    q4_codes(wa[g], a);
-                    q4_codes(wb[g], b);
+                    q4_codes<kBf16>(wa[g], a);
+                    q4_codes<kBf16>(wb[g], b);
                     float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                     for (int p = NP - 1; p >= 0; --p) {
@@ -385,6 +408,13 @@ __global__ void __launch_bounds__(kQdThreads, kQdCtas(kBf16)) q4_decode_kernel(c
                         gm_mma(c, {a[2], b[2], a[3], b[3]}, qf[p][g][2], qf[p][g][3]);
                     }
                     const float low = g & 1 ? q4_high(ca[g / 2]) : q4_low(ca[g / 2]), high = g & 1 ? q4_high(cb[g / 2]) : q4_low(cb[g / 2]);
+                    if (!kBf16) {
+                        const float za = fmaf(8.0f, low, g & 1 ? q4_high(oa[g / 2]) : q4_low(oa[g / 2])), zb = fmaf(8.0f, high, g & 1 ? q4_high(ob[g / 2]) : q4_low(ob[g / 2]));
+                        x[i][0] = fmaf(za, qsum[g][0], x[i][0]);
+                        x[i][1] = fmaf(za, qsum[g][1], x[i][1]);
+                        x[i][2] = fmaf(zb, qsum[g][0], x[i][2]);
+                        x[i][3] = fmaf(zb, qsum[g][1], x[i][3]);
+                    }
                     x[i][0] = fmaf(low, c[0], x[i][0]);
                     x[i][1] = fmaf(low, c[1], x[i][1]);
                     x[i][2] = fmaf(high, c[2], x[i][2]);
@@ -444,16 +474,20 @@ __global__ void __launch_bounds__(kQdThreads, kQdCtas(kBf16)) q4_decode_kernel(c
                 l[1] += x[i][1] + x[i][3];
 #pragma unroll
                 for (int g = 0; g < G; ++g) {
-                    const float low = g & 1 ? q4_high(oa[g / 2]) : q4_low(oa[g / 2]), high = g & 1 ? q4_high(ob[g / 2]) : q4_low(ob[g / 2]);
+                    float low = g & 1 ? q4_high(oa[g / 2]) : q4_low(oa[g / 2]), high = g & 1 ? q4_high(ob[g / 2]) : q4_low(ob[g / 2]);
                     const float sa = g & 1 ? q4_high(na[g / 2]) : q4_low(na[g / 2]), sb = g & 1 ? q4_high(nb[g / 2]) : q4_low(nb[g / 2]);
+                    if (!kBf16) {
+                        low = fmaf(8.0f, sa, low);
+                        high = fmaf(8.0f, sb, high);
+                    }
                     mins[g][0] = fmaf(x[i][0], low, fmaf(x[i][2], high, mins[g][0]));
                     mins[g][1] = fmaf(x[i][1], low, fmaf(x[i][3], high, mins[g][1]));
                     float y[4] = {x[i][0] * sa, x[i][1] * sa, x[i][2] * sb, x[i][3] * sb};
                     unsigned b0[NP], b1[NP], a[4], b[4];
 #pragma unroll
                     for (int p = 0; p < NP; ++p) { b0[p] = q4_turn(q4_part(y[0], y[1])); b1[p] = q4_turn(q4_part(y[2], y[3])); }
-                    q4_codes(wa[g], a);
-                    q4_codes(wb[g], b);
+                    q4_codes<kBf16>(wa[g], a);
+                    q4_codes<kBf16>(wb[g], b);
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
                         if (NP == 1) {
@@ -492,7 +526,7 @@ __global__ void __launch_bounds__(kQdThreads, kQdCtas(kBf16)) q4_decode_kernel(c
             for (int h = 0; h < 2; ++h) {
                 if (2 * t + h >= sum_heads) continue;
                 float* to = sums + (warp * sum_heads + 2 * t + h) * M::row + 32 * (m >> 1) + 4 * gq + 2 * (m & 1);
-                *reinterpret_cast<float2*>(to) = make_float2(fmaf(o[m][h], kQdCode, mins[m >> 1][h]), fmaf(o[m][h + 2], kQdCode / 16.0f, mins[m >> 1][h]));
+                *reinterpret_cast<float2*>(to) = make_float2(fmaf(o[m][h], kCode, mins[m >> 1][h]), fmaf(o[m][h + 2], kCode / 16.0f, mins[m >> 1][h]));
             }
         __syncthreads();
         unit += u1 - u0;

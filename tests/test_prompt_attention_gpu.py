@@ -82,6 +82,25 @@ def test_prompts_against_64_bits(cuda, dtype, hd, heads, share, lengths):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("hd,lengths,spread", [(128, [2000], 0), (64, [700, 300], 0), (128, [600], 12)])
+def test_fp32_keeps_fp32_accuracy(cuda, hd, lengths, spread):
+    """Over all results, errors add up as independent ones do: operands of 22 bits and fp32 sums leave less than 2^-21 of a result (as in
+    the test of the decode); twice that is allowed.  `spread`: rows of keys and values that differ by powers of two, up to 2^12."""
+    g, n = _gen(30 + hd), sum(lengths)
+    q, k, v = _randn(g, n, 4, hd), _randn(g, n, 2, hd), _randn(g, n, 2, hd)
+    if spread:
+        k = k * torch.exp2(-torch.randint(0, spread, (n, 2, 1), generator=g, device="cuda").float())
+        v = v * torch.exp2(-torch.randint(0, spread, (n, 2, 1), generator=g, device="cuda").float())
+    got, at, off, size = ops.prompt_attention(q, k, v, _ends(lengths)), 0, 0.0, 0.0
+    for m in lengths:
+        want = attend(q[at:at + m], k[at:at + m], v[at:at + m], 0)[0]
+        off += float((got[at:at + m].double() - want).square().sum())
+        size += float(want.square().sum())
+        at += m
+    assert (off / size) ** 0.5 <= 2.0 ** -20, (off / size) ** 0.5
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("hd,heads,share,lengths,key_lengths", [
     (128, 2, 4, [64], [1000]), (64, 1, 3, [1, 5, 0, 200, 17], [129, 5, 40, 333, 128]), (128, 1, 2, [300, 70, 4], [100, 0, 3]), (64, 2, 1, [1] * 5, [1, 127, 128, 129, 0])])

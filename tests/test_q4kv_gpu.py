@@ -317,6 +317,26 @@ def test_decode_against_64_bits(cuda, dtype, hd, heads, share, page, lengths):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("hd,heads,share,page,lengths", [(128, 8, 4, 64, [1000]), (64, 4, 7, 16, [5000, 333, 12000]), (128, 2, 16, 32, [2000] * 4)])
+def test_fp32_decode_keeps_fp32_accuracy(cuda, hd, heads, share, page, lengths):
+    """Over all results, errors add up as independent ones do.  Per score: operands of 22 bits (2^-23 each, two of them) and fp32 sums
+    of hd products, 2^-24 sqrt(hd) of a product's size at random, which is 2^-24 sqrt(2) of the score's spread of about 1; weights
+    of 22 bits and sums over tokens likewise.  Together below 2^-21 of a result; twice that is allowed."""
+    g = _gen(20)
+    c = ops.Q4PagedKVCache(sum(-(-n // page) for n in lengths), page, heads, heads * share, hd)
+    pool = random_pool(c, g)
+    table = random_table(c, lengths, g)
+    q = _randn(g, len(lengths), heads * share, hd)
+    got, off, size = c.decode(q, table, _ints(lengths)), 0.0, 0.0
+    for b, n in enumerate(lengths):
+        at = torch.arange(n, device="cuda")
+        want = attend(q[b:b + 1], *(gather(pool, x, table, b, at, page) for x in ("k", "v")), n - 1)[0]
+        off += float((got[b:b + 1].double() - want).square().sum())
+        size += float(want.square().sum())
+    assert (off / size) ** 0.5 <= 2.0 ** -20, (off / size) ** 0.5
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_decode_sees_nothing_behind_the_lengths(cuda, dtype):
     """Pages end inside a tile, and what is behind the last token is NaN."""

@@ -401,7 +401,8 @@ OJASX_API int ojasx_b200_paged_kv_decode(const void* d_q, void* d_out, const int
  * scale (the smallest not below (max - minimum) / 15); a value is a code 0..15 and reads as code * scale + minimum, within half a
  * scale of what it was.  A group that holds an infinity or a NaN reads as NaN.
  * d_block_table [batch, max_pages] int32 names the pages of every sequence.  Entries outside [0, num_pages) are no page: tokens
- * there are dropped by an append, read as zeros and weigh nothing in a decode, and *status becomes 1.
+ * there are dropped by an append, read as zeros and weigh nothing in a decode, and *status becomes 1; so it is with tokens beyond
+ * max_pages, and a sequence with a negative position is left out as a whole.
  *
  * append: token i of d_k, d_v [n_tokens, kv_heads, head_dim] goes to its place behind the d_positions[b] tokens of its sequence.
  * d_ends [batch + 1]: the tokens of sequence b are d_ends[b] .. d_ends[b + 1] - 1 (tokens behind the last one are left alone); NULL:
@@ -431,7 +432,7 @@ OJASX_API int ojasx_b200_q4kv_decode(const OjasxQ4Cache* cache, const void* d_q,
  * of a head in elements, the dimensions of a head together) into d_out [n_rows, q_heads, head_dim].  Rows d_ends[b] .. and keys
  * d_key_ends[b] .. belong to sequence b, whose last query sees its last key, the one before it the keys up to the one before, and so
  * on; a query that sees nothing gives zeros; rows behind the last sequence are left as they were.  Keys that a query does not see
- * have no part in its result, whatever they hold.  workspace: ojasx_b200_prompt_workspace bytes (0 for bf16) for this call alone,
+ * have no part in its result, whatever they hold.  fp32 values up to 2^100.  workspace: ojasx_b200_prompt_workspace bytes (0 for bf16) for this call alone,
  * 256-byte aligned; the others 16-byte aligned, strides whole multiples of 16 bytes. */
 OJASX_API size_t ojasx_b200_prompt_workspace(int n_keys, int kv_heads, int head_dim, int io_dtype);
 OJASX_API int ojasx_b200_prompt_attention(const void* d_q, long long q_row, long long q_head, const void* d_k, long long k_row,

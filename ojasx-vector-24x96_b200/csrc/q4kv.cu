@@ -168,7 +168,7 @@ __global__ void __launch_bounds__(128) q4_append_kernel(const __grid_constant__ 
     if (P.ends) {
         b = packed_owner(P.ends, P.batch, token);
         if (b < 0) return;   // (of the whole CTA)
-        pos = P.positions[b] + token - P.ends[b];
+        pos = P.positions[b] < 0 ? -1 : P.positions[b] + token - P.ends[b];   // (a sequence that begins nowhere has no place at all)
     } else {
         pos = P.positions[b];
     }
@@ -197,12 +197,17 @@ __global__ void __launch_bounds__(128) q4_append_kernel(const __grid_constant__ 
 // A tile of the cache that tokens `from` to `to` (in it) of a CTA's rows lie in: its sequence, the first one's row and position.
 struct Q4Span { int b, row, pos, from, to; };
 
-// Span `index` of the tiles that the packed tokens of all sequences touch; all lanes of a warp call it together.
-__device__ __forceinline__ bool q4_span(const int* ends, const int* positions, int batch, int rows, int index, Q4Span& S) {
+// Span `index` of the tiles that the packed tokens of all sequences touch; all lanes of a warp call it together.  A sequence that begins
+// at a negative position has none, which `status` tells.
+__device__ __forceinline__ bool q4_span(const int* ends, const int* positions, int batch, int rows, int index, int* status, Q4Span& S) {
     int part = 0;
     auto tiles = [&](int b) {
         const PackedRange r = packed_range(ends, b, rows);
-        if (r.count == 0 || (positions && positions[b] < 0)) return 0;
+        if (r.count == 0) return 0;
+        if (positions && positions[b] < 0) {
+            atomicExch(status, 1);
+            return 0;
+        }
         const int in = (positions ? positions[b] : 0) % kQ4Tile;
         return (in + r.count + kQ4Tile - 1) / kQ4Tile;
     };
@@ -229,7 +234,7 @@ __global__ void __launch_bounds__(256, 4) q4_append_tile_kernel(const __grid_con
     chain_begin();
     if (threadIdx.x < 32) {
         Q4Span S{-1, 0, 0, 0, 0};
-        if (!q4_span(P.ends, P.positions, P.batch, P.n_tokens, blockIdx.x / slices, S)) S.b = -1;
+        if (!q4_span(P.ends, P.positions, P.batch, P.n_tokens, blockIdx.x / slices, P.cache.status, S)) S.b = -1;
         if (threadIdx.x == 0) s_span = S;
     }
     __syncthreads();
@@ -329,7 +334,7 @@ __global__ void __launch_bounds__(256) q4_read_kernel(const __grid_constant__ Q4
     chain_begin();
     if (threadIdx.x < 32) {
         Q4Span S{-1, 0, 0, 0, 0};
-        if (!q4_span(P.ends, P.positions, P.batch, P.n_tokens, blockIdx.x, S)) S.b = -1;
+        if (!q4_span(P.ends, P.positions, P.batch, P.n_tokens, blockIdx.x, P.cache.status, S)) S.b = -1;
         if (threadIdx.x == 0) s_span = S;
     }
     __syncthreads();

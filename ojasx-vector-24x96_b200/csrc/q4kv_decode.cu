@@ -177,7 +177,9 @@ __global__ void __launch_bounds__(kQdThreads, kQdCtas(kBf16)) q4_decode_kernel(c
     }
     // an empty sequence has no units: its zeros come from here
     for (int b = blockIdx.x; b < P.batch; b += gridDim.x) {
-        if (Q4Place::length(P, b) > 0) continue;
+        const int length = Q4Place::length(P, b);
+        if (tid == 0 && P.lengths[b] > length) atomicExch(P.cache.status, 1);   // more tokens than the table has room for
+        if (length > 0) continue;
         for (int i = tid; i < P.q_heads * HD; i += kQdThreads) {
             if (kBf16) reinterpret_cast<__nv_bfloat16*>(P.out)[(size_t)b * P.q_heads * HD + i] = __float2bfloat16_rn(0.0f);
             else reinterpret_cast<float*>(P.out)[(size_t)b * P.q_heads * HD + i] = 0.0f;

@@ -577,7 +577,7 @@ class Q4PagedKVCache:
                q: Optional[torch.Tensor] = None, cu_seqlens: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
         """``k``, ``v`` [tokens, kv_heads, head_dim] behind the ``positions[b]`` tokens that sequence b has: one token per sequence, or
         with ``cu_seqlens`` int32 [batch + 1] the packed tokens ``cu_seqlens[b] .. cu_seqlens[b + 1]``.  ``q``
-        [tokens, q_heads, head_dim] is turned as the keys are and returned (its rows behind the last sequence are not written)."""
+        [tokens, q_heads, head_dim] is turned as the keys are and returned (its rows behind the last sequence, and those of a sequence whose position is negative, hold nothing)."""
         table, dtype, dev = self._table(block_table), k.dtype, self.device
         B, n = block_table.shape[0], k.shape[0]
         if dtype not in _DTYPE_CODES:
@@ -610,7 +610,7 @@ class Q4PagedKVCache:
         at = None if positions is None else _index32(positions, "positions", (B,), dev)
         if dtype not in _DTYPE_CODES:
             raise TypeError(f"values are read as float32 or bfloat16, not {dtype}")
-        k = torch.empty((int(tokens), self.kv_heads, self.head_dim), device=dev, dtype=dtype)
+        k = self.pool.new_empty((int(tokens), self.kv_heads, self.head_dim), dtype=dtype)
         v = torch.empty_like(k)
         if tokens and B:
             with _on_device(dev):
@@ -638,7 +638,7 @@ class Q4PagedKVCache:
             size = self._sizes.get(key)
             if size is None:
                 size = self._sizes[key] = lib().ojasx_b200_q4kv_decode_workspace(self._cache, B, pages, _DTYPE_CODES[dtype])
-            ws = torch.empty(size, device=dev, dtype=torch.uint8)     # of this call, so that calls on several streams do not share it
+            ws = self.pool.new_empty(size)     # of this call, so that calls on several streams do not share it
             with _on_device(dev):
                 rc = lib().ojasx_b200_q4kv_decode(self._cache, q.data_ptr(), o.data_ptr(), table, pages, n, B, scale, _DTYPE_CODES[dtype],
                                                   ws.data_ptr(), size, _stream_ptr(dev))

@@ -270,6 +270,41 @@ def test_tokens_without_a_page_are_dropped_and_reported(cuda, packed):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("tokens", [1, 3, 40])   # of a sequence: either kernel
+def test_a_negative_position_is_no_place(cuda, tokens):
+    g = _gen(11)
+    c = ops.Q4PagedKVCache(6, 32, 2, 4, 64, rope_theta=THETA)
+    table, ends = _ints([[0, 1], [2, 3]]), _ends([tokens, tokens])
+    k, v, q = _randn(g, 2 * tokens, 2, 64), _randn(g, 2 * tokens, 2, 64), _randn(g, 2 * tokens, 4, 64)
+    whole, before = c.append(k, v, table, _ints([0, 5]), q=q, cu_seqlens=ends), c.pool.clone()
+    c.check()
+    c.pool.zero_()
+    turned = c.append(k, v, table, _ints([-1, 5]), q=q, cu_seqlens=ends)
+    with pytest.raises(OjasxB200Error):
+        c.check()
+    assert not c.pool[:2].any() and torch.equal(c.pool[2:], before[2:]) and torch.equal(turned[tokens:], whole[tokens:])
+    c.read(table, ends, 2 * tokens, positions=_ints([0, -4]))
+    with pytest.raises(OjasxB200Error):
+        c.check()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_a_length_beyond_the_table_is_reported(cuda, dtype):
+    g = _gen(12)
+    c = ops.Q4PagedKVCache(6, 32, 2, 4, 64)
+    pool = random_pool(c, g)
+    table, q = random_table(c, [64, 50], g), _randn(g, 2, 4, 64, dtype=dtype)
+    _check_decode(c, pool, table, [64, 50], q, c.decode(q, table, _ints([64, 50])))
+    c.check()
+    got = c.decode(q, table, _ints([65, 50]))
+    with pytest.raises(OjasxB200Error):
+        c.check()
+    _check_decode(c, pool, table, [64, 50], q, got)   # the tokens that there is room for
+    c.check()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("hd,heads,page,starts,lengths", [(128, 2, 64, [0], [130]), (64, 3, 16, [3, 0, 16, 40], [5, 0, 33, 1])])
 def test_read_gives_the_values(cuda, dtype, hd, heads, page, starts, lengths):

@@ -152,7 +152,8 @@ __device__ __forceinline__ void q4_rotate(float4& a, float4& d, const float (&c)
 
 // Few tokens: 1024 / HD vectors (keys, values and queries of one token) per CTA, HD / 8 lanes to a vector, each with four dimensions of
 // either half (a rotated pair is in one lane, a group is eight lanes).  Bound by latency: everything that does not wait for the
-// position is asked for before it, the page while the angles are made.
+// position is asked for before it, the page while the angles are made.  One token of 8 KV heads and 32 query heads of 128: 2.3 us; with a
+// CTA per token, which takes its vectors in turn, 8.8.
 template <int HD, bool kBf16>
 __global__ void __launch_bounds__(128) q4_append_kernel(const __grid_constant__ Q4AppendProblem P) {
     constexpr int L = HD / 8, V = 128 / L;
@@ -224,7 +225,9 @@ __device__ __forceinline__ bool q4_span(const int* ends, const int* positions, i
 static long long q4_spans(int rows, int batch) { return rows / kQ4Tile + 2LL * std::min(rows, batch); }
 
 // Prompts: a tile of 16 tokens per CTA and some of the heads, a token to HD / 8 lanes (or two of them at head_dim 64), which make its
-// angles once.  A head's tile is put together in shared memory and written in 16-byte pieces: its words hold two tokens each.
+// angles once.  A head's tile is put together in shared memory and written in 16-byte pieces: its words hold two tokens each.  Bound by the
+// integer pipe (43 % busy) and by barriers between the heads' tiles: 16384 tokens of 8 KV heads of 128 in bf16 36.9 us, with 32 query
+// heads 78 (their 445 MB with the way back take 68), against 190 for a vector per eight lanes, which makes every angle 40 times.
 template <int HD, bool kBf16>
 __global__ void __launch_bounds__(256, 4) q4_append_tile_kernel(const __grid_constant__ Q4AppendProblem P, int slices) {
     constexpr int L = HD / 8, G = HD / 32, W = 256 / (kQ4Tile * L);   // W: vectors of a token at a time
@@ -323,7 +326,7 @@ struct Q4ReadProblem {
 };
 
 // A tile of 16 tokens and up to eight KV heads per CTA: the tiles of the heads come in 16-byte pieces, eight values of a token go out in
-// one or two.  Tokens without a page are read as zeros.
+// one or two.  Tokens without a page are read as zeros.  Bound by what it writes: 16384 tokens of 8 heads of 128 as bf16 in 19 us, 88 MB.
 constexpr int kQ4ReadHeads = 8;
 
 template <int HD, bool kBf16>
@@ -414,15 +417,21 @@ int ojasx_b200_q4kv_append(const OjasxQ4Cache* cache, const void* d_k, long long
     P.positions = d_positions; P.ends = d_ends; P.turns = cache->turns; P.n_tokens = n_tokens; P.batch = batch; P.q_heads = q_heads;
     const bool bf = io_dtype == OJX_BF16;
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (d_ends && n_tokens >= 4LL * batch) {
+    const int vectors = 1024 / head_dim, parts = (2 * kv_heads + (d_q ? q_heads : 0) + vectors - 1) / vectors;
+    // Few tokens by vectors, many by tiles, each sequence of which begins and ends with a part of one.  us of the two at 8 KV heads and 32
+    // query heads of 128 in bf16: one sequence of 64 tokens 2.9 and 4.7, 256 5.6 and 4.9, 1024 13.2 and 7.9; 16 sequences of 16 6.4 and 8.1,
+    // of 32 8.9 and 8.9, of 64 15.0 and 10.9; 64 of 4 7.1 and 8.9, of 16 15.9 and 14.5, of 64 55.7 and 28.4.
+    if (d_ends && (long long)n_tokens * parts > 12LL * num_sms() + 48LL * batch) {
         const long long tiles = q4_spans(n_tokens, batch);
-        const int slices = (int)std::min<long long>(kv_heads, std::max<long long>(1, (8LL * num_sms() + tiles - 1) / tiles));   // twice what the GPU holds
+        // equal slices of the heads while the CTAs are at most three times what the GPU holds (us with 8 heads in 1 and 5 slices for one
+        // sequence of 16384 tokens without queries: 36.2 and 43.9; in 4 and 7 for 64 of 16: 14.0 and 16.6; in 2 and 4 for 64 of 64: 30.0 and 28.1)
+        int slices = kv_heads;
+        while (slices > 1 && (kv_heads % slices || tiles * slices > 12LL * num_sms())) --slices;
         if (tiles * slices > 0x7fffffffLL) return OJX_ERR_TOO_LARGE;
         auto kernel = head_dim == 64 ? (bf ? q4_append_tile_kernel<64, true> : q4_append_tile_kernel<64, false>)
                                      : (bf ? q4_append_tile_kernel<128, true> : q4_append_tile_kernel<128, false>);
         OJX_CUDA_TRY(launch_chained(kernel, dim3((unsigned)(tiles * slices)), 256, 0, s, P, slices));
     } else {
-        const int vectors = 1024 / head_dim, parts = (2 * kv_heads + (d_q ? q_heads : 0) + vectors - 1) / vectors;
         if ((long long)n_tokens * parts > 0x7fffffffLL) return OJX_ERR_TOO_LARGE;
         auto kernel = head_dim == 64 ? (bf ? q4_append_kernel<64, true> : q4_append_kernel<64, false>)
                                      : (bf ? q4_append_kernel<128, true> : q4_append_kernel<128, false>);

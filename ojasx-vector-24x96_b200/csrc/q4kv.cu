@@ -152,8 +152,7 @@ __device__ __forceinline__ void q4_rotate(float4& a, float4& d, const float (&c)
 
 // Few tokens: 1024 / HD vectors (keys, values and queries of one token) per CTA, HD / 8 lanes to a vector, each with four dimensions of
 // either half (a rotated pair is in one lane, a group is eight lanes).  Bound by latency: everything that does not wait for the
-// position is asked for before it, the page while the angles are made.  One token of 8 KV heads and 32 query heads of 128: 2.3 us; with a
-// CTA per token, which takes its vectors in turn, 8.8.
+// position is asked for before it, the page while the angles are made.  One token of 8 KV heads and 32 query heads of 128: 2.3 us.
 template <int HD, bool kBf16>
 __global__ void __launch_bounds__(128) q4_append_kernel(const __grid_constant__ Q4AppendProblem P) {
     constexpr int L = HD / 8, V = 128 / L;
@@ -227,7 +226,8 @@ static long long q4_spans(int rows, int batch) { return rows / kQ4Tile + 2LL * s
 // Prompts: a tile of 16 tokens per CTA and some of the heads, a token to HD / 8 lanes (or two of them at head_dim 64), which make its
 // angles once.  A head's tile is put together in shared memory and written in 16-byte pieces: its words hold two tokens each.  Bound by the
 // integer pipe (43 % busy) and by barriers between the heads' tiles: 16384 tokens of 8 KV heads of 128 in bf16 36.9 us, with 32 query
-// heads 78 (their 445 MB with the way back take 68), against 190 for a vector per eight lanes, which makes every angle 40 times.
+// heads 78 (their 445 MB with the way back take 68), against 190 by single vectors, each of which
+// makes its angles anew.
 template <int HD, bool kBf16>
 __global__ void __launch_bounds__(256, 4) q4_append_tile_kernel(const __grid_constant__ Q4AppendProblem P, int slices) {
     constexpr int L = HD / 8, G = HD / 32, W = 256 / (kQ4Tile * L);   // W: vectors of a token at a time
@@ -423,8 +423,8 @@ int ojasx_b200_q4kv_append(const OjasxQ4Cache* cache, const void* d_k, long long
     // of 32 8.9 and 8.9, of 64 15.0 and 10.9; 64 of 4 7.1 and 8.9, of 16 15.9 and 14.5, of 64 55.7 and 28.4.
     if (d_ends && (long long)n_tokens * parts > 12LL * num_sms() + 48LL * batch) {
         const long long tiles = q4_spans(n_tokens, batch);
-        // equal slices of the heads while the CTAs are at most three times what the GPU holds (us with 8 heads in 1 and 5 slices for one
-        // sequence of 16384 tokens without queries: 36.2 and 43.9; in 4 and 7 for 64 of 16: 14.0 and 16.6; in 2 and 4 for 64 of 64: 30.0 and 28.1)
+        // equal slices of the heads while the CTAs are at most three times what the GPU holds (us with 8 heads in 1, 2 and 3 slices for one
+        // sequence of 16384 tokens without queries: 36.2, 39.1 and 43.9; in 4 and 7 for 64 of 16: 14.0 and 16.6; in 2 and 4 for 64 of 64: 30.0 and 28.1)
         int slices = kv_heads;
         while (slices > 1 && (kv_heads % slices || tiles * slices > 12LL * num_sms())) --slices;
         if (tiles * slices > 0x7fffffffLL) return OJX_ERR_TOO_LARGE;

@@ -20,6 +20,10 @@
 // Work: units of 128 tokens of a (sequence, KV head, eight query heads), all of them in a row, in equal shares for the CTAs whatever the
 // lengths are; the four warps of a CTA take two tiles of a unit each, from rings of their own that bulk copies fill.  A share that begins
 // or ends inside a sequence leaves its sums to q4_combine_kernel.
+//
+// Bound by the integer pipe (half of its slots at 380 instructions a tile and warp) next to the copies, which alone take 111 to 130 us: 16
+// sequences of 32768 tokens, 671 MB, in 151 us (4.4 TB/s) with 8 KV heads of 4 query heads of 128 in bf16; 48 of up to 20011, 4 heads of 7
+// of 64 in fp32, 106 MB, in 64 us, where the second planes of queries and weights double the products.
 #include <algorithm>
 #include <cmath>
 
@@ -139,10 +143,10 @@ struct QdSmem {
     static constexpr int bytes(int heads) { return kQdWarps * (ring + heads * row * 4); }
 };
 
-constexpr int kQdCtas(bool) { return 3; }   // per SM
+constexpr int kQdCtas = 3;   // per SM (16 sequences of 32768 tokens: 151 us; 2: 154, 4: 159)
 
 template <int HD, bool kBf16>
-__global__ void __launch_bounds__(kQdThreads, kQdCtas(kBf16)) q4_decode_kernel(const __grid_constant__ Q4DecodeProblem P) {
+__global__ void __launch_bounds__(kQdThreads, kQdCtas) q4_decode_kernel(const __grid_constant__ Q4DecodeProblem P) {
     constexpr int G = HD / 32, NP = kBf16 ? 1 : 2;
     constexpr float kCode = kBf16 ? 16777216.0f : 1.0f;   // what the operands are less than their codes
     using T = Q4Layout<HD>;
@@ -614,9 +618,9 @@ __global__ void __launch_bounds__(kQcThreads) q4_combine_kernel(const __grid_con
 }
 
 // CTAs of a decode: what the GPU holds at a time, or a unit each where the tables have room for fewer.
-static int q4_decode_ctas(int batch, int max_pages, int page_size, int kv_heads, int share, int dtype) {
+static int q4_decode_ctas(int batch, int max_pages, int page_size, int kv_heads, int share) {
     const long long units = (long long)batch * kv_heads * ((share + kQdHeads - 1) / kQdHeads) * (((long long)max_pages * page_size + kQdUnit - 1) / kQdUnit);
-    const int most = num_sms() * kQdCtas(dtype == OJX_BF16);
+    const int most = num_sms() * kQdCtas;
     return units < most ? (int)units : most;
 }
 static size_t q4_decode_bytes(int ctas, int head_dim) {
@@ -649,7 +653,7 @@ extern "C" {
 
 size_t ojasx_b200_q4kv_decode_workspace(const OjasxQ4Cache* cache, int batch, int max_pages, int io_dtype) {
     if (!cache || batch <= 0 || max_pages <= 0 || cache->page_size <= 0 || cache->kv_heads <= 0 || cache->q_heads <= 0) return 0;
-    return q4_decode_bytes(q4_decode_ctas(batch, max_pages, cache->page_size, cache->kv_heads, cache->q_heads / cache->kv_heads, io_dtype), cache->head_dim);
+    return q4_decode_bytes(q4_decode_ctas(batch, max_pages, cache->page_size, cache->kv_heads, cache->q_heads / cache->kv_heads), cache->head_dim);
 }
 
 int ojasx_b200_q4kv_decode(const OjasxQ4Cache* cache, const void* d_q, void* d_out, const int* d_block_table, int max_pages, const int* d_lengths,
@@ -658,7 +662,7 @@ int ojasx_b200_q4kv_decode(const OjasxQ4Cache* cache, const void* d_q, void* d_o
     if (rc != OJX_OK) return rc;
     const int kv_heads = cache->kv_heads, q_heads = cache->q_heads, head_dim = cache->head_dim;
     if (!d_q || !d_out || !d_lengths || !q4_aligned(d_q) || !q4_aligned(d_out)) return OJX_ERR_ARG;
-    const int share = q_heads / kv_heads, ctas = q4_decode_ctas(batch, max_pages, cache->page_size, kv_heads, share, io_dtype);
+    const int share = q_heads / kv_heads, ctas = q4_decode_ctas(batch, max_pages, cache->page_size, kv_heads, share);
     if (!workspace || !q4_aligned(workspace) || workspace_bytes < q4_decode_bytes(ctas, head_dim)) return OJX_ERR_ARG;
     if ((long long)batch * q_heads > 0x7fffffffLL) return OJX_ERR_TOO_LARGE;
     Q4DecodeProblem P{};

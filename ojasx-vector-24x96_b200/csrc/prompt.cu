@@ -527,8 +527,8 @@ static int launch_prompt_tc(const PromptProblem& P, cudaStream_t s) {
 // The high parts of Q are in tensor memory, where products take them without the shared memory's bandwidth; the low ones, and K and V
 // in steps of 64 keys, are in shared memory.  The tensor cores cut what they add to a sum, so a step's products with V are summed on
 // their own and join the row's fp32 sums, which are in its thread's registers.  Bound by what a row's thread does for a step (the two parts
-// of 64 weights, O of the step before); the tensor pipe is 41 % busy.  Two prompts of 2048 with 32 query heads and 8 KV heads of 128: 285 us,
-// 241 TFLOP/s of the formula, 723 of fp16 products (4750 us with fp32 FMA, 364 with all of Q in shared memory).
+// of 64 weights, O of the step before); the tensor pipe is 41 % busy.  Two prompts of 2048 with 32 query heads and 8 KV heads of 128: 283 us,
+// 243 TFLOP/s of the formula, 728 of fp16 products (4750 us with fp32 FMA, 364 with all of Q in shared memory).
 constexpr int kPpKeys = 64;
 constexpr float kPpRoom = 5.0f;   // y is 2^5 at most when the reference is set, 2^13 later on
 
@@ -547,24 +547,26 @@ struct PromptSplit {
     float2* factors;        // [kv_heads][n_keys]: 1 / scale of the key's row of K, e of its row of V
 };
 
-// A row of K or V per HD / 4 lanes.
+// A row of K or V per HD / 8 lanes, 16 bytes in and out; bound by the instructions of the split.  The two kernels take 283.3 us for two
+// prompts of 2048 (285.4 with HD / 4 lanes to a row).
 template <int HD>
 __global__ void __launch_bounds__(256) prompt_split_kernel(const __grid_constant__ PromptProblem P, const __grid_constant__ PromptSplit S) {
-    constexpr int L = HD / 4;
+    constexpr int L = HD / 8;
     chain_begin();
     const long long row = ((long long)blockIdx.x * 256 + threadIdx.x) / L, rows = (long long)P.n_keys * P.kv_heads;
     const int l = threadIdx.x % L;
-    if (row >= 2 * rows) return;   // (a whole warp's rows or half of them: the shuffles stay within L lanes)
+    if (row >= 2 * rows) return;   // (all L lanes of a row, within which the shuffles stay)
     const bool values = row >= rows;
     const long long r = values ? row - rows : row;
     const long long key = r / P.kv_heads;
     const int head = (int)(r - key * P.kv_heads);
-    const float4 x = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(values ? P.v : P.k) + key * (values ? P.v_row : P.k_row) +
-                                                      head * (values ? P.v_head : P.k_head) + 4 * l);
-    const float xs[4] = {x.x, x.y, x.z, x.w};
+    const float4* from = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(values ? P.v : P.k) + key * (values ? P.v_row : P.k_row) +
+                                                         head * (values ? P.v_head : P.k_head) + 8 * l);
+    const float4 x = from[0], y = from[1];
+    const float xs[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
     unsigned most = 0;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
+    for (int e = 0; e < 8; ++e) {
         const unsigned b = __float_as_uint(xs[e]) & 0x7fffffffu;
         if (b < 0x7f800000u) most = max(most, b);
     }
@@ -579,17 +581,17 @@ __global__ void __launch_bounds__(256) prompt_split_kernel(const __grid_constant
     } else {
         gm_scale(most, up, down);
     }
-    unsigned hi[2], lo[2];
+    unsigned hi[4], lo[4];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < 4; ++i) {
         const float a = xs[2 * i] * up, b = xs[2 * i + 1] * up;
         const __half2 h = __floats2half2_rn(a, b);
         hi[i] = *reinterpret_cast<const unsigned*>(&h);
         lo[i] = gm_pack(a - __low2float(h), b - __high2float(h));
     }
-    const size_t to = (size_t)r * HD + 4 * l;
-    *reinterpret_cast<uint2*>(S.planes[values ? 2 : 0] + to) = make_uint2(hi[0], hi[1]);
-    *reinterpret_cast<uint2*>(S.planes[values ? 3 : 1] + to) = make_uint2(lo[0], lo[1]);
+    const size_t to = (size_t)r * HD + 8 * l;
+    *reinterpret_cast<uint4*>(S.planes[values ? 2 : 0] + to) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+    *reinterpret_cast<uint4*>(S.planes[values ? 3 : 1] + to) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
     // (a value is 2^(14 - e) times as large, its weight 2^e: 2^14 is left for the end)
     if (l == 0) {
         float* f = reinterpret_cast<float*>(S.factors + (size_t)head * P.n_keys + key);
@@ -985,7 +987,7 @@ static int launch_prompt_pair(const PromptProblem& P, void* workspace, cudaStrea
     OJX_CUDA_TRY(opt_in_smem(reinterpret_cast<const void*>(prompt_pair_kernel<HD>), smem, opted));
     const int per = kPaRows / P.share;
     const long long parts = P.n_rows / (2 * per) + std::min(P.batch, P.n_rows);
-    const long long split = ((long long)P.n_keys * P.kv_heads * 2 * (HD / 4) + 255) / 256;
+    const long long split = ((long long)P.n_keys * P.kv_heads * 2 * (HD / 8) + 255) / 256;
     if (parts * P.kv_heads > 0x7fffffffLL || split > 0x7fffffffLL) return OJX_ERR_TOO_LARGE;
     PromptSplit S{};
     const size_t plane = prompt_split_plane(P.n_keys, P.kv_heads, HD);

@@ -87,7 +87,7 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_tc_kernel(const __grid_c
     constexpr int NS = M::slots, C = HD / 64;
     extern __shared__ unsigned char pa_raw[];
     unsigned char* smem = pa_raw + ((1024u - (tc_smem(pa_raw) & 1023u)) & 1023u);
-    __shared__ int s_gone, s_odd[2];
+    __shared__ int s_gone, s_odd[2][2];   // s_odd: of either S of a tile, since its rows may be a step ahead of the products
     __shared__ unsigned s_tmem;
     __shared__ __align__(16) int s_item[2][8];
     __shared__ __align__(16) int s_stolen[4];
@@ -110,7 +110,7 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_tc_kernel(const __grid_c
             tc_bar_init(q_empty + 8 * i, 1);
             tc_bar_init(item_full + 8 * i, 1);
             tc_bar_init(item_empty + 8 * i, 10);
-            s_odd[i] = 0;
+            s_odd[i][0] = s_odd[i][1] = 0;
         }
         tc_bar_init(want, 1);
         tc_bar_init(steal, 1);
@@ -274,7 +274,7 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_tc_kernel(const __grid_c
                         halves[i] ^= 1u << (j & 1);
                         tc_after();
                         // (values that are not finite behind what is seen: the rows have added their products themselves)
-                        if (!((j + 1) * kPaKeys - 1 > item.pos[i] + item.ahead && *reinterpret_cast<volatile int*>(&s_odd[i]) == (int)step)) {
+                        if (!((j + 1) * kPaKeys - 1 > item.pos[i] + item.ahead && *reinterpret_cast<volatile int*>(&s_odd[i][j & 1]) == (int)step)) {
                             const unsigned long long b = tc_at(ring_v, vr.slot * M::part);
 #pragma unroll
                             for (int k = 0; k < kPaKeys / 16; ++k)
@@ -397,11 +397,11 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_tc_kernel(const __grid_c
                     }
                     odd = __reduce_or_sync(0xffffffffu, odd);
                     if (lane == 0) {
-                        if (odd) *reinterpret_cast<volatile int*>(&s_odd[i]) = (int)step;
+                        if (odd) *reinterpret_cast<volatile int*>(&s_odd[i][j & 1]) = (int)step;
                         tc_bar_arrive(checked + 8 * i);
                     }
                     if (!(ok = wait(checked + 8 * i, checks++ & 1))) break;
-                    if (*reinterpret_cast<volatile int*>(&s_odd[i]) == (int)step) {
+                    if (*reinterpret_cast<volatile int*>(&s_odd[i][j & 1]) == (int)step) {
                         if (j > 0 && !(ok = wait(o_full + 8 * i, (step - 2) & 1))) break;
                         tc_after();
                         tc_wait_st();

@@ -149,6 +149,26 @@ def test_what_is_not_seen_has_no_part(cuda, dtype, hd, bad):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("hd,share", [(64, 1), (128, 1), (128, 4)])
+def test_rows_in_front_of_values_that_are_not_finite(cuda, dtype, hd, share):
+    """From some token on, every 31st value of a sequence is NaN, in every step of keys that a tile's mask cuts: the rows before that
+    token are what they are without, and those from it on are NaN."""
+    g = _gen(31)
+    lengths = [256] * 24 + [200, 129, 90, 333]
+    first = [5 + 17 * b % 80 for b in range(len(lengths))]
+    rows = sum(lengths)
+    q, k, v = (_randn(g, rows, h, hd, dtype=dtype) for h in (4 * share, 4, 4))
+    clean, at = v.clone(), np.cumsum([0] + lengths)
+    for a, n, f in zip(at, lengths, first):
+        v[a + f:a + n:31] = math.nan
+    got = ops.prompt_attention(q, k, v, _ends(lengths))
+    for a, n, f in zip(at, lengths, first):
+        _check(q[a:a + f], k[a:a + f], clean[a:a + f], [f], [f], got[a:a + f])
+        assert torch.isnan(got[a + f:a + n]).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("hd", [64, 128])
 def test_many_short_sequences(cuda, dtype, hd):
     """More parts than the GPU has SMs, of all kinds in turn: without queries, without keys, with values that are not finite behind what

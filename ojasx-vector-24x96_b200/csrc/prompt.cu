@@ -527,8 +527,9 @@ static int launch_prompt_tc(const PromptProblem& P, cudaStream_t s) {
 // The high parts of Q are in tensor memory, where products take them without the shared memory's bandwidth; the low ones, and K and V
 // in steps of 64 keys, are in shared memory.  The tensor cores cut what they add to a sum, so a step's products with V are summed on
 // their own and join the row's fp32 sums, which are in its thread's registers.  Bound by what a row's thread does for a step (the two parts
-// of 64 weights, O of the step before); the tensor pipe is 41 % busy.  Two prompts of 2048 with 32 query heads and 8 KV heads of 128: 283 us,
-// 243 TFLOP/s of the formula, 728 of fp16 products (4750 us with fp32 FMA, 364 with all of Q in shared memory).
+// of 64 weights, O of the step before); the tensor pipe is 41 % busy.  Two prompts of 2048 with 32 query heads and 8 KV heads of 128: 276 us,
+// 249 TFLOP/s of the formula, 747 of fp16 products (4750 us with fp32 FMA, 364 with all of Q in shared memory).  Two S of 32 keys a tile, so
+// that products and exponentials overlap within a tile too, took a fifth longer: every step has its waits, whatever its length.
 constexpr int kPpKeys = 64;
 constexpr float kPpRoom = 5.0f;   // y is 2^5 at most when the reference is set, 2^13 later on
 
@@ -889,8 +890,11 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_pair_kernel(const __grid
                     for (int u = 0; u < 2; ++u) {
                         const unsigned long long y = pa_exp2(pa_add2((unsigned long long)s[c + e + 2 * u + 1] << 32 | s[c + e + 2 * u], off2));
                         sum = pa_fma2(y, vfs[u], sum);
-                        const __half2 h = __floats2half2_rn(__uint_as_float((unsigned)y), __uint_as_float((unsigned)(y >> 32)));
-                        const unsigned long long rest = pa_add2(y, pa_pair(-__low2float(h), -__high2float(h)));
+                        // the high part is cut to 11 bits, which fp16 holds as they are (283 us with a
+                        // rounded one, which has to come back from fp16; 3.3e-7 and 3.4e-7 off 64 bits)
+                        const unsigned yl = (unsigned)y & 0xffffe000u, yh = (unsigned)(y >> 32) & 0xffffe000u;
+                        const __half2 h = __floats2half2_rn(__uint_as_float(yl), __uint_as_float(yh));
+                        const unsigned long long rest = pa_fma2((unsigned long long)yh << 32 | yl, pa_pair(-1.0f, -1.0f), y);
                         hi[e / 2 + u] = *reinterpret_cast<const unsigned*>(&h);
                         lo[e / 2 + u] = gm_pack(__uint_as_float((unsigned)rest), __uint_as_float((unsigned)(rest >> 32)));
                     }

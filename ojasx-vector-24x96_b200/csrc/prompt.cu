@@ -94,7 +94,7 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_tc_kernel(const __grid_c
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;   // (the same for a warp, as the compiler sees)
     const unsigned base = tc_smem(smem), bars = base + M::bars;
     const unsigned full = bars, empty = bars + 8 * NS, q_full = empty + 8 * NS, s_full = q_full + 16, p_full = s_full + 32, o_full = p_full + 32,
-                   checked = o_full + 16, q_empty = checked + 16, item_full = q_empty + 16, item_empty = item_full + 16,
+                   checked = o_full + 32, q_empty = checked + 16, item_full = q_empty + 16, item_empty = item_full + 16,
                    want = item_empty + 16, steal = want + 8, ended = steal + 8, gone = tc_smem(&s_gone);
     const int per = kPaRows / P.share;
     if (tid == 0) {
@@ -105,7 +105,8 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_tc_kernel(const __grid_c
             tc_bar_init(s_full + 16 * i + 8, 1);
             tc_bar_init(p_full + 16 * i, 4);
             tc_bar_init(p_full + 16 * i + 8, 4);
-            tc_bar_init(o_full + 8 * i, 1);
+            tc_bar_init(o_full + 16 * i, 1);
+            tc_bar_init(o_full + 16 * i + 8, 1);
             tc_bar_init(checked + 8 * i, 4);
             tc_bar_init(q_empty + 8 * i, 1);
             tc_bar_init(item_full + 8 * i, 1);
@@ -280,7 +281,7 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_tc_kernel(const __grid_c
                             for (int k = 0; k < kPaKeys / 16; ++k)
                                 tc_mma_ts(lead, tmem + 256 + i * 128, tmem + i * 128 + (j & 1) * 64 + k * 8, tc_at(b, k * 2048), iv, j > 0 || k > 0);
                         }
-                        tc_commit(lead, o_full + 8 * i);
+                        tc_commit(lead, o_full + 16 * i + 8 * (j & 1));
                         if (j + 2 < item.steps[i]) {
                             if (!loaded && !(ok = wait(full + 8 * kr.slot, kr.parity))) continue;
                             loaded = true;
@@ -310,6 +311,9 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_tc_kernel(const __grid_c
         const float scale = P.scale * 1.4426950408889634f;
         int checks = 0;
         unsigned done = 0, halves = 0, before = 0;   // steps of the tile so far, those with either S (a bit each), and the CTA's
+        // The products of step j, whose scores were the last that the row has waited for, or those before them.  (Either S has a barrier for its
+        // products: the scores of a step tell that the products of the second step before are done, not those of the one before.)
+        auto products = [&](int j) { return wait(o_full + 16 * i + 8 * (j & 1), (halves >> (j & 1) & 1) ^ 1); };
         auto rescale = [&](float by) {   // the warp's rows of O
             for (int c = 0; c < HD; c += 32) {
                 unsigned o[32];
@@ -364,7 +368,7 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_tc_kernel(const __grid_c
                 if (j == 0) {
                     top = now;
                 } else if (__any_sync(0xffffffffu, up)) {
-                    if (!(ok = wait(o_full + 8 * i, (step - 2) & 1))) break;   // the products of the step before
+                    if (!(ok = products(j - 1))) break;
                     tc_after();
                     const float to = up ? now : top, by = up ? exp2f((top - now) * scale) : 1.0f;
                     rescale(by);
@@ -402,7 +406,7 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_tc_kernel(const __grid_c
                     }
                     if (!(ok = wait(checked + 8 * i, checks++ & 1))) break;
                     if (*reinterpret_cast<volatile int*>(&s_odd[i][j & 1]) == (int)step) {
-                        if (j > 0 && !(ok = wait(o_full + 8 * i, (step - 2) & 1))) break;
+                        if (j > 0 && !(ok = products(j - 1))) break;
                         tc_after();
                         tc_wait_st();
                         const int see = min(last - j * kPaKeys, kPaKeys - 1);
@@ -456,7 +460,7 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_tc_kernel(const __grid_c
                 uint4* to = reinterpret_cast<uint4*>(reinterpret_cast<__nv_bfloat16*>(P.out) +
                                                      ((size_t)(what[0] + what[4] + i * per + (out ? position : 0)) * P.q_heads + what[3] * P.share + (out ? row % P.share : 0)) * HD);
                 if (steps) {
-                    ok = wait(o_full + 8 * i, (done - 1) & 1);
+                    ok = products(steps - 1);
                     tc_after();
                 }
                 for (int c = 0; c < HD && ok; c += 32) {

@@ -168,6 +168,26 @@ def test_rows_in_front_of_values_that_are_not_finite(cuda, dtype, hd, share):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("hd,heads,share", [(64, 4, 1), (128, 8, 4)])
+def test_every_step_of_short_prompts_counts(cuda, hd, heads, share):
+    """Weights are equal and the values of a sequence count its tokens, so that a step of keys whose products a result was read before shows;
+    the copies come from memory that the calls in between have pushed out of the cache."""
+    lengths = [65 + 7 * b % 130 for b in range(60)]
+    rows, at = sum(lengths), np.cumsum([0] + lengths)
+    q, k = torch.zeros(rows, heads * share, hd, device=cuda).bfloat16(), torch.zeros(rows, heads, hd, device=cuda).bfloat16()
+    place = torch.cat([torch.arange(n, device=cuda) for n in lengths])
+    v = (place[:, None, None] // 64).expand(rows, heads, hd).bfloat16().contiguous()       # 0, 1, 2, ...: of the step
+    # a row at place p sees p + 1 values whose sums are exact; the rounding to bf16 is off by 2^-8 at most, the reciprocal by far less
+    count = (place + 1).double()
+    want = torch.stack([(torch.clamp(count - 64 * s, 0, 64) * s) for s in range(4)]).sum(0) / count
+    away = torch.empty(64 << 20, dtype=torch.float32, device=cuda)
+    for turn in range(20):
+        away.fill_(turn)
+        got = ops.prompt_attention(q, k, v, _ends(lengths)).double()
+        assert bool(((got - want[:, None, None]).abs() <= want[:, None, None] * 2.0 ** -7).all()), turn
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("hd", [64, 128])
 def test_many_short_sequences(cuda, dtype, hd):

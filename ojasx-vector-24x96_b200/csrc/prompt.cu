@@ -80,7 +80,87 @@ __device__ __forceinline__ unsigned long long pa_exp2(unsigned long long x) {
 }
 static __device__ int g_prompt_error;   // raised when a bounded wait inside a kernel ran out
 
-template <int HD>
+// ---- Few rows over many keys: the CTAs of a cluster have the same rows and a share of the keys each.  Their sums go into their own shared
+// memory (copies and products are done by then), and after a cluster barrier every CTA joins the sums of some of the rows, in the
+// shares' order, and writes them.
+__device__ __forceinline__ void pa_cluster_sync() {
+    __syncwarp();
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ int pa_cluster_rank() {
+    unsigned rank;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+    return (int)rank;
+}
+__device__ __forceinline__ int pa_cluster_size() {
+    unsigned size;
+    asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(size));
+    return (int)size;
+}
+__device__ __forceinline__ void pa_rows_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }   // the rows' threads of both tiles
+// Steps of the keys that this CTA has of the n of its rows.
+struct PaShare {
+    int first, count;
+    __device__ __forceinline__ PaShare(int n, int rank, int size)
+        : first((int)((long long)n * rank / size)), count((int)((long long)n * (rank + 1) / size) - first) {}
+};
+// A row's sums: its products, and the reference of its weights (in powers of two) and their sum behind those of all rows.
+template <int HD> struct PaParts {
+    static constexpr int row = HD + 4, heads = 256 * row * 4, bytes = heads + 256 * 8;
+};
+template <int HD, bool kBf16>
+__device__ __forceinline__ void pa_join(const PromptProblem& P, const unsigned char* parts, int first_row, int head, int per, int live0, int live1, float unit) {
+    const int rank = pa_cluster_rank(), size = pa_cluster_size(), warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const unsigned at = static_cast<unsigned>(__cvta_generic_to_shared(parts));
+    constexpr int W = HD / 32;   // values of a lane
+    auto map = [](unsigned local, int z) {
+        unsigned far;
+        asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(far) : "r"(local), "r"(z));
+        return far;
+    };
+    for (int r = rank + size * warp; r < 2 * kPaRows; r += size * 8) {
+        const int tile = r / kPaRows, row = r % kPaRows, position = row / P.share;
+        if (row >= per * P.share || position >= (tile ? live1 : live0)) continue;
+        float top = -INFINITY, sum = 0.0f;
+        if (lane < size) asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(top), "=f"(sum) : "r"(map(at + PaParts<HD>::heads + r * 8, lane)) : "memory");
+        float most = top;
+#pragma unroll
+        for (int off = 1; off < 8; off <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, off));
+        const float keep = top == -INFINITY ? 0.0f : exp2f(top - most);   // (a share without keys for the row)
+        float x[W], total = 0.0f;
+#pragma unroll
+        for (int e = 0; e < W; ++e) x[e] = 0.0f;
+        for (int z = 0; z < size; ++z) {
+            const float k = __shfl_sync(0xffffffffu, keep, z);
+            const unsigned from = map(at + (r * PaParts<HD>::row + lane * W) * 4, z);
+            float y[W];
+            if constexpr (W == 4) asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(y[0]), "=f"(y[1]), "=f"(y[2]), "=f"(y[3]) : "r"(from) : "memory");
+            else asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(y[0]), "=f"(y[1]) : "r"(from) : "memory");
+#pragma unroll
+            for (int e = 0; e < W; ++e) x[e] = fmaf(y[e], k, x[e]);
+            total = fmaf(__shfl_sync(0xffffffffu, sum, z), k, total);
+        }
+        const float inv = total == 0.0f ? 0.0f : 1.0f / (total * unit);
+        const size_t to = ((size_t)(first_row + tile * per + position) * P.q_heads + head * P.share + row % P.share) * HD + lane * W;
+        if constexpr (kBf16) {
+            unsigned w[W / 2];
+#pragma unroll
+            for (int e = 0; e < W / 2; ++e) {
+                const __nv_bfloat162 h = __floats2bfloat162_rn(x[2 * e] * inv, x[2 * e + 1] * inv);
+                w[e] = *reinterpret_cast<const unsigned*>(&h);
+            }
+            unsigned* out = reinterpret_cast<unsigned*>(reinterpret_cast<__nv_bfloat16*>(P.out) + to);
+#pragma unroll
+            for (int e = 0; e < W / 2; ++e) out[e] = w[e];
+        } else {
+            float* out = reinterpret_cast<float*>(P.out) + to;
+#pragma unroll
+            for (int e = 0; e < W; ++e) out[e] = x[e] * inv;
+        }
+    }
+}
+
+template <int HD, bool kShares>
 __global__ void __launch_bounds__(kPaThreads, 1) prompt_tc_kernel(const __grid_constant__ PromptProblem P, const __grid_constant__ CUtensorMap q_map,
                                                                   const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map) {
     using M = PaSmem<HD>;
@@ -143,7 +223,7 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_tc_kernel(const __grid_c
         for (int i = 0; i < 2; ++i) {
             item.pos[i] = b.x + i * per;
             item.live[i] = i ? b.z : b.y;
-            item.steps[i] = item.live[i] > 0 ? max(0, item.pos[i] + item.live[i] + item.ahead + kPaKeys - 1) / kPaKeys : 0;
+            item.steps[i] = item.live[i] > 0 ? min(max(0, item.pos[i] + item.live[i] + item.ahead + kPaKeys - 1) / kPaKeys, b.w) : 0;
         }
         item.n = max(item.steps[0], item.steps[1]);
         return item.row >= 0;
@@ -154,11 +234,12 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_tc_kernel(const __grid_c
         if (warp == 11) {
             // Work: the CTA's own part of the prompts, and then those of CTAs that have not begun, asked for when the copies of the last one
             // have been issued.  The last parts of a sequence, which see the most keys, come first.
-            int cta = blockIdx.x, number = 0;
+            const int size = kShares ? pa_cluster_size() : 1, rank = kShares ? pa_cluster_rank() : 0;
+            int cta = (int)blockIdx.x / size, number = 0;
             unsigned asked = 0;
             while (ok) {
                 int seq = -1, part = 0;
-                const bool in = cta >= 0 && packed_part(P.batch, (int)(gridDim.x / P.kv_heads) - 1 - cta / P.kv_heads,
+                const bool in = cta >= 0 && packed_part(P.batch, (int)gridDim.x / size / P.kv_heads - 1 - cta / P.kv_heads,
                                                         [&](int b) { return (packed_range(P.ends, b, P.n_rows).count + 2 * per - 1) / (2 * per); }, seq, part);
                 if (in || cta < 0) {
                     if (number >= 2 && !(ok = wait(item_empty + 8 * (number & 1), ((number >> 1) - 1) & 1))) break;
@@ -168,7 +249,13 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_tc_kernel(const __grid_c
                             const PackedRange rows = packed_range(P.ends, seq, P.n_rows), keys = packed_range(P.key_ends, seq, P.n_keys);
                             const int pos = part * 2 * per;
                             a = make_int4(rows.first, keys.first, keys.count - rows.count, cta % P.kv_heads);
-                            b = make_int4(pos, min(per, rows.count - pos), max(0, min(per, rows.count - pos - per)), 0);
+                            b = make_int4(pos, min(per, rows.count - pos), max(0, min(per, rows.count - pos - per)), 0x7fffffff);
+                            if (kShares) {   // the keys begin with the first of this CTA's
+                                const PaShare share(max(0, pos + b.y + b.z + a.z + kPaKeys - 1) / kPaKeys, rank, size);
+                                a.y += share.first * kPaKeys;
+                                a.z -= share.first * kPaKeys;
+                                b.w = share.count;
+                            }
                         }
                         *reinterpret_cast<int4*>(s_item[number & 1]) = a;
                         *reinterpret_cast<int4*>(s_item[number & 1] + 4) = b;
@@ -177,6 +264,10 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_tc_kernel(const __grid_c
                     __syncwarp();
                     if (cta < 0 || !(ok = wait(want, number & 1))) break;
                     ++number;
+                }
+                if (kShares) {   // (the CTAs of a cluster stay at one part)
+                    cta = -1;
+                    continue;
                 }
                 if (lane == 0) {
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -310,6 +401,7 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_tc_kernel(const __grid_c
         const unsigned lanes = (unsigned)((warp & 3) * 32) << 16, st = tmem + i * 128 + lanes, ot = tmem + 256 + i * 128 + lanes;
         const float scale = P.scale * 1.4426950408889634f;
         int checks = 0;
+        bool met = false;   // (of the tiles' threads)
         unsigned done = 0, halves = 0, before = 0;   // steps of the tile so far, those with either S (a bit each), and the CTA's
         // The products of step j, whose scores were the last that the row has waited for, or those before them.  (Either S has a barrier for its
         // products: the scores of a step tell that the products of the second step before are done, not those of the one before.)
@@ -332,11 +424,11 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_tc_kernel(const __grid_c
             int steps, last, first, n;   // of the tile; last key that the row sees, and that the tile's first row sees; steps of both tiles
             {
                 const int pos = what[4] + i * per, live = what[5 + i], ahead = what[2], end = pos + live + ahead;
-                steps = live > 0 ? max(0, end + kPaKeys - 1) / kPaKeys : 0;
+                steps = live > 0 ? min(max(0, end + kPaKeys - 1) / kPaKeys, what[7]) : 0;
                 first = pos + ahead;
                 last = first + min(row, max(live * P.share - 1, 0)) / P.share;
                 const int other = what[6 - i], to = what[4] + (1 - i) * per + other + ahead;
-                n = max(steps, other > 0 ? max(0, to + kPaKeys - 1) / kPaKeys : 0);
+                n = max(steps, other > 0 ? min(max(0, to + kPaKeys - 1) / kPaKeys, what[7]) : 0);
             }
             float top = 0.0f;
             unsigned long long sum2[2] = {0, 0};
@@ -452,7 +544,31 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_tc_kernel(const __grid_c
                 if (lane == 0) tc_bar_arrive(p_full + 16 * i + 8 * (j & 1));
             }
             const int live = what[5 + i];
-            if (ok && live > 0) {
+            if constexpr (kShares) {
+                if (ok && steps) {
+                    ok = products(steps - 1);
+                    tc_after();
+                }
+                pa_rows_sync();   // (where Q, K and V were)
+                met = true;
+                sum2[0] = pa_add2(sum2[0], sum2[1]);
+                float* const parts = reinterpret_cast<float*>(smem);
+                for (int c = 0; c < HD; c += 32) {
+                    unsigned o[32];
+                    if (steps) {
+                        tc_ld32(ot + c, o);
+                        tc_wait_ld();
+                        tc_pin32(o);
+                    }
+#pragma unroll
+                    for (int e = 0; e < 32; e += 4)
+                        *reinterpret_cast<uint4*>(parts + tid * PaParts<HD>::row + c + e) =
+                            steps ? make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]) : make_uint4(0u, 0u, 0u, 0u);
+                }
+                reinterpret_cast<float2*>(smem + PaParts<HD>::heads)[tid] =
+                    steps ? make_float2(top * scale, __uint_as_float((unsigned)sum2[0]) + __uint_as_float((unsigned)(sum2[0] >> 32))) : make_float2(-INFINITY, 0.0f);
+            }
+            if (!kShares && ok && live > 0) {
                 const int position = row / P.share;
                 const bool out = position < live && row < per * P.share;
                 sum2[0] = pa_add2(sum2[0], sum2[1]);
@@ -490,6 +606,7 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_tc_kernel(const __grid_c
             __syncwarp();
             if (lane == 0) tc_bar_arrive(item_empty + 8 * (number & 1));
         }
+        if (kShares && !met) pa_rows_sync();   // (a warp that gave up must not leave the others waiting)
     }
     if (!ok) atomicExch(&g_prompt_error, 1);
     tc_before();
@@ -498,16 +615,35 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_tc_kernel(const __grid_c
         tc_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
     }
+    if constexpr (kShares) {
+        pa_cluster_sync();   // the sums of every share are in place
+        const volatile int* const what = s_item[0];
+        if (warp < 8 && what[0] >= 0) pa_join<HD, true>(P, smem, what[0] + what[4], what[3], per, what[5], what[6], 1.0f);
+        pa_cluster_sync();   // nobody leaves while its sums may still be read
+    }
 }
+
+// CTAs that share the keys of a part of the rows: as many as the GPU holds next to one another, with four steps of keys each on average.  The
+// cluster's launch and the joining cost 8 us in bf16, where there is also no work to take over, and 2 us next to the longer steps of fp32.
+// us without and with shares, 8 KV heads of 4 query heads of 128: 256 positions behind 768 cached ones 22 and 27 in bf16, 60 and 52 in
+// fp32, 300 behind 1700 37 and 34, 104 and 77, 64 behind 7936 124 and 30, 367 and 85; 512 alone 15 and 23, 38 and 40.
+static int prompt_shares(const PromptProblem& P, long long parts, bool bf16) {
+    const long long steps = (long long)P.n_keys / std::min(P.batch, P.n_rows) / 64;
+    int shares = 1;
+    if (steps < (bf16 ? 24 : 12)) return 1;
+    while (shares < 8 && parts * shares * 2 <= num_sms() && steps >= 8LL * shares) shares *= 2;
+    return shares;
+}
+static_assert(kPaKeys == 64, "steps of keys");
 
 template <int HD>
 static int launch_prompt_tc(const PromptProblem& P, cudaStream_t s) {
-    static std::atomic<bool> opted[64];
+    static std::atomic<bool> opted[2][64];
     constexpr int smem = PaSmem<HD>::bytes;
-    OJX_CUDA_TRY(opt_in_smem(reinterpret_cast<const void*>(prompt_tc_kernel<HD>), smem, opted));
+    static_assert(PaParts<HD>::bytes <= PaSmem<HD>::bars, "the sums of the rows lie where Q, K and V were");
     const int per = kPaRows / P.share;
     const long long parts = P.n_rows / (2 * per) + std::min(P.batch, P.n_rows);
-    if (parts * P.kv_heads > 0x7fffffffLL) return OJX_ERR_TOO_LARGE;
+    if (parts * P.kv_heads > 0x7fffffffLL) return OJX_ERR_TOO_LARGE;   // (with shares there are at most as many as SMs)
     CUtensorMap q, k, v;
     const bool none = P.n_keys == 0;
     if (!tc_map3(&q, true, P.q, HD, P.q_heads, P.n_rows, P.q_head, P.q_row, 64, P.share, per) ||
@@ -516,7 +652,11 @@ static int launch_prompt_tc(const PromptProblem& P, cudaStream_t s) {
         set_last_error_msg("prompt attention: the tensors' strides do not make a tensor map");
         return OJX_ERR_ARG;
     }
-    OJX_CUDA_TRY(launch_chained(prompt_tc_kernel<HD>, dim3((unsigned)(parts * P.kv_heads)), kPaThreads, smem, s, P, q, k, v));
+    const int shares = prompt_shares(P, parts * P.kv_heads, true);
+    auto kernel = shares > 1 ? prompt_tc_kernel<HD, true> : prompt_tc_kernel<HD, false>;
+    OJX_CUDA_TRY(opt_in_smem(reinterpret_cast<const void*>(kernel), smem, opted[shares > 1]));
+    if (shares > 1) OJX_CUDA_TRY(launch_chained_cluster(kernel, dim3((unsigned)(parts * P.kv_heads * shares)), kPaThreads, smem, s, (unsigned)shares, P, q, k, v));
+    else OJX_CUDA_TRY(launch_chained(kernel, dim3((unsigned)(parts * P.kv_heads)), kPaThreads, smem, s, P, q, k, v));
     count_launch(1);
     return OJX_OK;
 }
@@ -604,7 +744,7 @@ __global__ void __launch_bounds__(256) prompt_split_kernel(const __grid_constant
     }
 }
 
-template <int HD>
+template <int HD, bool kShares>
 __global__ void __launch_bounds__(kPaThreads, 1) prompt_pair_kernel(const __grid_constant__ PromptProblem P, const __grid_constant__ PromptSplit S,
                                                                     const __grid_constant__ CUtensorMap k_hi, const __grid_constant__ CUtensorMap k_lo,
                                                                     const __grid_constant__ CUtensorMap v_hi, const __grid_constant__ CUtensorMap v_lo) {
@@ -618,7 +758,8 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_pair_kernel(const __grid
     const unsigned base = tc_smem(smem), bars = base + M::bars;
     const unsigned full = bars, empty = bars + 8 * NS, q_full = empty + 8 * NS, s_full = q_full + 16, p_full = s_full + 16, o_full = p_full + 16,
                    checked = o_full + 16, f_full = checked + 16, f_empty = f_full + 16, ended = f_empty + 16, gone = tc_smem(&s_gone);
-    const int head = blockIdx.x % P.kv_heads, per = kPaRows / P.share;
+    const int size = kShares ? pa_cluster_size() : 1, unit = (int)blockIdx.x / size, units = (int)gridDim.x / size;
+    const int head = unit % P.kv_heads, per = kPaRows / P.share;
     if (tid == 0) {
         for (int i = 0; i < NS; ++i) { tc_bar_init(full + 8 * i, 1); tc_bar_init(empty + 8 * i, 1); }
         for (int i = 0; i < 2; ++i) {
@@ -638,7 +779,7 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_pair_kernel(const __grid
     chain_begin();
     if (warp == 0) {
         int seq = -1, part = 0;   // (the last parts first)
-        const bool in = packed_part(P.batch, (int)(gridDim.x / P.kv_heads) - 1 - (int)blockIdx.x / P.kv_heads,
+        const bool in = packed_part(P.batch, units / P.kv_heads - 1 - unit / P.kv_heads,
                                     [&](int b) { return (packed_range(P.ends, b, P.n_rows).count + 2 * per - 1) / (2 * per); }, seq, part);
         if (lane == 0) { s_seq = in ? seq : -1; s_part = part; }
     }
@@ -653,14 +794,22 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_pair_kernel(const __grid
     tc_after();
     // S and then the weights of tile i at 64 i (hi 32 columns, lo 32), Q's high parts at 128 + 64 i, a step's O at 256 + 128 i
     const unsigned tmem = __shfl_sync(0xffffffffu, s_tmem, 0);
-    const PackedRange rows = packed_range(P.ends, s_seq, P.n_rows), keys = packed_range(P.key_ends, s_seq, P.n_keys);
-    const int ahead = keys.count - rows.count;
-    int pos[2], live[2], steps[2];
+    const PackedRange rows = packed_range(P.ends, s_seq, P.n_rows);
+    PackedRange keys = packed_range(P.key_ends, s_seq, P.n_keys);
+    int ahead = keys.count - rows.count, pos[2], live[2], steps[2], most = 0x7fffffff;
+    if (kShares) {   // the keys begin with the first of this CTA's
+        const int end = min(rows.count, (s_part + 1) * 2 * per);
+        const PaShare share(max(0, end + ahead + N - 1) / N, pa_cluster_rank(), size);
+        keys.first += share.first * N;
+        keys.count -= share.first * N;
+        ahead -= share.first * N;
+        most = share.count;
+    }
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
         pos[i] = (s_part * 2 + i) * per;
         live[i] = max(0, min(per, rows.count - pos[i]));
-        steps[i] = live[i] > 0 ? max(0, pos[i] + live[i] + ahead + N - 1) / N : 0;
+        steps[i] = live[i] > 0 ? min(max(0, pos[i] + live[i] + ahead + N - 1) / N, most) : 0;
     }
     const int n = max(steps[0], steps[1]);
     bool ok = true;
@@ -960,7 +1109,20 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_pair_kernel(const __grid
                 tc_bar_arrive(p_full + 8 * i);
             }
         }
-        if (ok && live[i] > 0) {
+        if constexpr (kShares) {
+            if (ok && steps[i]) {
+                ok = wait(o_full + 8 * i, 0);
+                tc_after();
+                if (ok && parted) join();
+            }
+            pa_rows_sync();   // (where Q, K and V were)
+            float* const to = reinterpret_cast<float*>(smem) + tid * PaParts<HD>::row;
+#pragma unroll
+            for (int d = 0; d < HD / 2; d += 2) *reinterpret_cast<ulonglong2*>(to + 2 * d) = make_ulonglong2(o[d], o[d + 1]);
+            reinterpret_cast<float2*>(smem + PaParts<HD>::heads)[tid] =
+                make_float2(top, __uint_as_float((unsigned)sum) + __uint_as_float((unsigned)(sum >> 32)));
+        }
+        if (!kShares && ok && live[i] > 0) {
             if (steps[i]) {
                 ok = wait(o_full + 8 * i, 0);
                 tc_after();
@@ -983,6 +1145,11 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_pair_kernel(const __grid
         tc_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
     }
+    if constexpr (kShares) {
+        pa_cluster_sync();   // the sums of every share are in place
+        if (warp < 8) pa_join<HD, false>(P, smem, rows.first + pos[0], head, per, live[0], live[1], 16384.0f);
+        pa_cluster_sync();   // nobody leaves while its sums may still be read
+    }
 }
 
 // Bytes of the planes and factors of K and V.
@@ -990,9 +1157,9 @@ static size_t prompt_split_plane(int n_keys, int kv_heads, int head_dim) { retur
 
 template <int HD>
 static int launch_prompt_pair(const PromptProblem& P, void* workspace, cudaStream_t s) {
-    static std::atomic<bool> opted[64];
+    static std::atomic<bool> opted[2][64];
     constexpr int smem = PpSmem<HD>::bytes;
-    OJX_CUDA_TRY(opt_in_smem(reinterpret_cast<const void*>(prompt_pair_kernel<HD>), smem, opted));
+    static_assert(PaParts<HD>::bytes <= PpSmem<HD>::factors, "the sums of the rows lie where Q, K and V were");
     const int per = kPaRows / P.share;
     const long long parts = P.n_rows / (2 * per) + std::min(P.batch, P.n_rows);
     const long long split = ((long long)P.n_keys * P.kv_heads * 2 * (HD / 8) + 255) / 256;
@@ -1013,7 +1180,13 @@ static int launch_prompt_pair(const PromptProblem& P, void* workspace, cudaStrea
         OJX_CUDA_TRY(launch_chained(prompt_split_kernel<HD>, dim3((unsigned)split), 256, 0, s, P, S));
         count_launch(1);
     }
-    OJX_CUDA_TRY(launch_chained(prompt_pair_kernel<HD>, dim3((unsigned)(parts * P.kv_heads)), kPaThreads, smem, s, P, S, maps[0], maps[1], maps[2], maps[3]));
+    const int shares = prompt_shares(P, parts * P.kv_heads, false);
+    auto kernel = shares > 1 ? prompt_pair_kernel<HD, true> : prompt_pair_kernel<HD, false>;
+    OJX_CUDA_TRY(opt_in_smem(reinterpret_cast<const void*>(kernel), smem, opted[shares > 1]));
+    if (shares > 1)
+        OJX_CUDA_TRY(launch_chained_cluster(kernel, dim3((unsigned)(parts * P.kv_heads * shares)), kPaThreads, smem, s, (unsigned)shares, P, S, maps[0], maps[1],
+                                            maps[2], maps[3]));
+    else OJX_CUDA_TRY(launch_chained(kernel, dim3((unsigned)(parts * P.kv_heads)), kPaThreads, smem, s, P, S, maps[0], maps[1], maps[2], maps[3]));
     count_launch(1);
     return OJX_OK;
 }

@@ -189,6 +189,36 @@ def test_every_step_of_short_prompts_counts(cuda, hd, heads, share):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("hd,heads,share,lengths,key_lengths", [
+    (128, 1, 4, [7], [5000]), (128, 2, 4, [100, 33], [2100, 1900]), (64, 3, 3, [40, 1, 0, 130], [2900, 2500, 10, 1500]), (64, 1, 1, [2000], [1999]),
+    (128, 2, 8, [600], [600]), (64, 1, 2, [1, 1, 1], [6000, 0, 63]), (128, 1, 64, [3], [2049])])
+def test_few_rows_over_many_keys(cuda, dtype, hd, heads, share, lengths, key_lengths):
+    """Parts of the rows whose keys several CTAs share; keys behind the last sequence are not finite, and one row's scores end in an outlier."""
+    g = _gen(41)
+    n, m = sum(lengths), sum(key_lengths)
+    q = _randn(g, n + 2, heads * share, hd, dtype=dtype)
+    k, v = (_randn(g, m + 70, heads, hd, dtype=dtype) for _ in range(2))
+    k[m:], v[m:] = math.nan, math.inf
+    k[key_lengths[0] * 3 // 4] *= 6
+    got = ops.prompt_attention(q, k, v, _ends(lengths), _ends(key_lengths))
+    _check(q, k, v, lengths, key_lengths, got)
+    assert torch.equal(got[:n], ops.prompt_attention(q, k, v, _ends(lengths), _ends(key_lengths))[:n])   # joined in one order
+    out = torch.full_like(q, 7.0)
+    ops.prompt_attention(q, k, v, _ends(lengths), _ends(key_lengths), out=out)
+    assert (out[n:] == 7.0).all() and torch.equal(out[:n], got[:n])
+    # the values that a row does not see, not finite
+    first = lengths[0]
+    if first > 1 and key_lengths[0] >= first:
+        bad = v.clone()
+        bad[key_lengths[0] - 1] = math.nan
+        other = ops.prompt_attention(q, k, bad, _ends(lengths), _ends(key_lengths))
+        end = key_lengths[0] - 1
+        _check(q[:first - 1], k[:end], v[:end], [first - 1], [end], other[:first - 1])
+        assert torch.isnan(other[first - 1]).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("hd", [64, 128])
 def test_many_short_sequences(cuda, dtype, hd):
     """More parts than the GPU has SMs, of all kinds in turn: without queries, without keys, with values that are not finite behind what

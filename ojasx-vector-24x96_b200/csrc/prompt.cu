@@ -223,7 +223,8 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_tc_kernel(const __grid_c
         for (int i = 0; i < 2; ++i) {
             item.pos[i] = b.x + i * per;
             item.live[i] = i ? b.z : b.y;
-            item.steps[i] = item.live[i] > 0 ? min(max(0, item.pos[i] + item.live[i] + item.ahead + kPaKeys - 1) / kPaKeys, b.w) : 0;
+            item.steps[i] = item.live[i] > 0 ? max(0, item.pos[i] + item.live[i] + item.ahead + kPaKeys - 1) / kPaKeys : 0;
+            if (kShares) item.steps[i] = min(item.steps[i], b.w);
         }
         item.n = max(item.steps[0], item.steps[1]);
         return item.row >= 0;
@@ -235,11 +236,11 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_tc_kernel(const __grid_c
             // Work: the CTA's own part of the prompts, and then those of CTAs that have not begun, asked for when the copies of the last one
             // have been issued.  The last parts of a sequence, which see the most keys, come first.
             const int size = kShares ? pa_cluster_size() : 1, rank = kShares ? pa_cluster_rank() : 0;
-            int cta = (int)blockIdx.x / size, number = 0;
+            int cta = kShares ? (int)blockIdx.x / size : (int)blockIdx.x, number = 0;
             unsigned asked = 0;
             while (ok) {
                 int seq = -1, part = 0;
-                const bool in = cta >= 0 && packed_part(P.batch, (int)gridDim.x / size / P.kv_heads - 1 - cta / P.kv_heads,
+                const bool in = cta >= 0 && packed_part(P.batch, (int)((kShares ? gridDim.x / size : gridDim.x) / P.kv_heads) - 1 - cta / P.kv_heads,
                                                         [&](int b) { return (packed_range(P.ends, b, P.n_rows).count + 2 * per - 1) / (2 * per); }, seq, part);
                 if (in || cta < 0) {
                     if (number >= 2 && !(ok = wait(item_empty + 8 * (number & 1), ((number >> 1) - 1) & 1))) break;
@@ -249,7 +250,7 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_tc_kernel(const __grid_c
                             const PackedRange rows = packed_range(P.ends, seq, P.n_rows), keys = packed_range(P.key_ends, seq, P.n_keys);
                             const int pos = part * 2 * per;
                             a = make_int4(rows.first, keys.first, keys.count - rows.count, cta % P.kv_heads);
-                            b = make_int4(pos, min(per, rows.count - pos), max(0, min(per, rows.count - pos - per)), 0x7fffffff);
+                            b = make_int4(pos, min(per, rows.count - pos), max(0, min(per, rows.count - pos - per)), 0);
                             if (kShares) {   // the keys begin with the first of this CTA's
                                 const PaShare share(max(0, pos + b.y + b.z + a.z + kPaKeys - 1) / kPaKeys, rank, size);
                                 a.y += share.first * kPaKeys;
@@ -265,7 +266,7 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_tc_kernel(const __grid_c
                     if (cta < 0 || !(ok = wait(want, number & 1))) break;
                     ++number;
                 }
-                if (kShares) {   // (the CTAs of a cluster stay at one part)
+                if constexpr (kShares) {   // (the CTAs of a cluster stay at one part)
                     cta = -1;
                     continue;
                 }
@@ -424,11 +425,12 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_tc_kernel(const __grid_c
             int steps, last, first, n;   // of the tile; last key that the row sees, and that the tile's first row sees; steps of both tiles
             {
                 const int pos = what[4] + i * per, live = what[5 + i], ahead = what[2], end = pos + live + ahead;
-                steps = live > 0 ? min(max(0, end + kPaKeys - 1) / kPaKeys, what[7]) : 0;
+                steps = live > 0 ? max(0, end + kPaKeys - 1) / kPaKeys : 0;
                 first = pos + ahead;
                 last = first + min(row, max(live * P.share - 1, 0)) / P.share;
                 const int other = what[6 - i], to = what[4] + (1 - i) * per + other + ahead;
-                n = max(steps, other > 0 ? min(max(0, to + kPaKeys - 1) / kPaKeys, what[7]) : 0);
+                n = max(steps, other > 0 ? max(0, to + kPaKeys - 1) / kPaKeys : 0);
+                if (kShares) steps = min(steps, what[7]);   // (n is for the parts behind this one, and there are none)
             }
             float top = 0.0f;
             unsigned long long sum2[2] = {0, 0};

@@ -717,7 +717,7 @@ __global__ void __launch_bounds__(256) prompt_split_kernel(const __grid_constant
         const unsigned b = __float_as_uint(xs[e]) & 0x7fffffffu;
         if (b < 0x7f800000u) most = max(most, b);
     }
-    const unsigned lanes = __activemask();
+    const unsigned lanes = ((1u << L) - 1u) << (threadIdx.x % 32 / L * L);   // the row's: they are all here, or none of them
 #pragma unroll
     for (int off = L / 2; off >= 1; off >>= 1) most = max(most, __shfl_xor_sync(lanes, most, off));
     float up, down, e = 0.0f;

@@ -1,0 +1,19 @@
+"""What the kernels' sources must not do, checked by reading them."""
+import glob
+import os
+import re
+
+CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "ojasx-vector-24x96_b200", "csrc")
+
+
+def _code(path):
+    """A source without its comments."""
+    with open(path) as f:
+        return re.sub(r"//[^\n]*|/\*.*?\*/", "", f.read(), flags=re.S)
+
+
+def test_masks_of_shuffles_name_the_lanes_that_take_part():
+    """__activemask() gives the lanes that happen to be together at that place, not those that a shuffle is meant for."""
+    sources = glob.glob(os.path.join(CSRC, "*.cu")) + glob.glob(os.path.join(CSRC, "*.cuh"))
+    assert sources
+    assert [os.path.basename(p) for p in sources if "__activemask" in _code(p)] == []

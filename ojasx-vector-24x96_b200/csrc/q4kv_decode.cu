@@ -13,17 +13,20 @@
 //   S[token][head]  = codes of K (16 x 16 a step) x q (16 x 8)           a group's steps have sums of their own
 //   O[dim][head]   += codes of V, transposed (16 x 16) x p * s_g (16 x 8)    p * s_g turned by movmatrix
 // A bf16 query is one fp16 number where a power of two brings the head's largest to 2^15 (what is 2^29 below it loses bits), an fp32
-// one two of them (22 bits); so is p * s, one with bf16 activations (11 bits, below the rounding of the result), two with fp32.  The
-// reference of the weights is the largest score plus the exponent of the largest scale so far, so that p * s is in the range of fp16
-// whatever the scales are.
+// one two of them (22 bits); so is p * s * 2^u, one with bf16 activations (11 bits, below the rounding of the result), two with fp32.
+// Each head has an exponent u for each group of dimensions, which goes down where a product would pass 2^14, so that the largest so far is at
+// 2^5: scales that differ from token to token or from group to group, by 2^22 in the tests, cost one another no bits.  (One exponent for
+// all of them, that of the largest scale met so far, took 64 and 152 us in the place of the 71 and 158 below, but a token of large scale and next to
+// no weight cost all others theirs: 1.4e-4 off 64 bits at 2^16, 8e-3 at 2^22.)  u is 100 at most: scales below 2^-100 weigh nothing.
 //
 // Work: units of 128 tokens of a (sequence, KV head, eight query heads), all of them in a row, in equal shares for the CTAs whatever the
 // lengths are; the four warps of a CTA take two tiles of a unit each, from rings of their own that bulk copies fill.  A share that begins
 // or ends inside a sequence leaves its sums to q4_combine_kernel.
 //
-// Bound by the integer pipe (half of its slots at 380 instructions a tile and warp) next to the copies, which alone take 111 to 130 us: 16
-// sequences of 32768 tokens, 671 MB, in 151 us (4.4 TB/s) with 8 KV heads of 4 query heads of 128 in bf16; 48 of up to 20011, 4 heads of 7
-// of 64 in fp32, 106 MB, in 64 us, where the second planes of queries and weights double the products.
+// No pipe is full (integer pipe about half, tensor pipe a fifth, 12 warps an SM): warps wait for their chains of product, exponential and
+// product, next to the copies, which alone take 111 to 130 us: 16 sequences of 32768 tokens, 671 MB, in 158 us (4.2 TB/s) with 8 KV heads of
+// 4 query heads of 128 in bf16; 48 of up to 20011, 4 heads of 7 of 64 in fp32, 106 MB, in 71 us, where the second planes of queries and
+// weights double the products.  fp32 at head_dim 128 spills 92 bytes (168 registers for three CTAs an SM).
 #include <algorithm>
 #include <cmath>
 
@@ -38,8 +41,10 @@ namespace ojx {
 constexpr int kQdThreads = 128, kQdWarps = 4, kQdStages = 2, kQdHeads = 8, kQdPair = 2;
 constexpr int kQdUnit = kQdWarps * kQdPair * kQ4Tile;   // tokens
 constexpr float kQdLowest = -3.0e38f;         // finite: scores of -inf weigh nothing, a NaN makes its head's result one
-constexpr float kQdSlack = 8.0f;              // sums are relative to a reference, until a score is 2^8 above it ...
-constexpr float kQdRoom = 5.0f;               // ... and the largest p * s is 2^5 then: 2^14 at most
+constexpr float kQdSlack = 8.0f;              // weights are relative to a reference, until a score is 2^8 above it
+constexpr int kQdRoom = 5;                    // the largest p * s * 2^u is 2^5 to 2^6 when u is set ...
+constexpr unsigned kQdTooLarge = 0x74007400u; // ... and 2^14 at most (two fp16 numbers)
+constexpr int kQdMost = 127 + 100;            // u at most, as the exponent of a float
 
 static __device__ int g_q4_error;   // raised when a bounded wait inside a kernel ran out
 
@@ -97,8 +102,17 @@ __device__ __forceinline__ unsigned q4_part(float& a, float& b) {
     b -= __high2float(h);
     return *reinterpret_cast<const unsigned*>(&h);
 }
-// Exponent of a positive bf16 number, kept in -20..100.
-__device__ __forceinline__ float q4_exponent(unsigned bits) { return (float)(min(max((int)(bits >> 7), 107), 227) - 127); }
+// Two products in one instruction.
+__device__ __forceinline__ float2 q4_mul2(float2 a, float2 b) {
+    float2 c;
+    asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmul.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}"
+        : "=f"(c.x), "=f"(c.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return c;
+}
+// The power of two with this exponent field (zero where the field would be negative), and the field of a number that is not negative.
+__device__ __forceinline__ float q4_power(int field) { return __uint_as_float((unsigned)max(field, 0) << 23); }
+__device__ __forceinline__ int q4_bits(float x) { return (int)(__float_as_uint(x) >> 23); }
 
 // Quotient of numbers that are not negative (64-bit division takes some hundred instructions).
 __device__ __forceinline__ long long q4_quotient(long long a, long long b) {
@@ -143,7 +157,7 @@ struct QdSmem {
     static constexpr int bytes(int heads) { return kQdWarps * (ring + heads * row * 4); }
 };
 
-constexpr int kQdCtas = 3;   // per SM (16 sequences of 32768 tokens: 151 us; 2: 154, 4: 159)
+constexpr int kQdCtas = 3;   // per SM (16 sequences of 32768 tokens, with one exponent for all groups: 151 us; 2: 154, 4: 159)
 
 template <int HD, bool kBf16>
 __global__ void __launch_bounds__(kQdThreads, kQdCtas) q4_decode_kernel(const __grid_constant__ Q4DecodeProblem P) {
@@ -154,7 +168,9 @@ __global__ void __launch_bounds__(kQdThreads, kQdCtas) q4_decode_kernel(const __
     using Words = typename Q4Words<G>::type;
     using Metas = typename Q4Words<G / 2>::type;   // a token's scales or minima
     extern __shared__ __align__(128) unsigned char qd_smem[];
+    constexpr int kAtOnce = kBf16 ? kQdPair : 1;   // tiles whose weights are looked at together
     __shared__ float s_m[kQdWarps][kQdHeads], s_l[kQdWarps][kQdHeads];
+    __shared__ __align__(8) float s_up[kQdWarps][G * kQdHeads];   // [group][head] 2^u
     __shared__ __align__(8) unsigned long long s_bar[kQdWarps][kQdStages];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, gq = lane >> 2, t = lane & 3, sum_heads = min(P.share, kQdHeads);
     unsigned char* ring = qd_smem + warp * M::ring;
@@ -320,17 +336,17 @@ __global__ void __launch_bounds__(kQdThreads, kQdCtas) q4_decode_kernel(const __
             }
             most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
             most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
-            float up, down;
-            gm_scale(most, up, down);
+            float grow, down;
+            gm_scale(most, grow, down);
             // what a score comes out of the products with
-            const float back = fminf(down * (P.scale * kCode), 3.0e38f);
+            const float back = fminf(fmaxf(down * (P.scale * kCode), 0x1p-126f), 3.0e38f);   // (not zero: what is not seen is -inf times it)
             unscale[0] = __shfl_sync(0xffffffffu, back, 8 * t);        // heads 2 t and 2 t + 1
             unscale[1] = __shfl_sync(0xffffffffu, back, 8 * t + 4);
             float total[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int g = 0; g < G; ++g) {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) x[g][e] *= up;
+                for (int e = 0; e < 8; ++e) x[g][e] *= grow;
                 float sum = ((x[g][0] + x[g][1]) + (x[g][2] + x[g][3])) + ((x[g][4] + x[g][5]) + (x[g][6] + x[g][7]));
                 sum += __shfl_xor_sync(0xffffffffu, sum, 1);
                 sum += __shfl_xor_sync(0xffffffffu, sum, 2);
@@ -367,8 +383,9 @@ __global__ void __launch_bounds__(kQdThreads, kQdCtas) q4_decode_kernel(const __
 #pragma unroll
         for (int g = 0; g < G; ++g) mins[g][0] = mins[g][1] = 0.0f;
 
-        unsigned most = 0, bound = 0;                  // largest scales of the values, two at a time: seen by the lane, and in use
-        float above = -kQdSlack - kQdRoom;             // the exponent in use, less what p * s may be above the reference
+        if (lane < kQdHeads * G) s_up[warp][lane] = 1.0f;
+        __syncwarp();
+        float2* const up = reinterpret_cast<float2*>(s_up[warp]) + t;   // of group g at 4 g: 2^u for the heads 2 t and 2 t + 1
         const int u0 = at.u, u1 = (int)min((long long)at.units, at.u + (last - unit));
         for (int u = u0; u < u1 && ok; ++u) {
             const int token = (u * kQdWarps + warp) * kQdPair * kQ4Tile;
@@ -426,84 +443,157 @@ __global__ void __launch_bounds__(kQdThreads, kQdCtas) q4_decode_kernel(const __
                     x[i][2] = fmaf(high, c[2], x[i][2]);
                     x[i][3] = fmaf(high, c[3], x[i][3]);
                 }
-                Metas va = *reinterpret_cast<const Metas*>(tile + T::value_scales + T::meta_at(gq, 0)), vb = *reinterpret_cast<const Metas*>(tile + T::value_scales + T::meta_at(gq + 8, 0));
                 if (part) {   // what is behind the last token may be anything
-                    if (gq >= seen[i]) { x[i][0] = x[i][1] = -INFINITY; va = Metas{}; }
-                    if (gq + 8 >= seen[i]) { x[i][2] = x[i][3] = -INFINITY; vb = Metas{}; }
+                    if (gq >= seen[i]) x[i][0] = x[i][1] = -INFINITY;
+                    if (gq + 8 >= seen[i]) x[i][2] = x[i][3] = -INFINITY;
                 }
-                const unsigned *ua = reinterpret_cast<const unsigned*>(&va), *ub = reinterpret_cast<const unsigned*>(&vb);
-#pragma unroll
-                for (int g = 0; g < G / 2; ++g) most = __vmaxu2(most, __vmaxu2(ua[g], ub[g]));
                 now[0] = fmaxf(now[0], fmaxf(x[i][0], x[i][2]));
                 now[1] = fmaxf(now[1], fmaxf(x[i][1], x[i][3]));
             }
-            // the reference moves where a lane sees a score too far above it, or scales larger than those before
-            if (__any_sync(0xffffffffu, most != bound || fmaf(now[0], unscale[0], above) > top[0] || fmaf(now[1], unscale[1], above) > top[1])) {
-                const unsigned both = __reduce_max_sync(0xffffffffu, max(most & 0xffffu, most >> 16));
-                most = bound = both | both << 16;
-                above = q4_exponent(both) - (kQdSlack + kQdRoom);
-#pragma unroll
-                for (int off = 4; off < 32; off <<= 1) {
-                    now[0] = fmaxf(now[0], __shfl_xor_sync(0xffffffffu, now[0], off));
-                    now[1] = fmaxf(now[1], __shfl_xor_sync(0xffffffffu, now[1], off));
-                }
+            // the reference moves where a lane sees a score too far above it; by a whole number, so that all factors are powers of two
+            if (__any_sync(0xffffffffu, fmaf(now[0], unscale[0], -kQdSlack) > top[0] || fmaf(now[1], unscale[1], -kQdSlack) > top[1])) {
+                int rise[2];
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    const float score = fmaf(now[h], unscale[h], above);
-                    const bool up = score > top[h];
-                    const float to = up ? score + kQdSlack : top[h], keep = up ? q4_exp2(top[h] - to) : 1.0f;
+#pragma unroll
+                    for (int off = 4; off < 32; off <<= 1) now[h] = fmaxf(now[h], __shfl_xor_sync(0xffffffffu, now[h], off));
+                    const float to = fmaf(now[h], unscale[h], -kQdSlack) > top[h] ? ceilf(now[h] * unscale[h]) : top[h];
+                    rise[h] = (int)fminf(to - top[h], 1000.0f);
                     top[h] = to;
+                    const float keep = q4_power(127 - rise[h]);
                     l[h] *= keep;
 #pragma unroll
                     for (int g = 0; g < G; ++g) mins[g][h] *= keep;
-#pragma unroll
-                    for (int m = 0; m < 2 * G; ++m) { o[m][h] *= keep; o[m][h + 2] *= keep; }
                 }
-            }
-#pragma unroll
-            for (int i = 0; i < kQdPair; ++i) {
-                const unsigned char* tile = stage + i * T::bytes;
-                const Words va = *reinterpret_cast<const Words*>(tile + T::values + (gq * 4 + t) * (4 * G)),
-                            vb = *reinterpret_cast<const Words*>(tile + T::values + (32 + gq * 4 + t) * (4 * G));
-                Metas ma = *reinterpret_cast<const Metas*>(tile + T::value_scales + T::meta_at(gq, 0)), mb = *reinterpret_cast<const Metas*>(tile + T::value_scales + T::meta_at(gq + 8, 0));
-                Metas la = *reinterpret_cast<const Metas*>(tile + T::value_mins + T::meta_at(gq, 0)), lb = *reinterpret_cast<const Metas*>(tile + T::value_mins + T::meta_at(gq + 8, 0));
-                if (part) {
-                    if (gq >= seen[i]) ma = la = Metas{};
-                    if (gq + 8 >= seen[i]) mb = lb = Metas{};
-                }
-                const unsigned *na = reinterpret_cast<const unsigned*>(&ma), *nb = reinterpret_cast<const unsigned*>(&mb);
-                const unsigned *oa = reinterpret_cast<const unsigned*>(&la), *ob = reinterpret_cast<const unsigned*>(&lb);
-                const unsigned *wa = reinterpret_cast<const unsigned*>(&va), *wb = reinterpret_cast<const unsigned*>(&vb);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) x[i][e] = q4_exp2(fmaf(x[i][e], unscale[e & 1], -top[e & 1]));
-                l[0] += x[i][0] + x[i][2];
-                l[1] += x[i][1] + x[i][3];
+                // what the operands are made of grows by as much: the sums stay, unless a group's factor would leave its range
 #pragma unroll
                 for (int g = 0; g < G; ++g) {
-                    float low = g & 1 ? q4_high(oa[g / 2]) : q4_low(oa[g / 2]), high = g & 1 ? q4_high(ob[g / 2]) : q4_low(ob[g / 2]);
-                    const float sa = g & 1 ? q4_high(na[g / 2]) : q4_low(na[g / 2]), sb = g & 1 ? q4_high(nb[g / 2]) : q4_low(nb[g / 2]);
-                    if (!kBf16) {
-                        low = fmaf(8.0f, sa, low);
-                        high = fmaf(8.0f, sb, high);
+                    const float2 f = up[g * 4];
+                    const int e0 = q4_bits(f.x) + rise[0], e1 = q4_bits(f.y) + rise[1];
+                    __syncwarp();
+                    if (gq == 0) up[g * 4] = make_float2(q4_power(min(e0, kQdMost)), q4_power(min(e1, kQdMost)));
+                    const float keep[2] = {q4_power(127 + min(kQdMost - e0, 0)), q4_power(127 + min(kQdMost - e1, 0))};
+#pragma unroll
+                    for (int m = 2 * g; m < 2 * g + 2; ++m)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) { o[m][h] *= keep[h]; o[m][h + 2] *= keep[h]; }
+                }
+                __syncwarp();
+            }
+#pragma unroll
+            for (int i0 = 0; i0 < kQdPair; i0 += kAtOnce) {
+                // a token's scales, or minima, as far as it is there
+                auto metas = [&](int i, int at, Metas& a, Metas& b) {
+                    const unsigned char* tile = stage + (i0 + i) * T::bytes;
+                    a = *reinterpret_cast<const Metas*>(tile + at + T::meta_at(gq, 0));
+                    b = *reinterpret_cast<const Metas*>(tile + at + T::meta_at(gq + 8, 0));
+                    if (part) {
+                        if (gq >= seen[i0 + i]) a = Metas{};
+                        if (gq + 8 >= seen[i0 + i]) b = Metas{};
                     }
-                    mins[g][0] = fmaf(x[i][0], low, fmaf(x[i][2], high, mins[g][0]));
-                    mins[g][1] = fmaf(x[i][1], low, fmaf(x[i][3], high, mins[g][1]));
-                    float y[4] = {x[i][0] * sa, x[i][1] * sa, x[i][2] * sb, x[i][3] * sb};
-                    unsigned b0[NP], b1[NP], a[4], b[4];
+                };
+                auto of_group = [](const Metas& m, int g) {
+                    const unsigned w = reinterpret_cast<const unsigned*>(&m)[g / 2];
+                    return g & 1 ? q4_high(w) : q4_low(w);
+                };
 #pragma unroll
-                    for (int p = 0; p < NP; ++p) { b0[p] = q4_turn(q4_part(y[0], y[1])); b1[p] = q4_turn(q4_part(y[2], y[3])); }
-                    q4_codes<kBf16>(wa[g], a);
-                    q4_codes<kBf16>(wb[g], b);
+                for (int i = 0; i < kAtOnce; ++i) {
+                    float (&p)[4] = x[i0 + i];
+                    Metas sa, sb, ma, mb;
+                    if (!kBf16) metas(i, T::value_scales, sa, sb);
+                    metas(i, T::value_mins, ma, mb);
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        if (NP == 1) {
-                            gm_mma(o[2 * g + h], {a[2 * h], a[2 * h + 1], b[2 * h], b[2 * h + 1]}, b0[0], b1[0]);
-                        } else {   // (the tensor cores cut what they add to a sum: a tile's products are summed on their own)
-                            float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                    for (int e = 0; e < 4; ++e) p[e] = q4_exp2(fmaf(p[e], unscale[e & 1], -top[e & 1]));
+                    l[0] += p[0] + p[2];
+                    l[1] += p[1] + p[3];
 #pragma unroll
-                            for (int p = NP - 1; p >= 0; --p) gm_mma(c, {a[2 * h], a[2 * h + 1], b[2 * h], b[2 * h + 1]}, b0[p], b1[p]);
+                    for (int g = 0; g < G; ++g) {
+                        float low = of_group(ma, g), high = of_group(mb, g);
+                        if (!kBf16) {
+                            low = fmaf(8.0f, of_group(sa, g), low);
+                            high = fmaf(8.0f, of_group(sb, g), high);
+                        }
+                        mins[g][0] = fmaf(p[0], low, fmaf(p[2], high, mins[g][0]));
+                        mins[g][1] = fmaf(p[1], low, fmaf(p[3], high, mins[g][1]));
+                    }
+                }
+                // p * s * 2^u as fp16 parts; where one is too large, the exponents u go down and they are made again
+                unsigned y[kAtOnce][G][NP][2];
+                for (bool again = false;; again = true) {
+                    unsigned most = 0;
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) o[2 * g + h][e] += c[e];
+                    for (int i = 0; i < kAtOnce; ++i) {
+                        const float (&p)[4] = x[i0 + i];
+                        Metas sa, sb;
+                        metas(i, T::value_scales, sa, sb);
+#pragma unroll
+                        for (int g = 0; g < G; ++g) {
+                            const float2 f = up[g * 4];
+                            const float a = of_group(sa, g), b = of_group(sb, g);
+                            float2 w0 = q4_mul2(q4_mul2(make_float2(p[0], p[1]), make_float2(a, a)), f);
+                            float2 w1 = q4_mul2(q4_mul2(make_float2(p[2], p[3]), make_float2(b, b)), f);
+#pragma unroll
+                            for (int n = 0; n < NP; ++n) { y[i][g][n][0] = q4_part(w0.x, w0.y); y[i][g][n][1] = q4_part(w1.x, w1.y); }
+                            most = __vimax3_u16x2(most, y[i][g][0][0], y[i][g][0][1]);
+                        }
+                    }
+                    if (again || !__any_sync(0xffffffffu, (most + (0x80008000u - kQdTooLarge)) & 0x80008000u)) break;
+#pragma unroll
+                    for (int g = 0; g < G; ++g) {
+                        float high[2] = {0.0f, 0.0f};
+#pragma unroll
+                        for (int i = 0; i < kAtOnce; ++i) {
+                            Metas sa, sb;
+                            metas(i, T::value_scales, sa, sb);
+#pragma unroll
+                            for (int h = 0; h < 2; ++h) high[h] = fmaxf(high[h], fmaxf(fabsf(x[i0 + i][h] * of_group(sa, g)), fabsf(x[i0 + i][h + 2] * of_group(sb, g))));
+                        }
+                        const float2 f = up[g * 4];
+                        const int was[2] = {q4_bits(f.x), q4_bits(f.y)};
+                        int now_at[2];
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+                            for (int off = 4; off < 32; off <<= 1) high[h] = fmaxf(high[h], __shfl_xor_sync(0xffffffffu, high[h], off));
+                            now_at[h] = min(was[h], 254 + kQdRoom - q4_bits(high[h]));
+                        }
+                        __syncwarp();
+                        if (gq == 0) up[g * 4] = make_float2(q4_power(now_at[0]), q4_power(now_at[1]));
+#pragma unroll
+                        for (int m = 2 * g; m < 2 * g + 2; ++m)
+#pragma unroll
+                            for (int h = 0; h < 2; ++h) {
+                                const float keep = q4_power(127 + now_at[h] - was[h]);
+                                o[m][h] *= keep;
+                                o[m][h + 2] *= keep;
+                            }
+                    }
+                    __syncwarp();
+                }
+#pragma unroll
+                for (int i = 0; i < kAtOnce; ++i) {
+                    const unsigned char* tile = stage + (i0 + i) * T::bytes;
+                    const Words va = *reinterpret_cast<const Words*>(tile + T::values + (gq * 4 + t) * (4 * G)),
+                                vb = *reinterpret_cast<const Words*>(tile + T::values + (32 + gq * 4 + t) * (4 * G));
+                    const unsigned *wa = reinterpret_cast<const unsigned*>(&va), *wb = reinterpret_cast<const unsigned*>(&vb);
+#pragma unroll
+                    for (int g = 0; g < G; ++g) {
+                        unsigned b0[NP], b1[NP], a[4], b[4];
+#pragma unroll
+                        for (int n = 0; n < NP; ++n) { b0[n] = q4_turn(y[i][g][n][0]); b1[n] = q4_turn(y[i][g][n][1]); }
+                        q4_codes<kBf16>(wa[g], a);
+                        q4_codes<kBf16>(wb[g], b);
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            if (NP == 1) {
+                                gm_mma(o[2 * g + h], {a[2 * h], a[2 * h + 1], b[2 * h], b[2 * h + 1]}, b0[0], b1[0]);
+                            } else {   // (the tensor cores cut what they add to a sum: a tile's products are summed on their own)
+                                float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                                for (int n = NP - 1; n >= 0; --n) gm_mma(c, {a[2 * h], a[2 * h + 1], b[2 * h], b[2 * h + 1]}, b0[n], b1[n]);
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) o[2 * g + h][e] += c[e];
+                            }
                         }
                     }
                 }
@@ -532,7 +622,9 @@ __global__ void __launch_bounds__(kQdThreads, kQdCtas) q4_decode_kernel(const __
             for (int h = 0; h < 2; ++h) {
                 if (2 * t + h >= sum_heads) continue;
                 float* to = sums + (warp * sum_heads + 2 * t + h) * M::row + 32 * (m >> 1) + 4 * gq + 2 * (m & 1);
-                *reinterpret_cast<float2*>(to) = make_float2(fmaf(o[m][h], kCode, mins[m >> 1][h]), fmaf(o[m][h + 2], kCode / 16.0f, mins[m >> 1][h]));
+                const float2 f = up[(m >> 1) * 4];
+                const float down = q4_power(254 - q4_bits(h ? f.y : f.x));
+                *reinterpret_cast<float2*>(to) = make_float2(fmaf(o[m][h] * down, kCode, mins[m >> 1][h]), fmaf(o[m][h + 2] * down, kCode / 16.0f, mins[m >> 1][h]));
             }
         __syncthreads();
         unit += u1 - u0;

@@ -535,7 +535,7 @@ class Q4PagedKVCache:
         return k.view(*lead, 16, 4, G), ks, km, v.view(*lead, 2, 8, 4, G), vs, vm
 
     def load(self, k_codes, k_scales, k_mins, v_codes, v_scales, v_mins) -> None:
-        """Fills the pool: codes uint8 0..15 [num_pages, kv_heads, page_size, head_dim], scales and minima bf16
+        """Fills the pool: codes uint8 0..15 [num_pages, kv_heads, page_size, head_dim], scales (not negative) and minima bf16
         [num_pages, kv_heads, page_size, head_dim / 32]."""
         G, T = self.head_dim // 32, self.page_size // 16
         lead = (self.num_pages, self.kv_heads, T)
@@ -544,6 +544,10 @@ class Q4PagedKVCache:
                                      ("v_scales", v_scales, G, torch.bfloat16), ("v_mins", v_mins, G, torch.bfloat16)):
             if tuple(t.shape) != (self.num_pages, self.kv_heads, self.page_size, last) or t.dtype != dtype:
                 raise ValueError(f"{name} must be {dtype} of shape {(self.num_pages, self.kv_heads, self.page_size, last)}")
+        for name, t in (("k_scales", k_scales), ("v_scales", v_scales)):
+            if bool((t < 0).any()):
+                raise ValueError(f"{name} must not be negative")
+        k_scales, v_scales = k_scales.abs(), v_scales.abs()      # (zeros and NaN without a sign)
         k, ks, km, v, vs, vm = self._tiles()
 
         def bytes_of(codes):    # two codes to a byte: [..., head_dim / 2]

@@ -105,3 +105,20 @@ def test_decode_of_peaked_scores_and_values_that_are_not_finite(cuda, dtype):
         bad["k_mins"][table[0, 3].long(), 0, 9, 2] = math.nan
         c.load(**bad)
         assert torch.isnan(c.decode(q, table, n)).all()
+
+
+def test_scales_with_a_sign_are_refused_or_lose_it(cuda):
+    c = ops.Q4PagedKVCache(2, 16, 1, 1, 64)
+    pool = random_pool(c, _gen(22))
+    for name in ("k_scales", "v_scales"):
+        kept = c.pool.clone()
+        with pytest.raises(ValueError):
+            c.load(**{**pool, name: -pool[name]})
+        assert torch.equal(c.pool, kept)
+        zero = pool[name].clone()
+        zero[0, 0, 3], zero[1, 0, 5, 1] = 0.0, math.nan
+        c.load(**{**pool, name: zero})
+        kept = c.pool.clone()
+        zero[0, 0, 3] = -0.0
+        c.load(**{**pool, name: zero})
+        assert torch.equal(c.pool, kept) and not bool((c.unload()[name].view(torch.int16) < 0).any())

@@ -145,9 +145,9 @@ int num_sms();
 #ifdef __CUDACC__
 // Waits for a phase of an mbarrier (shared-space address) for at most about an eighth of a second: between the warps of a CTA a
 // phase takes microseconds, and a wait that has not ended by then never will.  False: it ran out.  gone: shared-space address
-// of a word that such a wait sets and that makes the others on it give up at once (0: none).
+// of a word that such a wait sets and that makes the others on it give up at once (0: none).  clocks: another limit, for what takes longer.
 constexpr long long kBarClocks = 1LL << 28;
-__device__ __forceinline__ bool bar_wait(unsigned bar, unsigned parity, unsigned gone = 0) {
+__device__ __forceinline__ bool bar_wait(unsigned bar, unsigned parity, unsigned gone = 0, long long clocks = kBarClocks) {
     long long begin = 0;
     for (bool first = true;; first = false) {
         unsigned done;
@@ -166,7 +166,7 @@ __device__ __forceinline__ bool bar_wait(unsigned bar, unsigned parity, unsigned
         }
         const long long now = clock64();
         if (first) begin = now;
-        else if (now - begin > kBarClocks) {
+        else if (now - begin > clocks) {
             if (gone != 0) asm volatile("st.volatile.shared.s32 [%0], %1;" ::"r"(gone), "r"(1) : "memory");
             return false;
         }

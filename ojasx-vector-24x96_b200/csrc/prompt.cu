@@ -41,6 +41,7 @@ struct PromptProblem {
 // 128 take 524 us, 1050 TFLOP/s.  Products issued by a warp as a whole with an elected lane, and not by one lane in a branch: 610 -> 562.
 constexpr int kPaRows = 128, kPaKeys = 64, kPaThreads = 384;
 constexpr float kPaSlack = 8.0f;
+constexpr long long kPaPartClocks = 1LL << 35;   // 18 s: a step of 64 keys takes a microsecond, and 10^9 keys do not fit into the memory
 
 template <int HD>
 struct PaSmem {
@@ -211,10 +212,12 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_tc_kernel(const __grid_c
     const unsigned tmem = __shfl_sync(0xffffffffu, s_tmem, 0);
     bool ok = true;
     auto wait = [&](unsigned bar, unsigned parity) { return tc_wait(bar, parity, gone); };
+    // For the end of what another warp does with all keys of a part: its own waits end soon, and this one with them.
+    auto wait_part = [&](unsigned bar, unsigned parity) { return tc_wait(bar, parity, gone, kPaPartClocks); };
     // Item `number` of the CTA, as warp 11 has put it down; false behind the last one (or where a wait ran out).
     struct { int row, key, ahead, head, pos[2], live[2], steps[2], n; } item;   // first row and key; first position, positions and steps of the tiles
     auto take = [&](int number) {
-        if (!(ok = wait(item_full + 8 * (number & 1), (number >> 1) & 1))) return false;
+        if (!(ok = wait_part(item_full + 8 * (number & 1), (number >> 1) & 1))) return false;
         const int4 a = *reinterpret_cast<const int4*>(s_item[number & 1]), b = *reinterpret_cast<const int4*>(s_item[number & 1] + 4);
         __syncwarp();
         if (lane == 0) tc_bar_arrive(item_empty + 8 * (number & 1));
@@ -263,7 +266,7 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_tc_kernel(const __grid_c
                         tc_bar_arrive(item_full + 8 * (number & 1));
                     }
                     __syncwarp();
-                    if (cta < 0 || !(ok = wait(want, number & 1))) break;
+                    if (cta < 0 || !(ok = wait_part(want, number & 1))) break;
                     ++number;
                 }
                 if constexpr (kShares) {   // (the CTAs of a cluster stay at one part)
@@ -421,7 +424,7 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_tc_kernel(const __grid_c
         for (int number = 0;; ++number) {
             // (read again where it is needed: registers are short between)
             const volatile int* const what = s_item[number & 1];
-            if (!(ok = wait(item_full + 8 * (number & 1), (number >> 1) & 1)) || what[0] < 0) break;
+            if (!(ok = wait_part(item_full + 8 * (number & 1), (number >> 1) & 1)) || what[0] < 0) break;
             int steps, last, first, n;   // of the tile; last key that the row sees, and that the tile's first row sees; steps of both tiles
             {
                 const int pos = what[4] + i * per, live = what[5 + i], ahead = what[2], end = pos + live + ahead;

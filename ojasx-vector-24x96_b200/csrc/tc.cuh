@@ -18,10 +18,10 @@ __device__ __forceinline__ void tc_bar_expect(unsigned bar, unsigned bytes) {
 }
 
 // Waits of a warp for a phase: one look where it is there already, else as bar_wait waits.  False: it ran out.
-__device__ __forceinline__ bool tc_wait(unsigned bar, unsigned parity, unsigned gone) {
+__device__ __forceinline__ bool tc_wait(unsigned bar, unsigned parity, unsigned gone, long long clocks = kBarClocks) {
     unsigned done;
     asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(done) : "r"(bar), "r"(parity) : "memory");
-    return __all_sync(0xffffffffu, done) || __all_sync(0xffffffffu, bar_wait(bar, parity, gone));
+    return __all_sync(0xffffffffu, done) || __all_sync(0xffffffffu, bar_wait(bar, parity, gone, clocks));
 }
 // Asks for a CTA of the grid that has not begun, to do its work in its place: 16 bytes at `to` and on `bar` (whose transaction count
 // the caller raises); then its number, or -1 where there is none any more (after which nothing may be asked again).

@@ -121,7 +121,7 @@ OJASX_API int ojasx_b200_linear_forward_tensor(OjasxLinearHandle handle, const v
  * and did nothing.  Bit 2: a bounded wait for a bulk copy of a lookup table ran out, or a whole-expert
  * MoE kernel of the chain walk found the same placement and did nothing.  Bit 3: a kernel that walks four
  * vectors at a time gave up on a wait (its results are NaN) or found that placement.  Bit 4: a launch of
- * attention over prompts gave up on a wait; bit 5: one over the 4-bit cache.  Negative = CUDA error. */
+ * attention over prompts gave up on a wait; bit 5: one over the 4-bit cache (what they did not finish is NaN).  Negative = CUDA error. */
 OJASX_API int ojasx_b200_take_device_error(void);
 
 /* Same computation on borrowed device arrays, no handle: the device twin of

@@ -49,4 +49,14 @@ __device__ __forceinline__ bool packed_part(int batch, int index, Parts parts, i
     return false;
 }
 
+// NaN for results that a launch gave up on: `heads` heads from `head` on of `rows` rows from `row` on of a [.., all_heads, HD] tensor.
+// `thread` of `threads` that call it.
+template <int HD, class T>
+__device__ __forceinline__ void packed_give_up(T* out, size_t row, int rows, int head, int heads, int all_heads, int thread, int threads) {
+    for (int i = thread; i < rows * heads * HD; i += threads) {
+        const int r = i / (heads * HD);
+        out[((row + r) * all_heads + head) * HD + i - r * (heads * HD)] = T(__int_as_float(0x7fffffff));
+    }
+}
+
 }  // namespace ojx

@@ -170,7 +170,7 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_tc_kernel(const __grid_c
     unsigned char* smem = pa_raw + ((1024u - (tc_smem(pa_raw) & 1023u)) & 1023u);
     __shared__ int s_gone, s_odd[2][2];   // s_odd: of either S of a tile, since its rows may be a step ahead of the products
     __shared__ unsigned s_tmem;
-    __shared__ __align__(16) int s_item[2][8];
+    __shared__ __align__(16) int s_item[3][8];   // two in turn, and one that was found when a wait had run out
     __shared__ __align__(16) int s_stolen[4];
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;   // (the same for a warp, as the compiler sees)
     const unsigned base = tc_smem(smem), bars = base + M::bars;
@@ -193,6 +193,7 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_tc_kernel(const __grid_c
             tc_bar_init(item_full + 8 * i, 1);
             tc_bar_init(item_empty + 8 * i, 10);
             s_odd[i][0] = s_odd[i][1] = 0;
+            s_item[i][0] = s_item[2][0] = -1;
         }
         tc_bar_init(want, 1);
         tc_bar_init(steal, 1);
@@ -241,12 +242,13 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_tc_kernel(const __grid_c
             const int size = kShares ? pa_cluster_size() : 1, rank = kShares ? pa_cluster_rank() : 0;
             int cta = kShares ? (int)blockIdx.x / size : (int)blockIdx.x, number = 0;
             unsigned asked = 0;
-            while (ok) {
+            bool room = true;   // false: a wait ran out
+            for (;;) {
                 int seq = -1, part = 0;
                 const bool in = cta >= 0 && packed_part(P.batch, (int)((kShares ? gridDim.x / size : gridDim.x) / P.kv_heads) - 1 - cta / P.kv_heads,
                                                         [&](int b) { return (packed_range(P.ends, b, P.n_rows).count + 2 * per - 1) / (2 * per); }, seq, part);
                 if (in || cta < 0) {
-                    if (number >= 2 && !(ok = wait(item_empty + 8 * (number & 1), ((number >> 1) - 1) & 1))) break;
+                    room = room && (number < 2 || wait(item_empty + 8 * (number & 1), ((number >> 1) - 1) & 1));
                     if (lane == 0) {
                         int4 a = make_int4(-1, 0, 0, 0), b = make_int4(0, 0, 0, 0);
                         if (in) {
@@ -261,14 +263,16 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_tc_kernel(const __grid_c
                                 b.w = share.count;
                             }
                         }
-                        *reinterpret_cast<int4*>(s_item[number & 1]) = a;
-                        *reinterpret_cast<int4*>(s_item[number & 1] + 4) = b;
-                        tc_bar_arrive(item_full + 8 * (number & 1));
+                        int* const to = s_item[room ? number & 1 : 2];
+                        *reinterpret_cast<int4*>(to) = a;
+                        *reinterpret_cast<int4*>(to + 4) = b;
+                        if (room) tc_bar_arrive(item_full + 8 * (number & 1));
                     }
                     __syncwarp();
-                    if (cta < 0 || !(ok = wait_part(want, number & 1))) break;
+                    if (!(ok = room) || cta < 0 || !(ok = wait_part(want, number & 1))) break;
                     ++number;
                 }
+                if (!(ok = room)) break;
                 if constexpr (kShares) {   // (the CTAs of a cluster stay at one part)
                     cta = -1;
                     continue;
@@ -279,8 +283,9 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_tc_kernel(const __grid_c
                     tc_steal(tc_smem(s_stolen), steal);
                 }
                 __syncwarp();
-                if (!(ok = wait(steal, asked & 1))) {   // nothing may land after the CTA has left
-                    bar_wait(steal, asked & 1);
+                room = wait(steal, asked & 1);
+                if (!room && !__all_sync(0xffffffffu, bar_wait(steal, asked & 1))) {   // nothing may land after the CTA has left
+                    ok = false;
                     break;
                 }
                 ++asked;
@@ -626,6 +631,12 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_tc_kernel(const __grid_c
         if (warp < 8 && what[0] >= 0) pa_join<HD, true>(P, smem, what[0] + what[4], what[3], per, what[5], what[6], 1.0f);
         pa_cluster_sync();   // nobody leaves while its sums may still be read
     }
+    if (*reinterpret_cast<volatile int*>(&s_gone) && threadIdx.x < 256)   // what the CTA had last and before, and what it took from another one
+        for (int i = 0; i < 3; ++i) {
+            const volatile int* const what = s_item[i];
+            if (what[0] >= 0)
+                packed_give_up<HD>(static_cast<__nv_bfloat16*>(P.out), (size_t)(what[0] + what[4]), what[5] + what[6], what[3] * P.share, P.share, P.q_heads, threadIdx.x, 256);
+        }
 }
 
 // CTAs that share the keys of a part of the rows: as many as the GPU holds next to one another, with four steps of keys each on average.  The
@@ -1154,6 +1165,12 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_pair_kernel(const __grid
         pa_cluster_sync();   // the sums of every share are in place
         if (warp < 8) pa_join<HD, false>(P, smem, rows.first + pos[0], head, per, live[0], live[1], 16384.0f);
         pa_cluster_sync();   // nobody leaves while its sums may still be read
+    }
+    if (*reinterpret_cast<volatile int*>(&s_gone) && threadIdx.x < 256) {
+        const PackedRange of = packed_range(P.ends, s_seq, P.n_rows);
+        const int first = s_part * 2 * (kPaRows / P.share), share = P.share;
+        packed_give_up<HD>(static_cast<float*>(P.out), (size_t)(of.first + first), min(2 * (kPaRows / share), of.count - first),
+                           (int)blockIdx.x / (kShares ? pa_cluster_size() : 1) % P.kv_heads * share, share, P.q_heads, threadIdx.x, 256);
     }
 }
 

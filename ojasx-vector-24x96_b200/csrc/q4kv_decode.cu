@@ -614,7 +614,7 @@ __global__ void __launch_bounds__(kQdThreads, kQdCtas) q4_decode_kernel(const __
             }
         if (gq == 0) {
 #pragma unroll
-            for (int h = 0; h < 2; ++h) { s_m[warp][2 * t + h] = top[h]; s_l[warp][2 * t + h] = l[h]; }
+            for (int h = 0; h < 2; ++h) { s_m[warp][2 * t + h] = top[h]; s_l[warp][2 * t + h] = ok ? l[h] : NAN; }   // (a wait ran out: no result)
         }
 #pragma unroll
         for (int m = 0; m < 2 * G; ++m)

@@ -401,14 +401,15 @@ OJASX_API int ojasx_b200_paged_kv_decode(const void* d_q, void* d_out, const int
  * scale (the smallest not below (max - minimum) / 15); a value is a code 0..15 and reads as code * scale + minimum, within half a
  * scale of what it was.  A group that holds an infinity or a NaN reads as NaN.
  * d_block_table [batch, max_pages] int32 names the pages of every sequence.  Entries outside [0, num_pages) are no page: tokens
- * there are dropped by an append, read as zeros and weigh nothing in a decode, and *status becomes 1; so it is with tokens beyond
- * max_pages, and a sequence with a negative position is left out as a whole.
+ * there are dropped by an append, read as zeros and weigh nothing in a decode or a prefill, and *status becomes 1; so it is with
+ * tokens beyond max_pages, and a sequence with a negative position is left out as a whole.
  *
  * append: token i of d_k, d_v [n_tokens, kv_heads, head_dim] goes to its place behind the d_positions[b] tokens of its sequence.
  * d_ends [batch + 1]: the tokens of sequence b are d_ends[b] .. d_ends[b + 1] - 1 (tokens behind the last one are left alone); NULL:
  * one token per sequence.  Keys, and the queries d_q [n_tokens, q_heads, head_dim] if there are any, are turned on the way where the
  * cache has `turns`; the queries go to d_q_out.
- * read: tokens d_positions[b] (NULL: 0) and on of every sequence into d_k, d_v, packed as d_ends says.
+ * read: tokens d_positions[b] (NULL: 0) and on of every sequence into d_k, d_v, packed as d_ends says.  read_marked also says in d_none
+ * (a byte per token, 16-byte aligned, NULL: not wanted) which of them have no page (1, else 0): attention over what was read takes it.
  * decode: one query per sequence, d_q, d_out [batch, q_heads, head_dim], over its first d_lengths[b] tokens; a length of zero gives
  * zeros; scale <= 0 means 1/sqrt(head_dim).  Values up to 2^100.  workspace: ojasx_b200_q4kv_decode_workspace bytes for this call.
  * None of them waits for the GPU; lengths, positions and tables are read on the device, so the calls can be captured in a graph. */
@@ -424,6 +425,9 @@ OJASX_API int ojasx_b200_q4kv_append(const OjasxQ4Cache* cache, const void* d_k,
                                      const int* d_positions, const int* d_ends, int n_tokens, int batch, int io_dtype, void* stream);
 OJASX_API int ojasx_b200_q4kv_read(const OjasxQ4Cache* cache, const int* d_block_table, int max_pages, const int* d_ends,
                                    const int* d_positions, void* d_k, void* d_v, int n_tokens, int batch, int io_dtype, void* stream);
+OJASX_API int ojasx_b200_q4kv_read_marked(const OjasxQ4Cache* cache, const int* d_block_table, int max_pages, const int* d_ends,
+                                          const int* d_positions, void* d_k, void* d_v, unsigned char* d_none, int n_tokens, int batch,
+                                          int io_dtype, void* stream);
 OJASX_API size_t ojasx_b200_q4kv_decode_workspace(const OjasxQ4Cache* cache, int batch, int max_pages, int io_dtype);
 OJASX_API int ojasx_b200_q4kv_decode(const OjasxQ4Cache* cache, const void* d_q, void* d_out, const int* d_block_table, int max_pages,
                                      const int* d_lengths, int batch, float scale, int io_dtype, void* workspace, size_t workspace_bytes,
@@ -433,13 +437,20 @@ OJASX_API int ojasx_b200_q4kv_decode(const OjasxQ4Cache* cache, const void* d_q,
  * d_key_ends[b] .. belong to sequence b, whose last query sees its last key, the one before it the keys up to the one before, and so
  * on; a query that sees nothing gives zeros; rows behind the last sequence are left as they were.  Keys that a query does not see
  * have no part in its result, whatever they hold.  fp32 values up to 2^100.  workspace: ojasx_b200_prompt_workspace bytes (0 for bf16) for this call alone,
- * 256-byte aligned; the others 16-byte aligned, strides whole multiples of 16 bytes. */
+ * 256-byte aligned; the others 16-byte aligned, strides whole multiples of 16 bytes.
+ * _marked: d_none [n_keys] bytes (NULL: none) are not zero for keys that no query sees, of the caches' tokens without a page those;
+ * it is read in pieces of 16 bytes, the last of which ends behind n_keys. */
 OJASX_API size_t ojasx_b200_prompt_workspace(int n_keys, int kv_heads, int head_dim, int io_dtype);
 OJASX_API int ojasx_b200_prompt_attention(const void* d_q, long long q_row, long long q_head, const void* d_k, long long k_row,
                                           long long k_head, const void* d_v, long long v_row, long long v_head, void* d_out,
                                           const int* d_ends, const int* d_key_ends, int batch, int n_rows, int n_keys, int q_heads,
                                           int kv_heads, int head_dim, float scale, int io_dtype, void* workspace,
                                           size_t workspace_bytes, void* stream);
+OJASX_API int ojasx_b200_prompt_attention_marked(const void* d_q, long long q_row, long long q_head, const void* d_k, long long k_row,
+                                                 long long k_head, const void* d_v, long long v_row, long long v_head, void* d_out,
+                                                 const int* d_ends, const int* d_key_ends, const unsigned char* d_none, int batch, int n_rows,
+                                                 int n_keys, int q_heads, int kv_heads, int head_dim, float scale, int io_dtype,
+                                                 void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

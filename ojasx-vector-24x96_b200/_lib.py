@@ -130,10 +130,12 @@ SIGNATURES = {
     "ojasx_b200_q4kv_page_bytes": (_sz, [_i, _i, _i]),
     "ojasx_b200_q4kv_append": (_i, [_vp, _vp, _ll, _vp, _ll, _vp, _ll, _vp, _vp, _i, _vp, _vp, _i, _i, _i, _vp]),
     "ojasx_b200_q4kv_read": (_i, [_vp, _vp, _i, _vp, _vp, _vp, _vp, _i, _i, _i, _vp]),
+    "ojasx_b200_q4kv_read_marked": (_i, [_vp, _vp, _i, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _vp]),
     "ojasx_b200_q4kv_decode_workspace": (_sz, [_vp, _i, _i, _i]),
     "ojasx_b200_q4kv_decode": (_i, [_vp, _vp, _vp, _vp, _i, _vp, _i, _f, _i, _vp, _sz, _vp]),
     "ojasx_b200_prompt_workspace": (_sz, [_i] * 4),
     "ojasx_b200_prompt_attention": (_i, [_vp, _ll, _ll] * 3 + [_vp] * 3 + [_i] * 6 + [_f, _i, _vp, _sz, _vp]),
+    "ojasx_b200_prompt_attention_marked": (_i, [_vp, _ll, _ll] * 3 + [_vp] * 4 + [_i] * 6 + [_f, _i, _vp, _sz, _vp]),
 }
 
 _lib = None

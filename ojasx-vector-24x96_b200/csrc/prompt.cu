@@ -19,6 +19,7 @@ struct PromptProblem {
     void* out;                                     // [n_rows][q_heads][head_dim]
     long long q_row, q_head, k_row, k_head, v_row, v_head;   // strides in elements
     const int *ends, *key_ends;
+    const unsigned char* none;                     // [n_keys, up to a multiple of 16] or null: not zero for keys that nobody sees
     int batch, n_rows, n_keys, q_heads, kv_heads, share;
     float scale;
 };
@@ -161,7 +162,8 @@ __device__ __forceinline__ void pa_join(const PromptProblem& P, const unsigned c
     }
 }
 
-template <int HD, bool kShares>
+// kHoles: P.none may name keys.  In a kernel of its own, since the test of it in every step costs the others 2 to 6 %.
+template <int HD, bool kShares, bool kHoles>
 __global__ void __launch_bounds__(kPaThreads, 1) prompt_tc_kernel(const __grid_constant__ PromptProblem P, const __grid_constant__ CUtensorMap q_map,
                                                                   const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map) {
     using M = PaSmem<HD>;
@@ -440,6 +442,16 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_tc_kernel(const __grid_c
                 n = max(steps, other > 0 ? max(0, to + kPaKeys - 1) / kPaKeys : 0);
                 if (kShares) steps = min(steps, what[7]);   // (n is for the parts behind this one, and there are none)
             }
+            bool holes = false;   // keys among the tile's that nobody sees (or some of the 15 before and behind them, as they are read)
+            if constexpr (kHoles) {
+                unsigned some = 0;
+                const long long to = min((long long)what[1] + steps * kPaKeys, (long long)P.n_keys);
+                for (long long key = (what[1] & ~15) + 16 * lane; key < to; key += 512) {
+                    const uint4 x = *reinterpret_cast<const uint4*>(P.none + key);
+                    some |= x.x | x.y | x.z | x.w;
+                }
+                holes = __any_sync(0xffffffffu, some != 0);
+            }
             float top = 0.0f;
             unsigned long long sum2[2] = {0, 0};
             for (int j = 0; j < steps; ++j) {
@@ -455,10 +467,20 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_tc_kernel(const __grid_c
                 tc_pin32(s);
                 tc_pin32(s + 32);
                 const bool masked = (j + 1) * kPaKeys - 1 > first;   // some row does not see all of these keys
-                if (masked) {
-                    const int see = last - j * kPaKeys;
+                if (kHoles ? masked || holes : masked) {
+                    const int see = masked ? last - j * kPaKeys : kPaKeys;
+                    if constexpr (kHoles) {
+                        const long long key = (long long)what[1] + j * kPaKeys + lane;
+                        unsigned long long not_seen = see < 0 ? ~0ull : see < 63 ? ~0ull << (see + 1) : 0ull;
+                        if (holes)
+                            not_seen |= __ballot_sync(0xffffffffu, key < P.n_keys && P.none[key]) |
+                                        (unsigned long long)__ballot_sync(0xffffffffu, key + 32 < P.n_keys && P.none[key + 32]) << 32;
 #pragma unroll
-                    for (int e = 0; e < 64; ++e) s[e] = e > see ? 0xff800000u : s[e];
+                        for (int e = 0; e < 64; ++e) s[e] = not_seen >> e & 1u ? 0xff800000u : s[e];
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 64; ++e) s[e] = e > see ? 0xff800000u : s[e];
+                    }
                 }
                 float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
@@ -654,7 +676,7 @@ static_assert(kPaKeys == 64, "steps of keys");
 
 template <int HD>
 static int launch_prompt_tc(const PromptProblem& P, cudaStream_t s) {
-    static std::atomic<bool> opted[2][64];
+    static std::atomic<bool> opted[4][64];
     constexpr int smem = PaSmem<HD>::bytes;
     static_assert(PaParts<HD>::bytes <= PaSmem<HD>::bars, "the sums of the rows lie where Q, K and V were");
     const int per = kPaRows / P.share;
@@ -669,8 +691,9 @@ static int launch_prompt_tc(const PromptProblem& P, cudaStream_t s) {
         return OJX_ERR_ARG;
     }
     const int shares = prompt_shares(P, parts * P.kv_heads, true);
-    auto kernel = shares > 1 ? prompt_tc_kernel<HD, true> : prompt_tc_kernel<HD, false>;
-    OJX_CUDA_TRY(opt_in_smem(reinterpret_cast<const void*>(kernel), smem, opted[shares > 1]));
+    auto kernel = P.none ? (shares > 1 ? prompt_tc_kernel<HD, true, true> : prompt_tc_kernel<HD, false, true>)
+                         : (shares > 1 ? prompt_tc_kernel<HD, true, false> : prompt_tc_kernel<HD, false, false>);
+    OJX_CUDA_TRY(opt_in_smem(reinterpret_cast<const void*>(kernel), smem, opted[(shares > 1) + 2 * (P.none != nullptr)]));
     if (shares > 1) OJX_CUDA_TRY(launch_chained_cluster(kernel, dim3((unsigned)(parts * P.kv_heads * shares)), kPaThreads, smem, s, (unsigned)shares, P, q, k, v));
     else OJX_CUDA_TRY(launch_chained(kernel, dim3((unsigned)(parts * P.kv_heads)), kPaThreads, smem, s, P, q, k, v));
     count_launch(1);
@@ -738,7 +761,7 @@ __global__ void __launch_bounds__(256) prompt_split_kernel(const __grid_constant
     if (values) {
         const int p = min(max((int)(most >> 23) - 127, -20), 100);
         up = __uint_as_float((unsigned)(127 + 14 - p) << 23);
-        e = (float)p;
+        e = P.none && P.none[key] ? -INFINITY : (float)p;   // a key that nobody sees: its scores, which e is added to, are -inf
     } else {
         gm_scale(most, up, down);
     }
@@ -856,7 +879,7 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_pair_kernel(const __grid
                     const float2 x = key < keys.count ? S.factors[(size_t)head * P.n_keys + keys.first + key] : make_float2(0.0f, 0.0f);
                     f[c] = x.x;
                     f[N + c] = x.y;
-                    f[2 * N + c] = __uint_as_float((unsigned)(127 - (int)x.y) << 23);
+                    f[2 * N + c] = x.y == -INFINITY ? 1.0f : __uint_as_float((unsigned)(127 - (int)x.y) << 23);
                 }
                 tc_bar_arrive(f_full + 8 * (j & 1));
             }
@@ -1236,6 +1259,14 @@ int ojasx_b200_prompt_attention(const void* d_q, long long q_row, long long q_he
                                 const void* d_v, long long v_row, long long v_head, void* d_out, const int* d_ends, const int* d_key_ends,
                                 int batch, int n_rows, int n_keys, int q_heads, int kv_heads, int head_dim, float scale, int io_dtype,
                                 void* workspace, size_t workspace_bytes, void* stream) {
+    return ojasx_b200_prompt_attention_marked(d_q, q_row, q_head, d_k, k_row, k_head, d_v, v_row, v_head, d_out, d_ends, d_key_ends, nullptr, batch, n_rows,
+                                              n_keys, q_heads, kv_heads, head_dim, scale, io_dtype, workspace, workspace_bytes, stream);
+}
+
+int ojasx_b200_prompt_attention_marked(const void* d_q, long long q_row, long long q_head, const void* d_k, long long k_row, long long k_head,
+                                       const void* d_v, long long v_row, long long v_head, void* d_out, const int* d_ends, const int* d_key_ends,
+                                       const unsigned char* d_none, int batch, int n_rows, int n_keys, int q_heads, int kv_heads, int head_dim,
+                                       float scale, int io_dtype, void* workspace, size_t workspace_bytes, void* stream) {
     if (!d_q || (n_keys > 0 && (!d_k || !d_v)) || !d_out || !d_ends || !d_key_ends || batch <= 0 || n_rows < 0 || n_keys < 0 || kv_heads <= 0 ||
         q_heads <= 0 || q_heads % kv_heads)
         return OJX_ERR_ARG;
@@ -1243,7 +1274,7 @@ int ojasx_b200_prompt_attention(const void* d_q, long long q_row, long long q_he
     const int unit = io_dtype == OJX_F32 ? 4 : 8;   // elements of 16 bytes
     for (const long long stride : {q_row, q_head, k_row, k_head, v_row, v_head})
         if (stride < 0 || stride % unit) return OJX_ERR_ARG;
-    for (const void* p : {d_q, d_k, d_v, static_cast<const void*>(d_out)})
+    for (const void* p : {d_q, d_k, d_v, static_cast<const void*>(d_out), static_cast<const void*>(d_none)})
         if (reinterpret_cast<uintptr_t>(p) & 15) return OJX_ERR_ARG;
     if ((head_dim != 64 && head_dim != 128) || q_heads / kv_heads > 64) return OJX_ERR_UNSUPPORTED;
     const size_t need = ojasx_b200_prompt_workspace(n_keys, kv_heads, head_dim, io_dtype);
@@ -1252,7 +1283,7 @@ int ojasx_b200_prompt_attention(const void* d_q, long long q_row, long long q_he
     PromptProblem P{};
     P.q = d_q; P.k = d_k; P.v = d_v; P.out = d_out;
     P.q_row = q_row; P.q_head = q_head; P.k_row = k_row; P.k_head = k_head; P.v_row = v_row; P.v_head = v_head;
-    P.ends = d_ends; P.key_ends = d_key_ends; P.batch = batch; P.n_rows = n_rows; P.n_keys = n_keys;
+    P.ends = d_ends; P.key_ends = d_key_ends; P.none = d_none; P.batch = batch; P.n_rows = n_rows; P.n_keys = n_keys;
     P.q_heads = q_heads; P.kv_heads = kv_heads; P.share = q_heads / kv_heads;
     P.scale = scale > 0.0f ? scale : 1.0f / sqrtf((float)head_dim);
     const cudaStream_t s = static_cast<cudaStream_t>(stream);

@@ -322,6 +322,7 @@ struct Q4ReadProblem {
     Q4Cache cache;
     void *k, *v;                // [n_tokens][kv_heads][head_dim]
     const int *ends, *positions;   // positions null: from the first token
+    unsigned char* none;        // [n_tokens] or null: 1 for a token without a page, 0 for the others
     int n_tokens, batch;
 };
 
@@ -352,6 +353,7 @@ __global__ void __launch_bounds__(256) q4_read_kernel(const __grid_constant__ Q4
     } else if (threadIdx.x == 0) {
         atomicExch(P.cache.status, 1);
     }
+    if (P.none && blockIdx.y == 0 && threadIdx.x >= S.from && threadIdx.x < S.to) P.none[S.row + threadIdx.x] = tile ? 0 : 1;
     __syncthreads();
     // eight dimensions of a token and head per thread
     constexpr int E = HD / 8, R = 256 / (2 * kQ4ReadHeads * E);   // R: tokens at a time
@@ -443,14 +445,19 @@ int ojasx_b200_q4kv_append(const OjasxQ4Cache* cache, const void* d_k, long long
 
 int ojasx_b200_q4kv_read(const OjasxQ4Cache* cache, const int* d_block_table, int max_pages, const int* d_ends, const int* d_positions, void* d_k,
                          void* d_v, int n_tokens, int batch, int io_dtype, void* stream) {
+    return ojasx_b200_q4kv_read_marked(cache, d_block_table, max_pages, d_ends, d_positions, d_k, d_v, nullptr, n_tokens, batch, io_dtype, stream);
+}
+
+int ojasx_b200_q4kv_read_marked(const OjasxQ4Cache* cache, const int* d_block_table, int max_pages, const int* d_ends, const int* d_positions,
+                                void* d_k, void* d_v, unsigned char* d_none, int n_tokens, int batch, int io_dtype, void* stream) {
     const int rc = q4_check(cache, d_block_table, max_pages, batch, io_dtype);
     if (rc != OJX_OK) return rc;
-    if (!d_ends || !d_k || !d_v || n_tokens < 0 || !q4_aligned(d_k) || !q4_aligned(d_v)) return OJX_ERR_ARG;
+    if (!d_ends || !d_k || !d_v || n_tokens < 0 || !q4_aligned(d_k) || !q4_aligned(d_v) || !q4_aligned(d_none)) return OJX_ERR_ARG;
     const int kv_heads = cache->kv_heads, head_dim = cache->head_dim;
     if (n_tokens == 0) return OJX_OK;
     Q4ReadProblem P{};
     P.cache = q4_cache(cache, d_block_table, max_pages);
-    P.k = d_k; P.v = d_v; P.ends = d_ends; P.positions = d_positions; P.n_tokens = n_tokens; P.batch = batch;
+    P.k = d_k; P.v = d_v; P.ends = d_ends; P.positions = d_positions; P.none = d_none; P.n_tokens = n_tokens; P.batch = batch;
     const bool bf = io_dtype == OJX_BF16;
     auto kernel = head_dim == 64 ? (bf ? q4_read_kernel<64, true> : q4_read_kernel<64, false>)
                                  : (bf ? q4_read_kernel<128, true> : q4_read_kernel<128, false>);

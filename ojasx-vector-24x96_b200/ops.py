@@ -609,6 +609,10 @@ class Q4PagedKVCache:
              dtype: torch.dtype = torch.bfloat16):
         """(k, v) [tokens, kv_heads, head_dim]: the values of ``cu_seqlens[b + 1] - cu_seqlens[b]`` tokens of every sequence, from
         ``positions[b]`` (default 0) on.  Rows behind the last sequence are not written."""
+        return self._read(block_table, cu_seqlens, tokens, positions, dtype)
+
+    def _read(self, block_table, cu_seqlens, tokens, positions, dtype, none: Optional[torch.Tensor] = None):
+        """``none``: a byte per token that becomes 1 where the token has no page."""
         table, B, dev = self._table(block_table), block_table.shape[0], self.device
         ends = _index32(cu_seqlens, "cu_seqlens", (B + 1,), dev)
         at = None if positions is None else _index32(positions, "positions", (B,), dev)
@@ -618,8 +622,8 @@ class Q4PagedKVCache:
         v = torch.empty_like(k)
         if tokens and B:
             with _on_device(dev):
-                rc = lib().ojasx_b200_q4kv_read(self._cache, table, block_table.shape[1], ends, at, k.data_ptr(), v.data_ptr(), int(tokens), B,
-                                                _DTYPE_CODES[dtype], _stream_ptr(dev))
+                rc = lib().ojasx_b200_q4kv_read_marked(self._cache, table, block_table.shape[1], ends, at, k.data_ptr(), v.data_ptr(),
+                                                       None if none is None else none.data_ptr(), int(tokens), B, _DTYPE_CODES[dtype], _stream_ptr(dev))
             if rc:
                 check(rc, "ojasx_b200_q4kv_read")
         return k, v
@@ -654,11 +658,13 @@ class Q4PagedKVCache:
                 cu_seqlens: torch.Tensor, cu_context: torch.Tensor, context_tokens: int, scale: float = -1.0,
                 out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """A chunk of every sequence's prompt, packed by ``cu_seqlens``: its keys and values are appended and every query attends to the
-        cached tokens up to its own, as the cache holds them.  ``cu_context`` int32 [batch + 1]: the tokens of the sequences with the
+        cached tokens up to its own, as the cache holds them (tokens without a page weigh nothing; rows of a sequence whose position is
+        negative hold nothing).  ``cu_context`` int32 [batch + 1]: the tokens of the sequences with the
         chunk, ends of ``positions[b] + chunk`` each; ``context_tokens``: their sum."""
         turned = self.append(k, v, block_table, positions, q=q, cu_seqlens=cu_seqlens)
-        keys, values = self.read(block_table, cu_context, context_tokens, dtype=q.dtype)
-        return prompt_attention(turned, keys, values, cu_seqlens, cu_context, scale=scale, out=out)
+        none = self.pool.new_empty((int(context_tokens) + 15) // 16 * 16)
+        keys, values = self._read(block_table, cu_context, context_tokens, None, q.dtype, none)
+        return _prompt_attention(turned, keys, values, cu_seqlens, cu_context, scale, out, none.data_ptr())
 
 
 def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor, cu_keys: Optional[torch.Tensor] = None,
@@ -667,6 +673,10 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     bfloat16, head_dim 64 or 128.  Sequence b has the rows ``cu_seqlens[b] .. cu_seqlens[b + 1]`` and the keys ``cu_keys[b] ..``
     (default: the same); its last query sees its last key, the one before it the keys up to the one before, and so on.  A query that
     sees nothing gives zeros; rows behind the last sequence are not written; ``scale <= 0`` is 1/sqrt(head_dim)."""
+    return _prompt_attention(q, k, v, cu_seqlens, cu_keys, scale, out, None)
+
+
+def _prompt_attention(q, k, v, cu_seqlens, cu_keys, scale, out, none):
     if q.dim() != 3 or k.dim() != 3 or k.shape[1] == 0 or q.shape[1] % k.shape[1]:
         raise ValueError("q must be [tokens, q_heads, head_dim] and k [keys, kv_heads, head_dim], q_heads a multiple of kv_heads")
     T, Hq, hd = q.shape
@@ -695,9 +705,9 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
             size = lib().ojasx_b200_prompt_workspace(M, Hkv, hd, F32)
             ws = torch.empty(size, device=dev, dtype=torch.uint8)
         with _on_device(dev):
-            rc = lib().ojasx_b200_prompt_attention(q.data_ptr(), q.stride(0), hd, k.data_ptr(), k.stride(0), hd, v.data_ptr(), v.stride(0), hd,
-                                                   o.data_ptr(), ends, key_ends, B, T, M, Hq, Hkv, hd, scale, _DTYPE_CODES[dtype],
-                                                   None if ws is None else ws.data_ptr(), size, _stream_ptr(dev))
+            rc = lib().ojasx_b200_prompt_attention_marked(q.data_ptr(), q.stride(0), hd, k.data_ptr(), k.stride(0), hd, v.data_ptr(), v.stride(0), hd,
+                                                          o.data_ptr(), ends, key_ends, none, B, T, M, Hq, Hkv, hd, scale, _DTYPE_CODES[dtype],
+                                                          None if ws is None else ws.data_ptr(), size, _stream_ptr(dev))
         if rc:
             check(rc, "ojasx_b200_prompt_attention")
     return o

@@ -200,6 +200,19 @@ class VQDecoderStack:
         self._move_to(0)
         self.position = 0
 
+    def crop(self, max_length: int) -> int:
+        """Forget the tokens beyond ``max_length`` of every sequence: the next token takes their place and sees none of them.  Returns the
+        new length."""
+        if max_length < 0:
+            raise ValueError("max_length must be nonnegative")
+        length = min(int(max_length), self.position)
+        if not self.q4:
+            for l in self.layers:
+                l.cache.crop(length)
+        self._move_to(length)
+        self.position = length
+        return length
+
     def _move_to(self, position: int) -> None:
         self.pos.fill_(position)
         self.lengths.fill_(position + 1)

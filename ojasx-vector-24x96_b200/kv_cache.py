@@ -5,9 +5,10 @@ The reference manager watches whatever a HuggingFace model returns as ``past_key
 and trims it.  Here the caches are the codebook-quantised ``ops.VQKVCache`` objects of this package (one
 per decoder layer): the manager admits a sequence length against ``max_context_length``, reports the bytes
 the code storage occupies, and ``crop`` / ``reset`` act on the device-side lengths, so a cropped cache
-decodes over the shorter context; a 4-bit paged cache (``ops.Q4PagedKVCache``) is counted with its pages, the
-lengths of its sequences are the caller's (``update(..., sequence_length=n)``, and a crop is a smaller length in the
-next call).  Plain tensor structures (``((k, v), ...)`` tuples, lists, dicts) are
+decodes over the shorter context.  A decoder stack (``inference_engine.VQDecoderStack``) is cropped with its positions,
+whatever caches it has.  A 4-bit paged cache (``ops.Q4PagedKVCache``) by itself is counted with its pages; the lengths of
+its sequences are the caller's and come with every call, so that ``update`` asks for them (``sequence_length=n``) and
+``crop`` below them is refused.  Plain tensor structures (``((k, v), ...)`` tuples, lists, dicts) are
 still counted and cropped along their sequence axis, which keeps callers of the reference class working.
 """
 from __future__ import annotations
@@ -54,6 +55,11 @@ def _walk(obj: Any, depth: int = 0) -> Iterable[Any]:
         yield from _walk(getattr(obj, "layers"), depth + 1)
 
 
+def _is_stack(obj: Any) -> bool:
+    """A decoder stack of this package: it holds the positions that belong to its caches."""
+    return hasattr(obj, "position") and hasattr(obj, "crop") and any(isinstance(l, _CACHES) for l in _walk(getattr(obj, "layers", None)))
+
+
 class OjasXKVCacheManager:
     def __init__(self, max_context_length: int = 2048, default_dtype: Union[torch.dtype, str] = torch.float16) -> None:
         if max_context_length <= 0:
@@ -81,6 +87,8 @@ class OjasXKVCacheManager:
         return out
 
     def _infer_sequence_length(self) -> Optional[int]:
+        if _is_stack(self.past_key_values):
+            return int(self.past_key_values.position)
         for leaf in self._leaves():
             if isinstance(leaf, VQKVCache):
                 return int(leaf.seq_len)
@@ -121,6 +129,8 @@ class OjasXKVCacheManager:
 
     # ------------------------------------------------------------------ the reference's four calls
     def update(self, past_key_values: Any, sequence_length: Optional[int] = None) -> None:
+        if sequence_length is None and not _is_stack(past_key_values) and any(isinstance(l, Q4PagedKVCache) for l in _walk(past_key_values)):
+            raise ValueError("the lengths of a 4-bit cache's sequences are the caller's: give sequence_length")
         self.past_key_values = past_key_values
         if sequence_length is not None:
             self._seen_tokens = int(sequence_length)
@@ -147,12 +157,17 @@ class OjasXKVCacheManager:
     def crop(self, max_length: int) -> None:
         if max_length < 0:
             raise ValueError("max_length must be nonnegative")
+        if max_length < self.sequence_length and not _is_stack(self.past_key_values) and any(isinstance(l, Q4PagedKVCache) for l in self._leaves()):
+            raise ValueError("the lengths of a 4-bit cache's sequences are the caller's: give update the shorter one")
 
         def trim(obj: Any) -> Any:
             if isinstance(obj, VQKVCache):
                 obj.crop(max_length)
                 return obj
             if isinstance(obj, Q4PagedKVCache):
+                return obj
+            if _is_stack(obj):
+                obj.crop(max_length)
                 return obj
             if isinstance(obj, torch.Tensor):
                 return obj[..., :max_length, :] if obj.ndim >= 2 and obj.shape[-2] > max_length else obj

@@ -747,12 +747,14 @@ __global__ void __launch_bounds__(256) prompt_split_kernel(const __grid_constant
     const float4* from = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(values ? P.v : P.k) + key * (values ? P.v_row : P.k_row) +
                                                          head * (values ? P.v_head : P.k_head) + 8 * l);
     const float4 x = from[0], y = from[1];
-    const float xs[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+    float xs[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
     unsigned most = 0;
+    bool odd = false;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
         const unsigned b = __float_as_uint(xs[e]) & 0x7fffffffu;
         if (b < 0x7f800000u) most = max(most, b);
+        else odd = true;
     }
     const unsigned lanes = ((1u << L) - 1u) << (threadIdx.x % 32 / L * L);   // the row's: they are all here, or none of them
 #pragma unroll
@@ -764,6 +766,14 @@ __global__ void __launch_bounds__(256) prompt_split_kernel(const __grid_constant
         e = P.none && P.none[key] ? -INFINITY : (float)p;   // a key that nobody sees: its scores, which e is added to, are -inf
     } else {
         gm_scale(most, up, down);
+        // A key with infinities: their signs alone, times infinity, so that its scores are infinite or, where the query is zero, NaN.  (Two
+        // infinities that cancel in a score, as far as the queries' sizes let them, are taken for the larger one.)
+        if (__any_sync(lanes, odd)) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) xs[i] = isinf(xs[i]) ? copysignf(1.0f, xs[i]) : isnan(xs[i]) ? xs[i] : 0.0f;
+            up = 1.0f;
+            down = INFINITY;
+        }
     }
     unsigned hi[4], lo[4];
 #pragma unroll

@@ -5,6 +5,9 @@ import torch
 from ojasx_b200 import ops
 from ojasx_b200._lib import lib
 
+from q4_plain import tolerance
+from test_prefill_holes_gpu import _masked as masked
+
 pytestmark = pytest.mark.gpu
 
 
@@ -30,3 +33,28 @@ def test_a_context_longer_than_a_wait(cuda):
     # each of the first rows sees up to 299 keys less, in a step that its mask cuts: sums beyond 2^24 are then off by one part in 2^24
     assert bool(((out.float() - 1).abs() <= 2.0 ** -8).all()), float((out.float() - 1).abs().max())
     print(f"{start.elapsed_time(end):.0f} ms")
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("hd,n,m", [(64, 150, 150), (128, 40, 3000)])
+def test_a_key_with_an_infinity(cuda, dtype, hd, n, m):
+    """A score of -inf weighs nothing, one of +inf or NaN leaves no result: by the sign of the one element of a query that meets it."""
+    g = torch.Generator(device="cuda").manual_seed(hd)
+    q, k, v = (torch.randn(r, h, hd, generator=g, device=cuda).to(dtype) for r, h in ((n, 4), (m, 2), (m, 2)))
+    at, first = m - n // 2, n - n // 2          # the key, and the first query that sees it
+    k[at, 0, 5] = -float("inf")                 # (of the first KV head, which two query heads share)
+    q[:, :2, 5] = q[:, :2, 5].abs().clamp(min=0.25)
+    q[first + 3, 0, 5] *= -1
+    q[first + 4, 1, 5] = 0
+    got = ops.prompt_attention(q, k, v, _ints(0, n), _ints(0, m)).double()
+    finite = torch.ones(n, 4, dtype=torch.bool, device=cuda)
+    finite[first + 3, 0] = finite[first + 4, 1] = False
+    assert torch.equal(torch.isfinite(got).all(-1), finite) and not torch.isfinite(got[~finite]).any()
+    keys = k.clone()
+    keys[at, 0] = 0
+    seen = torch.arange(m, device=cuda) <= torch.arange(m - n, m, device=cuda)[:, None]
+    for heads, see in ((slice(0, 2), seen & (torch.arange(m, device=cuda) != at)), (slice(2, 4), seen)):
+        kv = slice(heads.start // 2, heads.start // 2 + 1)
+        want, big, spread, mass = masked(q[:, heads], keys[:, kv].double(), v[:, kv].double(), see)
+        tol = tolerance(dtype, want, big, spread, mass, hd)
+        assert bool(((got[:, heads] - want).abs() <= tol)[finite[:, heads]].all())

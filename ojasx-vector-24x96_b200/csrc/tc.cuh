@@ -118,17 +118,9 @@ __device__ __forceinline__ void tc_st32(unsigned addr, const unsigned* v) {
         "%21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};" ::OJX_I8(v, 0), OJX_I8(v, 8), OJX_I8(v, 16), OJX_I8(v, 24), "r"(addr)
         : "memory");
 }
-__device__ __forceinline__ void tc_ld16(unsigned addr, unsigned* v) {
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
-                 : OJX_R8(v, 0), OJX_R8(v, 8)
-                 : "r"(addr));
-}
 __device__ __forceinline__ void tc_st16(unsigned addr, const unsigned* v) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};" ::OJX_I8(v, 0), OJX_I8(v, 8), "r"(addr)
                  : "memory");
-}
-__device__ __forceinline__ void tc_st8(unsigned addr, const unsigned* v) {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%8], {%0, %1, %2, %3, %4, %5, %6, %7};" ::OJX_I8(v, 0), "r"(addr) : "memory");
 }
 __device__ __forceinline__ unsigned tc_ld1(unsigned addr) {
     unsigned v;
@@ -138,7 +130,6 @@ __device__ __forceinline__ unsigned tc_ld1(unsigned addr) {
 #define OJX_P8(v, i) "+r"((v)[i]), "+r"((v)[i + 1]), "+r"((v)[i + 2]), "+r"((v)[i + 3]), "+r"((v)[i + 4]), "+r"((v)[i + 5]), "+r"((v)[i + 6]), "+r"((v)[i + 7])
 // Keeps the uses of loaded columns behind the wait for them.
 __device__ __forceinline__ void tc_pin32(unsigned* v) { asm volatile("" : OJX_P8(v, 0), OJX_P8(v, 8), OJX_P8(v, 16), OJX_P8(v, 24)); }
-__device__ __forceinline__ void tc_pin16(unsigned* v) { asm volatile("" : OJX_P8(v, 0), OJX_P8(v, 8)); }
 #undef OJX_R8
 #undef OJX_I8
 #undef OJX_P8

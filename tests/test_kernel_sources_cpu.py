@@ -17,3 +17,11 @@ def test_masks_of_shuffles_name_the_lanes_that_take_part():
     sources = glob.glob(os.path.join(CSRC, "*.cu")) + glob.glob(os.path.join(CSRC, "*.cuh"))
     assert sources
     assert [os.path.basename(p) for p in sources if "__activemask" in _code(p)] == []
+
+
+def test_every_wrapper_has_a_caller():
+    """Device functions of the header of instruction wrappers are called by a kernel (or by one another)."""
+    code = {os.path.basename(p): _code(p) for p in glob.glob(os.path.join(CSRC, "*.cu")) + glob.glob(os.path.join(CSRC, "*.cuh"))}
+    names = set(re.findall(r"\b(tc_\w+)\(", code["tc.cuh"]))
+    assert len(names) > 20
+    assert [n for n in sorted(names) if sum(len(re.findall(rf"\b{n}\b", text)) for text in code.values()) < 2] == []

@@ -745,6 +745,7 @@ extern "C" {
 
 size_t ojasx_b200_q4kv_decode_workspace(const OjasxQ4Cache* cache, int batch, int max_pages, int io_dtype) {
     if (!cache || batch <= 0 || max_pages <= 0 || cache->page_size <= 0 || cache->kv_heads <= 0 || cache->q_heads <= 0) return 0;
+    if (io_dtype != OJX_F32 && io_dtype != OJX_BF16) return 0;
     return q4_decode_bytes(q4_decode_ctas(batch, max_pages, cache->page_size, cache->kv_heads, cache->q_heads / cache->kv_heads), cache->head_dim);
 }
 

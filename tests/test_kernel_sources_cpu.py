@@ -25,3 +25,11 @@ def test_every_wrapper_has_a_caller():
     names = set(re.findall(r"\b(tc_\w+)\(", code["tc.cuh"]))
     assert len(names) > 20
     assert [n for n in sorted(names) if sum(len(re.findall(rf"\b{n}\b", text)) for text in code.values()) < 2] == []
+
+
+def test_the_decode_has_no_workspace_for_other_types():
+    import ctypes
+    from ojasx_b200._lib import Q4Cache, lib
+    c = Q4Cache(pool=4096, status=4096, turns=None, num_pages=1, page_size=16, kv_heads=2, q_heads=4, head_dim=128)
+    size = [lib().ojasx_b200_q4kv_decode_workspace(ctypes.addressof(c), 1, 1, t) for t in (0, 1, 2, -1)]
+    assert size[0] == size[1] > 0 and size[2:] == [0, 0]

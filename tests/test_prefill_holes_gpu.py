@@ -103,3 +103,63 @@ def test_a_chunk_of_one_is_a_step(cuda, dtype):
     one = c.prefill(q, k, v, table, _ints([n]), _ends([1]), _ends([n + 1]), n + 1)
     step = c.decode(c.append(k, v, table, _ints([n]), q=q), table, _ints([n + 1]))
     assert float((step.float() - one.float()).abs().max()) <= (2.0 ** -14 if dtype == torch.float32 else 0.08)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("page", [48, 80, 144, 1008])
+def test_pages_of_any_multiple_of_a_tile(cuda, dtype, page):
+    """The same tokens in pages of 16 and of other sizes: the same codes and the same bits from every call."""
+    g, hd, pasts, lengths = _gen(page), 64, [0, 37, 1000], [300, 1, 77]
+    totals = [p + n for p, n in zip(pasts, lengths)]
+    n, m = sum(lengths), sum(totals)
+    k, v, q = (torch.randn(m, h, hd, generator=g, device=cuda).to(dtype) for h in (2, 2, 6))
+    got = []
+    for size in (16, page):
+        c = ops.Q4PagedKVCache(sum(-(-t // size) for t in totals) + 2, size, 2, 6, hd, rope_theta=THETA)
+        table = random_table(c, totals, g)
+        first = torch.cat([torch.arange(e - t, e - t + p) for e, t, p in zip(np.cumsum(totals), totals, pasts)]).to(cuda)
+        then = torch.cat([torch.arange(e - t + p, e) for e, t, p in zip(np.cumsum(totals), totals, pasts)]).to(cuda)
+        c.append(k[first], v[first], table, _ints([0] * 3), cu_seqlens=_ends(pasts))
+        out = c.prefill(q[then], k[then], v[then], table, _ints(pasts), _ends(lengths), _ends(totals), m)
+        got.append((out, c.decode(q[:3], table, _ints(totals)), *c.read(table, _ends(totals), m, dtype=dtype)))
+        c.check()
+    for a, b in zip(*got):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_a_captured_prefill_follows_tables_and_positions(cuda, dtype):
+    """One graph for chunks of up to 64 tokens over up to 400 cached ones; replayed on two streams in turn, with holes the second time."""
+    g, hd, most = _gen(13), 128, 400
+    c = ops.Q4PagedKVCache(60, 16, 2, 8, hd, rope_theta=THETA)
+    random_pool(c, g)
+    q, k, v = (torch.randn(64, h, hd, generator=g, device=cuda).to(dtype) for h in (8, 2, 2))
+    tables, pos, ends, totals = random_table(c, [200, 200], g, width=13), _ints([0, 0]), _ends([10, 20]), _ends([10, 20])
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        out = c.prefill(q, k, v, tables, pos, ends, totals, most)
+    for turn, (pasts, lengths) in enumerate((([100, 0], [30, 34]), ([3, 150], [1, 50]), ([136, 136], [64, 0]))):
+        now = random_table(c, [200, 200], g, width=13)
+        if turn == 1:
+            now[1, 4] = now[0, 0] = -1
+        tables.copy_(now)
+        pos.copy_(_ints(pasts))
+        ends.copy_(_ends(lengths))
+        totals.copy_(_ends([p + n for p, n in zip(pasts, lengths)]))
+        kept = c.pool.clone()
+        with torch.cuda.stream(torch.cuda.current_stream() if turn % 2 else side):
+            side.wait_stream(torch.cuda.default_stream())
+            graph.replay()
+        torch.cuda.synchronize()
+        pool = c.pool.clone()
+        c.pool.copy_(kept)
+        want = c.prefill(q, k, v, now, _ints(pasts), _ends(lengths), _ends([p + n for p, n in zip(pasts, lengths)]), sum(pasts) + sum(lengths))
+        rows = sum(lengths)
+        assert torch.equal(c.pool, pool)
+        # the plan of the captured call is for 400 keys: sums may be shared out differently
+        bound = 2.0 ** -15 if dtype == torch.float32 else 2.0 ** -6
+        assert float((out[:rows].float() - want[:rows].float()).abs().max()) <= bound * float(want[:rows].float().abs().max())

@@ -16,17 +16,17 @@
 // one two of them (22 bits); so is p * s * 2^u, one with bf16 activations (11 bits, below the rounding of the result), two with fp32.
 // Each head has an exponent u for each group of dimensions, which goes down where a product would pass 2^14, so that the largest so far is at
 // 2^5: scales that differ from token to token or from group to group, by 2^22 in the tests, cost one another no bits.  (One exponent for
-// all of them, that of the largest scale met so far, took 64 and 152 us in the place of the 71 and 158 below, but a token of large scale and next to
+// all of them, that of the largest scale met so far, took 64 and 145 us in the place of the 67 and 149 below, but a token of large scale and next to
 // no weight cost all others theirs: 1.4e-4 off 64 bits at 2^16, 8e-3 at 2^22.)  u is 100 at most: scales below 2^-100 weigh nothing.
 //
 // Work: units of 128 tokens of a (sequence, KV head, eight query heads), all of them in a row, in equal shares for the CTAs whatever the
 // lengths are; the four warps of a CTA take two tiles of a unit each, from rings of their own that bulk copies fill.  A share that begins
 // or ends inside a sequence leaves its sums to q4_combine_kernel.
 //
-// No pipe is full (integer pipe about half, tensor pipe a fifth, 12 warps an SM): warps wait for their chains of product, exponential and
-// product, next to the copies, which alone take 111 to 130 us: 16 sequences of 32768 tokens, 671 MB, in 158 us (4.2 TB/s) with 8 KV heads of
-// 4 query heads of 128 in bf16; 48 of up to 20011, 4 heads of 7 of 64 in fp32, 106 MB, in 71 us, where the second planes of queries and
-// weights double the products.  fp32 at head_dim 128 spills 92 bytes (168 registers for three CTAs an SM).
+// No pipe is full (integer pipe 55 %, tensor pipe 20 %, 12 warps an SM, 391 instructions a tile and warp): warps wait for their chains of
+// product, exponential and product, next to the copies, which alone take 111 to 130 us: 16 sequences of 32768 tokens, 671 MB, in 149 us
+// (4.5 TB/s) with 8 KV heads of 4 query heads of 128 in bf16; 48 of up to 20011, 4 heads of 7 of 64 in fp32, 106 MB, in 67 us, where the
+// second planes of queries and weights double the products.  fp32 at head_dim 128 spills 48 bytes (168 registers for three CTAs an SM).
 #include <algorithm>
 #include <cmath>
 
@@ -451,8 +451,9 @@ __global__ void __launch_bounds__(kQdThreads, kQdCtas) q4_decode_kernel(const __
                 now[1] = fmaxf(now[1], fmaxf(x[i][1], x[i][3]));
             }
             // the reference moves where a lane sees a score too far above it; by a whole number, so that all factors are powers of two
-            if (__any_sync(0xffffffffu, fmaf(now[0], unscale[0], -kQdSlack) > top[0] || fmaf(now[1], unscale[1], -kQdSlack) > top[1])) {
-                int rise[2];
+            int rise[2] = {0, 0};
+            bool update = __any_sync(0xffffffffu, fmaf(now[0], unscale[0], -kQdSlack) > top[0] || fmaf(now[1], unscale[1], -kQdSlack) > top[1]);
+            if (update) {
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
 #pragma unroll
@@ -460,25 +461,16 @@ __global__ void __launch_bounds__(kQdThreads, kQdCtas) q4_decode_kernel(const __
                     const float to = fmaf(now[h], unscale[h], -kQdSlack) > top[h] ? ceilf(now[h] * unscale[h]) : top[h];
                     rise[h] = (int)fminf(to - top[h], 1000.0f);
                     top[h] = to;
-                    const float keep = q4_power(127 - rise[h]);
-                    l[h] *= keep;
-#pragma unroll
-                    for (int g = 0; g < G; ++g) mins[g][h] *= keep;
                 }
-                // what the operands are made of grows by as much: the sums stay, unless a group's factor would leave its range
+                if (u > u0) {
 #pragma unroll
-                for (int g = 0; g < G; ++g) {
-                    const float2 f = up[g * 4];
-                    const int e0 = q4_bits(f.x) + rise[0], e1 = q4_bits(f.y) + rise[1];
-                    __syncwarp();
-                    if (gq == 0) up[g * 4] = make_float2(q4_power(min(e0, kQdMost)), q4_power(min(e1, kQdMost)));
-                    const float keep[2] = {q4_power(127 + min(kQdMost - e0, 0)), q4_power(127 + min(kQdMost - e1, 0))};
+                    for (int h = 0; h < 2; ++h) {
+                        const float keep = q4_power(127 - rise[h]);
+                        l[h] *= keep;
 #pragma unroll
-                    for (int m = 2 * g; m < 2 * g + 2; ++m)
-#pragma unroll
-                        for (int h = 0; h < 2; ++h) { o[m][h] *= keep[h]; o[m][h + 2] *= keep[h]; }
+                        for (int g = 0; g < G; ++g) mins[g][h] *= keep;
+                    }
                 }
-                __syncwarp();
             }
 #pragma unroll
             for (int i0 = 0; i0 < kQdPair; i0 += kAtOnce) {
@@ -517,9 +509,59 @@ __global__ void __launch_bounds__(kQdThreads, kQdCtas) q4_decode_kernel(const __
                         mins[g][1] = fmaf(p[1], low, fmaf(p[3], high, mins[g][1]));
                     }
                 }
-                // p * s * 2^u as fp16 parts; where one is too large, the exponents u go down and they are made again
+                // p * s * 2^u as fp16 parts.  Where the reference has risen, u has with it, and the sums stay; u goes down where a product would be
+                // too large (of the first ones always), and the sums with it.
                 unsigned y[kAtOnce][G][NP][2];
-                for (bool again = false;; again = true) {
+                for (;; update = true) {
+                    if (update) {
+                        float high[G][2];
+                        int was[G][2];
+#pragma unroll
+                        for (int g = 0; g < G; ++g) {
+                            const float2 f = up[g * 4];
+                            was[g][0] = q4_bits(f.x) + rise[0];
+                            was[g][1] = q4_bits(f.y) + rise[1];
+                            high[g][0] = high[g][1] = 0.0f;
+                        }
+#pragma unroll
+                        for (int i = 0; i < kAtOnce; ++i) {
+                            Metas sa, sb;
+                            metas(i, T::value_scales, sa, sb);
+#pragma unroll
+                            for (int g = 0; g < G; ++g)
+#pragma unroll
+                                for (int h = 0; h < 2; ++h)
+                                    high[g][h] = fmaxf(high[g][h], fmaxf(fabsf(x[i0 + i][h] * of_group(sa, g)), fabsf(x[i0 + i][h + 2] * of_group(sb, g))));
+                        }
+#pragma unroll
+                        for (int off = 4; off < 32; off <<= 1)
+#pragma unroll
+                            for (int g = 0; g < G; ++g)
+#pragma unroll
+                                for (int h = 0; h < 2; ++h) high[g][h] = fmaxf(high[g][h], __shfl_xor_sync(0xffffffffu, high[g][h], off));
+                        __syncwarp();
+#pragma unroll
+                        for (int g = 0; g < G; ++g) {
+                            int to[2];
+#pragma unroll
+                            for (int h = 0; h < 2; ++h) {
+                                to[h] = min(min(was[g][h], kQdMost), 254 + kQdRoom - q4_bits(high[g][h]));
+                                was[g][h] = to[h] - was[g][h];
+                            }
+                            if (gq == 0) up[g * 4] = make_float2(q4_power(to[0]), q4_power(to[1]));
+                        }
+                        if (u > u0 || i0 > 0) {   // (there are no sums before)
+#pragma unroll
+                            for (int g = 0; g < G; ++g)
+#pragma unroll
+                                for (int h = 0; h < 2; ++h) {
+                                    const float keep = q4_power(127 + was[g][h]);
+#pragma unroll
+                                    for (int m = 2 * g; m < 2 * g + 2; ++m) { o[m][h] *= keep; o[m][h + 2] *= keep; }
+                                }
+                        }
+                        __syncwarp();
+                    }
                     unsigned most = 0;
 #pragma unroll
                     for (int i = 0; i < kAtOnce; ++i) {
@@ -537,39 +579,10 @@ __global__ void __launch_bounds__(kQdThreads, kQdCtas) q4_decode_kernel(const __
                             most = __vimax3_u16x2(most, y[i][g][0][0], y[i][g][0][1]);
                         }
                     }
-                    if (again || !__any_sync(0xffffffffu, (most + (0x80008000u - kQdTooLarge)) & 0x80008000u)) break;
-#pragma unroll
-                    for (int g = 0; g < G; ++g) {
-                        float high[2] = {0.0f, 0.0f};
-#pragma unroll
-                        for (int i = 0; i < kAtOnce; ++i) {
-                            Metas sa, sb;
-                            metas(i, T::value_scales, sa, sb);
-#pragma unroll
-                            for (int h = 0; h < 2; ++h) high[h] = fmaxf(high[h], fmaxf(fabsf(x[i0 + i][h] * of_group(sa, g)), fabsf(x[i0 + i][h + 2] * of_group(sb, g))));
-                        }
-                        const float2 f = up[g * 4];
-                        const int was[2] = {q4_bits(f.x), q4_bits(f.y)};
-                        int now_at[2];
-#pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-#pragma unroll
-                            for (int off = 4; off < 32; off <<= 1) high[h] = fmaxf(high[h], __shfl_xor_sync(0xffffffffu, high[h], off));
-                            now_at[h] = min(was[h], 254 + kQdRoom - q4_bits(high[h]));
-                        }
-                        __syncwarp();
-                        if (gq == 0) up[g * 4] = make_float2(q4_power(now_at[0]), q4_power(now_at[1]));
-#pragma unroll
-                        for (int m = 2 * g; m < 2 * g + 2; ++m)
-#pragma unroll
-                            for (int h = 0; h < 2; ++h) {
-                                const float keep = q4_power(127 + now_at[h] - was[h]);
-                                o[m][h] *= keep;
-                                o[m][h + 2] *= keep;
-                            }
-                    }
-                    __syncwarp();
+                    if (update || !__any_sync(0xffffffffu, (most + (0x80008000u - kQdTooLarge)) & 0x80008000u)) break;
                 }
+                update = false;
+                rise[0] = rise[1] = 0;
 #pragma unroll
                 for (int i = 0; i < kAtOnce; ++i) {
                     const unsigned char* tile = stage + (i0 + i) * T::bytes;
@@ -604,6 +617,13 @@ __global__ void __launch_bounds__(kQdThreads, kQdCtas) q4_decode_kernel(const __
         }
 
         // the warps' sums joined, and out
+        float down[G][2];   // 2^-u
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+            const float2 f = up[g * 4];
+            down[g][0] = q4_power(254 - q4_bits(f.x));
+            down[g][1] = q4_power(254 - q4_bits(f.y));
+        }
 #pragma unroll
         for (int off = 4; off < 32; off <<= 1)
 #pragma unroll
@@ -622,9 +642,7 @@ __global__ void __launch_bounds__(kQdThreads, kQdCtas) q4_decode_kernel(const __
             for (int h = 0; h < 2; ++h) {
                 if (2 * t + h >= sum_heads) continue;
                 float* to = sums + (warp * sum_heads + 2 * t + h) * M::row + 32 * (m >> 1) + 4 * gq + 2 * (m & 1);
-                const float2 f = up[(m >> 1) * 4];
-                const float down = q4_power(254 - q4_bits(h ? f.y : f.x));
-                *reinterpret_cast<float2*>(to) = make_float2(fmaf(o[m][h] * down, kCode, mins[m >> 1][h]), fmaf(o[m][h + 2] * down, kCode / 16.0f, mins[m >> 1][h]));
+                *reinterpret_cast<float2*>(to) = make_float2(fmaf(o[m][h] * down[m >> 1][h], kCode, mins[m >> 1][h]), fmaf(o[m][h + 2] * down[m >> 1][h], kCode / 16.0f, mins[m >> 1][h]));
             }
         __syncthreads();
         unit += u1 - u0;

@@ -399,7 +399,7 @@ OJASX_API int ojasx_b200_paged_kv_decode(const void* d_q, void* d_out, const int
  *
  * Format: 32 consecutive dimensions of a token's key or value share a bf16 minimum (the largest not above their own) and a bf16
  * scale (the smallest not below (max - minimum) / 15); a value is a code 0..15 and reads as code * scale + minimum, within half a
- * scale of what it was.  A group that holds an infinity or a NaN reads as NaN.
+ * scale of what it was.  A group that holds an infinity, a NaN or a value below bf16's lowest reads as NaN.
  * d_block_table [batch, max_pages] int32 names the pages of every sequence.  Entries outside [0, num_pages) are no page: tokens
  * there are dropped by an append, read as zeros and weigh nothing in a decode or a prefill, and *status becomes 1; so it is with
  * tokens beyond max_pages, and a sequence with a negative position is left out as a whole.

@@ -30,16 +30,17 @@ struct PromptProblem {
 // time.  Per tile and step: S = Q K^T into tensor memory, one thread per row takes the maximum, the exponentials and their sum, writes
 // the weights back over S as bf16, O += P V with P read from tensor memory.  A tile has S twice: the products of a step are made while
 // the row's threads are at the step before, and those of the tiles go on in turn.  (With one S of 128 keys a tile, whose products wait
-// for its weights: 526 us at 8192 positions, 139 packed.)
+// for its weights: 139 against 129 us for packed prompts, 306 against 299 for 1024 positions behind 7000.)
 //   warps 0..3, 4..7: the rows of the two tiles; warp 8: issues the products; warp 9: the copies of Q, K and V (K and V in a ring);
 //   warp 11: what to do next, so that a CTA's copies and products for one part of the prompts begin while it is at the last results of
-//   another (packed prompts 171 us without, 150 with it); warp 10: none.  Registers move between groups of four warps: 384 * 168 are
+//   another (packed prompts 171 us without and 154 with it, when they were that slow); warp 10: none.  Registers move between groups of four warps: 384 * 168 are
 //   2 * 128 * 200 + 128 * 96 and some.
 // Maxima are left behind: a row's sums are relative to the maximum it had when a score was last more than 2^8 above it, so that
 // O is rescaled a few times per row and not once per step (weights up to 2^8 cost nothing in bf16 or in fp32 sums).
 // Weights are rounded to bf16, below the rounding of the result.  Bound by the chain from a product through maximum and exponentials to the
-// next one (tensor pipe 54 %, exponentials 54 % of their pipe, at 1.66 GHz under load): 8192 positions of 32 query heads and 8 KV heads of
-// 128 take 524 us, 1050 TFLOP/s.  Products issued by a warp as a whole with an elected lane, and not by one lane in a branch: 610 -> 562.
+// next one (tensor pipe 56 %, exponentials 56 % of their pipe): 8192 positions of 32 query heads and 8 KV heads of 128 take 497 to 523 us by
+// CUDA events, call after call, on several GPUs whose power limit sets their clocks (1.66 GHz), 1050 to 1110 TFLOP/s.  Products issued
+// by a warp as a whole with an elected lane, and not by one lane in a branch: 610 -> 562.
 constexpr int kPaRows = 128, kPaKeys = 64, kPaThreads = 384;
 constexpr float kPaSlack = 8.0f;
 constexpr long long kPaPartClocks = 1LL << 35;   // 18 s: a step of 64 keys takes a microsecond, and 10^9 keys do not fit into the memory
@@ -710,8 +711,9 @@ static int launch_prompt_tc(const PromptProblem& P, cudaStream_t s) {
 // The high parts of Q are in tensor memory, where products take them without the shared memory's bandwidth; the low ones, and K and V
 // in steps of 64 keys, are in shared memory.  The tensor cores cut what they add to a sum, so a step's products with V are summed on
 // their own and join the row's fp32 sums, which are in its thread's registers.  Bound by what a row's thread does for a step (the two parts
-// of 64 weights, O of the step before); the tensor pipe is 41 % busy.  Two prompts of 2048 with 32 query heads and 8 KV heads of 128: 276 us,
-// 249 TFLOP/s of the formula, 747 of fp16 products (4750 us with fp32 FMA, 364 with all of Q in shared memory).  Two S of 32 keys a tile, so
+// of 64 weights, O of the step before, and at head_dim 128 some of the 312 bytes that do not fit into its registers, 116 at 64); the tensor
+// pipe is 41 % busy.  Two prompts of 2048 with 32 query heads and 8 KV heads of 128: 263 to 272 us, 253 to 261 TFLOP/s of the formula, three
+// times as many of fp16 products (4750 us with fp32 FMA, 364 with all of Q in shared memory).  Two S of 32 keys a tile, so
 // that products and exponentials overlap within a tile too, took a fifth longer: every step has its waits, whatever its length.
 constexpr int kPpKeys = 64;
 constexpr float kPpRoom = 5.0f;   // y is 2^5 at most when the reference is set, 2^13 later on
@@ -731,8 +733,8 @@ struct PromptSplit {
     float2* factors;        // [kv_heads][n_keys]: 1 / scale of the key's row of K, e of its row of V
 };
 
-// A row of K or V per HD / 8 lanes, 16 bytes in and out; bound by the instructions of the split.  The two kernels take 283.3 us for two
-// prompts of 2048 (285.4 with HD / 4 lanes to a row).
+// A row of K or V per HD / 8 lanes, 16 bytes in and out; bound by the instructions of the split and the latency of its loads.  (With HD / 4
+// lanes to a row the two kernels took 285.4 us for two prompts of 2048, with HD / 8 283.3 then.)
 template <int HD>
 __global__ void __launch_bounds__(256) prompt_split_kernel(const __grid_constant__ PromptProblem P, const __grid_constant__ PromptSplit S) {
     constexpr int L = HD / 8;
@@ -1092,8 +1094,8 @@ __global__ void __launch_bounds__(kPaThreads, 1) prompt_pair_kernel(const __grid
                     for (int u = 0; u < 2; ++u) {
                         const unsigned long long y = pa_exp2(pa_add2((unsigned long long)s[c + e + 2 * u + 1] << 32 | s[c + e + 2 * u], off2));
                         sum = pa_fma2(y, vfs[u], sum);
-                        // the high part is cut to 11 bits, which fp16 holds as they are (283 us with a
-                        // rounded one, which has to come back from fp16; 3.3e-7 and 3.4e-7 off 64 bits)
+                        // the high part is cut to 11 bits, which fp16 holds as they are (266 us with a
+                        // rounded one, which has to come back from fp16, and 254.5 so on one box; 3.3e-7 and 3.4e-7 off 64 bits)
                         const unsigned yl = (unsigned)y & 0xffffe000u, yh = (unsigned)(y >> 32) & 0xffffe000u;
                         const __half2 h = __floats2half2_rn(__uint_as_float(yl), __uint_as_float(yh));
                         const unsigned long long rest = pa_fma2((unsigned long long)yh << 32 | yl, pa_pair(-1.0f, -1.0f), y);

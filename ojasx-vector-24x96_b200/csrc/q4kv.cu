@@ -224,10 +224,10 @@ __device__ __forceinline__ bool q4_span(const int* ends, const int* positions, i
 static long long q4_spans(int rows, int batch) { return rows / kQ4Tile + 2LL * std::min(rows, batch); }
 
 // Prompts: a tile of 16 tokens per CTA and some of the heads, a token to HD / 8 lanes (or two of them at head_dim 64), which make its
-// angles once.  A head's tile is put together in shared memory and written in 16-byte pieces: its words hold two tokens each.  Bound by the
-// integer pipe (43 % busy) and by barriers between the heads' tiles: 16384 tokens of 8 KV heads of 128 in bf16 36.9 us, with 32 query
-// heads 78 (their 445 MB with the way back take 68), against 190 by single vectors, each of which
-// makes its angles anew.
+// angles once.  A head's tile is put together in shared memory and written in 16-byte pieces: its words hold two tokens each.  No pipe is
+// full (integer pipe 43 %): warps wait for their loads, one vector ahead in 64 registers, and at the barrier of every turn of heads.
+// 16384 tokens of 8 KV heads of 128 in bf16 take 36.9 us, 88 MB; with 32 query heads 78, 357 MB, against 190 by single vectors, each of
+// which makes its angles anew.  In fp32 it spills 8 to 20 bytes.
 template <int HD, bool kBf16>
 __global__ void __launch_bounds__(256, 4) q4_append_tile_kernel(const __grid_constant__ Q4AppendProblem P, int slices) {
     constexpr int L = HD / 8, G = HD / 32, W = 256 / (kQ4Tile * L);   // W: vectors of a token at a time

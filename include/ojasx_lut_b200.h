@@ -399,7 +399,7 @@ OJASX_API int ojasx_b200_paged_kv_decode(const void* d_q, void* d_out, const int
  *
  * Format: 32 consecutive dimensions of a token's key or value share a bf16 minimum (the largest not above their own) and a bf16
  * scale (the smallest not below (max - minimum) / 15); a value is a code 0..15 and reads as code * scale + minimum, within half a
- * scale of what it was.  A group that holds an infinity, a NaN or a value below bf16's lowest reads as NaN.
+ * scale of what it was.  A group that holds an infinity or a NaN reads as NaN; beyond 3.37e38 a value may read as infinite, or its group as NaN.
  * d_block_table [batch, max_pages] int32 names the pages of every sequence.  Entries outside [0, num_pages) are no page: tokens
  * there are dropped by an append, read as zeros and weigh nothing in a decode or a prefill, and *status becomes 1; so it is with
  * tokens beyond max_pages, and a sequence with a negative position is left out as a whole.
@@ -436,8 +436,10 @@ OJASX_API int ojasx_b200_q4kv_decode(const OjasxQ4Cache* cache, const void* d_q,
  * of a head in elements, the dimensions of a head together) into d_out [n_rows, q_heads, head_dim].  Rows d_ends[b] .. and keys
  * d_key_ends[b] .. belong to sequence b, whose last query sees its last key, the one before it the keys up to the one before, and so
  * on; a query that sees nothing gives zeros; rows behind the last sequence are left as they were.  Keys that a query does not see
- * have no part in its result, whatever they hold.  fp32 values up to 2^100.  workspace: ojasx_b200_prompt_workspace bytes (0 for bf16) for this call alone,
- * 256-byte aligned; the others 16-byte aligned, strides whole multiples of 16 bytes.
+ * have no part in its result, whatever they hold.  fp32 operands are kept as two fp16 numbers under a power of two of their row: 22
+ * bits for what is within 2^-17 of the row's largest, an error of 2^-40 of that for the rest; keys and queries of any size, values up to
+ * 2^100, with errors of 2^-59 where they are below 2^-37 and weights off by up to 2^-17 where they are near 2^100 (2^-24 for each power of two).  workspace: ojasx_b200_prompt_workspace bytes (0 for bf16) for this call
+ * alone, 256-byte aligned; the others 16-byte aligned, strides whole multiples of 16 bytes.
  * _marked: d_none [n_keys] bytes (NULL: none) are not zero for keys that no query sees, of the caches' tokens without a page those;
  * it is read in pieces of 16 bytes, the last of which ends behind n_keys. */
 OJASX_API size_t ojasx_b200_prompt_workspace(int n_keys, int kv_heads, int head_dim, int io_dtype);

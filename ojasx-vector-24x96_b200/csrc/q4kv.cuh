@@ -3,7 +3,8 @@
 // 32 consecutive dimensions of a token's key or value form a group with a bf16 minimum and a bf16 scale: minimum = floor(min x) and
 // scale = ceil((max x - minimum) / 15), to the neighbouring bf16 number, code = round((x - minimum) / scale) in 0..15.  Rounding the
 // two outwards keeps every x of the group inside the 16 steps, so that it is read back within half a step.  A group with a value
-// that is not finite, or below the lowest bf16 number, has a scale of zero and a NaN for its minimum, and is read back as NaN.
+// that is not finite, or below the lowest bf16 number, has a scale of zero and a NaN for its minimum, and is read back as NaN.  (The
+// largest code of a group whose maximum is beyond 3.37e38 may stand for an infinity.)
 //
 // A page of one KV head is page_size / 16 tiles of 16 tokens, each contiguous (2560 bytes at head_dim 128), pools are
 // [pages][kv_heads][tiles].  A tile is laid out as the operands of mma.sync m16n8k16 that the decode kernel makes of it, so that

@@ -672,7 +672,8 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     """Causal attention over packed prompts: ``q`` [tokens, q_heads, head_dim], ``k``, ``v`` [keys, kv_heads, head_dim], all float32 or all
     bfloat16, head_dim 64 or 128.  Sequence b has the rows ``cu_seqlens[b] .. cu_seqlens[b + 1]`` and the keys ``cu_keys[b] ..``
     (default: the same); its last query sees its last key, the one before it the keys up to the one before, and so on.  A query that
-    sees nothing gives zeros; rows behind the last sequence are not written; ``scale <= 0`` is 1/sqrt(head_dim)."""
+    sees nothing gives zeros; rows behind the last sequence are not written; ``scale <= 0`` is 1/sqrt(head_dim).  float32 operands keep
+    22 bits (of what is within 2^-17 of the largest of their row; values from 2^-37 to 2^100)."""
     return _prompt_attention(q, k, v, cu_seqlens, cu_keys, scale, out, None)
 
 

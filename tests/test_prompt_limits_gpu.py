@@ -58,3 +58,33 @@ def test_a_key_with_an_infinity(cuda, dtype, hd, n, m):
         want, big, spread, mass = masked(q[:, heads], keys[:, kv].double(), v[:, kv].double(), see)
         tol = tolerance(dtype, want, big, spread, mass, hd)
         assert bool(((got[:, heads] - want).abs() <= tol)[finite[:, heads]].all())
+
+
+@pytest.mark.parametrize("power", [-120, -45, -37, 0, 60, 95])
+@pytest.mark.parametrize("what", ["keys", "values", "one dimension"])
+def test_fp32_operands_of_any_size(cuda, what, power):
+    """Keys of any size against queries that bring the scores back; values of any size up to 2^100, with errors of 2^-59 where they are small;
+    one dimension of all rows far above or below the others.  Relative errors are independent ones as in the tests of fp32 accuracy, 2^-20;
+    what is more than 2^-17 below its row's largest is off by 2^-40 of that at most, and so is a mean of such values.  The exponent of a
+    row of values is added to its scores (up to 16 here, in powers of two), whose sum fp32 rounds to 2^-24 of its size, power + 16; a
+    weight moves by ln 2 of that, and a result by twice what its weights do."""
+    if what == "one dimension" and abs(power) > 60:
+        power //= 4
+    g = torch.Generator(device="cuda").manual_seed(7)
+    n = 400
+    q, k, v = (torch.randn(n, h, 64, generator=g, device=cuda) for h in (4, 2, 2))
+    if what == "keys":
+        k, q = k * 2.0 ** power, q * 2.0 ** -power
+    elif what == "values":
+        v = v * 2.0 ** power
+    else:
+        v[..., 9] *= 2.0 ** power
+    got = ops.prompt_attention(q, k, v, _ints(0, n)).double()
+    seen = torch.arange(n, device=cuda) <= torch.arange(n, device=cuda)[:, None]
+    want, _, _, _ = masked(q, k.double(), v.double(), seen)
+    most = float(v.abs().max())
+    floor = max(2.0 ** -59, 2.0 ** -40 * most)
+    for part in ((slice(9), slice(10, 64)), (slice(9, 10),)):
+        off, size = (torch.cat([x[..., s] for s in part], -1).square().mean().sqrt() for x in (got - want, want))
+        weights = 2 * 0.7 * 2.0 ** -24 * (abs(power) + 16) if what == "values" else 0.0
+        assert float(off) <= (2.0 ** -20 + weights) * float(size) + floor, (float(off), float(size))

@@ -122,3 +122,24 @@ def test_scales_with_a_sign_are_refused_or_lose_it(cuda):
         zero[0, 0, 3] = -0.0
         c.load(**{**pool, name: zero})
         assert torch.equal(c.pool, kept) and not bool((c.unload()[name].view(torch.int16) < 0).any())
+
+
+def test_values_at_the_ends_of_fp32(cuda):
+    """The lowest bf16 number is above the lowest fp32 ones: a group with one of those reads as NaN.  Fifteen scales, rounded up, may end
+    beyond fp32: the highest reads as infinite.  Up to 3.37e38 everything is finite, and whatever a group holds, the others are kept."""
+    c = ops.Q4PagedKVCache(1, 16, 1, 1, 64)
+    top = torch.finfo(torch.float32).max
+    x = torch.zeros(4, 1, 64, device=cuda)
+    x[0, 0, 3], x[1, 0, 40], x[2, 0, 5], x[3, 0, 50] = top, -top, -3.38e38, 3.37e38
+    c.append(x, x, _ints([[0]]), _ints([0]), cu_seqlens=_ints([0, 4]))
+    k, v = c.read(_ints([[0]]), _ints([0, 4]), 4, dtype=torch.float32)
+    bad = torch.zeros(4, 1, 64, dtype=torch.bool, device=cuda)
+    bad[1, 0, 32:] = True
+    scale = c.unload()["k_scales"][0, 0, :4].float()[:, None].repeat_interleave(32, -1)
+    for got in (k, v):
+        assert torch.equal(torch.isnan(got), bad) and not bool(torch.isfinite(got[0, 0, 3]))
+        bad[0, 0, 3] = True
+        assert torch.equal(torch.isfinite(got), ~bad)
+        # half a step, and the fp32 rounding of code * scale + minimum
+        assert bool(((got / 4 - x / 4).abs() <= scale / 4 * 0.5001 + x.abs() / 4 * 2.0 ** -22)[~bad].all())
+        bad[0, 0, 3] = False

@@ -658,8 +658,8 @@ class Q4PagedKVCache:
                 cu_seqlens: torch.Tensor, cu_context: torch.Tensor, context_tokens: int, scale: float = -1.0,
                 out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """A chunk of every sequence's prompt, packed by ``cu_seqlens``: its keys and values are appended and every query attends to the
-        cached tokens up to its own, as the cache holds them (tokens without a page weigh nothing; rows of a sequence whose position is
-        negative hold nothing).  ``cu_context`` int32 [batch + 1]: the tokens of the sequences with the
+        cached tokens up to its own, as the cache holds them, rounded to q's dtype (tokens without a page weigh nothing; rows of a sequence
+        whose position is negative hold nothing).  ``cu_context`` int32 [batch + 1]: the tokens of the sequences with the
         chunk, ends of ``positions[b] + chunk`` each; ``context_tokens``: their sum."""
         turned = self.append(k, v, block_table, positions, q=q, cu_seqlens=cu_seqlens)
         none = self.pool.new_empty((int(context_tokens) + 15) // 16 * 16)
